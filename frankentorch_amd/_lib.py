@@ -69,6 +69,31 @@ class SdpaDesc(C.Structure):
     ] + [("causal", C.c_int32), ("kv_group", C.c_int32)]
 
 
+class PagedCache(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("num_pages", "page_size", "kv_heads", "head_dim", "page_stride", "head_stride", "row_stride",
+                                         "num_seqs", "max_pages", "table_stride")] + [("dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+class PagedAppendDesc(C.Structure):
+    _fields_ = [
+        (n, C.c_int64)
+        for n in (
+            "tokens", "q_heads",
+            "q_row_stride", "q_head_stride", "k_row_stride", "k_head_stride", "v_row_stride", "v_head_stride",
+            "out_row_stride", "out_head_stride", "rotary_dim", "max_pos",
+        )
+    ] + [("interleaved", C.c_int32), ("reserved", C.c_int32)]
+
+
+class PagedSdpaDesc(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("q_heads", "new_tokens", "max_len", "q_seq_stride", "q_row_stride", "q_head_stride",
+                                         "o_seq_stride", "o_row_stride", "o_head_stride")]
+
+
+class LogitsDesc(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("rows", "vocab", "logits_stride", "out_stride", "history_stride", "bias_stride", "mask_stride")]
+
+
 class LayerWeights(C.Structure):
     _fields_ = [
         (n, C.c_void_p)
@@ -80,6 +105,7 @@ _SCALARS = {
     "int8_t": C.c_int8,
     "int32_t": C.c_int32,
     "int64_t": C.c_int64,
+    "uint32_t": C.c_uint32,
     "uint64_t": C.c_uint64,
     "size_t": C.c_size_t,
     "float": C.c_float,

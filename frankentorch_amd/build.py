@@ -36,6 +36,9 @@ HIP_SOURCES = [
     "lossops.hip",
     "ingest.hip",
     "int8ops.hip",
+    "paged_append.hip",
+    "paged_sdpa.hip",
+    "logits.hip",
     "host_api.hip",
     "resident.hip",
 ]

@@ -1,0 +1,144 @@
+// Keys and values of new tokens into a paged cache, with the position rotation of keys and queries on the way.
+//
+// One pass over the packed projection: every K, V and query element is read once and written once. A thread owns pairs of a
+// rotation (both elements of each, so queries may be rotated in place) or the same number of elements that are only copied; no
+// two threads touch one element. -ffp-contract=off rounds a c, b s and their difference one by one.
+
+#include "paged.hpp"
+
+namespace {
+
+constexpr int kBlock = 256;
+
+struct AppendArgs {
+    fth_paged_cache c;
+    fth_paged_append_desc d;
+    const float *q, *k, *v, *cosines, *sines;
+    const int32_t *table, *seq_ids, *positions;
+    float *q_out;
+    void *k_cache, *v_cache;
+    int64_t *bad;
+    int pair_units, k_units, units;  // per head: of a rotated one, pairs first; of the V rows; per token
+};
+
+__device__ __forceinline__ void store_as(float *p, float x) { *p = x; }
+__device__ __forceinline__ void store_as(fth::f16 *p, float x) { *p = (fth::f16)x; }
+__device__ __forceinline__ void store_as(fth::bf16 *p, float x) { *reinterpret_cast<__bf16 *>(p) = (__bf16)x; }
+
+// Unit u of one head's row: a pair while u < pairs, one element that is copied from there on.
+template <typename T> __device__ __forceinline__ void head_unit(const float *src, T *dst, int u, int pairs, bool interleaved, const float *c, const float *s) {
+    if (u >= pairs) {
+        store_as(dst + pairs + u, src[pairs + u]);
+        return;
+    }
+    const int ia = interleaved ? 2 * u : u, ib = interleaved ? 2 * u + 1 : u + pairs;
+    const float a = src[ia], b = src[ib], cc = c[u], ss = s[u];
+    store_as(dst + ia, a * cc - b * ss);
+    store_as(dst + ib, b * cc + a * ss);
+}
+
+template <typename T> __global__ __launch_bounds__(kBlock) void paged_append_kernel(const AppendArgs p, int blocks_per_token) {
+    const int64_t t = blockIdx.x / blocks_per_token;
+    const int part = (int)(blockIdx.x % blocks_per_token);
+    const int pos = p.positions[t];
+    if (pos == -1) return;
+    const int seq = p.seq_ids[t], page_size = (int)p.c.page_size;
+    bool ok = seq >= 0 && seq < p.c.num_seqs && pos >= 0 && pos < p.c.max_pages * p.c.page_size && (p.d.rotary_dim == 0 || pos < p.d.max_pos);
+    int page = -1;
+    if (ok) page = p.table[(int64_t)seq * p.c.table_stride + pos / page_size];
+    if (!ok || page < 0 || page >= p.c.num_pages) {
+        if (part == 0 && threadIdx.x == 0) fth::report_bad_entry(p.bad, t);
+        return;
+    }
+    const int64_t slot = (int64_t)page * p.c.page_stride + (int64_t)(pos % page_size) * p.c.row_stride;
+    const int pairs = (int)p.d.rotary_dim / 2, hd = (int)p.c.head_dim, hq = (int)p.d.q_heads, hkv = (int)p.c.kv_heads;
+    const float *c = p.cosines + (int64_t)pos * pairs, *s = p.sines + (int64_t)pos * pairs;
+    const bool inter = p.d.interleaved != 0;
+    const int rotated = (hq + hkv) * p.pair_units;
+    for (int u = part * kBlock + threadIdx.x; u < p.units; u += blocks_per_token * kBlock) {
+        if (u < rotated) {
+            const int h = u / p.pair_units, i = u % p.pair_units;
+            if (h < hq) {
+                head_unit(p.q + t * p.d.q_row_stride + h * p.d.q_head_stride, p.q_out + t * p.d.out_row_stride + h * p.d.out_head_stride, i, pairs, inter, c, s);
+            } else {
+                head_unit(p.k + t * p.d.k_row_stride + (h - hq) * p.d.k_head_stride, static_cast<T *>(p.k_cache) + slot + (h - hq) * p.c.head_stride, i, pairs, inter, c, s);
+            }
+        } else {
+            const int h = (u - rotated) / hd, i = (u - rotated) % hd;
+            head_unit(p.v + t * p.d.v_row_stride + h * p.d.v_head_stride, static_cast<T *>(p.v_cache) + slot + h * p.c.head_stride, i, 0, false, c, s);
+        }
+    }
+}
+
+template <typename T> int32_t launch(const AppendArgs &a, hipStream_t st) {
+    const int64_t per_token = fth::ceil_div(a.units, kBlock);
+    FTH_ARG(a.d.tokens * per_token <= 2147483647LL, "paged_append: too many tokens for one launch");
+    paged_append_kernel<T><<<dim3((unsigned)(a.d.tokens * per_token)), dim3(kBlock), 0, st>>>(a, (int)per_token);
+    FTH_CHECK_LAUNCH("paged_append");
+    return FTH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+void fth_dev_paged_cache_contiguous(fth_paged_cache *c, int64_t num_pages, int64_t page_size, int64_t kv_heads, int64_t head_dim, int64_t num_seqs, int64_t max_pages,
+                                int32_t dtype) {
+    if (!c) return;
+    std::memset(c, 0, sizeof *c);
+    c->num_pages = num_pages;
+    c->page_size = page_size;
+    c->kv_heads = kv_heads;
+    c->head_dim = head_dim;
+    c->row_stride = head_dim;
+    // wrapped products of sizes that no memory holds; the calls refuse such caches
+    c->head_stride = (int64_t)((uint64_t)page_size * (uint64_t)head_dim);
+    c->page_stride = (int64_t)((uint64_t)kv_heads * (uint64_t)c->head_stride);
+    c->num_seqs = num_seqs;
+    c->max_pages = c->table_stride = max_pages;
+    c->dtype = dtype;
+}
+
+int32_t fth_dev_paged_append_f32(const fth_paged_cache *c, const fth_paged_append_desc *d, const float *q, const float *k, const float *v, const float *cosines,
+                                 const float *sines, const int32_t *block_table, const int32_t *seq_ids, const int32_t *positions, float *q_out, void *k_cache,
+                                 void *v_cache, int64_t *bad_index, fth_stream s) {
+    if (int32_t rc = fth::check_paged_cache(c, "paged_append", nullptr)) return rc;
+    FTH_ARG(d, "paged_append: NULL descriptor");
+    FTH_ARG(d->tokens >= 0 && d->q_heads >= 0, "paged_append: negative extent");
+    FTH_ARG(d->rotary_dim >= 0 && d->rotary_dim % 2 == 0 && d->rotary_dim <= c->head_dim, "paged_append: rotary_dim %lld is odd or outside 0..head_dim",
+            (long long)d->rotary_dim);
+    FTH_ARG(d->rotary_dim == 0 || d->max_pos >= 0, "paged_append: negative max_pos");
+    for (int64_t x : {d->q_row_stride, d->q_head_stride, d->k_row_stride, d->k_head_stride, d->v_row_stride, d->v_head_stride, d->out_row_stride, d->out_head_stride})
+        FTH_ARG(fth::stride_in_range(x), "paged_append: a stride is negative or over 2^40");
+    if (d->q_heads + c->kv_heads > (1 << 20) || d->tokens > 2147483647LL) return fth::set_error(FTH_ERR_SIZE_OVERFLOW, "paged_append: extents overflow");
+    if (d->tokens > 0) {
+        FTH_ARG(k && v && seq_ids && positions && (block_table || c->max_pages == 0) && ((k_cache && v_cache) || c->num_pages == 0), "paged_append: NULL operand");
+        FTH_ARG(d->q_heads == 0 || (q && q_out), "paged_append: NULL queries");
+        FTH_ARG(d->rotary_dim == 0 || (cosines && sines), "paged_append: NULL rotation tables");
+        FTH_ARG(q != q_out || d->q_heads == 0 || (d->q_row_stride == d->out_row_stride && d->q_head_stride == d->out_head_stride),
+                "paged_append: queries rotated in place need the strides they have");
+    }
+    FTH_REQUIRE_DEVICE();
+    hipStream_t st = fth::resolve_stream(s);
+    if (bad_index) {
+        fth::reset_bad_kernel<<<1, 1, 0, st>>>(bad_index);
+        FTH_CHECK_LAUNCH("paged_append(bad_index reset)");
+    }
+    if (d->tokens == 0) return FTH_OK;
+    AppendArgs a;
+    a.c = *c;
+    a.d = *d;
+    a.q = q; a.k = k; a.v = v; a.cosines = cosines; a.sines = sines;
+    a.table = block_table; a.seq_ids = seq_ids; a.positions = positions;
+    a.q_out = q_out; a.k_cache = k_cache; a.v_cache = v_cache; a.bad = bad_index;
+    a.pair_units = (int)(c->head_dim - d->rotary_dim / 2);
+    a.k_units = (int)c->head_dim;
+    a.units = (int)((d->q_heads + c->kv_heads) * a.pair_units + c->kv_heads * a.k_units);
+    switch (c->dtype) {
+        case FTH_DTYPE_F32: return launch<float>(a, st);
+        case FTH_DTYPE_F16: return launch<fth::f16>(a, st);
+        default: return launch<fth::bf16>(a, st);
+    }
+}
+
+}  // extern "C"

@@ -463,5 +463,78 @@ def linear_int8_dynamic(x, m, k, w_i8, w_scales, n, bias, out, workspace=None, s
     return workspace
 
 
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 1, 2, 3
+_STORAGE = {"f32": DTYPE_F32, "f16": DTYPE_F16, "bf16": DTYPE_BF16}
+
+
+def paged_cache(num_pages, page_size, kv_heads, head_dim, num_seqs, max_pages, dtype="f32") -> _lib.PagedCache:
+    """Contiguous [num_pages, kv_heads, page_size, head_dim] K and V arrays of type "f32", "f16" or "bf16", and a
+    [num_seqs, max_pages] int32 block table. Other layouts: set the strides of the result."""
+    c = _lib.PagedCache()
+    _lib.load().fth_dev_paged_cache_contiguous(C.byref(c), num_pages, page_size, kv_heads, head_dim, num_seqs, max_pages, _STORAGE[dtype])
+    return c
+
+
+def paged_append_desc(cache, tokens, q_heads=0, rotary_dim=0, max_pos=0, interleaved=False, row_stride=None) -> _lib.PagedAppendDesc:
+    """Operands [tokens, heads, head_dim]; row_stride: the row pitch of q, k and v where they are columns of one packed projection."""
+    d = _lib.PagedAppendDesc()
+    d.tokens, d.q_heads, d.rotary_dim, d.max_pos, d.interleaved = tokens, q_heads, rotary_dim, max_pos, 1 if interleaved else 0
+    d.q_head_stride = d.k_head_stride = d.v_head_stride = d.out_head_stride = cache.head_dim
+    d.q_row_stride = q_heads * cache.head_dim if row_stride is None else row_stride
+    d.k_row_stride = d.v_row_stride = cache.kv_heads * cache.head_dim if row_stride is None else row_stride
+    d.out_row_stride = q_heads * cache.head_dim
+    return d
+
+
+def paged_append(cache, desc, q, k, v, cosines, sines, block_table, seq_ids, positions, q_out, k_cache, v_cache, bad_index=None, stream=None):
+    """K (rotated) and V of desc.tokens tokens into the paged cache, rotated queries into q_out (q and q_out None: no queries)."""
+    check(_lib.load().fth_dev_paged_append_f32(C.byref(cache), C.byref(desc), _ptr(q), _ptr(k), _ptr(v), _ptr(cosines), _ptr(sines), _ptr(block_table),
+                                               _ptr(seq_ids), _ptr(positions), _ptr(q_out), _ptr(k_cache), _ptr(v_cache), _ptr(bad_index), stream))
+
+
+def rotary_tables(max_pos, rotary_dim, base=10000.0):
+    """cosines, sines [max_pos, rotary_dim / 2] of position * base^(-2 i / rotary_dim), computed in double precision (host arrays)."""
+    angle = np.arange(max_pos)[:, None] * float(base) ** (-np.arange(0, rotary_dim, 2) / rotary_dim)
+    return np.cos(angle).astype(np.float32), np.sin(angle).astype(np.float32)
+
+
+def paged_sdpa_desc(cache, q_heads, new_tokens=1, max_len=None) -> _lib.PagedSdpaDesc:
+    """Contiguous q and out [num_seqs, new_tokens, q_heads, head_dim]; max_len: no sequence is longer (default: what the table holds)."""
+    d = _lib.PagedSdpaDesc()
+    d.q_heads, d.new_tokens = q_heads, new_tokens
+    d.max_len = cache.max_pages * cache.page_size if max_len is None else max_len
+    d.q_head_stride = d.o_head_stride = cache.head_dim
+    d.q_row_stride = d.o_row_stride = q_heads * cache.head_dim
+    d.q_seq_stride = d.o_seq_stride = new_tokens * q_heads * cache.head_dim
+    return d
+
+
+def paged_sdpa_workspace(cache, desc) -> DeviceBuffer:
+    """A workspace for paged_sdpa calls with these descriptors."""
+    return _workspace(_lib.load().fth_dev_paged_sdpa_workspace_bytes(C.byref(cache), C.byref(desc)), None)
+
+
+def paged_sdpa(cache, desc, scale, q, k_cache, v_cache, block_table, lens, out, bad_index=None, workspace=None, stream=None):
+    """Attention of the last desc.new_tokens tokens of every sequence over the paged cache; returns the workspace for the next call."""
+    workspace = paged_sdpa_workspace(cache, desc) if workspace is None else workspace
+    check(_lib.load().fth_dev_paged_sdpa_f32(C.byref(cache), C.byref(desc), scale, _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_table), _ptr(lens),
+                                             _ptr(out), _ptr(bad_index), workspace.ptr, workspace.nbytes, stream))
+    return workspace
+
+
+def logits_desc(rows, vocab, history_stride=0, shared_bias=False) -> _lib.LogitsDesc:
+    """Contiguous logits, out and bias [rows, vocab] (shared_bias: bias [vocab]), history [rows, history_stride], mask [rows, words of 32 bits]."""
+    d = _lib.LogitsDesc()
+    d.rows, d.vocab, d.logits_stride, d.out_stride, d.history_stride = rows, vocab, vocab, vocab, history_stride
+    d.bias_stride, d.mask_stride = 0 if shared_bias else vocab, (vocab + 31) // 32
+    return d
+
+
+def logits_process(desc, logits, history, history_len, prompt_len, repetition, frequency, presence, bias, mask, out, bad_index=None, stream=None):
+    """Penalties for repeated tokens, a bias and a mask of allowed tokens on the logits of a step; each of them may be None."""
+    check(_lib.load().fth_dev_logits_process_f32(C.byref(desc), _ptr(logits), _ptr(history), _ptr(history_len), _ptr(prompt_len), _ptr(repetition),
+                                                 _ptr(frequency), _ptr(presence), _ptr(bias), _ptr(mask), _ptr(out), _ptr(bad_index), stream))
+
+
 def default_scale(head_dim: int) -> float:
     return 1.0 / math.sqrt(head_dim)

@@ -432,6 +432,81 @@ int32_t fth_dev_sdpa_forward_masked_f32(const fth_sdpa_desc *d, float scale, con
 int32_t fth_dev_sdpa_forward_masked_f64(const fth_sdpa_desc *d, double scale, const double *q, const double *k, const double *v,
                                         const double *mask, int64_t mask_bh_stride, double *out, fth_stream s);
 
+/* ---- token-by-token generation: a paged K/V cache, attention over it, and the logits of a step ----
+ * The cache is two arrays of pages, k and v, laid out alike: element c of the K (V) row of K/V head h at position p of
+ * sequence s is cache[block_table[s * table_stride + p / page_size] * page_stride + h * head_stride
+ * + (p % page_size) * row_stride + c]. Any page may belong to several sequences (a shared prompt), in any order. Entries of a
+ * sequence's row of the table past its last page are not read. dtype is the storage type (FTH_DTYPE_F32, F16 or BF16; stores
+ * round to nearest even, and what is over the largest F16 becomes infinite); queries, new keys and values, and outputs are
+ * fp32, and so is all arithmetic. The reference has no cache: its decoder recomputes every position. */
+typedef struct fth_paged_cache {
+    int64_t num_pages, page_size, kv_heads, head_dim; /* head_dim <= 256 */
+    int64_t page_stride, head_stride, row_stride;     /* elements, each >= head_dim */
+    int64_t num_seqs, max_pages, table_stride;        /* rows, usable columns and row pitch of block_table (int32) */
+    int32_t dtype;
+    int32_t reserved; /* 0 */
+} fth_paged_cache;
+/* Fills the strides for contiguous [num_pages, kv_heads, page_size, head_dim] arrays and a [num_seqs, max_pages] table. */
+void fth_dev_paged_cache_contiguous(fth_paged_cache *c, int64_t num_pages, int64_t page_size, int64_t kv_heads, int64_t head_dim,
+                                int64_t num_seqs, int64_t max_pages, int32_t dtype);
+/* Appends k and v of `tokens` tokens: token t goes to position positions[t] of sequence seq_ids[t]. Element (t, h, c) of an
+ * operand is x[t * x_row_stride + h * x_head_stride + c], so a packed QKV projection is read in place. With rotary_dim > 0
+ * the first rotary_dim elements of every K row are rotated on the way, in pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1)
+ * when `interleaved`: (a, b) -> (a c - b s, b c + a s), c = cosines[position * rotary_dim / 2 + i], s = sines[the same]
+ * (fp32 [max_pos, rotary_dim / 2] tables, not read when rotary_dim == 0). With q_heads > 0 the queries are rotated likewise
+ * into q_out (fp32; q_out == q with the same strides is allowed; otherwise no operand may overlap another).
+ * A token at position -1 is skipped: nothing of it is read or written (the padding of a captured graph). A token whose
+ * sequence, position, page or row of the tables does not exist is left out the same way and reported: bad_index (device, may
+ * be NULL) receives the lowest such t, or -1. Two tokens at one place leave either of them there. */
+typedef struct fth_paged_append_desc {
+    int64_t tokens, q_heads;
+    int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride, out_row_stride, out_head_stride;
+    int64_t rotary_dim, max_pos; /* rotary_dim even, <= head_dim */
+    int32_t interleaved;
+    int32_t reserved; /* 0 */
+} fth_paged_append_desc;
+int32_t fth_dev_paged_append_f32(const fth_paged_cache *c, const fth_paged_append_desc *d, const float *q, const float *k, const float *v,
+                                 const float *cosines, const float *sines, const int32_t *block_table, const int32_t *seq_ids,
+                                 const int32_t *positions, float *q_out, void *k_cache, void *v_cache, int64_t *bad_index, fth_stream s);
+/* Attention of the last new_tokens tokens of every sequence (1 to 8; their K and V are in the cache) over the cache:
+ * lens[s] positions are filled, and query i of sequence s sees positions 0 .. lens[s] - new_tokens + i:
+ * out = softmax(scale * q . k) v. Element (s, i, h, c) of q is q[s * q_seq_stride + i * q_row_stride + h * q_head_stride + c];
+ * likewise out (o_*). Query head h reads K/V head h / (q_heads / kv_heads). A query that sees nothing (lens[s] too small, 0 for
+ * an unused slot of a batch) gives zeros. What the cache holds past a sequence's length is never used, NaN included.
+ * max_len is a bound on lens that the host knows (it sizes the launch; a captured graph serves every length up to it). A
+ * sequence with lens[s] outside [0, min(max_len, max_pages * page_size)] or with a page that does not exist has NaN in all its
+ * outputs, and bad_index (device, may be NULL) receives the lowest such s, or -1.
+ * The workspace (device memory, contents ignored and overwritten) holds the partial results of shares of the keys, which are
+ * joined in a fixed order. */
+typedef struct fth_paged_sdpa_desc {
+    int64_t q_heads, new_tokens, max_len;
+    int64_t q_seq_stride, q_row_stride, q_head_stride, o_seq_stride, o_row_stride, o_head_stride;
+} fth_paged_sdpa_desc;
+/* Bytes that the call needs, or 0 for arguments it would refuse (or when it needs none). */
+size_t fth_dev_paged_sdpa_workspace_bytes(const fth_paged_cache *c, const fth_paged_sdpa_desc *d);
+int32_t fth_dev_paged_sdpa_f32(const fth_paged_cache *c, const fth_paged_sdpa_desc *d, float scale, const float *q, const void *k_cache,
+                               const void *v_cache, const int32_t *block_table, const int32_t *lens, float *out, int64_t *bad_index,
+                               void *workspace, size_t workspace_bytes, fth_stream s);
+/* The logits of a step made ready for the choice of a token. Row r has the tokens so far in history[r * history_stride ...],
+ * history_len[r] of them, the first prompt_len[r] given and the others generated. For every v < vocab, in this order:
+ *   seen anywhere in the history:                   x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *   n times among the generated ones, n > 0:        x = x - frequency[r] * n;  x = x - presence[r]
+ *   x = x + bias[r * bias_stride + v]               (bias_stride 0: one bias for all rows)
+ *   bit v % 32 of mask[r * mask_stride + v / 32] is 0:  x = -inf, whatever it was
+ * each step rounded to fp32. repetition, frequency, presence, bias and mask may each be NULL (that step is left out), and so
+ * may history (then all of repetition, frequency and presence are left out). A mask row of zeros leaves -inf everywhere.
+ * out == logits with the same stride is allowed. A row whose lengths are out of range (0 <= prompt_len <= history_len <=
+ * history_stride) or whose history has a token outside [0, vocab) is not written; bad_index (device, may be NULL) receives the
+ * lowest such row, or -1. Counts are integers and every row's result is independent of the others: runs repeat bit for bit. */
+typedef struct fth_logits_desc {
+    int64_t rows, vocab;
+    int64_t logits_stride, out_stride;                  /* elements, >= vocab */
+    int64_t history_stride, bias_stride, mask_stride;   /* elements; bias_stride 0 or >= vocab; mask_stride in 32-bit words */
+} fth_logits_desc;
+int32_t fth_dev_logits_process_f32(const fth_logits_desc *d, const float *logits, const int32_t *history, const int32_t *history_len,
+                                   const int32_t *prompt_len, const float *repetition, const float *frequency, const float *presence,
+                                   const float *bias, const uint32_t *mask, float *out, int64_t *bad_index, fth_stream s);
+
 /* ------------------------------------------------------------------------------------------ */
 /* Tier A: host slices in, host buffer out (the ft_kernel_cpu surface)                        */
 /* ------------------------------------------------------------------------------------------ */

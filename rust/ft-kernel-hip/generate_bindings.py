@@ -27,7 +27,7 @@ HEADER = os.path.join(ROOT, "include", "ft_kernel_hip.h")
 # ------------------------------------------------------------------------------------------------
 # header -> ffi.rs
 # ------------------------------------------------------------------------------------------------
-SCALAR = {"int8_t": "i8", "int32_t": "i32", "int64_t": "i64", "uint64_t": "u64", "size_t": "usize", "float": "f32",
+SCALAR = {"int8_t": "i8", "int32_t": "i32", "int64_t": "i64", "uint32_t": "u32", "uint64_t": "u64", "size_t": "usize", "float": "f32",
           "double": "f64", "void": "c_void", "char": "c_char", "fth_stream": "fth_stream", "fth_event": "fth_event"}
 RUST_KEYWORDS = {"in", "type", "fn", "ref", "match", "mod", "move", "use", "where", "impl", "loop", "box", "as"}
 

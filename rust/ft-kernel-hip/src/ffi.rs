@@ -122,6 +122,68 @@ pub struct fth_sdpa_desc {
 
 #[repr(C)]
 #[derive(Debug, Clone, Copy)]
+pub struct fth_paged_cache {
+    pub num_pages: i64,
+    pub page_size: i64,
+    pub kv_heads: i64,
+    pub head_dim: i64,
+    pub page_stride: i64,
+    pub head_stride: i64,
+    pub row_stride: i64,
+    pub num_seqs: i64,
+    pub max_pages: i64,
+    pub table_stride: i64,
+    pub dtype: i32,
+    pub reserved: i32,
+}
+
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct fth_paged_append_desc {
+    pub tokens: i64,
+    pub q_heads: i64,
+    pub q_row_stride: i64,
+    pub q_head_stride: i64,
+    pub k_row_stride: i64,
+    pub k_head_stride: i64,
+    pub v_row_stride: i64,
+    pub v_head_stride: i64,
+    pub out_row_stride: i64,
+    pub out_head_stride: i64,
+    pub rotary_dim: i64,
+    pub max_pos: i64,
+    pub interleaved: i32,
+    pub reserved: i32,
+}
+
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct fth_paged_sdpa_desc {
+    pub q_heads: i64,
+    pub new_tokens: i64,
+    pub max_len: i64,
+    pub q_seq_stride: i64,
+    pub q_row_stride: i64,
+    pub q_head_stride: i64,
+    pub o_seq_stride: i64,
+    pub o_row_stride: i64,
+    pub o_head_stride: i64,
+}
+
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct fth_logits_desc {
+    pub rows: i64,
+    pub vocab: i64,
+    pub logits_stride: i64,
+    pub out_stride: i64,
+    pub history_stride: i64,
+    pub bias_stride: i64,
+    pub mask_stride: i64,
+}
+
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
 pub struct fth_layer_weights {
     pub ln1_w: *const f32,
     pub ln1_b: *const f32,
@@ -278,6 +340,11 @@ extern "C" {
     pub fn fth_dev_sdpa_forward_f64(d: *const fth_sdpa_desc, scale: f64, q: *const f64, k: *const f64, v: *const f64, out: *mut f64, s: fth_stream) -> i32;
     pub fn fth_dev_sdpa_forward_masked_f32(d: *const fth_sdpa_desc, scale: f32, q: *const f32, k: *const f32, v: *const f32, mask: *const f32, mask_bh_stride: i64, out: *mut f32, s: fth_stream) -> i32;
     pub fn fth_dev_sdpa_forward_masked_f64(d: *const fth_sdpa_desc, scale: f64, q: *const f64, k: *const f64, v: *const f64, mask: *const f64, mask_bh_stride: i64, out: *mut f64, s: fth_stream) -> i32;
+    pub fn fth_dev_paged_cache_contiguous(c: *mut fth_paged_cache, num_pages: i64, page_size: i64, kv_heads: i64, head_dim: i64, num_seqs: i64, max_pages: i64, dtype: i32);
+    pub fn fth_dev_paged_append_f32(c: *const fth_paged_cache, d: *const fth_paged_append_desc, q: *const f32, k: *const f32, v: *const f32, cosines: *const f32, sines: *const f32, block_table: *const i32, seq_ids: *const i32, positions: *const i32, q_out: *mut f32, k_cache: *mut c_void, v_cache: *mut c_void, bad_index: *mut i64, s: fth_stream) -> i32;
+    pub fn fth_dev_paged_sdpa_workspace_bytes(c: *const fth_paged_cache, d: *const fth_paged_sdpa_desc) -> usize;
+    pub fn fth_dev_paged_sdpa_f32(c: *const fth_paged_cache, d: *const fth_paged_sdpa_desc, scale: f32, q: *const f32, k_cache: *const c_void, v_cache: *const c_void, block_table: *const i32, lens: *const i32, out: *mut f32, bad_index: *mut i64, workspace: *mut c_void, workspace_bytes: usize, s: fth_stream) -> i32;
+    pub fn fth_dev_logits_process_f32(d: *const fth_logits_desc, logits: *const f32, history: *const i32, history_len: *const i32, prompt_len: *const i32, repetition: *const f32, frequency: *const f32, presence: *const f32, bias: *const f32, mask: *const u32, out: *mut f32, bad_index: *mut i64, s: fth_stream) -> i32;
     pub fn fth_matmul_tensor_contiguous_f32(lhs: *const f32, lhs_len: usize, rhs: *const f32, rhs_len: usize, lhs_meta: *const fth_meta, rhs_meta: *const fth_meta, out: *mut f32, out_cap: usize, out_len: *mut usize) -> i32;
     pub fn fth_matmul_tensor_contiguous_f64(lhs: *const f64, lhs_len: usize, rhs: *const f64, rhs_len: usize, lhs_meta: *const fth_meta, rhs_meta: *const fth_meta, out: *mut f64, out_cap: usize, out_len: *mut usize) -> i32;
     pub fn fth_bmm_tensor_contiguous_f32(lhs: *const f32, lhs_len: usize, rhs: *const f32, rhs_len: usize, lhs_meta: *const fth_meta, rhs_meta: *const fth_meta, out: *mut f32, out_cap: usize, out_len: *mut usize) -> i32;
