@@ -2,14 +2,29 @@
 //
 //   out[s, i, h] = sum_j w_j v_j / sum_j w_j,   w_j = exp(x_j - max x),   x_j = scale q . k_j,   j < lens[s] - new_tokens + i + 1
 //
-// One wavefront a query row: 64 keys at a time, a key per lane for the scores, columns over the lanes for the outputs, a
-// running maximum and sum (fp32) in between. Bound by reading the cache; every query head of a group reads its K/V head again.
+// Bound by reading the cache once. The keys of a sequence are cut into shares of equal length; a workgroup takes one share of
+// one K/V head for up to 16 of the query rows that read it (query heads of the group x new tokens), so K and V are read once for
+// all of them. Its four wavefronts walk the share in tiles of 32 keys, each on its own (running maximum and sum per row in fp32,
+// no barrier), and are joined through LDS at the end; a second small kernel joins the shares of a row in order.
+//   * S^T[key, row] = K . Q^T on v_mfma_f32_16x16x4_f32: lane (lr, g) brings a quarter of K row lr and of query row lr; 16-bit
+//     values become floats on the way, so scores and outputs are fp32 sums of exact products' roundings, whatever the storage.
+//   * It then holds the scores of keys 16 s + 4 g + r of row lr, which is the B operand of O^T[d, row] += V^T . P^T: P never
+//     moves, and V rows are read whole (16 lanes side by side).
+//   * The loads of the next tile's K go out when the scores have consumed this one's, those of V after the outputs have.
+// Pages: with a page size that is a multiple of 16 each half tile lies in one page, whose number is a scalar load one tile
+// ahead. Other page sizes, head sizes and alignments that the 128-bit loads cannot take go to a kernel of one wavefront a row.
+
+#include <type_traits>
 
 #include "paged.hpp"
 
 namespace {
 
+using F4 = float __attribute__((ext_vector_type(4)));
+using U4 = uint32_t __attribute__((ext_vector_type(4)));
+
 constexpr float kLog2e = 1.44269502162933349609375f;
+constexpr int kTile = 32, kWaves = 4;
 
 struct PagedArgs {
     fth_paged_cache c;
@@ -19,36 +34,73 @@ struct PagedArgs {
     const int32_t *table, *lens;
     float *out;
     int64_t *bad;
-    float scale;
+    float *part_o;   // [row][split][pitch] unnormalised outputs of the shares (rows with more than one)
+    float *part_ml;  // [row][split][2] their maxima (of scores times log2 e) and sums
+    float scale2;    // scale * log2(e)
+    int64_t most;    // the longest valid sequence
+    int group, row_tiles, nsplit, share, pitch;
+    uint32_t page_mul, page_shift;  // n / page_size, see Plan
 };
 
+// n / d for 0 <= n < 2^31 by a multiplication: shift = ceil(log2 d), mul = ceil(2^(32 + shift) / d) - 2^32.
+struct Divisor {
+    uint32_t mul, shift;
+    explicit Divisor(uint32_t d) : shift(0) {
+        while (((uint64_t)1 << shift) < d) ++shift;
+        mul = (uint32_t)(((((uint64_t)1 << shift) - d) << 32) / d + 1);
+    }
+};
+__device__ __forceinline__ uint32_t divide(uint32_t n, uint32_t mul, uint32_t shift) { return (uint32_t)(((uint64_t)__umulhi(n, mul) + n) >> shift); }
+
+struct MaxOp { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct AddOp { __device__ float operator()(float a, float b) const { return a + b; } };
 template <typename F> __device__ __forceinline__ float wave_reduce(float x, F op) {
 #pragma unroll
     for (int m = 32; m > 0; m >>= 1) x = op(x, __shfl_xor(x, m));
     return x;
 }
+// over the four 16-lane rows of a wavefront, the result in every lane
+template <typename F> __device__ __forceinline__ float rows_reduce(float x, F op) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// Where a row (sequence, new token, query head) of the output lies, and its number.
+__device__ __forceinline__ float *out_row(const PagedArgs &p, int64_t seq, int i, int h) {
+    return p.out + seq * p.d.o_seq_stride + i * p.d.o_row_stride + h * p.d.o_head_stride;
+}
+__device__ __forceinline__ int64_t row_number(const PagedArgs &p, int64_t seq, int i, int h) { return (seq * p.d.new_tokens + i) * p.d.q_heads + h; }
+
+// ---- one wavefront a row and share: any page size, head size, stride and alignment ----------------------------------------
 
 template <typename T> __global__ __launch_bounds__(64) void paged_sdpa_rows_kernel(const PagedArgs p) {
     __shared__ float qs[256], ps[64];
     __shared__ int64_t at[64];
     const int lane = threadIdx.x, hd = (int)p.c.head_dim, page_size = (int)p.c.page_size;
-    const int64_t row = blockIdx.x;  // (sequence * new_tokens + i) * q_heads + h
+    const int split = (int)(blockIdx.x % (unsigned)p.nsplit);
+    const int64_t row = blockIdx.x / (unsigned)p.nsplit;
     const int h = (int)(row % p.d.q_heads), i = (int)(row / p.d.q_heads % p.d.new_tokens);
     const int64_t seq = row / p.d.q_heads / p.d.new_tokens;
-    const int64_t hk = h / (p.d.q_heads / p.c.kv_heads);
+    const int64_t hk = h / p.group;
     const T *K = static_cast<const T *>(p.k) + hk * p.c.head_stride, *V = static_cast<const T *>(p.v) + hk * p.c.head_stride;
-    const int64_t most = p.c.max_pages * p.c.page_size < p.d.max_len ? p.c.max_pages * p.c.page_size : p.d.max_len;
-    const int len = p.lens[seq];
-    bool bad = len < 0 || len > most;
-    const int sees = bad ? 0 : len - (int)p.d.new_tokens + i + 1;
+    int len = p.lens[seq];
+    bool bad = len < 0 || len > p.most;
+    if (bad) len = 0;
+    const int key_lo = split * p.share;
+    if (split > 0 && key_lo >= len) return;
+    const bool alone = len <= p.share;  // no other share of this row
+    const int end = len - key_lo < p.share ? len : key_lo + p.share;
+    const int sees = len - (int)p.d.new_tokens + i + 1, key_hi = sees < end ? sees : end;  // pages are looked at up to `end`, so that all rows of a sequence find a bad one
     const float *q = p.q + seq * p.d.q_seq_stride + i * p.d.q_row_stride + h * p.d.q_head_stride;
     for (int c = lane; c < hd; c += 64) qs[c] = q[c];
     __syncthreads();
     float o[4] = {0.f, 0.f, 0.f, 0.f}, m = -__builtin_inff(), l = 0.f;
-    for (int key0 = 0; key0 < sees; key0 += 64) {
-        const int key = key0 + lane, n = sees - key0 < 64 ? sees - key0 : 64;
+    for (int key0 = key_lo; key0 < end; key0 += 64) {
+        const int key = key0 + lane, n = key_hi - key0 < 64 ? key_hi - key0 : 64;
         float x = -__builtin_inff();
-        if (lane < n) {
+        if (key < end) {
             int page = p.table[seq * p.c.table_stride + key / page_size];
             if (page < 0 || page >= p.c.num_pages) {
                 bad = true;
@@ -56,17 +108,17 @@ template <typename T> __global__ __launch_bounds__(64) void paged_sdpa_rows_kern
             }
             const int64_t off = page < 0 ? -1 : (int64_t)page * p.c.page_stride + (int64_t)(key % page_size) * p.c.row_stride;
             at[lane] = off;
-            if (page >= 0) {
+            if (page >= 0 && lane < n) {
                 float dot = 0.f;
                 for (int c = 0; c < hd; ++c) dot = __builtin_fmaf(qs[c], fth::to_f32(K[off + c]), dot);
-                x = dot * p.scale;
+                x = dot * p.scale2;
             }
         }
-        const float m_new = fmaxf(m, wave_reduce(x, [](float a, float b) { return fmaxf(a, b); }));
+        const float m_new = fmaxf(m, wave_reduce(x, MaxOp()));
         const float ref = m_new == -__builtin_inff() ? 0.f : m_new;
-        const float alpha = __builtin_amdgcn_exp2f((m - ref) * kLog2e), w = lane < n ? __builtin_amdgcn_exp2f((x - ref) * kLog2e) : 0.f;
+        const float alpha = __builtin_amdgcn_exp2f(m - ref), w = lane < n ? __builtin_amdgcn_exp2f(x - ref) : 0.f;
         m = m_new;
-        l = l * alpha + wave_reduce(w, [](float a, float b) { return a + b; });
+        l = l * alpha + wave_reduce(w, AddOp());
         ps[lane] = w;
         __syncthreads();
         for (int j = 0; j < 4; ++j) {
@@ -81,30 +133,368 @@ template <typename T> __global__ __launch_bounds__(64) void paged_sdpa_rows_kern
     }
     bad = __any(bad);
     if (bad && lane == 0) fth::report_bad_entry(p.bad, seq);
-    float *out = p.out + seq * p.d.o_seq_stride + i * p.d.o_row_stride + h * p.d.o_head_stride;
+    if (bad) l = __builtin_nanf("");
+    float *dst = out_row(p, seq, i, h);
+    if (!alone) {
+        const int64_t slot = row * p.nsplit + split;
+        dst = p.part_o + slot * p.pitch;
+        if (lane == 0) {
+            p.part_ml[2 * slot] = m;
+            p.part_ml[2 * slot + 1] = l;
+        }
+    }
     for (int j = 0; j < 4; ++j) {
         const int c = lane + 64 * j;
-        if (c < hd) out[c] = bad ? __builtin_nanf("") : sees <= 0 ? 0.f : o[j] / l;
+        if (c < hd) dst[c] = !alone ? o[j] : sees <= 0 && !bad ? 0.f : o[j] / l;
     }
 }
 
-template <typename T> int32_t launch(const PagedArgs &a, hipStream_t st) {
-    paged_sdpa_rows_kernel<T><<<dim3((unsigned)(a.c.num_seqs * a.d.new_tokens * a.d.q_heads)), dim3(64), 0, st>>>(a);
-    FTH_CHECK_LAUNCH("paged_sdpa");
-    return FTH_OK;
+// ---- tiles of 32 keys on the matrix units ---------------------------------------------------------------------------------
+
+// Element e of 16 bytes of storage, as a float.
+template <typename T> struct Chunk {  // f16, bf16
+    static constexpr int kElems = 8;
+    static __device__ __forceinline__ float get(const U4 &v, int e) {
+        const uint32_t w = v[e >> 1];
+        if constexpr (std::is_same<T, fth::bf16>::value) {
+            return __uint_as_float((e & 1) ? w & 0xffff0000u : w << 16);
+        } else {
+            return (float)__builtin_bit_cast(fth::f16, (uint16_t)((e & 1) ? w >> 16 : w));
+        }
+    }
+};
+template <> struct Chunk<float> {
+    static constexpr int kElems = 4;
+    static __device__ __forceinline__ float get(const U4 &v, int e) { return __uint_as_float(v[e]); }
+};
+
+template <typename T, int DP> struct TileShape {
+    static constexpr int CH = Chunk<T>::kElems;     // elements of a 128-bit load
+    static constexpr int NK = DP / 4 / CH;          // loads of a lane's quarter of a K row
+    static constexpr int NE = DP / 16;              // output columns of a lane
+    static constexpr int CV = NE < CH ? NE : CH;    // consecutive ones
+    static constexpr int NV = NE / CV;              // loads of its part of a V row
+    static constexpr int kLds = kWaves * 16 * (DP + 4);
+};
+
+// FULL: head_dim == DP; otherwise what lies past head_dim counts as zero.
+template <typename T, int DP, bool FULL> __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void paged_sdpa_tiles_kernel(const PagedArgs p) {
+    using S = TileShape<T, DP>;
+    constexpr int CH = S::CH, NK = S::NK, NE = S::NE, CV = S::CV, NV = S::NV;
+    __shared__ __attribute__((aligned(16))) float lds_o[S::kLds];
+    __shared__ float lds_ml[kWaves * 16 * 2];
+    const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int units = (int)(p.c.num_seqs * p.c.kv_heads) * p.row_tiles;
+    const int split = (int)(blockIdx.x / (unsigned)units), unit = (int)(blockIdx.x % (unsigned)units);
+    const int rt = unit % p.row_tiles, hk = unit / p.row_tiles % (int)p.c.kv_heads;
+    const int64_t seq = unit / p.row_tiles / (int)p.c.kv_heads;
+    const int hd = (int)p.c.head_dim, new_tokens = (int)p.d.new_tokens, rows = p.group * new_tokens;
+    int len = p.lens[seq];
+    bool bad = len < 0 || len > p.most;
+    if (bad) len = 0;
+    const int key_lo = split * p.share;
+    if (split > 0 && key_lo >= len) return;
+    const bool alone = len <= p.share;
+    const int key_hi = len - key_lo < p.share ? len : key_lo + p.share;
+    const int tiles = (key_hi - key_lo + kTile - 1) / kTile, last16 = (key_hi - 1) >> 4;
+    const T *K = static_cast<const T *>(p.k) + hk * p.c.head_stride, *V = static_cast<const T *>(p.v) + hk * p.c.head_stride;
+    const int32_t *table = p.table + seq * p.c.table_stride;
+    const int rs = (int)p.c.row_stride;
+
+    // this lane's query row (rows past the last repeat it and are never stored) and how many keys it sees
+    int rr = rt * 16 + lr;
+    rr = rr < rows ? rr : rows - 1;
+    const int qi = rr % new_tokens, qh = hk * p.group + rr / new_tokens;
+    const int sees = len - new_tokens + 1 + qi;
+    float q[NK][CH];
+    {
+        const float *qr = p.q + seq * p.d.q_seq_stride + qi * p.d.q_row_stride + qh * p.d.q_head_stride;
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+#pragma unroll
+            for (int e = 0; e < CH; ++e) {
+                const int c = (4 * i + g) * CH + e;
+                q[i][e] = FULL || c < hd ? qr[c] : 0.f;
+            }
+    }
+
+    // page and first row of the 16 keys number t16 (of the sequence)
+    auto page_of = [&](int t16) __attribute__((always_inline)) {
+        t16 = t16 < last16 ? t16 : last16;  // half tiles past the end repeat the last one
+        const int index = (int)divide((uint32_t)t16 << 4, p.page_mul, p.page_shift);
+        return make_int2(table[index], (t16 << 4) - index * (int)p.c.page_size);
+    };
+    auto offset_of = [&](int2 page) __attribute__((always_inline)) {
+        if (page.x < 0 || page.x >= p.c.num_pages) {
+            bad = true;
+            page.x = 0;
+        }
+        return (int64_t)page.x * p.c.page_stride + (int64_t)page.y * rs;
+    };
+    U4 kf[2][NK], vf[2][4][NV];
+    auto load_k = [&](const int64_t (&off)[2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < NK; ++i) {
+                const int c = (4 * i + g) * CH;
+                kf[s][i] = U4{0u, 0u, 0u, 0u};
+                if (FULL || c < hd) kf[s][i] = *reinterpret_cast<const U4 *>(K + off[s] + (uint32_t)(lr * rs + c));
+            }
+    };
+    auto load_v = [&](const int64_t (&off)[2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const int c = (16 * i + lr) * CV;
+                    const T *src = V + off[s] + (uint32_t)((4 * g + r) * rs + c);
+                    vf[s][r][i] = U4{0u, 0u, 0u, 0u};
+                    if (FULL || c < hd) {
+                        if constexpr (CV * sizeof(T) == 16) {
+                            vf[s][r][i] = *reinterpret_cast<const U4 *>(src);
+                        } else {
+                            const uint2 w = *reinterpret_cast<const uint2 *>(src);
+                            vf[s][r][i][0] = w.x;
+                            vf[s][r][i][1] = w.y;
+                        }
+                    }
+                }
+    };
+
+    F4 o[NE];
+#pragma unroll
+    for (int e = 0; e < NE; ++e) o[e] = F4{0.f, 0.f, 0.f, 0.f};
+    float m_run = -__builtin_inff(), l_run = 0.f;  // the sum: this lane's keys only
+
+    const int t16_lo = key_lo >> 4;
+    int64_t off[2], off_next[2];
+    int2 ahead[2];
+    if (wave < tiles) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            off[s] = offset_of(page_of(t16_lo + 2 * wave + s));
+            ahead[s] = page_of(t16_lo + 2 * (wave + kWaves) + s);
+        }
+        load_k(off);
+        load_v(off);
+    }
+    for (int t = wave; t < tiles; t += kWaves) {
+        const int key0 = key_lo + t * kTile;
+        const bool more = t + kWaves < tiles;
+        F4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+#pragma unroll
+            for (int e = 0; e < CH; ++e)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) sc[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(Chunk<T>::get(kf[s][i], e), q[i][e], sc[s], 0, 0, 0);
+        if (more) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                off_next[s] = offset_of(ahead[s]);
+                ahead[s] = page_of(t16_lo + 2 * (t + 2 * kWaves) + s);
+            }
+            load_k(off_next);
+        }
+        float mx = -__builtin_inff();
+        const bool edge = key0 + kTile > len - new_tokens + 1 || key0 + kTile > key_hi;
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float x = sc[s][r] * p.scale2;
+                if (edge) {
+                    const int key = key0 + 16 * s + 4 * g + r;
+                    x = key >= sees || key >= key_hi ? -__builtin_inff() : x;
+                }
+                sc[s][r] = x;
+                mx = fmaxf(mx, x);
+            }
+        mx = rows_reduce(mx, MaxOp());
+        if (__any(mx > m_run)) {
+            const float m_new = fmaxf(m_run, mx);
+            const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -__builtin_inff() ? 0.f : m_new));
+            m_run = m_new;
+            l_run *= alpha;
+#pragma unroll
+            for (int e = 0; e < NE; ++e)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[e][r] *= alpha;
+        }
+        const float ref = m_run == -__builtin_inff() ? 0.f : m_run;  // nothing visible so far: every weight is exp(-inf) = 0
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                sc[s][r] = __builtin_amdgcn_exp2f(sc[s][r] - ref);
+                l_run += sc[s][r];
+            }
+        if (key0 + kTile > key_hi) {  // weight 0 times what an unused row holds would be NaN
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (key0 + 16 * s + 4 * g + r >= key_hi)
+#pragma unroll
+                        for (int i = 0; i < NV; ++i) vf[s][r][i] = U4{0u, 0u, 0u, 0u};
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int e = 0; e < NE; ++e)
+                    o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(Chunk<T>::get(vf[s][r][e / CV], e % CV), sc[s][r], o[e], 0, 0, 0);
+        if (more) load_v(off_next);
+    }
+
+    // join the wavefronts: MFMA row 4 g + r of column tile e is output column ((e / CV) * 16 + 4 g + r) * CV + e % CV
+    constexpr int P = DP + 4;
+    const float l_wave = rows_reduce(l_run, AddOp());
+    if (g == 0) {
+        lds_ml[(wave * 16 + lr) * 2] = m_run;
+        lds_ml[(wave * 16 + lr) * 2 + 1] = bad ? __builtin_nanf("") : l_wave;
+    }
+#pragma unroll
+    for (int e = 0; e < NE; ++e)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) lds_o[(wave * 16 + lr) * P + ((e / CV) * 16 + 4 * g + r) * CV + e % CV] = o[e][r];
+    if (bad && lane == 0) fth::report_bad_entry(p.bad, seq);
+    __syncthreads();
+    const int stored = rows - rt * 16 < 16 ? rows - rt * 16 : 16;
+    for (int x = threadIdx.x; x < stored * (DP / 4); x += 64 * kWaves) {
+        const int row = x / (DP / 4), c = x % (DP / 4) * 4;
+        if (c >= hd) continue;
+        float m = -__builtin_inff(), l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) m = fmaxf(m, lds_ml[(w * 16 + row) * 2]);
+        const float ref = m == -__builtin_inff() ? 0.f : m;
+        F4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float weight = __builtin_amdgcn_exp2f(lds_ml[(w * 16 + row) * 2] - ref);
+            l += lds_ml[(w * 16 + row) * 2 + 1] * weight;
+            const F4 part = *reinterpret_cast<const F4 *>(&lds_o[(w * 16 + row) * P + c]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] += part[j] * weight;
+        }
+        const int ri = (rt * 16 + row) % new_tokens, rh = hk * p.group + (rt * 16 + row) / new_tokens;
+        if (alone) {
+            float *dst = out_row(p, seq, ri, rh);
+            const bool nothing = !(l != l) && len - new_tokens + 1 + ri <= 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) dst[c + j] = nothing ? 0.f : acc[j] / l;
+        } else {
+            const int64_t slot = row_number(p, seq, ri, rh) * p.nsplit + split;
+            *reinterpret_cast<F4 *>(p.part_o + slot * p.pitch + c) = acc;
+            if (c == 0) {
+                p.part_ml[2 * slot] = m;
+                p.part_ml[2 * slot + 1] = l;
+            }
+        }
+    }
 }
+
+// ---- shares joined in their order -----------------------------------------------------------------------------------------
+
+__global__ __launch_bounds__(64) void paged_sdpa_join_kernel(const PagedArgs p) {
+    const int64_t row = blockIdx.x;
+    const int h = (int)(row % p.d.q_heads), i = (int)(row / p.d.q_heads % p.d.new_tokens);
+    const int64_t seq = row / p.d.q_heads / p.d.new_tokens;
+    const int len = p.lens[seq];
+    if (len <= p.share || len > p.most) return;  // written by its only share
+    const int shares = (len - 1) / p.share + 1;
+    const int64_t slot0 = row * p.nsplit;
+    float m = -__builtin_inff();
+    for (int s = 0; s < shares; ++s) m = fmaxf(m, p.part_ml[2 * (slot0 + s)]);
+    const float ref = m == -__builtin_inff() ? 0.f : m;
+    float *dst = out_row(p, seq, i, h);
+    for (int c = threadIdx.x; c < p.c.head_dim; c += 64) {
+        float acc = 0.f, l = 0.f;
+        for (int s = 0; s < shares; ++s) {
+            const float w = __builtin_amdgcn_exp2f(p.part_ml[2 * (slot0 + s)] - ref);
+            l += p.part_ml[2 * (slot0 + s) + 1] * w;
+            acc += p.part_o[(slot0 + s) * p.pitch + c] * w;
+        }
+        dst[c] = acc / l;
+    }
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------------
+
+// How a call is cut: the same for its workspace and its launch.
+struct Plan {
+    bool tiles;   // pages, head size and strides that the 128-bit loads take (the pointers' alignment is looked at later)
+    int nsplit, share, pitch;
+    int64_t rows;
+};
+
+Plan plan(const fth_paged_cache &c, const fth_paged_sdpa_desc &d) {
+    Plan p;
+    const int64_t ch = c.dtype == FTH_DTYPE_F32 ? 4 : 8;
+    p.rows = c.num_seqs * d.new_tokens * d.q_heads;
+    p.tiles = c.page_size % 16 == 0 && c.head_dim % ch == 0 && c.row_stride % ch == 0 && c.head_stride % ch == 0 && c.page_stride % ch == 0 &&
+              c.row_stride <= ((int64_t)1 << 24) && c.num_pages > 0;
+    const int64_t most = c.max_pages * c.page_size < d.max_len ? c.max_pages * c.page_size : d.max_len;
+    const int64_t row_tiles = fth::ceil_div(d.q_heads / c.kv_heads * d.new_tokens, 16);
+    const int64_t units = p.tiles ? c.num_seqs * c.kv_heads * row_tiles : p.rows;
+    const int64_t step = kTile * kWaves;
+    int64_t want = units > 0 ? 2048 / units : 1;
+    const int64_t longest = fth::ceil_div(most, 4 * step);
+    want = want > longest ? longest : want;
+    want = want < 1 ? 1 : want;
+    p.share = (int)(fth::ceil_div(fth::ceil_div(most, want), step) * step);
+    if (p.share < step) p.share = (int)step;
+    // (most is at most 2^30: nothing here overflows an int)
+    p.nsplit = (int)fth::ceil_div(most, p.share);
+    if (p.nsplit < 1) p.nsplit = 1;
+    p.pitch = (int)fth::ceil_div(c.head_dim, 4) * 4;
+    return p;
+}
+
+size_t workspace_bytes_of(const Plan &p) { return p.nsplit > 1 ? (size_t)p.rows * p.nsplit * (p.pitch + 2) * sizeof(float) : 0; }
 
 int32_t check(const fth_paged_cache *c, const fth_paged_sdpa_desc *d) {
     if (int32_t rc = fth::check_paged_cache(c, "paged_sdpa", nullptr)) return rc;
     FTH_ARG(d, "paged_sdpa: NULL descriptor");
     FTH_ARG(d->q_heads >= 1 && d->q_heads % c->kv_heads == 0, "paged_sdpa: %lld query heads on %lld K/V heads", (long long)d->q_heads, (long long)c->kv_heads);
     FTH_ARG(d->new_tokens >= 1 && d->new_tokens <= 8, "paged_sdpa: new_tokens %lld is outside 1..8", (long long)d->new_tokens);
-    FTH_ARG(d->max_len >= 0 && d->max_len <= 2147483647LL, "paged_sdpa: max_len %lld is outside 0..2^31 - 1", (long long)d->max_len);
+    FTH_ARG(d->max_len >= 0 && d->max_len <= (1 << 30), "paged_sdpa: max_len %lld is outside 0..2^30", (long long)d->max_len);
     for (int64_t x : {d->q_seq_stride, d->q_row_stride, d->q_head_stride, d->o_seq_stride, d->o_row_stride, d->o_head_stride})
         FTH_ARG(fth::stride_in_range(x), "paged_sdpa: a stride is negative or over 2^40");
     int64_t rows = 0;
-    if (__builtin_mul_overflow(c->num_seqs * d->new_tokens, d->q_heads, &rows) || rows > 2147483647LL)
-        return fth::set_error(FTH_ERR_SIZE_OVERFLOW, "paged_sdpa: too many query rows for one launch");
+    if (__builtin_mul_overflow(c->num_seqs * d->new_tokens, d->q_heads, &rows) || rows > (1 << 24))
+        return fth::set_error(FTH_ERR_SIZE_OVERFLOW, "paged_sdpa: more than 2^24 query rows");
+    return FTH_OK;
+}
+
+template <typename T> int32_t launch(PagedArgs &a, const Plan &pl, bool tiles, hipStream_t st) {
+    if (tiles) {
+        const int64_t grid = a.c.num_seqs * a.c.kv_heads * a.row_tiles * a.nsplit;
+        FTH_ARG(grid <= 2147483647LL, "paged_sdpa: too many workgroups for one launch");
+        const dim3 blocks((unsigned)grid), threads(64 * kWaves);
+        switch (a.c.head_dim) {
+            case 64: paged_sdpa_tiles_kernel<T, 64, true><<<blocks, threads, 0, st>>>(a); break;
+            case 128: paged_sdpa_tiles_kernel<T, 128, true><<<blocks, threads, 0, st>>>(a); break;
+            case 256: paged_sdpa_tiles_kernel<T, 256, true><<<blocks, threads, 0, st>>>(a); break;
+            default:
+                if (a.c.head_dim < 64) paged_sdpa_tiles_kernel<T, 64, false><<<blocks, threads, 0, st>>>(a);
+                else if (a.c.head_dim < 128) paged_sdpa_tiles_kernel<T, 128, false><<<blocks, threads, 0, st>>>(a);
+                else paged_sdpa_tiles_kernel<T, 256, false><<<blocks, threads, 0, st>>>(a);
+        }
+    } else {
+        FTH_ARG(pl.rows * a.nsplit <= 2147483647LL, "paged_sdpa: too many rows for one launch");
+        paged_sdpa_rows_kernel<T><<<dim3((unsigned)(pl.rows * a.nsplit)), dim3(64), 0, st>>>(a);
+    }
+    FTH_CHECK_LAUNCH("paged_sdpa");
+    if (a.nsplit > 1) {
+        paged_sdpa_join_kernel<<<dim3((unsigned)pl.rows), dim3(64), 0, st>>>(a);
+        FTH_CHECK_LAUNCH("paged_sdpa_join");
+    }
     return FTH_OK;
 }
 
@@ -113,7 +503,7 @@ int32_t check(const fth_paged_cache *c, const fth_paged_sdpa_desc *d) {
 extern "C" {
 
 size_t fth_dev_paged_sdpa_workspace_bytes(const fth_paged_cache *c, const fth_paged_sdpa_desc *d) {
-    return check(c, d) == FTH_OK ? 0 : 0;
+    return check(c, d) == FTH_OK ? workspace_bytes_of(plan(*c, *d)) : 0;
 }
 
 int32_t fth_dev_paged_sdpa_f32(const fth_paged_cache *c, const fth_paged_sdpa_desc *d, float scale, const float *q, const void *k_cache, const void *v_cache,
@@ -121,6 +511,9 @@ int32_t fth_dev_paged_sdpa_f32(const fth_paged_cache *c, const fth_paged_sdpa_de
                                fth_stream s) {
     if (int32_t rc = check(c, d)) return rc;
     FTH_ARG(c->num_seqs == 0 || (q && lens && out && (block_table || c->max_pages == 0) && ((k_cache && v_cache) || c->num_pages == 0)), "paged_sdpa: NULL operand");
+    const Plan pl = plan(*c, *d);
+    const size_t need = workspace_bytes_of(pl);
+    FTH_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15u) == 0), "paged_sdpa: needs a workspace of %zu bytes, 16-byte aligned", need);
     FTH_REQUIRE_DEVICE();
     hipStream_t st = fth::resolve_stream(s);
     if (bad_index) {
@@ -128,17 +521,25 @@ int32_t fth_dev_paged_sdpa_f32(const fth_paged_cache *c, const fth_paged_sdpa_de
         FTH_CHECK_LAUNCH("paged_sdpa(bad_index reset)");
     }
     if (c->num_seqs == 0) return FTH_OK;
-    (void)workspace;
-    (void)workspace_bytes;
     PagedArgs a;
     a.c = *c;
     a.d = *d;
     a.q = q; a.k = k_cache; a.v = v_cache; a.table = block_table; a.lens = lens; a.out = out; a.bad = bad_index;
-    a.scale = scale;
+    a.part_o = static_cast<float *>(workspace);
+    a.part_ml = need ? a.part_o + pl.rows * pl.nsplit * pl.pitch : nullptr;
+    a.scale2 = scale * kLog2e;
+    a.most = c->max_pages * c->page_size < d->max_len ? c->max_pages * c->page_size : d->max_len;
+    a.group = (int)(d->q_heads / c->kv_heads);
+    a.row_tiles = (int)fth::ceil_div((int64_t)a.group * d->new_tokens, 16);
+    a.nsplit = pl.nsplit; a.share = pl.share; a.pitch = pl.pitch;
+    const Divisor by_page((uint32_t)c->page_size);
+    a.page_mul = by_page.mul;
+    a.page_shift = by_page.shift;
+    const bool tiles = pl.tiles && (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15u) == 0;
     switch (c->dtype) {
-        case FTH_DTYPE_F32: return launch<float>(a, st);
-        case FTH_DTYPE_F16: return launch<fth::f16>(a, st);
-        default: return launch<fth::bf16>(a, st);
+        case FTH_DTYPE_F32: return launch<float>(a, pl, tiles, st);
+        case FTH_DTYPE_F16: return launch<fth::f16>(a, pl, tiles, st);
+        default: return launch<fth::bf16>(a, pl, tiles, st);
     }
 }
 

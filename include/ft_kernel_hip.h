@@ -473,7 +473,7 @@ int32_t fth_dev_paged_append_f32(const fth_paged_cache *c, const fth_paged_appen
  * out = softmax(scale * q . k) v. Element (s, i, h, c) of q is q[s * q_seq_stride + i * q_row_stride + h * q_head_stride + c];
  * likewise out (o_*). Query head h reads K/V head h / (q_heads / kv_heads). A query that sees nothing (lens[s] too small, 0 for
  * an unused slot of a batch) gives zeros. What the cache holds past a sequence's length is never used, NaN included.
- * max_len is a bound on lens that the host knows (it sizes the launch; a captured graph serves every length up to it). A
+ * max_len (<= 2^30) is a bound on lens that the host knows (it sizes the launch; a captured graph serves every length up to it). A
  * sequence with lens[s] outside [0, min(max_len, max_pages * page_size)] or with a page that does not exist has NaN in all its
  * outputs, and bad_index (device, may be NULL) receives the lowest such s, or -1.
  * The workspace (device memory, contents ignored and overwritten) holds the partial results of shares of the keys, which are
