@@ -6,13 +6,21 @@
 // one K/V head for up to 16 of the query rows that read it (query heads of the group x new tokens), so K and V are read once for
 // all of them. Its four wavefronts walk the share in tiles of 32 keys, each on its own (running maximum and sum per row in fp32,
 // no barrier), and are joined through LDS at the end; a second small kernel joins the shares of a row in order.
-//   * S^T[key, row] = K . Q^T on v_mfma_f32_16x16x4_f32: lane (lr, g) brings a quarter of K row lr and of query row lr; 16-bit
-//     values become floats on the way, so scores and outputs are fp32 sums of exact products' roundings, whatever the storage.
-//   * It then holds the scores of keys 16 s + 4 g + r of row lr, which is the B operand of O^T[d, row] += V^T . P^T: P never
-//     moves, and V rows are read whole (16 lanes side by side).
-//   * The loads of the next tile's K go out when the scores have consumed this one's, those of V after the outputs have.
+//   * S^T[key, row] = K . Q^T with a key row and a query row per lane (16 x 16 tiles); the lane that gets scores of row lr holds
+//     them as it needs them for O^T[d, row] += V^T . P^T, so P never moves; V rows are read whole (16 lanes side by side).
+//   * 16-bit caches: both products run on the 16-bit matrix units against the bits as they are stored. The fp32 side is cut into
+//     parts of the storage type whose sum it is (struct Parts), so that the result is that of fp32 arithmetic; what parts cannot
+//     do (values that are not finite) is found and computed again. fp32 caches: fp32 matrix units, 16 times slower a product.
+//   * The loads of the next tile's K go out when the scores have consumed this one's, those of V after the outputs have, with
+//     nothing conditional in between: the waits are then for K or V alone, never for both.
 // Pages: with a page size that is a multiple of 16 each half tile lies in one page, whose number is a scalar load one tile
-// ahead. Other page sizes, head sizes and alignments that the 128-bit loads cannot take go to a kernel of one wavefront a row.
+// ahead. Other page sizes, and strides and alignments that 128-bit loads cannot take, go to a kernel of one wavefront a row.
+//
+// Measured: 64 sequences of 1024 to 8191 keys, 32 query heads on 8 K/V heads of 128, bf16 (1.22 GB): 7.6 ms on one wavefront a
+// row, 283 us with both products on fp32 units, 235 with the scores on 16-bit ones (MFMA-busy 0.31, wavefronts waiting to
+// issue), 217 + 5 with both (5.7 TB/s; a kernel that only reads pages of 4 KB in random order reaches 5.9, with nontemporal
+// loads 6.5). One sequence of 131071: 87 + 6 us (6.2 TB/s). Joining the shares in the last workgroup to arrive instead of a
+// second launch was slower in every case (release and acquire across the XCDs): 90 -> 109 us.
 
 #include <type_traits>
 
@@ -22,6 +30,7 @@ namespace {
 
 using F4 = float __attribute__((ext_vector_type(4)));
 using U4 = uint32_t __attribute__((ext_vector_type(4)));
+using U2 = uint32_t __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.44269502162933349609375f;
 constexpr int kTile = 32, kWaves = 4;
@@ -168,6 +177,49 @@ template <> struct Chunk<float> {
     static __device__ __forceinline__ float get(const U4 &v, int e) { return __uint_as_float(v[e]); }
 };
 
+// Scores against 16-bit keys go to the 16-bit matrix units: a query row is scaled by a power of two so that its largest element
+// lies in [2^kTop, 2^(kTop + 1)), and cut into parts of the keys' type whose sum it is (bf16: 3 x 8 bits; f16: 2 x 11 bits, off by
+// 2^-22 of an element or 2^-39 of the largest).
+template <typename T> struct Parts {  // fp32 keys and values: none
+    static constexpr int kParts = 0, kArray = 1, kTop = 0, kWeight = 0;
+    using Vec = __attribute__((ext_vector_type(8))) _Float16;
+    static __device__ __forceinline__ F4 mfma(const U4 &, const U4 &, F4 c) { return c; }
+};
+template <> struct Parts<fth::bf16> {
+    static constexpr int kParts = 3, kArray = 3, kTop = 0, kWeight = 64;
+    using Vec = __attribute__((ext_vector_type(8))) __bf16;
+    static __device__ __forceinline__ F4 mfma(const U4 &a, const U4 &b, F4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Vec, a), __builtin_bit_cast(Vec, b), c, 0, 0, 0);
+    }
+};
+template <> struct Parts<fth::f16> {
+    static constexpr int kParts = 2, kArray = 2, kTop = 14, kWeight = 14;
+    using Vec = __attribute__((ext_vector_type(8))) _Float16;
+    static __device__ __forceinline__ F4 mfma(const U4 &a, const U4 &b, F4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(Vec, a), __builtin_bit_cast(Vec, b), c, 0, 0, 0);
+    }
+};
+
+template <bool NT> __device__ __forceinline__ U4 load128(const void *p) {
+    const U4 *v = static_cast<const U4 *>(p);
+    return NT ? __builtin_nontemporal_load(v) : *v;
+}
+
+// v[0..7] as kParts vectors of the storage type whose sum they are (up to the last part's rounding).
+template <typename T> __device__ __forceinline__ void split_parts(float *v, U4 (&parts)[Parts<T>::kArray]) {
+    using V8 = typename Parts<T>::Vec;
+#pragma unroll
+    for (int j = 0; j < Parts<T>::kParts; ++j) {
+        V8 part;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            part[e] = (typename std::remove_reference<decltype(part[0])>::type)v[e];
+            v[e] -= (float)part[e];
+        }
+        parts[j] = __builtin_bit_cast(U4, part);
+    }
+}
+
 template <typename T, int DP> struct TileShape {
     static constexpr int CH = Chunk<T>::kElems;     // elements of a 128-bit load
     static constexpr int NK = DP / 4 / CH;          // loads of a lane's quarter of a K row
@@ -177,10 +229,10 @@ template <typename T, int DP> struct TileShape {
     static constexpr int kLds = kWaves * 16 * (DP + 4);
 };
 
-// FULL: head_dim == DP; otherwise what lies past head_dim counts as zero.
-template <typename T, int DP, bool FULL> __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void paged_sdpa_tiles_kernel(const PagedArgs p) {
+// FULL: head_dim == DP; otherwise what lies past head_dim counts as zero. NT: K and V leave no trace in the caches.
+template <typename T, int DP, bool FULL, bool NT> __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void paged_sdpa_tiles_kernel(const PagedArgs p) {
     using S = TileShape<T, DP>;
-    constexpr int CH = S::CH, NK = S::NK, NE = S::NE, CV = S::CV, NV = S::NV;
+    constexpr int CH = S::CH, NK = S::NK, NE = S::NE, CV = S::CV, NV = S::NV, kParts = Parts<T>::kParts;
     __shared__ __attribute__((aligned(16))) float lds_o[S::kLds];
     __shared__ float lds_ml[kWaves * 16 * 2];
     const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
@@ -200,120 +252,194 @@ template <typename T, int DP, bool FULL> __global__ __launch_bounds__(64 * kWave
     const int tiles = (key_hi - key_lo + kTile - 1) / kTile, last16 = (key_hi - 1) >> 4;
     const T *K = static_cast<const T *>(p.k) + hk * p.c.head_stride, *V = static_cast<const T *>(p.v) + hk * p.c.head_stride;
     const int32_t *table = p.table + seq * p.c.table_stride;
-    const int rs = (int)p.c.row_stride;
+    const int rs = (int)p.c.row_stride, num_pages = (int)p.c.num_pages;
+
+    const int stored = rows - rt * 16 < 16 ? rows - rt * 16 : 16;
+    if (len == 0) {
+        if (bad && threadIdx.x == 0) fth::report_bad_entry(p.bad, seq);
+        for (int x = threadIdx.x; x < stored * hd; x += 64 * kWaves) {
+            const int row = rt * 16 + x / hd;
+            out_row(p, seq, row % new_tokens, hk * p.group + row / new_tokens)[x % hd] = bad ? __builtin_nanf("") : 0.f;
+        }
+        return;
+    }
 
     // this lane's query row (rows past the last repeat it and are never stored) and how many keys it sees
     int rr = rt * 16 + lr;
     rr = rr < rows ? rr : rows - 1;
     const int qi = rr % new_tokens, qh = hk * p.group + rr / new_tokens;
     const int sees = len - new_tokens + 1 + qi;
+    const float *qr = p.q + seq * p.d.q_seq_stride + qi * p.d.q_row_stride + qh * p.d.q_head_stride;
     float q[NK][CH];
-    {
-        const float *qr = p.q + seq * p.d.q_seq_stride + qi * p.d.q_row_stride + qh * p.d.q_head_stride;
 #pragma unroll
-        for (int i = 0; i < NK; ++i)
+    for (int i = 0; i < NK; ++i)
 #pragma unroll
-            for (int e = 0; e < CH; ++e) {
-                const int c = (4 * i + g) * CH + e;
-                q[i][e] = FULL || c < hd ? qr[c] : 0.f;
-            }
-    }
+        for (int e = 0; e < CH; ++e) {
+            const int c = (4 * i + g) * CH + e;
+            q[i][e] = FULL || c < hd ? qr[c] : 0.f;
+        }
 
-    // page and first row of the 16 keys number t16 (of the sequence)
+    // The 16 keys number t16 (of the sequence): the page and the first row in it; half tiles past the end repeat the last one.
     auto page_of = [&](int t16) __attribute__((always_inline)) {
-        t16 = t16 < last16 ? t16 : last16;  // half tiles past the end repeat the last one
+        t16 = t16 < last16 ? t16 : last16;
         const int index = (int)divide((uint32_t)t16 << 4, p.page_mul, p.page_shift);
         return make_int2(table[index], (t16 << 4) - index * (int)p.c.page_size);
     };
     auto offset_of = [&](int2 page) __attribute__((always_inline)) {
-        if (page.x < 0 || page.x >= p.c.num_pages) {
-            bad = true;
-            page.x = 0;
-        }
-        return (int64_t)page.x * p.c.page_stride + (int64_t)page.y * rs;
+        const bool there = page.x >= 0 && page.x < num_pages;
+        bad = bad || !there;
+        const int64_t at = (int64_t)(there ? page.x : 0) * p.c.page_stride + (int64_t)page.y * rs;
+        return (int64_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)at);  // one for all lanes
     };
     U4 kf[2][NK], vf[2][4][NV];
+    const uint32_t k_lane = (uint32_t)((lr * rs + g * CH) * (int)sizeof(T));
+    uint32_t v_lane[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v_lane[r] = (uint32_t)(((4 * g + r) * rs + lr * CV) * (int)sizeof(T));
     auto load_k = [&](const int64_t (&off)[2]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < 2; ++s) {
+            const char *base = reinterpret_cast<const char *>(K + off[s]);
 #pragma unroll
             for (int i = 0; i < NK; ++i) {
-                const int c = (4 * i + g) * CH;
-                kf[s][i] = U4{0u, 0u, 0u, 0u};
-                if (FULL || c < hd) kf[s][i] = *reinterpret_cast<const U4 *>(K + off[s] + (uint32_t)(lr * rs + c));
+                if (!FULL) kf[s][i] = U4{0u, 0u, 0u, 0u};
+                if (FULL || (4 * i + g) * CH < hd) kf[s][i] = load128<NT>(base + k_lane + 64 * i);
             }
+        }
     };
     auto load_v = [&](const int64_t (&off)[2]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < 2; ++s) {
+            const char *base = reinterpret_cast<const char *>(V + off[s]);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    const int c = (16 * i + lr) * CV;
-                    const T *src = V + off[s] + (uint32_t)((4 * g + r) * rs + c);
-                    vf[s][r][i] = U4{0u, 0u, 0u, 0u};
-                    if (FULL || c < hd) {
+                    const char *src = base + v_lane[r] + 16 * CV * (int)sizeof(T) * i;
+                    if (!FULL) vf[s][r][i] = U4{0u, 0u, 0u, 0u};
+                    if (FULL || (16 * i + lr) * CV < hd) {
                         if constexpr (CV * sizeof(T) == 16) {
-                            vf[s][r][i] = *reinterpret_cast<const U4 *>(src);
+                            vf[s][r][i] = load128<NT>(src);
                         } else {
-                            const uint2 w = *reinterpret_cast<const uint2 *>(src);
-                            vf[s][r][i][0] = w.x;
-                            vf[s][r][i][1] = w.y;
+                            const U2 w = NT ? __builtin_nontemporal_load(reinterpret_cast<const U2 *>(src)) : *reinterpret_cast<const U2 *>(src);
+                            vf[s][r][i][0] = w[0];
+                            vf[s][r][i][1] = w[1];
                         }
                     }
                 }
+        }
     };
+
+    const int t16_lo = key_lo >> 4;
+    int64_t off[2];
+    int2 ahead[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        off[s] = offset_of(page_of(t16_lo + 2 * wave + s));
+        ahead[s] = page_of(t16_lo + 2 * (wave + kWaves) + s);
+    }
+    load_k(off);  // (a wavefront without a tile reads the last one)
+    load_v(off);
+    __builtin_amdgcn_sched_barrier(0);
+
+    U4 qp[Parts<T>::kArray][NK];
+    float scale2 = p.scale2;
+    bool finite = true;  // the query row
+    if constexpr (kParts != 0) {
+        float big = 0.f, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+#pragma unroll
+            for (int e = 0; e < CH; ++e) {
+                big = fmaxf(big, fabsf(q[i][e]));
+                sum += q[i][e] * 0.f;
+            }
+        big = rows_reduce(big, MaxOp());
+        finite = rows_reduce(sum, AddOp()) == 0.f;
+        const int up = big > 0.f && big < __builtin_inff() ? Parts<T>::kTop + 1 - __builtin_amdgcn_frexp_expf(big) : 0;
+        scale2 = __builtin_ldexpf(scale2, -up);
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+            U4 parts[Parts<T>::kArray];
+#pragma unroll
+            for (int e = 0; e < CH; ++e) q[i][e] = __builtin_ldexpf(q[i][e], up);
+            split_parts<T>(q[i], parts);
+#pragma unroll
+            for (int j = 0; j < kParts; ++j) qp[j][i] = parts[j];
+        }
+    }
 
     F4 o[NE];
 #pragma unroll
     for (int e = 0; e < NE; ++e) o[e] = F4{0.f, 0.f, 0.f, 0.f};
     float m_run = -__builtin_inff(), l_run = 0.f;  // the sum: this lane's keys only
+    const int limit = sees < key_hi ? sees : key_hi;
 
-    const int t16_lo = key_lo >> 4;
-    int64_t off[2], off_next[2];
-    int2 ahead[2];
-    if (wave < tiles) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            off[s] = offset_of(page_of(t16_lo + 2 * wave + s));
-            ahead[s] = page_of(t16_lo + 2 * (wave + kWaves) + s);
-        }
-        load_k(off);
-        load_v(off);
-    }
-    for (int t = wave; t < tiles; t += kWaves) {
+    // One tile of 32 keys. Constants: `more`: another one of this wavefront follows, whose loads go out on the way (what a query
+    // may not see lies in the last two tiles of the sequence, which are the last ones of their wavefronts); `parts`: weights
+    // and V on the 16-bit matrix units.
+    auto step = [&](int t, auto more, auto parts) __attribute__((always_inline)) {
         const int key0 = key_lo + t * kTile;
-        const bool more = t + kWaves < tiles;
-        F4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        F4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, low[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int i = 0; i < NK; ++i)
+        for (int i = 0; i < NK; ++i) {
+            if constexpr (kParts == 0) {
 #pragma unroll
-            for (int e = 0; e < CH; ++e)
+                for (int e = 0; e < CH; ++e)
 #pragma unroll
-                for (int s = 0; s < 2; ++s) sc[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(Chunk<T>::get(kf[s][i], e), q[i][e], sc[s], 0, 0, 0);
-        if (more) {
+                    for (int s = 0; s < 2; ++s) sc[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(Chunk<T>::get(kf[s][i], e), q[i][e], sc[s], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int j = kParts - 1; j >= 0; --j)
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) (j ? low : sc)[s] = Parts<T>::mfma(kf[s][i], qp[j][i], (j ? low : sc)[s]);
+            }
+        }
+        int64_t next[2];
+        if constexpr (more) {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                off_next[s] = offset_of(ahead[s]);
+                next[s] = offset_of(ahead[s]);
                 ahead[s] = page_of(t16_lo + 2 * (t + 2 * kWaves) + s);
             }
-            load_k(off_next);
+            load_k(next);
         }
-        float mx = -__builtin_inff();
-        const bool edge = key0 + kTile > len - new_tokens + 1 || key0 + kTile > key_hi;
+        float check = 0.f;
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float x = sc[s][r] * p.scale2;
-                if (edge) {
-                    const int key = key0 + 16 * s + 4 * g + r;
-                    x = key >= sees || key >= key_hi ? -__builtin_inff() : x;
-                }
-                sc[s][r] = x;
-                mx = fmaxf(mx, x);
+                float x = (kParts ? sc[s][r] + low[s][r] : sc[s][r]) * scale2;
+                const bool seen = more || key0 + 16 * s + 4 * g + r < limit;
+                check = __builtin_fmaf(seen ? x : 0.f, 0.f, check);
+                sc[s][r] = seen ? x : -__builtin_inff();
             }
+        if constexpr (kParts != 0) {
+            // An infinity against the parts of a query is no longer what it is against the query, and the scaled query may
+            // overflow where it does not: such scores are computed again. (A query row that is not finite gives NaN either way.)
+            if (__any(!(check == 0.f) && finite)) {
+#pragma unroll 1
+                for (int j = 0; j < 8; ++j) {
+                    float x = sc[0][0];
+#pragma unroll
+                    for (int y = 1; y < 8; ++y) x = j == y ? sc[y >> 2][y & 3] : x;
+                    const int row = 16 * (j >> 2) + 4 * g + (j & 3);
+                    if (finite && !(fabsf(x) < __builtin_inff()) && key0 + row < limit) {
+                        const T *kr = K + off[j >> 2] + (4 * g + (j & 3)) * rs;
+                        float dot = 0.f;
+                        for (int c = 0; c < hd; ++c) dot = __builtin_fmaf(qr[c], fth::to_f32(kr[c]), dot);
+                        x = dot * p.scale2;
+                    }
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) sc[y >> 2][y & 3] = j == y ? x : sc[y >> 2][y & 3];
+                }
+            }
+        }
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[s][r]);
         mx = rows_reduce(mx, MaxOp());
         if (__any(mx > m_run)) {
             const float m_new = fmaxf(m_run, mx);
@@ -325,38 +451,102 @@ template <typename T, int DP, bool FULL> __global__ __launch_bounds__(64 * kWave
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[e][r] *= alpha;
         }
-        const float ref = m_run == -__builtin_inff() ? 0.f : m_run;  // nothing visible so far: every weight is exp(-inf) = 0
+        // nothing visible so far: every weight is exp(-inf) = 0
+        const float ref = (m_run == -__builtin_inff() ? 0.f : m_run) - (parts ? (float)Parts<T>::kWeight : 0.f);
+        float w[8];
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                sc[s][r] = __builtin_amdgcn_exp2f(sc[s][r] - ref);
-                l_run += sc[s][r];
+                w[4 * s + r] = __builtin_amdgcn_exp2f(sc[s][r] - ref);
+                l_run += w[4 * s + r];
             }
-        if (key0 + kTile > key_hi) {  // weight 0 times what an unused row holds would be NaN
+        if constexpr (!more) {  // weight 0 times what an unused row holds would be NaN
+            if (key0 + kTile > key_hi) {
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (key0 + 16 * s + 4 * g + r >= key_hi)
+#pragma unroll
+                            for (int i = 0; i < NV; ++i) vf[s][r][i] = U4{0u, 0u, 0u, 0u};
+            }
+        }
+        if constexpr (parts) {
+            U4 wp[Parts<T>::kArray];
+            split_parts<T>(w, wp);
+#pragma unroll
+            for (int e = 0; e < NE; ++e) {
+                // elements e of the eight V rows, in the order of the weights
+                U4 column;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t a = vf[j >> 1][2 * (j & 1)][e / CV][e % CV / 2], b = vf[j >> 1][2 * (j & 1) + 1][e / CV][e % CV / 2];
+                    column[j] = __builtin_amdgcn_perm(b, a, e & 1 ? 0x07060302u : 0x05040100u);
+                }
+#pragma unroll
+                for (int j = kParts - 1; j >= 0; --j) o[e] = Parts<T>::mfma(column, wp[j], o[e]);
+            }
+        } else {
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (key0 + 16 * s + 4 * g + r >= key_hi)
 #pragma unroll
-                        for (int i = 0; i < NV; ++i) vf[s][r][i] = U4{0u, 0u, 0u, 0u};
+                    for (int e = 0; e < NE; ++e)
+                        o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(Chunk<T>::get(vf[s][r][e / CV], e % CV), w[4 * s + r], o[e], 0, 0, 0);
         }
+        if constexpr (more) {
+            load_v(next);
+            off[0] = next[0];
+            off[1] = next[1];
+        }
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+    auto walk = [&](auto parts) __attribute__((always_inline)) {
+        int t = wave;
+        for (; t + kWaves < tiles; t += kWaves) step(t, Yes(), parts);
+        step(t, No(), parts);
+    };
+    float weight = 0.f;  // the exponent of two in the weights
+    if (wave < tiles) {
+        if constexpr (kParts == 0) {
+            walk(No());
+        } else {
+            walk(Yes());
+            weight = (float)Parts<T>::kWeight;
+            float check = 0.f;
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+            for (int e = 0; e < NE; ++e)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+                for (int r = 0; r < 4; ++r) check = __builtin_fmaf(o[e][r] * 0x1p28f, 0.f, check);
+            // What is not finite in V meets the parts of a weight, not the weight, and large values times the scaled weights
+            // may overflow (here or when shares are added up) where they do not: from 2^100 on once more on fp32 units, unless
+            // the query row gives NaN anyway.
+            if (__any(!(check == 0.f) && finite)) {
+                weight = 0.f;
+                m_run = -__builtin_inff();
+                l_run = 0.f;
 #pragma unroll
-                for (int e = 0; e < NE; ++e)
-                    o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(Chunk<T>::get(vf[s][r][e / CV], e % CV), sc[s][r], o[e], 0, 0, 0);
-        if (more) load_v(off_next);
+                for (int e = 0; e < NE; ++e) o[e] = F4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    off[s] = offset_of(page_of(t16_lo + 2 * wave + s));
+                    ahead[s] = page_of(t16_lo + 2 * (wave + kWaves) + s);
+                }
+                load_k(off);
+                load_v(off);
+                walk(No());
+            }
+        }
     }
 
     // join the wavefronts: MFMA row 4 g + r of column tile e is output column ((e / CV) * 16 + 4 g + r) * CV + e % CV
     constexpr int P = DP + 4;
     const float l_wave = rows_reduce(l_run, AddOp());
     if (g == 0) {
-        lds_ml[(wave * 16 + lr) * 2] = m_run;
+        lds_ml[(wave * 16 + lr) * 2] = m_run - weight;  // weights times 2^k relative to m are weights relative to m - k
         lds_ml[(wave * 16 + lr) * 2 + 1] = bad ? __builtin_nanf("") : l_wave;
     }
 #pragma unroll
@@ -365,7 +555,6 @@ template <typename T, int DP, bool FULL> __global__ __launch_bounds__(64 * kWave
         for (int r = 0; r < 4; ++r) lds_o[(wave * 16 + lr) * P + ((e / CV) * 16 + 4 * g + r) * CV + e % CV] = o[e][r];
     if (bad && lane == 0) fth::report_bad_entry(p.bad, seq);
     __syncthreads();
-    const int stored = rows - rt * 16 < 16 ? rows - rt * 16 : 16;
     for (int x = threadIdx.x; x < stored * (DP / 4); x += 64 * kWaves) {
         const int row = x / (DP / 4), c = x % (DP / 4) * 4;
         if (c >= hd) continue;
@@ -401,27 +590,50 @@ template <typename T, int DP, bool FULL> __global__ __launch_bounds__(64 * kWave
 
 // ---- shares joined in their order -----------------------------------------------------------------------------------------
 
-__global__ __launch_bounds__(64) void paged_sdpa_join_kernel(const PagedArgs p) {
-    const int64_t row = blockIdx.x;
+// SL lanes of a wavefront walk the shares of four columns of a row side by side (each over every SL-th of them, in order) and are
+// added up in a fixed tree; 64 / SL neighbouring groups of columns make the wavefront. SL grows with the shares, so that no lane
+// has more than a few loads to wait for.
+template <int SL> __global__ __launch_bounds__(256) void paged_sdpa_join_kernel(const PagedArgs p, int64_t items) {
+    constexpr int CL = 64 / SL;
+    const int64_t item = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * CL + (threadIdx.x & (CL - 1));
+    const int lane_s = (threadIdx.x & 63) / CL, groups = p.pitch / 4;
+    const bool there = item < items;
+    const int64_t row = there ? item / groups : 0;
+    const int c = (int)(item % groups) * 4;
     const int h = (int)(row % p.d.q_heads), i = (int)(row / p.d.q_heads % p.d.new_tokens);
     const int64_t seq = row / p.d.q_heads / p.d.new_tokens;
     const int len = p.lens[seq];
-    if (len <= p.share || len > p.most) return;  // written by its only share
-    const int shares = (len - 1) / p.share + 1;
-    const int64_t slot0 = row * p.nsplit;
+    // rows of one share are written; so are those of an invalid length
+    const int shares = there && len > p.share && len <= p.most ? (len - 1) / p.share + 1 : 0;
+    const float2 *ml = reinterpret_cast<const float2 *>(p.part_ml) + row * p.nsplit;
+    const float *o = p.part_o + row * p.nsplit * p.pitch + c;
     float m = -__builtin_inff();
-    for (int s = 0; s < shares; ++s) m = fmaxf(m, p.part_ml[2 * (slot0 + s)]);
+    for (int s = lane_s; s < shares; s += SL) m = fmaxf(m, ml[s].x);
+#pragma unroll
+    for (int d = CL; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
     const float ref = m == -__builtin_inff() ? 0.f : m;
-    float *dst = out_row(p, seq, i, h);
-    for (int c = threadIdx.x; c < p.c.head_dim; c += 64) {
-        float acc = 0.f, l = 0.f;
-        for (int s = 0; s < shares; ++s) {
-            const float w = __builtin_amdgcn_exp2f(p.part_ml[2 * (slot0 + s)] - ref);
-            l += p.part_ml[2 * (slot0 + s) + 1] * w;
-            acc += p.part_o[(slot0 + s) * p.pitch + c] * w;
-        }
-        dst[c] = acc / l;
+    F4 acc = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+#pragma unroll 8
+    for (int s = lane_s; s < shares; s += SL) {
+        const float2 part = ml[s];
+        const F4 v = *reinterpret_cast<const F4 *>(o + (int64_t)s * p.pitch);
+        const float w = __builtin_amdgcn_exp2f(part.x - ref);
+        l += part.y * w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] += v[j] * w;
     }
+#pragma unroll
+    for (int d = CL; d < 64; d <<= 1) {
+        l += __shfl_xor(l, d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor(acc[j], d);
+    }
+    if (shares == 0 || lane_s != 0) return;
+    float *dst = out_row(p, seq, i, h) + c;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (c + j < p.c.head_dim) dst[j] = acc[j] / l;
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
@@ -429,6 +641,7 @@ __global__ __launch_bounds__(64) void paged_sdpa_join_kernel(const PagedArgs p) 
 // How a call is cut: the same for its workspace and its launch.
 struct Plan {
     bool tiles;   // pages, head size and strides that the 128-bit loads take (the pointers' alignment is looked at later)
+    bool nt;      // loads that leave no trace in the caches
     int nsplit, share, pitch;
     int64_t rows;
 };
@@ -443,16 +656,22 @@ Plan plan(const fth_paged_cache &c, const fth_paged_sdpa_desc &d) {
     const int64_t row_tiles = fth::ceil_div(d.q_heads / c.kv_heads * d.new_tokens, 16);
     const int64_t units = p.tiles ? c.num_seqs * c.kv_heads * row_tiles : p.rows;
     const int64_t step = kTile * kWaves;
-    int64_t want = units > 0 ? 2048 / units : 1;
-    const int64_t longest = fth::ceil_div(most, 4 * step);
-    want = want > longest ? longest : want;
-    want = want < 1 ? 1 : want;
-    p.share = (int)(fth::ceil_div(fth::ceil_div(most, want), step) * step);
-    if (p.share < step) p.share = (int)step;
-    // (most is at most 2^30: nothing here overflows an int)
+    // Shares: about 256 workgroups, of 256 to 2048 keys. A join costs 4 to 5 us, so nothing is cut that fills the chip whole (32
+    // sequences of 1000 keys: 18.6 us in one share, 23.6 in two) or has 512 keys (8 K/V heads of 128: 10.5 / 12.0); longer shares than
+    // 2048 leave the chip empty behind the longest sequence (64 of up to 8191: 241 us in one share, 235 in four). 128 keys where
+    // 256 would not make 128 workgroups (12 heads of 64, 1024 keys: 10.6 / 12.4; 8 of 128, 4096 keys: 13.4 / 14.7).
+    int64_t share = fth::ceil_div(most, units > 0 && units < 256 ? 256 / units : 1);
+    const int64_t least = units * fth::ceil_div(most, 256) <= 128 ? 128 : 256;
+    share = share < least ? least : share > 2048 ? 2048 : share;
+    if (p.tiles && most <= 512) share = most;
+    p.share = (int)(fth::ceil_div(share > 0 ? share : 1, step) * step);
     p.nsplit = (int)fth::ceil_div(most, p.share);
     if (p.nsplit < 1) p.nsplit = 1;
     p.pitch = (int)fth::ceil_div(c.head_dim, 4) * 4;
+    // Nontemporal loads for what the 256 MB last-level cache cannot hold until the next call, if sequences are half of max_len on
+    // average, and that is read once (us, with / without: one sequence of 131071, bf16 87 / 99, fp32 180 / 196; 64 of up to 8191,
+    // bf16 217 / 229; 16 of up to 3967, four queries, f16, 260 MB 38.5 / 36.3, fp32, 520 MB 79 / 72).
+    p.nt = row_tiles == 1 && 2.0 * (double)c.num_seqs * (double)most * (double)c.kv_heads * (double)c.head_dim * (c.dtype == FTH_DTYPE_F32 ? 4 : 2) > 500.0 * (1 << 20);
     return p;
 }
 
@@ -477,14 +696,16 @@ template <typename T> int32_t launch(PagedArgs &a, const Plan &pl, bool tiles, h
         const int64_t grid = a.c.num_seqs * a.c.kv_heads * a.row_tiles * a.nsplit;
         FTH_ARG(grid <= 2147483647LL, "paged_sdpa: too many workgroups for one launch");
         const dim3 blocks((unsigned)grid), threads(64 * kWaves);
+        const bool nt = pl.nt;
+        auto go = [&](auto kernel) { kernel<<<blocks, threads, 0, st>>>(a); };
         switch (a.c.head_dim) {
-            case 64: paged_sdpa_tiles_kernel<T, 64, true><<<blocks, threads, 0, st>>>(a); break;
-            case 128: paged_sdpa_tiles_kernel<T, 128, true><<<blocks, threads, 0, st>>>(a); break;
-            case 256: paged_sdpa_tiles_kernel<T, 256, true><<<blocks, threads, 0, st>>>(a); break;
+            case 64: go(nt ? paged_sdpa_tiles_kernel<T, 64, true, true> : paged_sdpa_tiles_kernel<T, 64, true, false>); break;
+            case 128: go(nt ? paged_sdpa_tiles_kernel<T, 128, true, true> : paged_sdpa_tiles_kernel<T, 128, true, false>); break;
+            case 256: go(nt ? paged_sdpa_tiles_kernel<T, 256, true, true> : paged_sdpa_tiles_kernel<T, 256, true, false>); break;
             default:
-                if (a.c.head_dim < 64) paged_sdpa_tiles_kernel<T, 64, false><<<blocks, threads, 0, st>>>(a);
-                else if (a.c.head_dim < 128) paged_sdpa_tiles_kernel<T, 128, false><<<blocks, threads, 0, st>>>(a);
-                else paged_sdpa_tiles_kernel<T, 256, false><<<blocks, threads, 0, st>>>(a);
+                if (a.c.head_dim < 64) go(paged_sdpa_tiles_kernel<T, 64, false, false>);
+                else if (a.c.head_dim < 128) go(paged_sdpa_tiles_kernel<T, 128, false, false>);
+                else go(paged_sdpa_tiles_kernel<T, 256, false, false>);
         }
     } else {
         FTH_ARG(pl.rows * a.nsplit <= 2147483647LL, "paged_sdpa: too many rows for one launch");
@@ -492,7 +713,14 @@ template <typename T> int32_t launch(PagedArgs &a, const Plan &pl, bool tiles, h
     }
     FTH_CHECK_LAUNCH("paged_sdpa");
     if (a.nsplit > 1) {
-        paged_sdpa_join_kernel<<<dim3((unsigned)pl.rows), dim3(64), 0, st>>>(a);
+        const int64_t items = pl.rows * (a.pitch / 4);  // at most 2^24 rows of 64 groups
+        // (us, 1 / 4 / 16 / 64 lanes: 2048 rows of up to 16 shares 5.9 / 5.1 / 11.8 / 41; 32 rows of 256 shares 44 / 15 / 9.6 / 6.3)
+        const int lanes = a.nsplit <= 4 ? 1 : a.nsplit <= 16 ? 4 : a.nsplit <= 64 ? 16 : 64;
+        const dim3 blocks((unsigned)fth::ceil_div(items * lanes, 256));
+        if (lanes == 1) paged_sdpa_join_kernel<1><<<blocks, dim3(256), 0, st>>>(a, items);
+        else if (lanes == 4) paged_sdpa_join_kernel<4><<<blocks, dim3(256), 0, st>>>(a, items);
+        else if (lanes == 16) paged_sdpa_join_kernel<16><<<blocks, dim3(256), 0, st>>>(a, items);
+        else paged_sdpa_join_kernel<64><<<blocks, dim3(256), 0, st>>>(a, items);
         FTH_CHECK_LAUNCH("paged_sdpa_join");
     }
     return FTH_OK;

@@ -238,3 +238,25 @@ def test_a_workspace_that_is_too_small_is_refused(hip):
     assert fn(*args(ws.ptr, need)) == 0
     hip.synchronize()
     assert np.all(out.to_host() != 7.0)
+
+
+@pytest.mark.parametrize("dtype,std", [("f16", 2e-5), ("f16", 6e-7), ("f16", 6e3), ("bf16", 1e-39), ("bf16", 1e30), ("f32", 1e-39), ("f32", 1e15)])
+def test_small_and_large_caches(hip, dtype, std):
+    """Keys and values among the subnormal numbers of their type, and near its ends: scores of a few units by the scale."""
+    for q_std in (1.0, 1e-5, 1e5):
+        p = Paged(21, [130, 5], 2, 64, 16, dtype, std=std)
+        q, scale = queries(p, 4, 1, std=q_std), np.float32(min(1e37, 0.3 / (std * q_std)))
+        got, ref = run(hip, p, q, scale), attention(q, p.k, p.v, scale, p.lens)
+        # results below 2^-126 may be rounded to multiples of 2^-149 at each of 130 steps, or flushed
+        assert np.max(np.abs(got - ref)) <= TOL_GEMM_F32 * np.max(np.abs(ref)) + 2.0 ** -126, (q_std,)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_queries_that_are_not_finite(hip, dtype):
+    """A query row with NaN or an infinity gives NaN, as the formula does; the rows beside it do not see it."""
+    p = Paged(22, [200, 3], 2, 64, 16, dtype)
+    q = queries(p, 8, 2)
+    q[0, 0, 1, 5], q[0, 1, 6, 0], q[1, 1, 3, 63] = np.nan, np.inf, -np.inf
+    got, ref = run(hip, p, q, 0.125), attention(q, p.k, p.v, 0.125, p.lens)
+    assert np.array_equal(np.isnan(got), np.isnan(ref)) and np.isnan(ref).sum() == 3 * 64
+    assert rel_err(got[~np.isnan(ref)], ref[~np.isnan(ref)]) <= TOL_GEMM_F32
