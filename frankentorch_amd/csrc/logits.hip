@@ -2,14 +2,27 @@
 //
 // A workgroup owns one row's logits over a stretch of the vocabulary. It counts the history's tokens that fall into its stretch
 // in LDS (integer atomics: the counts do not depend on their order), then makes one pass over the logits. Each workgroup of a row
-// scans the whole history, which comes from L2; in return nothing is handed from one launch to another.
+// scans the whole history, which comes from L2; in return nothing is handed from one launch to another. HBM-bound: every logit
+// is read and written once, a row's own bias read once.
+//   * A scan costs about eight instructions an id and is repeated by every stretch of the row: with 2048 steps of 4096 logits and
+//     more, a stretch is two of them (200 rows of 131071, up to 8000 tokens before: 67 -> 60 us; four steps leave too few
+//     workgroups: 64). The loads of a step go out before the one before it is finished, those of the first before the barrier.
+//   * What a thread loads and stores is 128 bits at 4-byte alignment, since rows of an odd vocabulary start anywhere (65 us where
+//     131072 takes 61).
+//   * A bias of the row's own is loaded past the caches, where it would push out logits (64.5 -> 60 us); one for all rows is not
+//     (64 rows of 50257: 9.9 us, past the caches 11.5). Outputs over 8 MiB are stored past them (200 rows 72 -> 60 us; 64 rows
+//     11.1 -> 9.5, and the argmax after it as fast as before in all: 27 us; 8 rows lose 1.2 of 22 us with the argmax).
+//
+// Measured: 200 rows of 131071, a bias each, a mask, up to 8000 tokens before 60 us (318 MB, 5.3 TB/s; one entry a thread and
+// stretches of 4096: 143); 64 rows of 50257, one bias, a mask 9.5 us (27 MB; 17.3); one row 4.6 us.
+
+#include <type_traits>
 
 #include "paged.hpp"
 
 namespace {
 
-constexpr int kBlock = 256, kStretch = 4096;
-constexpr uint32_t kGiven = 0x80000000u;  // bit 31: among the given tokens; below it: times generated
+constexpr int kThreads = 512, kVecs = 2, kStep = kThreads * kVecs * 4, kMostSteps = 2;
 
 struct LogitsArgs {
     fth_logits_desc d;
@@ -18,54 +31,124 @@ struct LogitsArgs {
     const uint32_t *mask;
     float *out;
     int64_t *bad;
-    int stretches;
+    int stretches, steps;  // stretches of a row, steps of a stretch
 };
 
-__global__ __launch_bounds__(kBlock) void logits_process_kernel(const LogitsArgs p) {
-    __shared__ uint32_t seen[kStretch];
-    const int64_t r = blockIdx.x / p.stretches;
-    const int64_t v0 = (int64_t)(blockIdx.x % p.stretches) * kStretch;
-    const int n = (int)(p.d.vocab - v0 < kStretch ? p.d.vocab - v0 : kStretch);
-    float rep = 1.f, freq = 0.f, pres = 0.f;
-    if (p.history) {
-        for (int i = threadIdx.x; i < n; i += kBlock) seen[i] = 0;
-        __syncthreads();
-        const int len = p.history_len[r], prompt = p.prompt_len[r];
-        bool bad = len < 0 || len > p.d.history_stride || prompt < 0 || prompt > len;
-        for (int i = threadIdx.x; i < (bad ? 0 : len); i += kBlock) {
-            const int64_t id = p.history[r * p.d.history_stride + i];
-            if (id < 0 || id >= p.d.vocab) bad = true;
-            else if (id >= v0 && id < v0 + n) {
-                if (i < prompt) atomicOr(&seen[id - v0], kGiven);
-                else atomicAdd(&seen[id - v0], 1u);
-            }
-        }
-        if (__syncthreads_or(bad)) {
-            if (threadIdx.x == 0 && v0 == 0) fth::report_bad_entry(p.bad, r);
-            return;
-        }
-        if (p.repetition) rep = p.repetition[r];
-        if (p.frequency) freq = p.frequency[r];
-        if (p.presence) pres = p.presence[r];
-    }
+using F4u = float __attribute__((ext_vector_type(4), aligned(4)));  // rows start anywhere
+using I4u = int32_t __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr uint32_t kGiven = 0x80000000u;  // bit 31: among the given tokens; below it: times generated
+
+struct Step {  // one step's inputs of a thread
+    F4u z[kVecs], b[kVecs];
+    uint32_t bits[kVecs];
+};
+
+// NTB: a bias that no other row reads; NTS: more output than the caches hold.
+template <bool NTB, bool NTS> __global__ __launch_bounds__(kThreads) void logits_process_kernel(const LogitsArgs p) {
+    __shared__ __attribute__((aligned(16))) uint32_t seen[kMostSteps * kStep];
+    const int64_t r = blockIdx.x / (unsigned)p.stretches;
+    const int64_t v0 = (int64_t)(blockIdx.x % (unsigned)p.stretches) * (p.steps * kStep);
+    const int n = (int)(p.d.vocab - v0 < p.steps * kStep ? p.d.vocab - v0 : p.steps * kStep);
     const float *x = p.logits + r * p.d.logits_stride + v0, *bias = p.bias ? p.bias + r * p.d.bias_stride + v0 : nullptr;
     const uint32_t *mask = p.mask ? p.mask + r * p.d.mask_stride + v0 / 32 : nullptr;
-    float *y = p.out + r * p.d.out_stride + v0;
-    for (int i = threadIdx.x; i < n; i += kBlock) {
-        float z = x[i];
-        if (p.history) {
-            const uint32_t c = seen[i];
-            if (c) {
-                if (p.repetition) z = z > 0.f ? z / rep : z * rep;
-                if (c & ~kGiven) {
-                    if (p.frequency) z = z - freq * (float)(c & ~kGiven);
-                    if (p.presence) z = z - pres;
+    auto place = [&](int step, int j) { return step * kStep + (j * kThreads + (int)threadIdx.x) * 4; };
+    auto load4 = [&](const float *src, int i, auto nt) __attribute__((always_inline)) {
+        F4u v = {0.f, 0.f, 0.f, 0.f};
+        if (i + 4 <= n) v = nt ? __builtin_nontemporal_load(reinterpret_cast<const F4u *>(src + i)) : *reinterpret_cast<const F4u *>(src + i);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (i + e < n) v[e] = src[i + e];
+        return v;
+    };
+    auto load = [&](int step) __attribute__((always_inline)) {
+        Step s;
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) {
+            const int i = place(step, j);
+            s.z[j] = load4(x, i, std::false_type());
+            if (bias) s.b[j] = load4(bias, i, std::bool_constant<NTB>());
+            s.bits[j] = mask && i < n ? mask[i / 32] >> (i % 32) : 15u;
+        }
+        return s;
+    };
+
+    Step now;
+    float rep = 1.f, freq = 0.f, pres = 0.f;
+    bool counted = false;
+    if (p.history) {
+        const int len = p.history_len[r], prompt = p.prompt_len[r];
+        const int32_t *history = p.history + r * p.d.history_stride;
+        const bool bad = len < 0 || len > p.d.history_stride || prompt < 0 || prompt > len;
+        const int count = bad ? 0 : len;
+        uint32_t largest = 0;  // as unsigned numbers, negative ids are beyond every vocabulary
+        counted = count > 0;
+        if (counted) {
+            for (int i = (int)threadIdx.x * 4; i < n; i += kThreads * 4) *reinterpret_cast<uint4 *>(&seen[i]) = make_uint4(0, 0, 0, 0);
+            __syncthreads();
+            auto note = [&](int32_t id, int i) __attribute__((always_inline)) {
+                largest = (uint32_t)id > largest ? (uint32_t)id : largest;
+                const uint32_t at = (uint32_t)id - (uint32_t)v0;
+                if (at < (uint32_t)n) {
+                    if (i < prompt) atomicOr(&seen[at], kGiven);
+                    else atomicAdd(&seen[at], 1u);
+                }
+            };
+            for (int i = (int)threadIdx.x * 4; i < count; i += kThreads * 4) {
+                if (i + 4 <= count) {
+                    const I4u ids = *reinterpret_cast<const I4u *>(history + i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) note(ids[e], i + e);
+                } else {
+                    for (int e = i; e < count; ++e) note(history[e], e);
                 }
             }
         }
-        if (bias) z = z + bias[i];
-        if (mask && !((mask[i / 32] >> (i % 32)) & 1u)) z = -__builtin_inff();
-        y[i] = z;
+        now = load(0);
+        if (p.repetition) rep = p.repetition[r];
+        if (p.frequency) freq = p.frequency[r];
+        if (p.presence) pres = p.presence[r];
+        if (__syncthreads_or(bad || (counted && largest >= (uint32_t)p.d.vocab))) {
+            if (threadIdx.x == 0 && v0 == 0) fth::report_bad_entry(p.bad, r);
+            return;
+        }
+    } else {
+        now = load(0);
+    }
+    float *y = p.out + r * p.d.out_stride + v0;
+    auto finish = [&](float t, uint32_t c, float b, bool allowed) __attribute__((always_inline)) {
+        if (c) {
+            if (p.repetition) t = t > 0.f ? t / rep : t * rep;
+            if (c & ~kGiven) {
+                if (p.frequency) t = t - freq * (float)(c & ~kGiven);
+                if (p.presence) t = t - pres;
+            }
+        }
+        if (bias) t = t + b;
+        return allowed ? t : -__builtin_inff();
+    };
+    for (int step = 0; step < p.steps && step * kStep < n; ++step) {
+        Step next;
+        if (step + 1 < p.steps) next = load(step + 1);
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) {
+            const int i = place(step, j);
+            if (i >= n) break;
+            const uint4 counts = counted ? *reinterpret_cast<const uint4 *>(&seen[i]) : make_uint4(0, 0, 0, 0);
+            const uint32_t c[4] = {counts.x, counts.y, counts.z, counts.w};
+            F4u t;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[e] = finish(now.z[j][e], c[e], now.b[j][e], (now.bits[j] >> e) & 1u);
+            if (i + 4 <= n) {
+                if constexpr (NTS) __builtin_nontemporal_store(t, reinterpret_cast<F4u *>(y + i));
+                else *reinterpret_cast<F4u *>(y + i) = t;
+            } else
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (i + e < n) y[i + e] = t[e];
+        }
+        now = next;
     }
 }
 
@@ -100,11 +183,16 @@ extern "C" int32_t fth_dev_logits_process_f32(const fth_logits_desc *d, const fl
     a.logits = logits;
     a.history = repetition || frequency || presence ? history : nullptr;
     a.history_len = history_len; a.prompt_len = prompt_len;
-    a.repetition = repetition; a.frequency = frequency; a.presence = presence;
+    a.repetition = a.history ? repetition : nullptr; a.frequency = a.history ? frequency : nullptr; a.presence = a.history ? presence : nullptr;
     a.bias = bias; a.mask = mask; a.out = out; a.bad = bad_index;
-    a.stretches = (int)fth::ceil_div(d->vocab, kStretch);
+    const int64_t steps = fth::ceil_div(d->vocab, kStep);
+    a.steps = a.history && d->rows * steps >= 2048 ? kMostSteps : 1;
+    a.stretches = (int)fth::ceil_div(steps, a.steps);
     FTH_ARG(d->rows * a.stretches <= 2147483647LL, "logits_process: too many rows for one launch");
-    logits_process_kernel<<<dim3((unsigned)(d->rows * a.stretches)), dim3(kBlock), 0, st>>>(a);
+    const bool ntb = bias && d->bias_stride != 0, nts = d->rows * d->vocab > (2 << 20);
+    auto go = [&](auto kernel) { kernel<<<dim3((unsigned)(d->rows * a.stretches)), dim3(kThreads), 0, st>>>(a); };
+    if (ntb) go(nts ? logits_process_kernel<true, true> : logits_process_kernel<true, false>);
+    else go(nts ? logits_process_kernel<false, true> : logits_process_kernel<false, false>);
     FTH_CHECK_LAUNCH("logits_process");
     return FTH_OK;
 }

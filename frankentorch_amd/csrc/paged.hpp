@@ -41,6 +41,17 @@ inline int32_t check_paged_cache(const fth_paged_cache *c, const char *who, int6
     return FTH_OK;
 }
 
+// n / d for 0 <= n < 2^31 by a multiplication: shift = ceil(log2 d), mul = ceil(2^(32 + shift) / d) - 2^32.
+struct Divisor {
+    uint32_t mul = 1, shift = 0;
+    Divisor() = default;
+    explicit Divisor(uint32_t d) {
+        while (((uint64_t)1 << shift) < d) ++shift;
+        mul = (uint32_t)(((((uint64_t)1 << shift) - d) << 32) / d + 1);
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (uint32_t)(((uint64_t)__umulhi(n, mul) + n) >> shift); }
+};
+
 inline bool stride_in_range(int64_t s) { return s >= 0 && s <= ((int64_t)1 << 40); }
 
 }  // namespace fth

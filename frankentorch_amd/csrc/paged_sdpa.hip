@@ -48,18 +48,8 @@ struct PagedArgs {
     float scale2;    // scale * log2(e)
     int64_t most;    // the longest valid sequence
     int group, row_tiles, nsplit, share, pitch;
-    uint32_t page_mul, page_shift;  // n / page_size, see Plan
+    fth::Divisor by_page;
 };
-
-// n / d for 0 <= n < 2^31 by a multiplication: shift = ceil(log2 d), mul = ceil(2^(32 + shift) / d) - 2^32.
-struct Divisor {
-    uint32_t mul, shift;
-    explicit Divisor(uint32_t d) : shift(0) {
-        while (((uint64_t)1 << shift) < d) ++shift;
-        mul = (uint32_t)(((((uint64_t)1 << shift) - d) << 32) / d + 1);
-    }
-};
-__device__ __forceinline__ uint32_t divide(uint32_t n, uint32_t mul, uint32_t shift) { return (uint32_t)(((uint64_t)__umulhi(n, mul) + n) >> shift); }
 
 struct MaxOp { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
 struct AddOp { __device__ float operator()(float a, float b) const { return a + b; } };
@@ -282,7 +272,7 @@ template <typename T, int DP, bool FULL, bool NT> __global__ __launch_bounds__(6
     // The 16 keys number t16 (of the sequence): the page and the first row in it; half tiles past the end repeat the last one.
     auto page_of = [&](int t16) __attribute__((always_inline)) {
         t16 = t16 < last16 ? t16 : last16;
-        const int index = (int)divide((uint32_t)t16 << 4, p.page_mul, p.page_shift);
+        const int index = (int)p.by_page((uint32_t)t16 << 4);
         return make_int2(table[index], (t16 << 4) - index * (int)p.c.page_size);
     };
     auto offset_of = [&](int2 page) __attribute__((always_inline)) {
@@ -760,9 +750,7 @@ int32_t fth_dev_paged_sdpa_f32(const fth_paged_cache *c, const fth_paged_sdpa_de
     a.group = (int)(d->q_heads / c->kv_heads);
     a.row_tiles = (int)fth::ceil_div((int64_t)a.group * d->new_tokens, 16);
     a.nsplit = pl.nsplit; a.share = pl.share; a.pitch = pl.pitch;
-    const Divisor by_page((uint32_t)c->page_size);
-    a.page_mul = by_page.mul;
-    a.page_shift = by_page.shift;
+    a.by_page = fth::Divisor((uint32_t)c->page_size);
     const bool tiles = pl.tiles && (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15u) == 0;
     switch (c->dtype) {
         case FTH_DTYPE_F32: return launch<float>(a, pl, tiles, st);
