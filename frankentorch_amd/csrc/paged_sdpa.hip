@@ -14,7 +14,8 @@
 //   * The loads of the next tile's K go out when the scores have consumed this one's, those of V after the outputs have, with
 //     nothing conditional in between: the waits are then for K or V alone, never for both.
 // Pages: with a page size that is a multiple of 16 each half tile lies in one page, whose number is a scalar load one tile
-// ahead. Other page sizes, and strides and alignments that 128-bit loads cannot take, go to a kernel of one wavefront a row.
+// ahead; with other sizes every lane looks up a row. Strides, head sizes and alignments that 128-bit loads cannot take go to a
+// kernel of one wavefront a row.
 //
 // Measured: 64 sequences of 1024 to 8191 keys, 32 query heads on 8 K/V heads of 128, bf16 (1.22 GB): 7.6 ms on one wavefront a
 // row, 283 us with both products on fp32 units, 235 with the scores on 16-bit ones (MFMA-busy 0.31, wavefronts waiting to
@@ -108,9 +109,9 @@ template <typename T> __global__ __launch_bounds__(64) void paged_sdpa_rows_kern
             const int64_t off = page < 0 ? -1 : (int64_t)page * p.c.page_stride + (int64_t)(key % page_size) * p.c.row_stride;
             at[lane] = off;
             if (page >= 0 && lane < n) {
-                float dot = 0.f;
-                for (int c = 0; c < hd; ++c) dot = __builtin_fmaf(qs[c], fth::to_f32(K[off + c]), dot);
-                x = dot * p.scale2;
+                float dot[4] = {0.f, 0.f, 0.f, 0.f};  // short chains of roundings
+                for (int c = 0; c < hd; ++c) dot[c & 3] = __builtin_fmaf(qs[c], fth::to_f32(K[off + c]), dot[c & 3]);
+                x = ((dot[0] + dot[1]) + (dot[2] + dot[3])) * p.scale2;
             }
         }
         const float m_new = fmaxf(m, wave_reduce(x, MaxOp()));
@@ -123,10 +124,10 @@ template <typename T> __global__ __launch_bounds__(64) void paged_sdpa_rows_kern
         for (int j = 0; j < 4; ++j) {
             const int c = lane + 64 * j;
             if (c >= hd) break;
-            float acc = o[j] * alpha;
+            float acc = 0.f;
             for (int r = 0; r < n; ++r)
                 if (at[r] >= 0) acc = __builtin_fmaf(ps[r], fth::to_f32(V[at[r] + c]), acc);
-            o[j] = acc;
+            o[j] = o[j] * alpha + acc;
         }
         __syncthreads();
     }
@@ -219,8 +220,9 @@ template <typename T, int DP> struct TileShape {
     static constexpr int kLds = kWaves * 16 * (DP + 4);
 };
 
-// FULL: head_dim == DP; otherwise what lies past head_dim counts as zero. NT: K and V leave no trace in the caches.
-template <typename T, int DP, bool FULL, bool NT> __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void paged_sdpa_tiles_kernel(const PagedArgs p) {
+// FULL: head_dim == DP; otherwise what lies past head_dim counts as zero. NT: K and V leave no trace in the caches. ANY: pages of any
+// size: every lane looks its K row up, and V rows are found through the lane that has the same key.
+template <typename T, int DP, bool FULL, bool NT, bool ANY> __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void paged_sdpa_tiles_kernel(const PagedArgs p) {
     using S = TileShape<T, DP>;
     constexpr int CH = S::CH, NK = S::NK, NE = S::NE, CV = S::CV, NV = S::NV, kParts = Parts<T>::kParts;
     __shared__ __attribute__((aligned(16))) float lds_o[S::kLds];
@@ -269,23 +271,36 @@ template <typename T, int DP, bool FULL, bool NT> __global__ __launch_bounds__(6
             q[i][e] = FULL || c < hd ? qr[c] : 0.f;
         }
 
-    // The 16 keys number t16 (of the sequence): the page and the first row in it; half tiles past the end repeat the last one.
+    // The 16 keys number t16 (of the sequence): the page and the row in it of the first (ANY: of this lane's); half tiles past the
+    // end repeat the last one (ANY: keys past the end repeat the last one).
     auto page_of = [&](int t16) __attribute__((always_inline)) {
-        t16 = t16 < last16 ? t16 : last16;
-        const int index = (int)p.by_page((uint32_t)t16 << 4);
-        return make_int2(table[index], (t16 << 4) - index * (int)p.c.page_size);
+        int key;
+        if constexpr (ANY) {
+            key = (t16 << 4) + lr;
+            key = key < len ? key : len - 1;
+        } else {
+            key = (t16 < last16 ? t16 : last16) << 4;
+        }
+        const int index = (int)p.by_page((uint32_t)key);
+        return make_int2(table[index], key - index * (int)p.c.page_size);
     };
     auto offset_of = [&](int2 page) __attribute__((always_inline)) {
         const bool there = page.x >= 0 && page.x < num_pages;
         bad = bad || !there;
         const int64_t at = (int64_t)(there ? page.x : 0) * p.c.page_stride + (int64_t)page.y * rs;
+        if constexpr (ANY) return at;
         return (int64_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)at);  // one for all lanes
     };
+    // the offset of row `row` of a half tile, from what offset_of gave
+    auto row_offset = [&](int64_t at, int row) __attribute__((always_inline)) {
+        if constexpr (ANY) return (int64_t)__shfl((int)(at >> 32), row) << 32 | (uint32_t)__shfl((int)at, row);
+        return at + row * rs;
+    };
     U4 kf[2][NK], vf[2][4][NV];
-    const uint32_t k_lane = (uint32_t)((lr * rs + g * CH) * (int)sizeof(T));
+    const uint32_t k_lane = (uint32_t)(((ANY ? 0 : lr * rs) + g * CH) * (int)sizeof(T));
     uint32_t v_lane[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v_lane[r] = (uint32_t)(((4 * g + r) * rs + lr * CV) * (int)sizeof(T));
+    for (int r = 0; r < 4; ++r) v_lane[r] = (uint32_t)(((ANY ? 0 : (4 * g + r) * rs) + lr * CV) * (int)sizeof(T));
     auto load_k = [&](const int64_t (&off)[2]) __attribute__((always_inline)) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -302,7 +317,8 @@ template <typename T, int DP, bool FULL, bool NT> __global__ __launch_bounds__(6
         for (int s = 0; s < 2; ++s) {
             const char *base = reinterpret_cast<const char *>(V + off[s]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < 4; ++r) {
+                if constexpr (ANY) base = reinterpret_cast<const char *>(V + row_offset(off[s], 4 * g + r));
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
                     const char *src = base + v_lane[r] + 16 * CV * (int)sizeof(T) * i;
@@ -317,6 +333,7 @@ template <typename T, int DP, bool FULL, bool NT> __global__ __launch_bounds__(6
                         }
                     }
                 }
+            }
         }
     };
 
@@ -414,8 +431,8 @@ template <typename T, int DP, bool FULL, bool NT> __global__ __launch_bounds__(6
 #pragma unroll
                     for (int y = 1; y < 8; ++y) x = j == y ? sc[y >> 2][y & 3] : x;
                     const int row = 16 * (j >> 2) + 4 * g + (j & 3);
+                    const T *kr = K + row_offset(off[j >> 2], row & 15);
                     if (finite && !(fabsf(x) < __builtin_inff()) && key0 + row < limit) {
-                        const T *kr = K + off[j >> 2] + (4 * g + (j & 3)) * rs;
                         float dot = 0.f;
                         for (int c = 0; c < hd; ++c) dot = __builtin_fmaf(qr[c], fth::to_f32(kr[c]), dot);
                         x = dot * p.scale2;
@@ -535,6 +552,7 @@ template <typename T, int DP, bool FULL, bool NT> __global__ __launch_bounds__(6
     // join the wavefronts: MFMA row 4 g + r of column tile e is output column ((e / CV) * 16 + 4 g + r) * CV + e % CV
     constexpr int P = DP + 4;
     const float l_wave = rows_reduce(l_run, AddOp());
+    if constexpr (ANY) bad = __any(bad);
     if (g == 0) {
         lds_ml[(wave * 16 + lr) * 2] = m_run - weight;  // weights times 2^k relative to m are weights relative to m - k
         lds_ml[(wave * 16 + lr) * 2 + 1] = bad ? __builtin_nanf("") : l_wave;
@@ -630,7 +648,7 @@ template <int SL> __global__ __launch_bounds__(256) void paged_sdpa_join_kernel(
 
 // How a call is cut: the same for its workspace and its launch.
 struct Plan {
-    bool tiles;   // pages, head size and strides that the 128-bit loads take (the pointers' alignment is looked at later)
+    bool tiles;   // head size and strides that the 128-bit loads take (the pointers' alignment is looked at later)
     bool nt;      // loads that leave no trace in the caches
     int nsplit, share, pitch;
     int64_t rows;
@@ -640,7 +658,7 @@ Plan plan(const fth_paged_cache &c, const fth_paged_sdpa_desc &d) {
     Plan p;
     const int64_t ch = c.dtype == FTH_DTYPE_F32 ? 4 : 8;
     p.rows = c.num_seqs * d.new_tokens * d.q_heads;
-    p.tiles = c.page_size % 16 == 0 && c.head_dim % ch == 0 && c.row_stride % ch == 0 && c.head_stride % ch == 0 && c.page_stride % ch == 0 &&
+    p.tiles = c.head_dim % ch == 0 && c.row_stride % ch == 0 && c.head_stride % ch == 0 && c.page_stride % ch == 0 &&
               c.row_stride <= ((int64_t)1 << 24) && c.num_pages > 0;
     const int64_t most = c.max_pages * c.page_size < d.max_len ? c.max_pages * c.page_size : d.max_len;
     const int64_t row_tiles = fth::ceil_div(d.q_heads / c.kv_heads * d.new_tokens, 16);
@@ -688,14 +706,18 @@ template <typename T> int32_t launch(PagedArgs &a, const Plan &pl, bool tiles, h
         const dim3 blocks((unsigned)grid), threads(64 * kWaves);
         const bool nt = pl.nt;
         auto go = [&](auto kernel) { kernel<<<blocks, threads, 0, st>>>(a); };
-        switch (a.c.head_dim) {
-            case 64: go(nt ? paged_sdpa_tiles_kernel<T, 64, true, true> : paged_sdpa_tiles_kernel<T, 64, true, false>); break;
-            case 128: go(nt ? paged_sdpa_tiles_kernel<T, 128, true, true> : paged_sdpa_tiles_kernel<T, 128, true, false>); break;
-            case 256: go(nt ? paged_sdpa_tiles_kernel<T, 256, true, true> : paged_sdpa_tiles_kernel<T, 256, true, false>); break;
+        if (a.c.page_size % 16 != 0) {
+            if (a.c.head_dim <= 64) go(paged_sdpa_tiles_kernel<T, 64, false, false, true>);
+            else if (a.c.head_dim <= 128) go(paged_sdpa_tiles_kernel<T, 128, false, false, true>);
+            else go(paged_sdpa_tiles_kernel<T, 256, false, false, true>);
+        } else switch (a.c.head_dim) {
+            case 64: go(nt ? paged_sdpa_tiles_kernel<T, 64, true, true, false> : paged_sdpa_tiles_kernel<T, 64, true, false, false>); break;
+            case 128: go(nt ? paged_sdpa_tiles_kernel<T, 128, true, true, false> : paged_sdpa_tiles_kernel<T, 128, true, false, false>); break;
+            case 256: go(nt ? paged_sdpa_tiles_kernel<T, 256, true, true, false> : paged_sdpa_tiles_kernel<T, 256, true, false, false>); break;
             default:
-                if (a.c.head_dim < 64) go(paged_sdpa_tiles_kernel<T, 64, false, false>);
-                else if (a.c.head_dim < 128) go(paged_sdpa_tiles_kernel<T, 128, false, false>);
-                else go(paged_sdpa_tiles_kernel<T, 256, false, false>);
+                if (a.c.head_dim < 64) go(paged_sdpa_tiles_kernel<T, 64, false, false, false>);
+                else if (a.c.head_dim < 128) go(paged_sdpa_tiles_kernel<T, 128, false, false, false>);
+                else go(paged_sdpa_tiles_kernel<T, 256, false, false, false>);
         }
     } else {
         FTH_ARG(pl.rows * a.nsplit <= 2147483647LL, "paged_sdpa: too many rows for one launch");
