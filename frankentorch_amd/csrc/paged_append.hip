@@ -27,8 +27,22 @@ struct AppendArgs {
     void *k_cache, *v_cache;
     int64_t *bad;
     fth::Divisor by_page;
-    int pair_units, k_units, units;  // per head: of a rotated one, pairs first; of the V rows; per token
+    int kv_heads;           // 0: queries only
+    int pair_units, units;  // of a rotated head, pairs first; of a token
 };
+
+// Where token t goes in the cache (nowhere without keys); false when there is no such place.
+__device__ __forceinline__ bool find_slot(const AppendArgs &p, int64_t t, int pos, int64_t *slot) {
+    if (pos < 0 || (p.d.rotary_dim > 0 && pos >= p.d.max_pos)) return false;
+    if (p.kv_heads == 0) return true;
+    const int seq = p.seq_ids[t];
+    if (seq < 0 || seq >= p.c.num_seqs || pos >= p.c.max_pages * p.c.page_size) return false;
+    const int index = (int)p.by_page((uint32_t)pos);
+    const int page = p.table[(int64_t)seq * p.c.table_stride + index];
+    if (page < 0 || page >= p.c.num_pages) return false;
+    *slot = (int64_t)page * p.c.page_stride + (int64_t)(pos - index * (int)p.c.page_size) * p.c.row_stride;
+    return true;
+}
 
 __device__ __forceinline__ void store_as(float *p, float x) { *p = x; }
 __device__ __forceinline__ void store_as(fth::f16 *p, float x) { *p = (fth::f16)x; }
@@ -51,16 +65,12 @@ template <typename T> __global__ __launch_bounds__(kBlock) void paged_append_ker
     const int part = (int)(blockIdx.x % blocks_per_token);
     const int pos = p.positions[t];
     if (pos == -1) return;
-    const int seq = p.seq_ids[t], page_size = (int)p.c.page_size;
-    bool ok = seq >= 0 && seq < p.c.num_seqs && pos >= 0 && pos < p.c.max_pages * p.c.page_size && (p.d.rotary_dim == 0 || pos < p.d.max_pos);
-    int page = -1;
-    if (ok) page = p.table[(int64_t)seq * p.c.table_stride + pos / page_size];
-    if (!ok || page < 0 || page >= p.c.num_pages) {
+    int64_t slot = 0;
+    if (!find_slot(p, t, pos, &slot)) {
         if (part == 0 && threadIdx.x == 0) fth::report_bad_entry(p.bad, t);
         return;
     }
-    const int64_t slot = (int64_t)page * p.c.page_stride + (int64_t)(pos % page_size) * p.c.row_stride;
-    const int pairs = (int)p.d.rotary_dim / 2, hd = (int)p.c.head_dim, hq = (int)p.d.q_heads, hkv = (int)p.c.kv_heads;
+    const int pairs = (int)p.d.rotary_dim / 2, hd = (int)p.c.head_dim, hq = (int)p.d.q_heads, hkv = p.kv_heads;
     const float *c = p.cosines + (int64_t)pos * pairs, *s = p.sines + (int64_t)pos * pairs;
     const bool inter = p.d.interleaved != 0;
     const int rotated = (hq + hkv) * p.pair_units;
@@ -108,22 +118,15 @@ template <typename T> __global__ __launch_bounds__(kBlock) void paged_append_vec
     const int part = (int)(blockIdx.x % (unsigned)blocks_per_token);
     const int pos = p.positions[t];
     if (pos == -1) return;
-    const int seq = p.seq_ids[t], hd = (int)p.c.head_dim, per_row = hd / 8, slots = kBlock / per_row;
-    bool ok = seq >= 0 && seq < p.c.num_seqs && pos >= 0 && pos < p.c.max_pages * p.c.page_size && (p.d.rotary_dim == 0 || pos < p.d.max_pos);
-    int page = -1, row = 0;
-    if (ok) {
-        const int index = (int)p.by_page((uint32_t)pos);
-        row = pos - index * (int)p.c.page_size;
-        page = p.table[(int64_t)seq * p.c.table_stride + index];
-    }
-    if (!ok || page < 0 || page >= p.c.num_pages) {
+    const int hd = (int)p.c.head_dim, per_row = hd / 8, slots = kBlock / per_row;
+    int64_t at = 0;
+    if (!find_slot(p, t, pos, &at)) {
         if (part == 0 && threadIdx.x == 0) fth::report_bad_entry(p.bad, t);
         return;
     }
     const int slot = (int)threadIdx.x / per_row, i = (int)threadIdx.x % per_row;
     if (slot >= slots) return;
-    const int64_t at = (int64_t)page * p.c.page_stride + (int64_t)row * p.c.row_stride;
-    const int rotary = (int)p.d.rotary_dim, hq = (int)p.d.q_heads, hkv = (int)p.c.kv_heads, heads = hq + 2 * hkv;
+    const int rotary = (int)p.d.rotary_dim, hq = (int)p.d.q_heads, hkv = p.kv_heads, heads = hq + 2 * hkv;
     const bool turns = 8 * i < rotary, inter = p.d.interleaved != 0;
     F4 c = {1.f, 1.f, 1.f, 1.f}, s = {0.f, 0.f, 0.f, 0.f};
     if (turns) {
@@ -186,16 +189,17 @@ bool aligned(const void *p, int64_t row_stride, int64_t head_stride, int64_t ele
 // Rows, pairs and strides that 128-bit accesses take.
 template <typename T> bool takes_vectors(const AppendArgs &a) {
     const int64_t ch = 16 / (int64_t)sizeof(T);
-    const bool cache = a.c.head_dim % 8 == 0 && a.d.rotary_dim % 8 == 0 && a.c.page_stride % ch == 0 && aligned(a.k_cache, a.c.row_stride, a.c.head_stride, ch) &&
-                       aligned(a.v_cache, a.c.row_stride, a.c.head_stride, ch);
-    const bool rows = aligned(a.k, a.d.k_row_stride, a.d.k_head_stride, 4) && aligned(a.v, a.d.v_row_stride, a.d.v_head_stride, 4) &&
+    const bool cache = a.kv_heads == 0 || (a.c.page_stride % ch == 0 && aligned(a.k_cache, a.c.row_stride, a.c.head_stride, ch) &&
+                                           aligned(a.v_cache, a.c.row_stride, a.c.head_stride, ch) && aligned(a.k, a.d.k_row_stride, a.d.k_head_stride, 4) &&
+                                           aligned(a.v, a.d.v_row_stride, a.d.v_head_stride, 4));
+    const bool rows = a.c.head_dim % 8 == 0 && a.d.rotary_dim % 8 == 0 &&
                       (a.d.q_heads == 0 || (aligned(a.q, a.d.q_row_stride, a.d.q_head_stride, 4) && aligned(a.q_out, a.d.out_row_stride, a.d.out_head_stride, 4)));
     return cache && rows && (a.d.rotary_dim == 0 || (((uintptr_t)a.cosines | (uintptr_t)a.sines) & 15u) == 0);
 }
 
 template <typename T> int32_t launch(const AppendArgs &a, hipStream_t st) {
     if (takes_vectors<T>(a)) {
-        const int64_t slots = kBlock / (a.c.head_dim / 8), heads = a.d.q_heads + 2 * a.c.kv_heads;
+        const int64_t slots = kBlock / (a.c.head_dim / 8), heads = a.d.q_heads + 2 * a.kv_heads;
         // A workgroup a token and four rows a thread; one row a thread where tokens are few (64 of 48 heads of 128: 4.5 -> 3.7 us).
         const int64_t blocks_per_token = fth::ceil_div(heads, a.d.tokens < 1024 ? slots : slots * kHeads);
         FTH_ARG(a.d.tokens * blocks_per_token <= 2147483647LL, "paged_append: too many tokens for one launch");
@@ -244,7 +248,8 @@ int32_t fth_dev_paged_append_f32(const fth_paged_cache *c, const fth_paged_appen
         FTH_ARG(fth::stride_in_range(x), "paged_append: a stride is negative or over 2^40");
     if (d->q_heads + c->kv_heads > (1 << 20) || d->tokens > 2147483647LL) return fth::set_error(FTH_ERR_SIZE_OVERFLOW, "paged_append: extents overflow");
     if (d->tokens > 0) {
-        FTH_ARG(k && v && seq_ids && positions && (block_table || c->max_pages == 0) && ((k_cache && v_cache) || c->num_pages == 0), "paged_append: NULL operand");
+        FTH_ARG(positions && (k != nullptr) == (v != nullptr) && (k || d->q_heads > 0), "paged_append: NULL operand");
+        FTH_ARG(!k || (seq_ids && (block_table || c->max_pages == 0) && ((k_cache && v_cache) || c->num_pages == 0)), "paged_append: NULL cache, table or sequences");
         FTH_ARG(d->q_heads == 0 || (q && q_out), "paged_append: NULL queries");
         FTH_ARG(d->rotary_dim == 0 || (cosines && sines), "paged_append: NULL rotation tables");
         FTH_ARG(q != q_out || d->q_heads == 0 || (d->q_row_stride == d->out_row_stride && d->q_head_stride == d->out_head_stride),
@@ -265,8 +270,8 @@ int32_t fth_dev_paged_append_f32(const fth_paged_cache *c, const fth_paged_appen
     a.q_out = q_out; a.k_cache = k_cache; a.v_cache = v_cache; a.bad = bad_index;
     a.by_page = fth::Divisor((uint32_t)c->page_size);
     a.pair_units = (int)(c->head_dim - d->rotary_dim / 2);
-    a.k_units = (int)c->head_dim;
-    a.units = (int)((d->q_heads + c->kv_heads) * a.pair_units + c->kv_heads * a.k_units);
+    a.kv_heads = k ? (int)c->kv_heads : 0;
+    a.units = (int)((d->q_heads + a.kv_heads) * a.pair_units + a.kv_heads * c->head_dim);
     switch (c->dtype) {
         case FTH_DTYPE_F32: return launch<float>(a, st);
         case FTH_DTYPE_F16: return launch<fth::f16>(a, st);

@@ -487,7 +487,8 @@ def paged_append_desc(cache, tokens, q_heads=0, rotary_dim=0, max_pos=0, interle
 
 
 def paged_append(cache, desc, q, k, v, cosines, sines, block_table, seq_ids, positions, q_out, k_cache, v_cache, bad_index=None, stream=None):
-    """K (rotated) and V of desc.tokens tokens into the paged cache, rotated queries into q_out (q and q_out None: no queries)."""
+    """K (rotated) and V of desc.tokens tokens into the paged cache, rotated queries into q_out (q and q_out None: no
+    queries; k, v, the caches, block_table and seq_ids None: queries alone)."""
     check(_lib.load().fth_dev_paged_append_f32(C.byref(cache), C.byref(desc), _ptr(q), _ptr(k), _ptr(v), _ptr(cosines), _ptr(sines), _ptr(block_table),
                                                _ptr(seq_ids), _ptr(positions), _ptr(q_out), _ptr(k_cache), _ptr(v_cache), _ptr(bad_index), stream))
 

@@ -454,7 +454,8 @@ void fth_dev_paged_cache_contiguous(fth_paged_cache *c, int64_t num_pages, int64
  * the first rotary_dim elements of every K row are rotated on the way, in pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1)
  * when `interleaved`: (a, b) -> (a c - b s, b c + a s), c = cosines[position * rotary_dim / 2 + i], s = sines[the same]
  * (fp32 [max_pos, rotary_dim / 2] tables, not read when rotary_dim == 0). With q_heads > 0 the queries are rotated likewise
- * into q_out (fp32; q_out == q with the same strides is allowed; otherwise no operand may overlap another).
+ * into q_out (fp32; q_out == q with the same strides is allowed; otherwise no operand may overlap another). k and v may both be
+ * NULL: then only queries are rotated, and caches, tables and seq_ids are not looked at.
  * A token at position -1 is skipped: nothing of it is read or written (the padding of a captured graph). A token whose
  * sequence, position, page or row of the tables does not exist is left out the same way and reported: bad_index (device, may
  * be NULL) receives the lowest such t, or -1. Two tokens at one place leave either of them there. */

@@ -64,6 +64,7 @@ def test_append_refusals():
         assert append(cache(), **kw) == INVALID, kw
     assert append(cache(), q_heads=1 << 40) == OVERFLOW
     assert append(cache(), tokens=1 << 31) == OVERFLOW
+    assert append(cache(), 1, none=("k", "v", "q", "out"), q_heads=0) == INVALID  # nothing to do
     for n in ("q", "k", "v", "cos", "sin", "table", "seq", "pos", "out", "kc", "vc"):
         assert append(cache(), 1, none=(n,)) == INVALID, n
 

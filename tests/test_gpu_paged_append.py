@@ -140,3 +140,28 @@ def test_nothing_to_append(hip):
     bad = DeviceBuffer.from_host(np.array([5], np.int64))
     hip.paged_append(p.cache, hip.paged_append_desc(p.cache, 0), None, None, None, None, None, p.dev_table, None, None, None, kc, vc, bad)
     assert bad.to_host()[0] == -1
+
+
+@pytest.mark.parametrize("d,rotary,interleaved", [(64, 64, False), (64, 32, True), (20, 6, False)])
+def test_queries_alone(hip, d, rotary, interleaved):
+    """Without keys and values only queries are rotated: no sequence, table or cache is looked at; positions still count."""
+    t, hq = 37, 5
+    q, pos = synth.normal(35, "q", (t, hq, d)), (np.arange(t) * 3 % 50).astype(np.int32)
+    cos, sin = hip.rotary_tables(50, rotary)
+    cache, bad = hip.paged_cache(0, 16, 1, d, 0, 0, "bf16"), DeviceBuffer((1,), np.int64)
+    bufs = [DeviceBuffer.from_host(x) for x in (cos, sin)]
+
+    def call(pos):
+        out = DeviceBuffer.from_host(np.full(q.shape, 7.0, np.float32))
+        hip.paged_append(cache, hip.paged_append_desc(cache, t, hq, rotary, 50, interleaved), DeviceBuffer.from_host(q), None, None, *bufs, None, None,
+                         DeviceBuffer.from_host(pos), out, None, None, bad)
+        hip.synchronize()
+        return out.to_host(), int(bad.to_host()[0])
+
+    ref = rotated(q, pos, cos, sin, rotary, interleaved, np.float32)
+    out, first = call(pos)
+    assert first == -1 and np.array_equal(out, ref)
+    pos[[4, 9, 30]] = -1, 50, -2
+    out, first = call(pos)
+    kept = np.delete(np.arange(t), [4, 9, 30])
+    assert first == 9 and np.array_equal(out[kept], ref[kept]) and np.all(out[[4, 9, 30]] == 7.0)
