@@ -46,7 +46,7 @@ struct Divisor {
     uint32_t mul = 1, shift = 0;
     Divisor() = default;
     explicit Divisor(uint32_t d) {
-        while (((uint64_t)1 << shift) < d) ++shift;
+        shift = d > 1 ? 32 - (uint32_t)__builtin_clz(d - 1) : 0;
         mul = (uint32_t)(((((uint64_t)1 << shift) - d) << 32) / d + 1);
     }
     __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (uint32_t)(((uint64_t)__umulhi(n, mul) + n) >> shift); }

@@ -19,8 +19,8 @@
 //
 // Measured: 64 sequences of 1024 to 8191 keys, 32 query heads on 8 K/V heads of 128, bf16 (1.22 GB): 7.6 ms on one wavefront a
 // row, 283 us with both products on fp32 units, 235 with the scores on 16-bit ones (MFMA-busy 0.31, wavefronts waiting to
-// issue), 217 + 5 with both (5.7 TB/s; a kernel that only reads pages of 4 KB in random order reaches 5.9, with nontemporal
-// loads 6.5). One sequence of 131071: 87 + 6 us (6.2 TB/s). Joining the shares in the last workgroup to arrive instead of a
+// issue), 212 + 5 with both (5.8 TB/s; a kernel that only reads pages of 4 KB in random order reaches 5.9, with nontemporal
+// loads 6.5). One sequence of 131071: 85 + 5 us (6.3 TB/s). Joining the shares in the last workgroup to arrive instead of a
 // second launch was slower in every case (release and acquire across the XCDs): 90 -> 109 us.
 
 #include <type_traits>
@@ -49,7 +49,9 @@ struct PagedArgs {
     float scale2;    // scale * log2(e)
     int64_t most;    // the longest valid sequence
     int group, row_tiles, nsplit, share, pitch;
-    fth::Divisor by_page;
+    int pairs;                                            // of a sequence and a K/V head
+    fth::Divisor by_page, by_tiles, by_pairs, by_heads;   // by page_size, row_tiles, pairs, kv_heads
+    fth::Divisor by_new, by_q_heads, by_group4;           // by new_tokens, q_heads, pitch / 4
 };
 
 struct MaxOp { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
@@ -79,10 +81,10 @@ template <typename T> __global__ __launch_bounds__(64) void paged_sdpa_rows_kern
     __shared__ float qs[256], ps[64];
     __shared__ int64_t at[64];
     const int lane = threadIdx.x, hd = (int)p.c.head_dim, page_size = (int)p.c.page_size;
-    const int split = (int)(blockIdx.x % (unsigned)p.nsplit);
-    const int64_t row = blockIdx.x / (unsigned)p.nsplit;
-    const int h = (int)(row % p.d.q_heads), i = (int)(row / p.d.q_heads % p.d.new_tokens);
-    const int64_t seq = row / p.d.q_heads / p.d.new_tokens;
+    const int split = (int)(blockIdx.x % (unsigned)p.nsplit), row32 = (int)(blockIdx.x / (unsigned)p.nsplit);
+    const int token = (int)p.by_q_heads((uint32_t)row32), h = row32 - token * (int)p.d.q_heads;
+    const int seq32 = (int)p.by_new((uint32_t)token), i = token - seq32 * (int)p.d.new_tokens;
+    const int64_t row = row32, seq = seq32;
     const int64_t hk = h / p.group;
     const T *K = static_cast<const T *>(p.k) + hk * p.c.head_stride, *V = static_cast<const T *>(p.v) + hk * p.c.head_stride;
     int len = p.lens[seq];
@@ -101,12 +103,13 @@ template <typename T> __global__ __launch_bounds__(64) void paged_sdpa_rows_kern
         const int key = key0 + lane, n = key_hi - key0 < 64 ? key_hi - key0 : 64;
         float x = -__builtin_inff();
         if (key < end) {
-            int page = p.table[seq * p.c.table_stride + key / page_size];
+            const int index = (int)p.by_page((uint32_t)key);
+            int page = p.table[seq * p.c.table_stride + index];
             if (page < 0 || page >= p.c.num_pages) {
                 bad = true;
                 page = -1;
             }
-            const int64_t off = page < 0 ? -1 : (int64_t)page * p.c.page_stride + (int64_t)(key % page_size) * p.c.row_stride;
+            const int64_t off = page < 0 ? -1 : (int64_t)page * p.c.page_stride + (int64_t)(key - index * page_size) * p.c.row_stride;
             at[lane] = off;
             if (page >= 0 && lane < n) {
                 float dot[4] = {0.f, 0.f, 0.f, 0.f};  // short chains of roundings
@@ -217,7 +220,6 @@ template <typename T, int DP> struct TileShape {
     static constexpr int NE = DP / 16;              // output columns of a lane
     static constexpr int CV = NE < CH ? NE : CH;    // consecutive ones
     static constexpr int NV = NE / CV;              // loads of its part of a V row
-    static constexpr int kLds = kWaves * 16 * (DP + 4);
 };
 
 // FULL: head_dim == DP; otherwise what lies past head_dim counts as zero. NT: K and V leave no trace in the caches. ANY: pages of any
@@ -225,14 +227,17 @@ template <typename T, int DP> struct TileShape {
 template <typename T, int DP, bool FULL, bool NT, bool ANY> __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void paged_sdpa_tiles_kernel(const PagedArgs p) {
     using S = TileShape<T, DP>;
     constexpr int CH = S::CH, NK = S::NK, NE = S::NE, CV = S::CV, NV = S::NV, kParts = Parts<T>::kParts;
-    __shared__ __attribute__((aligned(16))) float lds_o[S::kLds];
+    __shared__ __attribute__((aligned(16))) float lds_o[kWaves * 16 * (DP + 4)];
     __shared__ float lds_ml[kWaves * 16 * 2];
     const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int units = (int)(p.c.num_seqs * p.c.kv_heads) * p.row_tiles;
-    const int split = (int)(blockIdx.x / (unsigned)units), unit = (int)(blockIdx.x % (unsigned)units);
-    const int rt = unit % p.row_tiles, hk = unit / p.row_tiles % (int)p.c.kv_heads;
-    const int64_t seq = unit / p.row_tiles / (int)p.c.kv_heads;
+    // Workgroup ids go round the 8 XCDs: the row tiles of one share of a K/V head come 8 apart, so that they find its K and V in
+    // one L2 (16 sequences of up to 3967 keys, 64 query heads on 8 of 128: four queries, bf16 64.6 -> 57.3 us; eight, fp32 202 -> 155).
+    const int block8 = (int)(blockIdx.x >> 3), item8 = (int)p.by_tiles((uint32_t)block8), rt = block8 - item8 * p.row_tiles;
+    const int item = item8 * 8 + (int)(blockIdx.x & 7), split = (int)p.by_pairs((uint32_t)item), pair = item - split * p.pairs;
+    if (split >= p.nsplit) return;
+    const int seq32 = (int)p.by_heads((uint32_t)pair), hk = pair - seq32 * (int)p.c.kv_heads;
+    const int64_t seq = seq32;
     const int hd = (int)p.c.head_dim, new_tokens = (int)p.d.new_tokens, rows = p.group * new_tokens;
     int len = p.lens[seq];
     bool bad = len < 0 || len > p.most;
@@ -259,7 +264,7 @@ template <typename T, int DP, bool FULL, bool NT, bool ANY> __global__ __launch_
     // this lane's query row (rows past the last repeat it and are never stored) and how many keys it sees
     int rr = rt * 16 + lr;
     rr = rr < rows ? rr : rows - 1;
-    const int qi = rr % new_tokens, qh = hk * p.group + rr / new_tokens;
+    const int in_group = (int)p.by_new((uint32_t)rr), qi = rr - in_group * new_tokens, qh = hk * p.group + in_group;
     const int sees = len - new_tokens + 1 + qi;
     const float *qr = p.q + seq * p.d.q_seq_stride + qi * p.d.q_row_stride + qh * p.d.q_head_stride;
     float q[NK][CH];
@@ -579,7 +584,7 @@ template <typename T, int DP, bool FULL, bool NT, bool ANY> __global__ __launch_
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[j] += part[j] * weight;
         }
-        const int ri = (rt * 16 + row) % new_tokens, rh = hk * p.group + (rt * 16 + row) / new_tokens;
+        const int head = (int)p.by_new((uint32_t)(rt * 16 + row)), ri = rt * 16 + row - head * new_tokens, rh = hk * p.group + head;
         if (alone) {
             float *dst = out_row(p, seq, ri, rh);
             const bool nothing = !(l != l) && len - new_tokens + 1 + ri <= 0;
@@ -601,15 +606,15 @@ template <typename T, int DP, bool FULL, bool NT, bool ANY> __global__ __launch_
 // SL lanes of a wavefront walk the shares of four columns of a row side by side (each over every SL-th of them, in order) and are
 // added up in a fixed tree; 64 / SL neighbouring groups of columns make the wavefront. SL grows with the shares, so that no lane
 // has more than a few loads to wait for.
-template <int SL> __global__ __launch_bounds__(256) void paged_sdpa_join_kernel(const PagedArgs p, int64_t items) {
+template <int SL> __global__ __launch_bounds__(256) void paged_sdpa_join_kernel(const PagedArgs p, int items) {
     constexpr int CL = 64 / SL;
-    const int64_t item = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * CL + (threadIdx.x & (CL - 1));
-    const int lane_s = (threadIdx.x & 63) / CL, groups = p.pitch / 4;
+    const int item = (int)((blockIdx.x * 4 + (threadIdx.x >> 6)) * CL + (threadIdx.x & (CL - 1)));
+    const int lane_s = (threadIdx.x & 63) / CL;
     const bool there = item < items;
-    const int64_t row = there ? item / groups : 0;
-    const int c = (int)(item % groups) * 4;
-    const int h = (int)(row % p.d.q_heads), i = (int)(row / p.d.q_heads % p.d.new_tokens);
-    const int64_t seq = row / p.d.q_heads / p.d.new_tokens;
+    const int row32 = there ? (int)p.by_group4((uint32_t)item) : 0, c = there ? (item - row32 * (p.pitch / 4)) * 4 : 0;
+    const int token = (int)p.by_q_heads((uint32_t)row32), h = row32 - token * (int)p.d.q_heads;
+    const int seq32 = (int)p.by_new((uint32_t)token), i = token - seq32 * (int)p.d.new_tokens;
+    const int64_t row = row32, seq = seq32;
     const int len = p.lens[seq];
     // rows of one share are written; so are those of an invalid length
     const int shares = there && len > p.share && len <= p.most ? (len - 1) / p.share + 1 : 0;
@@ -664,13 +669,17 @@ Plan plan(const fth_paged_cache &c, const fth_paged_sdpa_desc &d) {
     const int64_t row_tiles = fth::ceil_div(d.q_heads / c.kv_heads * d.new_tokens, 16);
     const int64_t units = p.tiles ? c.num_seqs * c.kv_heads * row_tiles : p.rows;
     const int64_t step = kTile * kWaves;
-    // Shares: about 256 workgroups, of 256 to 2048 keys. A join costs 4 to 5 us, so nothing is cut that fills the chip whole (32
-    // sequences of 1000 keys: 18.6 us in one share, 23.6 in two) or has 512 keys (8 K/V heads of 128: 10.5 / 12.0); longer shares than
-    // 2048 leave the chip empty behind the longest sequence (64 of up to 8191: 241 us in one share, 235 in four). 128 keys where
-    // 256 would not make 128 workgroups (12 heads of 64, 1024 keys: 10.6 / 12.4; 8 of 128, 4096 keys: 13.4 / 14.7).
+    // Shares: about 256 workgroups, of 256 keys at least. A join costs 4 to 5 us, so nothing is cut that fills the chip whole (32
+    // sequences of 1000 keys: 18.6 us in one share, 23.6 in two) or has 512 keys (8 K/V heads of 128: 10.5 / 12.0). 128 keys where 256
+    // would not make 128 workgroups (12 heads of 64, 1024 keys: 10.6 / 12.4; 8 of 128, 4096 keys: 13.4 / 14.7). In a batch that
+    // fills the chip, shares of 512 KB where a sequence has more than 1 MB: the chip does not wait for the longest one (64 of up to
+    // 8191 keys, bf16: 244 us in one share each, 224 in shares of 1 MB, 218 of 512 KB, 227 of 256 KB; 64 of up to 4000, fp32: 255,
+    // 232, 225, 234; 32 of up to 1000, fp32: 39 in one, 45 in 512 KB).
     int64_t share = fth::ceil_div(most, units > 0 && units < 256 ? 256 / units : 1);
     const int64_t least = units * fth::ceil_div(most, 256) <= 128 ? 128 : 256;
-    share = share < least ? least : share > 2048 ? 2048 : share;
+    const int64_t key_bytes = 2 * c.head_dim * (c.dtype == FTH_DTYPE_F32 ? 4 : 2);
+    if (units >= 256 && most * key_bytes > (1 << 20)) share = share < (512 << 10) / key_bytes ? share : (512 << 10) / key_bytes;
+    share = share < least ? least : share;
     if (p.tiles && most <= 512) share = most;
     p.share = (int)(fth::ceil_div(share > 0 ? share : 1, step) * step);
     p.nsplit = (int)fth::ceil_div(most, p.share);
@@ -701,11 +710,11 @@ int32_t check(const fth_paged_cache *c, const fth_paged_sdpa_desc *d) {
 
 template <typename T> int32_t launch(PagedArgs &a, const Plan &pl, bool tiles, hipStream_t st) {
     if (tiles) {
-        const int64_t grid = a.c.num_seqs * a.c.kv_heads * a.row_tiles * a.nsplit;
+        const int64_t grid = fth::ceil_div(a.c.num_seqs * a.c.kv_heads * a.nsplit, 8) * 8 * a.row_tiles;
         FTH_ARG(grid <= 2147483647LL, "paged_sdpa: too many workgroups for one launch");
-        const dim3 blocks((unsigned)grid), threads(64 * kWaves);
+        const dim3 blocks((unsigned)grid);
         const bool nt = pl.nt;
-        auto go = [&](auto kernel) { kernel<<<blocks, threads, 0, st>>>(a); };
+        auto go = [&](auto kernel) { kernel<<<blocks, dim3(64 * kWaves), 0, st>>>(a); };
         if (a.c.page_size % 16 != 0) {
             if (a.c.head_dim <= 64) go(paged_sdpa_tiles_kernel<T, 64, false, false, true>);
             else if (a.c.head_dim <= 128) go(paged_sdpa_tiles_kernel<T, 128, false, false, true>);
@@ -725,10 +734,10 @@ template <typename T> int32_t launch(PagedArgs &a, const Plan &pl, bool tiles, h
     }
     FTH_CHECK_LAUNCH("paged_sdpa");
     if (a.nsplit > 1) {
-        const int64_t items = pl.rows * (a.pitch / 4);  // at most 2^24 rows of 64 groups
+        const int items = (int)(pl.rows * (a.pitch / 4));  // at most 2^24 rows of 64 groups
         // (us, 1 / 4 / 16 / 64 lanes: 2048 rows of up to 16 shares 5.9 / 5.1 / 11.8 / 41; 32 rows of 256 shares 44 / 15 / 9.6 / 6.3)
         const int lanes = a.nsplit <= 4 ? 1 : a.nsplit <= 16 ? 4 : a.nsplit <= 64 ? 16 : 64;
-        const dim3 blocks((unsigned)fth::ceil_div(items * lanes, 256));
+        const dim3 blocks((unsigned)fth::ceil_div((int64_t)items * lanes, 256));
         if (lanes == 1) paged_sdpa_join_kernel<1><<<blocks, dim3(256), 0, st>>>(a, items);
         else if (lanes == 4) paged_sdpa_join_kernel<4><<<blocks, dim3(256), 0, st>>>(a, items);
         else if (lanes == 16) paged_sdpa_join_kernel<16><<<blocks, dim3(256), 0, st>>>(a, items);
@@ -772,7 +781,14 @@ int32_t fth_dev_paged_sdpa_f32(const fth_paged_cache *c, const fth_paged_sdpa_de
     a.group = (int)(d->q_heads / c->kv_heads);
     a.row_tiles = (int)fth::ceil_div((int64_t)a.group * d->new_tokens, 16);
     a.nsplit = pl.nsplit; a.share = pl.share; a.pitch = pl.pitch;
+    a.pairs = (int)(c->num_seqs * c->kv_heads);
     a.by_page = fth::Divisor((uint32_t)c->page_size);
+    a.by_tiles = fth::Divisor((uint32_t)a.row_tiles);
+    a.by_pairs = fth::Divisor((uint32_t)a.pairs);
+    a.by_heads = fth::Divisor((uint32_t)c->kv_heads);
+    a.by_new = fth::Divisor((uint32_t)d->new_tokens);
+    a.by_q_heads = fth::Divisor((uint32_t)d->q_heads);
+    a.by_group4 = fth::Divisor((uint32_t)(a.pitch / 4));
     const bool tiles = pl.tiles && (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15u) == 0;
     switch (c->dtype) {
         case FTH_DTYPE_F32: return launch<float>(a, pl, tiles, st);
