@@ -500,13 +500,45 @@ template <typename T, int DP, bool FULL, bool NT, bool ANY> __global__ __launch_
                 for (int j = kParts - 1; j >= 0; --j) o[e] = Parts<T>::mfma(column, wp[j], o[e]);
             }
         } else {
+            // A key that only the later of the new tokens see: what is not finite in its V row would be NaN under a weight of 0. It
+            // counts as zero here and is added below to the rows that see it.
+            const int partly = len - new_tokens + 1;
+            bool held = false;
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
 #pragma unroll
-                    for (int e = 0; e < NE; ++e)
-                        o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(Chunk<T>::get(vf[s][r][e / CV], e % CV), w[4 * s + r], o[e], 0, 0, 0);
+                    for (int e = 0; e < NE; ++e) {
+                        float v = Chunk<T>::get(vf[s][r][e / CV], e % CV);
+                        if constexpr (!more) {
+                            const bool hold = key0 + 16 * s + 4 * g + r >= partly && !(fabsf(v) < __builtin_inff());
+                            held |= hold;
+                            v = hold ? 0.f : v;
+                        }
+                        o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, w[4 * s + r], o[e], 0, 0, 0);
+                    }
+            if constexpr (!more) {
+                if (__any(held)) {
+                    const int from = partly > key0 ? partly : key0, to = key_hi < key0 + kTile ? key_hi : key0 + kTile;
+                    for (int key = from; key < to; ++key) {
+                        const int at = key - key0, in_lane = 4 * (at >> 4) + (at & 3);
+                        float mine = w[0];
+#pragma unroll
+                        for (int y = 1; y < 8; ++y) mine = in_lane == y ? w[y] : mine;
+                        const float weight = __shfl(mine, (at >> 2 & 3) * 16 + lr);
+                        const T *vr = V + row_offset(off[at >> 4], at & 15);
+#pragma unroll
+                        for (int e = 0; e < NE; ++e)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const int c = ((e / CV) * 16 + 4 * g + r) * CV + e % CV;
+                                const float v = FULL || c < hd ? fth::to_f32(vr[c]) : 0.f;
+                                if (key < sees && !(fabsf(v) < __builtin_inff())) o[e][r] += weight * v;
+                            }
+                    }
+                }
+            }
         }
         if constexpr (more) {
             load_v(next);
@@ -697,6 +729,7 @@ size_t workspace_bytes_of(const Plan &p) { return p.nsplit > 1 ? (size_t)p.rows 
 int32_t check(const fth_paged_cache *c, const fth_paged_sdpa_desc *d) {
     if (int32_t rc = fth::check_paged_cache(c, "paged_sdpa", nullptr)) return rc;
     FTH_ARG(d, "paged_sdpa: NULL descriptor");
+    if (d->q_heads > (1 << 24)) return fth::set_error(FTH_ERR_SIZE_OVERFLOW, "paged_sdpa: more than 2^24 query heads");
     FTH_ARG(d->q_heads >= 1 && d->q_heads % c->kv_heads == 0, "paged_sdpa: %lld query heads on %lld K/V heads", (long long)d->q_heads, (long long)c->kv_heads);
     FTH_ARG(d->new_tokens >= 1 && d->new_tokens <= 8, "paged_sdpa: new_tokens %lld is outside 1..8", (long long)d->new_tokens);
     FTH_ARG(d->max_len >= 0 && d->max_len <= (1 << 30), "paged_sdpa: max_len %lld is outside 0..2^30", (long long)d->max_len);

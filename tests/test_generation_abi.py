@@ -76,7 +76,7 @@ def test_attention_refusals():
                dict(o_head_stride=-1), dict(q_row_stride=(1 << 40) + 1)):
         assert attend(cache(), **kw) == INVALID, kw
     assert attend(cache(), 1 << 30, q_heads=4) == OVERFLOW
-    assert attend(cache(), q_heads=1 << 62) == OVERFLOW
+    assert attend(cache(), q_heads=1 << 62) == OVERFLOW and attend(cache(), 0, q_heads=1 << 62) == OVERFLOW
     for n in ("q", "k", "v", "table", "lens", "out"):
         assert attend(cache(), none=(n,)) == INVALID, n
 

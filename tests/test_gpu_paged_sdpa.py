@@ -260,3 +260,25 @@ def test_queries_that_are_not_finite(hip, dtype):
     got, ref = run(hip, p, q, 0.125), attention(q, p.k, p.v, 0.125, p.lens)
     assert np.array_equal(np.isnan(got), np.isnan(ref)) and np.isnan(ref).sum() == 3 * 64
     assert rel_err(got[~np.isnan(ref)], ref[~np.isnan(ref)]) <= TOL_GEMM_F32
+
+
+@pytest.mark.parametrize("dtype,page,d", [("f32", 16, 64), ("f16", 16, 128), ("bf16", 16, 64), ("bf16", 5, 128), ("f16", 16, 40), ("f32", 16, 7), ("bf16", 16, 256)])
+@pytest.mark.parametrize("n", [1, 4, 33, 35, 64, 130, 515])
+def test_later_tokens_that_are_not_finite(hip, dtype, page, d, n):
+    """Infinities and NaN in K and V of the newest tokens: the queries before them do not see them, those after do, in their column."""
+    new, hq, hkv = 6, 4, 2
+    for what in ("inf", "nan", "k"):
+        for at in {n - 1, max(0, n - 3), max(0, n - new)}:
+            p = Paged(23, [n, 40], hkv, d, page, dtype)
+            q = np.abs(queries(p, hq, new)) + np.float32(0.25)
+            if what == "k":
+                p.k[0][0, at, 2 % d] = -np.inf  # weighs nothing where it is seen
+            else:
+                p.v[0][1, at, 3 % d] = {"inf": np.inf, "nan": np.nan}[what]
+                p.v[0][1, at, d - 1] = -np.inf
+            for x, store in ((p.k, p.stores[0]), (p.v, p.stores[1])):
+                store[p.index(0, np.arange(n))] = x[0].transpose(1, 0, 2)
+            got, ref = run(hip, p, q, 0.125), attention(q, p.k, p.v, 0.125, p.lens)
+            fine = np.isfinite(ref)
+            assert np.array_equal(got[~fine], ref[~fine], equal_nan=True), (what, at)
+            assert rel_err(got[fine], ref[fine]) <= TOL_GEMM_F32, (what, at)
