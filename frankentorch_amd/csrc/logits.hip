@@ -6,7 +6,7 @@
 // is read and written once, a row's own bias read once.
 //   * A scan costs about eight instructions an id and is repeated by every stretch of the row: with 2048 steps of 4096 logits and
 //     more, a stretch is two of them (200 rows of 131071, up to 8000 tokens before: 67 -> 60 us; four steps leave too few
-//     workgroups: 64). The loads of a step go out before the one before it is finished, those of the first before the barrier.
+//     workgroups: 64). The loads of a step go out before the one before it is finished, those of the first before the scan.
 //   * What a thread loads and stores is 128 bits at 4-byte alignment, since rows of an odd vocabulary start anywhere (65 us where
 //     131072 takes 61).
 //   * A bias of the row's own is loaded past the caches, where it would push out logits (64.5 -> 60 us); one for all rows is not
@@ -74,7 +74,7 @@ template <bool NTB, bool NTS> __global__ __launch_bounds__(kThreads) void logits
         return s;
     };
 
-    Step now;
+    Step now = load(0);
     float rep = 1.f, freq = 0.f, pres = 0.f;
     bool counted = false;
     if (p.history) {
@@ -105,7 +105,6 @@ template <bool NTB, bool NTS> __global__ __launch_bounds__(kThreads) void logits
                 }
             }
         }
-        now = load(0);
         if (p.repetition) rep = p.repetition[r];
         if (p.frequency) freq = p.frequency[r];
         if (p.presence) pres = p.presence[r];
@@ -113,8 +112,6 @@ template <bool NTB, bool NTS> __global__ __launch_bounds__(kThreads) void logits
             if (threadIdx.x == 0 && v0 == 0) fth::report_bad_entry(p.bad, r);
             return;
         }
-    } else {
-        now = load(0);
     }
     float *y = p.out + r * p.d.out_stride + v0;
     auto finish = [&](float t, uint32_t c, float b, bool allowed) __attribute__((always_inline)) {
