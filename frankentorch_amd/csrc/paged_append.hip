@@ -3,12 +3,12 @@
 // HBM-bound: one pass over the packed projection, every K, V and query element read once and written once. A thread owns pairs of
 // a rotation (both elements of each, so queries may be rotated in place) or the same number of elements that are only copied; no
 // two threads touch one element. -ffp-contract=off rounds a c, b s and their difference one by one.
-// Whole vectors: four pairs a thread, of several heads at one place of the row, so that its cosines and sines are read once and
-// four rows are in flight. What 128-bit accesses cannot take goes element by element.
+// What 128-bit accesses cannot take goes element by element.
 //
-// Measured: three prompts of up to 7001 tokens, 32 query and 8 K/V heads of 128, f16 (710 MB) 128 us, 5.5 TB/s (a copy of that
-// size reaches 6.3; element by element 447); eight of up to 1024 tokens, 12 heads of 64, fp32 (63 MB) 13.7 us (50); a step of 64
-// sequences 3.7 us. Nontemporal loads or stores or both are slower (133 to 140 us; the next reader finds less in the caches).
+// Measured: three prompts of up to 7001 tokens, 32 query and 8 K/V heads of 128, f16 (712 MB) 112 us, 6.3 TB/s, what a copy of that
+// size reaches (through the caches 134; element by element 447); eight of up to 1024 tokens, 12 heads of 64, fp32 (68 MB) 13.6 us
+// (50); a step of 64 sequences 3.7 us. Four tokens a workgroup where it holds all heads of one are slower (22 us for the eight
+// prompts: registers), and so is a workgroup that looks the next token up while this one's rows are on their way (145 us for the three).
 
 #include <type_traits>
 
@@ -91,29 +91,45 @@ template <typename T> __global__ __launch_bounds__(kBlock) void paged_append_ker
 
 using F4 = float __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ F4 load4(const float *p) { return *reinterpret_cast<const F4 *>(p); }
-// Eight elements as they are stored: four at `a` and four at `b` (the next four unless `apart`).
-__device__ __forceinline__ void store8(float *a, float *b, F4 x, F4 y, bool) {
-    *reinterpret_cast<F4 *>(a) = x;
-    *reinterpret_cast<F4 *>(b) = y;
+template <bool NT> __device__ __forceinline__ F4 load4(const float *p) {
+    const F4 *v = reinterpret_cast<const F4 *>(p);
+    return NT ? __builtin_nontemporal_load(v) : *v;
 }
-template <typename T> __device__ __forceinline__ void store8(T *a, T *b, F4 x, F4 y, bool apart) {
+// Two adjacent pairs.
+__device__ __forceinline__ F4 turned(F4 v, float c0, float s0, float c1, float s1) {
+    return F4{v[0] * c0 - v[1] * s0, v[1] * c0 + v[0] * s0, v[2] * c1 - v[3] * s1, v[3] * c1 + v[2] * s1};
+}
+// Eight elements as they are stored: four at `a` and four at `b`, which are the next four when `adjacent`.
+template <bool NT> __device__ __forceinline__ void store8(float *a, float *b, F4 x, F4 y, bool) {
+    if constexpr (NT) {
+        __builtin_nontemporal_store(x, reinterpret_cast<F4 *>(a));
+        __builtin_nontemporal_store(y, reinterpret_cast<F4 *>(b));
+    } else {
+        *reinterpret_cast<F4 *>(a) = x;
+        *reinterpret_cast<F4 *>(b) = y;
+    }
+}
+template <bool NT, typename T> __device__ __forceinline__ void store8(T *a, T *b, F4 x, F4 y, bool adjacent) {
     using E = typename std::conditional<std::is_same<T, fth::bf16>::value, __bf16, _Float16>::type;
     using E4 = E __attribute__((ext_vector_type(4)));
     using E8 = E __attribute__((ext_vector_type(8)));
     const E4 u = __builtin_convertvector(x, E4), v = __builtin_convertvector(y, E4);
-    if (apart) {
+    if (adjacent) {
+        *reinterpret_cast<E8 *>(a) = __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
         *reinterpret_cast<E4 *>(a) = u;
         *reinterpret_cast<E4 *>(b) = v;
-    } else {
-        *reinterpret_cast<E8 *>(a) = __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
     }
 }
 
-// Whole vectors: a thread owns eight elements of a row, four pairs or eight that are copied, and takes them from several heads, so
-// that the table's entries are read once. kHeads rows are in flight per thread.
+// Whole vectors: a thread owns two chunks of four elements at one place of the row and takes them from several heads, so that the
+// tables' entries are read once; kHeads rows are in flight per thread. The chunks are the two sides of four pairs
+// (i, i + rotary_dim / 2), else neighbours, which a 16-bit cache takes in one store.
+// STREAM, for what the caches cannot hold: operands and rotated queries go past them, and then every access has to cover whole lines,
+// so chunks that are no pairs come from the two halves of what they cover (an fp32 cache is stored the same way; 16-bit ones, whose
+// rows are then stored by half lines, go through the caches).
 constexpr int kHeads = 4;
-template <typename T> __global__ __launch_bounds__(kBlock) void paged_append_vec_kernel(const AppendArgs p, int blocks_per_token) {
+template <typename T, bool INTER, bool STREAM> __global__ __launch_bounds__(kBlock) void paged_append_vec_kernel(const AppendArgs p, int blocks_per_token) {
     const int64_t t = blockIdx.x / (unsigned)blocks_per_token;
     const int part = (int)(blockIdx.x % (unsigned)blocks_per_token);
     const int pos = p.positions[t];
@@ -127,13 +143,29 @@ template <typename T> __global__ __launch_bounds__(kBlock) void paged_append_vec
     const int slot = (int)threadIdx.x / per_row, i = (int)threadIdx.x % per_row;
     if (slot >= slots) return;
     const int rotary = (int)p.d.rotary_dim, hq = (int)p.d.q_heads, hkv = p.kv_heads, heads = hq + 2 * hkv;
-    const bool turns = 8 * i < rotary, inter = p.d.interleaved != 0;
+    const int va = STREAM ? 4 * i : 8 * i, vb = STREAM ? hd / 2 + 4 * i : 8 * i + 4;  // chunks of a row that is only copied
+    int ra = va, rb = vb;                                                           // of one that is rotated
+    bool turn_a = va < rotary, turn_b = vb < rotary;
     F4 c = {1.f, 1.f, 1.f, 1.f}, s = {0.f, 0.f, 0.f, 0.f};
-    if (turns) {
-        c = load4(p.cosines + (int64_t)pos * (rotary / 2) + 4 * i);
-        s = load4(p.sines + (int64_t)pos * (rotary / 2) + 4 * i);
+    const float *cosines = p.cosines + (int64_t)pos * (rotary / 2), *sines = p.sines + (int64_t)pos * (rotary / 2);
+    if constexpr (INTER) {  // two pairs a chunk
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            if (turn_a) c[e] = cosines[va / 2 + e], s[e] = sines[va / 2 + e];
+            if (turn_b) c[2 + e] = cosines[vb / 2 + e], s[2 + e] = sines[vb / 2 + e];
+        }
+    } else {
+        turn_a = turn_b = 8 * i < rotary;
+        if (turn_a) {
+            ra = 4 * i;
+            rb = rotary / 2 + 4 * i;
+            c = load4<false>(cosines + 4 * i);
+            s = load4<false>(sines + 4 * i);
+        } else if (STREAM) {
+            ra = rotary + 4 * (i - rotary / 8);
+            rb = ra + (hd - rotary) / 2;
+        }
     }
-    const int ia_pairs = inter ? 8 * i : 4 * i, ib_pairs = inter ? 8 * i + 4 : rotary / 2 + 4 * i;
     const int stride = slots * blocks_per_token;
     for (int h0 = part * slots + slot; h0 < heads; h0 += kHeads * stride) {
         F4 a[kHeads], b[kHeads];
@@ -144,39 +176,32 @@ template <typename T> __global__ __launch_bounds__(kBlock) void paged_append_vec
             const float *src = h < hq ? p.q + t * p.d.q_row_stride + h * p.d.q_head_stride
                                : h < hq + hkv ? p.k + t * p.d.k_row_stride + (h - hq) * p.d.k_head_stride
                                               : p.v + t * p.d.v_row_stride + (h - hq - hkv) * p.d.v_head_stride;
-            const bool pair = turns && h < hq + hkv;
-            a[j] = load4(src + (pair ? ia_pairs : 8 * i));
-            b[j] = load4(src + (pair ? ib_pairs : 8 * i + 4));
+            a[j] = load4<STREAM>(src + (h < hq + hkv ? ra : va));
+            b[j] = load4<STREAM>(src + (h < hq + hkv ? rb : vb));
         }
 #pragma unroll
         for (int j = 0; j < kHeads; ++j) {
             const int h = h0 + j * stride;
             if (h >= heads) continue;
-            const bool pair = turns && h < hq + hkv;
+            const bool turns = h < hq + hkv;
             F4 x = a[j], y = b[j];
-            if (pair && inter) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    x[2 * e] = a[j][2 * e] * c[e] - a[j][2 * e + 1] * s[e];
-                    x[2 * e + 1] = a[j][2 * e + 1] * c[e] + a[j][2 * e] * s[e];
-                    y[2 * e] = b[j][2 * e] * c[2 + e] - b[j][2 * e + 1] * s[2 + e];
-                    y[2 * e + 1] = b[j][2 * e + 1] * c[2 + e] + b[j][2 * e] * s[2 + e];
-                }
-            } else if (pair) {
+            if constexpr (INTER) {
+                if (turns && turn_a) x = turned(x, c[0], s[0], c[1], s[1]);
+                if (turns && turn_b) y = turned(y, c[2], s[2], c[3], s[3]);
+            } else if (turns && turn_a) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     x[e] = a[j][e] * c[e] - b[j][e] * s[e];
                     y[e] = b[j][e] * c[e] + a[j][e] * s[e];
                 }
             }
-            const int ia = pair ? ia_pairs : 8 * i, ib = pair ? ib_pairs : 8 * i + 4;
-            const bool apart = pair && !inter;
+            const int xa = turns ? ra : va, xb = turns ? rb : vb;
             if (h < hq) {
                 float *dst = p.q_out + t * p.d.out_row_stride + h * p.d.out_head_stride;
-                store8(dst + ia, dst + ib, x, y, apart);
+                store8<STREAM>(dst + xa, dst + xb, x, y, false);
             } else {
-                T *dst = h < hq + hkv ? static_cast<T *>(p.k_cache) + at + (h - hq) * p.c.head_stride : static_cast<T *>(p.v_cache) + at + (h - hq - hkv) * p.c.head_stride;
-                store8(dst + ia, dst + ib, x, y, apart);
+                T *dst = turns ? static_cast<T *>(p.k_cache) + at + (h - hq) * p.c.head_stride : static_cast<T *>(p.v_cache) + at + (h - hq - hkv) * p.c.head_stride;
+                store8<STREAM>(dst + xa, dst + xb, x, y, !STREAM && (INTER || !turns || !turn_a));
             }
         }
     }
@@ -203,7 +228,13 @@ template <typename T> int32_t launch(const AppendArgs &a, hipStream_t st) {
         // A workgroup a token and four rows a thread; one row a thread where tokens are few (64 of 48 heads of 128: 4.5 -> 3.7 us).
         const int64_t blocks_per_token = fth::ceil_div(heads, a.d.tokens < 1024 ? slots : slots * kHeads);
         FTH_ARG(a.d.tokens * blocks_per_token <= 2147483647LL, "paged_append: too many tokens for one launch");
-        paged_append_vec_kernel<T><<<dim3((unsigned)(a.d.tokens * blocks_per_token)), dim3(kBlock), 0, st>>>(a, (int)blocks_per_token);
+        // past the caches from their 256 MB on (us, with / without: 712 MB, f16 cache 112 / 134, 789 MB, fp32 cache 132 / 150, 271 MB,
+        // fp32 cache 54 / 59; 325 MB level; 68 MB 17.2 / 16.2)
+        const double bytes = (double)a.d.tokens * a.c.head_dim * (8.0 * a.d.q_heads + 2.0 * a.kv_heads * (4 + sizeof(T)));
+        const bool stream = bytes > 0x1p28;
+        auto go = [&](auto k) { k<<<dim3((unsigned)(a.d.tokens * blocks_per_token)), dim3(kBlock), 0, st>>>(a, (int)blocks_per_token); };
+        if (a.d.interleaved && a.d.rotary_dim > 0) go(stream ? paged_append_vec_kernel<T, true, true> : paged_append_vec_kernel<T, true, false>);
+        else go(stream ? paged_append_vec_kernel<T, false, true> : paged_append_vec_kernel<T, false, false>);
         FTH_CHECK_LAUNCH("paged_append");
         return FTH_OK;
     }
