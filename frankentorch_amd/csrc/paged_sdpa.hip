@@ -2,10 +2,12 @@
 //
 //   out[s, i, h] = sum_j w_j v_j / sum_j w_j,   w_j = exp(x_j - max x),   x_j = scale q . k_j,   j < lens[s] - new_tokens + i + 1
 //
-// Bound by reading the cache once. The keys of a sequence are cut into shares of equal length; a workgroup takes one share of
-// one K/V head for up to 16 of the query rows that read it (query heads of the group x new tokens), so K and V are read once for
-// all of them. Its four wavefronts walk the share in tiles of 32 keys, each on its own (running maximum and sum per row in fp32,
-// no barrier), and are joined through LDS at the end; a second small kernel joins the shares of a row in order.
+// Bound by reading the cache once. The keys of a sequence are cut into shares; a workgroup takes one share of one K/V head for up to
+// 16 of the query rows that read it (query heads of the group x new tokens), so K and V are read once for all of them. Shares
+// have one length, or, in large batches, are cut from the keys of the whole batch end to end, so that the chip does not wait for
+// long sequences (see steps_of). The four wavefronts of a workgroup walk a share in tiles of 32 keys, each on its own (running
+// maximum and sum per row in fp32, no barrier), and are joined through LDS at the end; a second small kernel joins the shares of a
+// row in order.
 //   * S^T[key, row] = K . Q^T with a key row and a query row per lane (16 x 16 tiles); the lane that gets scores of row lr holds
 //     them as it needs them for O^T[d, row] += V^T . P^T, so P never moves; V rows are read whole (16 lanes side by side).
 //   * 16-bit caches: both products run on the 16-bit matrix units against the bits as they are stored. The fp32 side is cut into
@@ -19,8 +21,8 @@
 //
 // Measured: 64 sequences of 1024 to 8191 keys, 32 query heads on 8 K/V heads of 128, bf16 (1.22 GB): 7.6 ms on one wavefront a
 // row, 283 us with both products on fp32 units, 235 with the scores on 16-bit ones (MFMA-busy 0.31, wavefronts waiting to
-// issue), 212 + 5 with both (5.8 TB/s; a kernel that only reads pages of 4 KB in random order reaches 5.9, with nontemporal
-// loads 6.5). One sequence of 131071: 85 + 5 us (6.3 TB/s). Joining the shares in the last workgroup to arrive instead of a
+// issue), 212 + 5 with both in shares of 512 KB, 194 + 5 in even ones (6.3 TB/s; a kernel that only reads pages of 4 KB in random
+// order reaches 5.9, with nontemporal loads 6.7). One sequence of 131071: 85 + 5 us (6.3 TB/s). Joining the shares in the last workgroup to arrive instead of a
 // second launch was slower in every case (release and acquire across the XCDs): 90 -> 109 us.
 
 #include <type_traits>
@@ -33,6 +35,10 @@ using F4 = float __attribute__((ext_vector_type(4)));
 using U4 = uint32_t __attribute__((ext_vector_type(4)));
 using U2 = uint32_t __attribute__((ext_vector_type(2)));
 
+// What no kernel here writes: such loads stay scalar ones also behind stores.
+using Const = const int32_t __attribute__((address_space(4))) *;
+__device__ __forceinline__ Const constant(const int32_t *x) { return (Const)(uintptr_t)x; }
+
 constexpr float kLog2e = 1.44269502162933349609375f;
 constexpr int kTile = 32, kWaves = 4;
 
@@ -44,15 +50,33 @@ struct PagedArgs {
     const int32_t *table, *lens;
     float *out;
     int64_t *bad;
-    float *part_o;   // [row][split][pitch] unnormalised outputs of the shares (rows with more than one)
-    float *part_ml;  // [row][split][2] their maxima (of scores times log2 e) and sums
-    float scale2;    // scale * log2(e)
-    int64_t most;    // the longest valid sequence
-    int group, row_tiles, nsplit, share, pitch;
+    float *part_o;    // [slot][pitch] unnormalised outputs of the shares (rows with more than one)
+    float *part_ml;   // [slot][2] their maxima (of scores times log2 e) and sums
+    int32_t *starts;  // even shares: where each sequence begins in the line of steps; behind the last one the length of a share
+    float scale2;     // scale * log2(e)
+    int64_t most;     // the longest valid sequence
+    int group, rows, row_tiles, pitch;                    // rows: queries that read a K/V head, group * new_tokens
     int pairs;                                            // of a sequence and a K/V head
+    int nsplit, share;                                    // shares of `share` keys from the first key of a pair on, nsplit of the longest
+    int even, step_log2, seqs_a_lane;                     // or this many even shares (0: the former)
     fth::Divisor by_page, by_tiles, by_pairs, by_heads;   // by page_size, row_tiles, pairs, kv_heads
-    fth::Divisor by_new, by_q_heads, by_group4;           // by new_tokens, q_heads, pitch / 4
+    fth::Divisor by_new, by_q_heads, by_group, by_group4, by_even;  // by new_tokens, q_heads, group, pitch / 4, even
 };
+
+// Even shares: all pairs of a sequence and a K/V head stand in one line, each as one step for beginning it and the steps of
+// 2^step_log2 keys that it has, and every workgroup takes the same stretch of that line. A stretch has at most two pairs in part, its
+// first and its last, so a workgroup has two groups of `rows` slots.
+__device__ __forceinline__ int steps_of(const PagedArgs &p, int len) { return len < 0 || len > p.most ? 0 : (int)(((uint32_t)len + (1u << p.step_log2) - 1) >> p.step_log2); }
+
+// All lines of the arguments at once: the compiler reads them as it needs them, in several round trips one after the other (8
+// sequences of up to 1024 keys, 12 heads of 64: 10.8 + 3.8 -> 10.3 + 3.1 us).
+__device__ __forceinline__ void fetch_arguments() {
+    const auto a = (const uint32_t __attribute__((address_space(4))) *)__builtin_amdgcn_kernarg_segment_ptr();
+    uint32_t any = 0;
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(PagedArgs) / 4; i += 16) any |= a[i];
+    asm volatile("" ::"s"(any));
+}
 
 struct MaxOp { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
 struct AddOp { __device__ float operator()(float a, float b) const { return a + b; } };
@@ -69,11 +93,10 @@ template <typename F> __device__ __forceinline__ float rows_reduce(float x, F op
     return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// Where a row (sequence, new token, query head) of the output lies, and its number.
+// Where a row (sequence, new token, query head) of the output lies.
 __device__ __forceinline__ float *out_row(const PagedArgs &p, int64_t seq, int i, int h) {
     return p.out + seq * p.d.o_seq_stride + i * p.d.o_row_stride + h * p.d.o_head_stride;
 }
-__device__ __forceinline__ int64_t row_number(const PagedArgs &p, int64_t seq, int i, int h) { return (seq * p.d.new_tokens + i) * p.d.q_heads + h; }
 
 // ---- one wavefront a row and share: any page size, head size, stride and alignment ----------------------------------------
 
@@ -84,8 +107,7 @@ template <typename T> __global__ __launch_bounds__(64) void paged_sdpa_rows_kern
     const int split = (int)(blockIdx.x % (unsigned)p.nsplit), row32 = (int)(blockIdx.x / (unsigned)p.nsplit);
     const int token = (int)p.by_q_heads((uint32_t)row32), h = row32 - token * (int)p.d.q_heads;
     const int seq32 = (int)p.by_new((uint32_t)token), i = token - seq32 * (int)p.d.new_tokens;
-    const int64_t row = row32, seq = seq32;
-    const int64_t hk = h / p.group;
+    const int64_t seq = seq32, hk = p.by_group((uint32_t)h);
     const T *K = static_cast<const T *>(p.k) + hk * p.c.head_stride, *V = static_cast<const T *>(p.v) + hk * p.c.head_stride;
     int len = p.lens[seq];
     bool bad = len < 0 || len > p.most;
@@ -139,7 +161,7 @@ template <typename T> __global__ __launch_bounds__(64) void paged_sdpa_rows_kern
     if (bad) l = __builtin_nanf("");
     float *dst = out_row(p, seq, i, h);
     if (!alone) {
-        const int64_t slot = row * p.nsplit + split;
+        const int64_t slot = ((seq * p.c.kv_heads + hk) * p.nsplit + split) * p.rows + (h - hk * p.group) * p.d.new_tokens + i;
         dst = p.part_o + slot * p.pitch;
         if (lane == 0) {
             p.part_ml[2 * slot] = m;
@@ -224,31 +246,20 @@ template <typename T, int DP> struct TileShape {
 
 // FULL: head_dim == DP; otherwise what lies past head_dim counts as zero. NT: K and V leave no trace in the caches. ANY: pages of any
 // size: every lane looks its K row up, and V rows are found through the lane that has the same key.
-template <typename T, int DP, bool FULL, bool NT, bool ANY> __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void paged_sdpa_tiles_kernel(const PagedArgs p) {
+//
+// One segment: keys key_lo .. key_hi - 1 of a pair of `len` keys, with row tile rt of its queries. `alone`: these are all of them, and
+// the outputs are written; otherwise they go to the slots from `slot` on.
+template <typename T, int DP, bool FULL, bool NT, bool ANY>
+__device__ __forceinline__ void tiles_segment(const PagedArgs &p, float *lds_o, float *lds_ml, int seq32, int hk, int rt, int len, bool bad, int key_lo, int key_hi, bool alone, int64_t slot0) {
     using S = TileShape<T, DP>;
     constexpr int CH = S::CH, NK = S::NK, NE = S::NE, CV = S::CV, NV = S::NV, kParts = Parts<T>::kParts;
-    __shared__ __attribute__((aligned(16))) float lds_o[kWaves * 16 * (DP + 4)];
-    __shared__ float lds_ml[kWaves * 16 * 2];
     const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // Workgroup ids go round the 8 XCDs: the row tiles of one share of a K/V head come 8 apart, so that they find its K and V in
-    // one L2 (16 sequences of up to 3967 keys, 64 query heads on 8 of 128: four queries, bf16 64.6 -> 57.3 us; eight, fp32 202 -> 155).
-    const int block8 = (int)(blockIdx.x >> 3), item8 = (int)p.by_tiles((uint32_t)block8), rt = block8 - item8 * p.row_tiles;
-    const int item = item8 * 8 + (int)(blockIdx.x & 7), split = (int)p.by_pairs((uint32_t)item), pair = item - split * p.pairs;
-    if (split >= p.nsplit) return;
-    const int seq32 = (int)p.by_heads((uint32_t)pair), hk = pair - seq32 * (int)p.c.kv_heads;
     const int64_t seq = seq32;
-    const int hd = (int)p.c.head_dim, new_tokens = (int)p.d.new_tokens, rows = p.group * new_tokens;
-    int len = p.lens[seq];
-    bool bad = len < 0 || len > p.most;
-    if (bad) len = 0;
-    const int key_lo = split * p.share;
-    if (split > 0 && key_lo >= len) return;
-    const bool alone = len <= p.share;
-    const int key_hi = len - key_lo < p.share ? len : key_lo + p.share;
+    const int hd = (int)p.c.head_dim, new_tokens = (int)p.d.new_tokens, rows = p.rows;
     const int tiles = (key_hi - key_lo + kTile - 1) / kTile, last16 = (key_hi - 1) >> 4;
     const T *K = static_cast<const T *>(p.k) + hk * p.c.head_stride, *V = static_cast<const T *>(p.v) + hk * p.c.head_stride;
-    const int32_t *table = p.table + seq * p.c.table_stride;
+    const Const table = constant(p.table) + seq * p.c.table_stride;
     const int rs = (int)p.c.row_stride, num_pages = (int)p.c.num_pages;
 
     const int stored = rows - rt * 16 < 16 ? rows - rt * 16 : 16;
@@ -623,7 +634,7 @@ template <typename T, int DP, bool FULL, bool NT, bool ANY> __global__ __launch_
 #pragma unroll
             for (int j = 0; j < 4; ++j) dst[c + j] = nothing ? 0.f : acc[j] / l;
         } else {
-            const int64_t slot = row_number(p, seq, ri, rh) * p.nsplit + split;
+            const int64_t slot = slot0 + rt * 16 + row;
             *reinterpret_cast<F4 *>(p.part_o + slot * p.pitch + c) = acc;
             if (c == 0) {
                 p.part_ml[2 * slot] = m;
@@ -633,27 +644,113 @@ template <typename T, int DP, bool FULL, bool NT, bool ANY> __global__ __launch_
     }
 }
 
+template <typename T, int DP, bool FULL, bool NT, bool ANY, bool EVEN> __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void paged_sdpa_tiles_kernel(const PagedArgs p) {
+    __shared__ __attribute__((aligned(16))) float lds_o[kWaves * 16 * (DP + 4)];
+    __shared__ float lds_ml[kWaves * 16 * 2];
+    fetch_arguments();
+    // Workgroup ids go round the 8 XCDs: the row tiles of one share of a K/V head come 8 apart, so that they find its K and V in
+    // one L2 (16 sequences of up to 3967 keys, 64 query heads on 8 of 128: four queries, bf16 64.6 -> 57.3 us; eight, fp32 202 -> 155).
+    const int block8 = (int)(blockIdx.x >> 3), item8 = (int)p.by_tiles((uint32_t)block8), rt = block8 - item8 * p.row_tiles;
+    const int item = item8 * 8 + (int)(blockIdx.x & 7), heads = (int)p.c.kv_heads;
+    const Const lens = constant(p.lens);
+    if constexpr (!EVEN) {
+        const int split = (int)p.by_pairs((uint32_t)item);
+        if (split >= p.nsplit) return;
+        const int pair = item - split * p.pairs, seq = (int)p.by_heads((uint32_t)pair), raw = lens[seq], key_lo = split * p.share;
+        const bool bad = raw < 0 || raw > p.most;
+        const int len = bad ? 0 : raw;
+        if (split > 0 && key_lo >= len) return;
+        tiles_segment<T, DP, FULL, NT, ANY>(p, lds_o, lds_ml, seq, pair - seq * heads, rt, len, bad, key_lo, len - key_lo < p.share ? len : key_lo + p.share, len <= p.share,
+                                            ((int64_t)pair * p.nsplit + split) * p.rows);
+    } else {
+        // this workgroup's place in the line
+        const int lane = threadIdx.x & 63, first = lane * p.seqs_a_lane, num_seqs = (int)p.c.num_seqs;
+        const int last = num_seqs - first < p.seqs_a_lane ? num_seqs : first + p.seqs_a_lane;
+        int mine = 0;
+        for (int j = first; j < last; ++j) mine += heads * (steps_of(p, lens[j]) + 1);
+        int upto = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int x = __shfl_up(upto, d);
+            upto += lane >= d ? x : 0;
+        }
+        const int total = __builtin_amdgcn_readlane(upto, 63), share = (int)p.by_even((uint32_t)(total + p.even - 1));
+        if (blockIdx.x == 0 && threadIdx.x < 64) {
+            int at = upto - mine;
+            for (int j = first; j < last; ++j) {
+                p.starts[j] = at;
+                at += heads * (steps_of(p, lens[j]) + 1);
+            }
+            if (lane == 0) p.starts[num_seqs] = share;
+        }
+        int pos = item * share;
+        if (pos >= total) return;
+        const int end = total - pos < share ? total : pos + share, in_lane = __builtin_ctzll(__ballot(upto > pos));
+        int at = __builtin_amdgcn_readlane(upto - mine, in_lane), seq = in_lane * p.seqs_a_lane, raw;
+        for (;;) {
+            raw = lens[seq];
+            const int behind = at + heads * (steps_of(p, raw) + 1);
+            if (pos < behind) break;
+            at = behind;
+            ++seq;
+        }
+        int hk = (pos - at) / (steps_of(p, raw) + 1), within = pos - at - hk * (steps_of(p, raw) + 1);
+        for (;;) {
+            const bool bad = raw < 0 || raw > p.most;
+            const int len = bad ? 0 : raw, steps = steps_of(p, raw), stop = steps + 1 - within < end - pos ? steps + 1 : within + end - pos;
+            const int key_lo = (within > 1 ? within - 1 : 0) << p.step_log2, key_hi = stop > steps ? len : (stop - 1) << p.step_log2;
+            if (key_lo < key_hi || len == 0)
+                tiles_segment<T, DP, FULL, NT, ANY>(p, lds_o, lds_ml, seq, hk, rt, len, bad, key_lo, key_hi, key_lo == 0 && key_hi == len,
+                                                    (int64_t)(2 * item + (within == 0)) * p.rows);
+            pos += stop - within;
+            if (pos >= end) break;
+            within = 0;
+            if (++hk == heads) {
+                hk = 0;
+                raw = lens[++seq];
+            }
+            __syncthreads();  // lds_o and lds_ml have been read
+        }
+    }
+}
+
 // ---- shares joined in their order -----------------------------------------------------------------------------------------
 
 // SL lanes of a wavefront walk the shares of four columns of a row side by side (each over every SL-th of them, in order) and are
 // added up in a fixed tree; 64 / SL neighbouring groups of columns make the wavefront. SL grows with the shares, so that no lane
 // has more than a few loads to wait for.
-template <int SL> __global__ __launch_bounds__(256) void paged_sdpa_join_kernel(const PagedArgs p, int items) {
+template <int SL, bool EVEN> __global__ __launch_bounds__(256) void paged_sdpa_join_kernel(const PagedArgs p, int items) {
     constexpr int CL = 64 / SL;
+    fetch_arguments();
     const int item = (int)((blockIdx.x * 4 + (threadIdx.x >> 6)) * CL + (threadIdx.x & (CL - 1)));
     const int lane_s = (threadIdx.x & 63) / CL;
     const bool there = item < items;
     const int row32 = there ? (int)p.by_group4((uint32_t)item) : 0, c = there ? (item - row32 * (p.pitch / 4)) * 4 : 0;
     const int token = (int)p.by_q_heads((uint32_t)row32), h = row32 - token * (int)p.d.q_heads;
     const int seq32 = (int)p.by_new((uint32_t)token), i = token - seq32 * (int)p.d.new_tokens;
-    const int64_t row = row32, seq = seq32;
-    const int len = p.lens[seq];
-    // rows of one share are written; so are those of an invalid length
-    const int shares = there && len > p.share && len <= p.most ? (len - 1) / p.share + 1 : 0;
-    const float2 *ml = reinterpret_cast<const float2 *>(p.part_ml) + row * p.nsplit;
-    const float *o = p.part_o + row * p.nsplit * p.pitch + c;
+    const int64_t seq = seq32;
+    const int len = p.lens[seq], hk = (int)p.by_group((uint32_t)h), in_pair = (h - hk * p.group) * (int)p.d.new_tokens + i;
+    // The slots of the row's shares, `apart` from each other; `first`: the first of even shares may stand further on. Rows of one share
+    // are written; so are those of an invalid length.
+    int shares = 0;
+    int64_t slot0, apart, first = 0;
+    if constexpr (!EVEN) {
+        if (there && len > p.share && len <= p.most) shares = (len - 1) / p.share + 1;
+        apart = p.rows;
+        slot0 = (seq * p.c.kv_heads + hk) * p.nsplit * apart + in_pair;
+    } else {
+        const int steps = steps_of(p, len), share = p.starts[p.c.num_seqs];
+        const int begin = p.starts[seq] + hk * (steps + 1) + 1, from = begin / share, to = (begin + steps - 1) / share;
+        if (there && steps > 0 && to > from) shares = to - from + 1;
+        apart = 2 * p.rows;
+        slot0 = from * apart + in_pair;
+        if (from * share < begin) first = p.rows;
+    }
+    const float2 *ml = reinterpret_cast<const float2 *>(p.part_ml);
+    auto slot = [&](int s) __attribute__((always_inline)) { return slot0 + s * apart + (EVEN && s == 0 ? first : 0); };
+    const float *o = p.part_o + c;
     float m = -__builtin_inff();
-    for (int s = lane_s; s < shares; s += SL) m = fmaxf(m, ml[s].x);
+    for (int s = lane_s; s < shares; s += SL) m = fmaxf(m, ml[slot(s)].x);
 #pragma unroll
     for (int d = CL; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
     const float ref = m == -__builtin_inff() ? 0.f : m;
@@ -661,8 +758,8 @@ template <int SL> __global__ __launch_bounds__(256) void paged_sdpa_join_kernel(
     float l = 0.f;
 #pragma unroll 8
     for (int s = lane_s; s < shares; s += SL) {
-        const float2 part = ml[s];
-        const F4 v = *reinterpret_cast<const F4 *>(o + (int64_t)s * p.pitch);
+        const float2 part = ml[slot(s)];
+        const F4 v = *reinterpret_cast<const F4 *>(o + slot(s) * p.pitch);
         const float w = __builtin_amdgcn_exp2f(part.x - ref);
         l += part.y * w;
 #pragma unroll
@@ -685,10 +782,10 @@ template <int SL> __global__ __launch_bounds__(256) void paged_sdpa_join_kernel(
 
 // How a call is cut: the same for its workspace and its launch.
 struct Plan {
-    bool tiles;   // head size and strides that the 128-bit loads take (the pointers' alignment is looked at later)
-    bool nt;      // loads that leave no trace in the caches
-    int nsplit, share, pitch;
-    int64_t rows;
+    bool tiles;  // head size and strides that the 128-bit loads take (the pointers' alignment is looked at later)
+    bool nt;     // loads that leave no trace in the caches
+    int even, step_log2, nsplit, share, pitch;
+    int64_t rows, row_tiles, most;
 };
 
 Plan plan(const fth_paged_cache &c, const fth_paged_sdpa_desc &d) {
@@ -697,34 +794,50 @@ Plan plan(const fth_paged_cache &c, const fth_paged_sdpa_desc &d) {
     p.rows = c.num_seqs * d.new_tokens * d.q_heads;
     p.tiles = c.head_dim % ch == 0 && c.row_stride % ch == 0 && c.head_stride % ch == 0 && c.page_stride % ch == 0 &&
               c.row_stride <= ((int64_t)1 << 24) && c.num_pages > 0;
-    const int64_t most = c.max_pages * c.page_size < d.max_len ? c.max_pages * c.page_size : d.max_len;
-    const int64_t row_tiles = fth::ceil_div(d.q_heads / c.kv_heads * d.new_tokens, 16);
-    const int64_t units = p.tiles ? c.num_seqs * c.kv_heads * row_tiles : p.rows;
-    const int64_t step = kTile * kWaves;
-    // Shares: about 256 workgroups, of 256 keys at least. A join costs 4 to 5 us, so nothing is cut that fills the chip whole (32
-    // sequences of 1000 keys: 18.6 us in one share, 23.6 in two) or has 512 keys (8 K/V heads of 128: 10.5 / 12.0). 128 keys where 256
-    // would not make 128 workgroups (12 heads of 64, 1024 keys: 10.6 / 12.4; 8 of 128, 4096 keys: 13.4 / 14.7). In a batch that
-    // fills the chip, shares of 512 KB where a sequence has more than 1 MB: the chip does not wait for the longest one (64 of up to
-    // 8191 keys, bf16: 244 us in one share each, 224 in shares of 1 MB, 218 of 512 KB, 227 of 256 KB; 64 of up to 4000, fp32: 255,
-    // 232, 225, 234; 32 of up to 1000, fp32: 39 in one, 45 in 512 KB).
-    int64_t share = fth::ceil_div(most, units > 0 && units < 256 ? 256 / units : 1);
-    const int64_t least = units * fth::ceil_div(most, 256) <= 128 ? 128 : 256;
+    p.pitch = (int)fth::ceil_div(c.head_dim, 4) * 4;
+    const int64_t most = p.most = c.max_pages * c.page_size < d.max_len ? c.max_pages * c.page_size : d.max_len;
+    p.row_tiles = fth::ceil_div(d.q_heads / c.kv_heads * d.new_tokens, 16);
+    const int64_t pairs = c.num_seqs * c.kv_heads, units = p.tiles ? pairs * p.row_tiles : p.rows;
     const int64_t key_bytes = 2 * c.head_dim * (c.dtype == FTH_DTYPE_F32 ? 4 : 2);
-    if (units >= 256 && most * key_bytes > (1 << 20)) share = share < (512 << 10) / key_bytes ? share : (512 << 10) / key_bytes;
+    // Shares of one length: about 256 workgroups, of 256 keys at least. A join costs 4 to 5 us, so nothing is cut that fills the chip whole (32
+    // sequences of 1000 keys: 18.6 us in one share, 23.6 in two) or has 512 keys (8 K/V heads of 128: 10.5 / 12.0). 128 keys where 256
+    // would not make 128 workgroups (12 heads of 64, 1024 keys: 10.6 / 12.4; 8 of 128, 4096 keys: 13.4 / 14.7).
+    const int64_t step = kTile * kWaves, least = units * fth::ceil_div(most, 256) <= 128 ? 128 : 256;
+    int64_t share = fth::ceil_div(most, units > 0 && units < 256 ? 256 / units : 1);
     share = share < least ? least : share;
     if (p.tiles && most <= 512) share = most;
     p.share = (int)(fth::ceil_div(share > 0 ? share : 1, step) * step);
     p.nsplit = (int)fth::ceil_div(most, p.share);
     if (p.nsplit < 1) p.nsplit = 1;
-    p.pitch = (int)fth::ceil_div(c.head_dim, 4) * 4;
+    // Even shares in a batch that fills the chip and whose sequences may have more than 1 MB (us, shares of 512 KB / even ones: 64 of up
+    // to 8191, bf16: 225 / 204; 64 of up to 4000, fp32: 225 / 202; 64 on 12 heads of 64 of up to 5000, bf16: 117 / 103; 128 on heads
+    // of 256 of up to 1500, bf16: 198 / 165; 32 sequences of 1000 keys take 18.6 in one share each, 23 in even ones). One workgroup a
+    // compute unit, two where their tiles would not keep enough bytes on the way (the first of these: 204 / 209, the second 202 / 210,
+    // heads of 64, bf16: 108 / 103).
+    p.even = 0;
+    p.step_log2 = 7;
+    static_assert(kTile * kWaves == 1 << 7, "a step is a tile of every wavefront");
+    if (p.tiles && units >= 256 && most * key_bytes > (1 << 20)) {
+        p.even = (int)((key_bytes < 512 ? 512 : 256) / p.row_tiles / 8 * 8);
+        p.even = p.even < 8 ? 8 : p.even;
+        while (pairs * ((most >> p.step_log2) + 2) > (1 << 30)) ++p.step_log2;  // places in the line are 32-bit numbers
+    }
     // Nontemporal loads for what the 256 MB last-level cache cannot hold until the next call, if sequences are half of max_len on
     // average, and that is read once (us, with / without: one sequence of 131071, bf16 87 / 99, fp32 180 / 196; 64 of up to 8191,
-    // bf16 217 / 229; 16 of up to 3967, four queries, f16, 260 MB 38.5 / 36.3, fp32, 520 MB 79 / 72).
-    p.nt = row_tiles == 1 && 2.0 * (double)c.num_seqs * (double)most * (double)c.kv_heads * (double)c.head_dim * (c.dtype == FTH_DTYPE_F32 ? 4 : 2) > 500.0 * (1 << 20);
+    // bf16 217 / 229 in shares of 512 KB; 16 of up to 3967, four queries, f16, 260 MB 38.5 / 36.3, fp32, 520 MB 79 / 72).
+    p.nt = p.row_tiles == 1 && 2.0 * (double)c.num_seqs * (double)most * (double)c.kv_heads * (double)c.head_dim * (c.dtype == FTH_DTYPE_F32 ? 4 : 2) > 500.0 * (1 << 20);
     return p;
 }
 
-size_t workspace_bytes_of(const Plan &p) { return p.nsplit > 1 ? (size_t)p.rows * p.nsplit * (p.pitch + 2) * sizeof(float) : 0; }
+// Partial results: of the shares of every row, or of two pairs a share.
+int64_t slots_of(const Plan &p, const fth_paged_cache &c, bool tiles) {
+    if (tiles && p.even) return 2 * p.even * (p.rows / (c.num_seqs * c.kv_heads));
+    return p.nsplit > 1 ? p.rows * p.nsplit : 0;
+}
+size_t workspace_bytes_of(const Plan &p, const fth_paged_cache &c) {
+    const int64_t even = slots_of(p, c, true), other = slots_of(p, c, false);
+    return (size_t)(even > other ? even : other) * (p.pitch + 2) * sizeof(float) + (p.even ? (size_t)(c.num_seqs + 1) * sizeof(int32_t) : 0);
+}
 
 int32_t check(const fth_paged_cache *c, const fth_paged_sdpa_desc *d) {
     if (int32_t rc = fth::check_paged_cache(c, "paged_sdpa", nullptr)) return rc;
@@ -743,38 +856,46 @@ int32_t check(const fth_paged_cache *c, const fth_paged_sdpa_desc *d) {
 
 template <typename T> int32_t launch(PagedArgs &a, const Plan &pl, bool tiles, hipStream_t st) {
     if (tiles) {
-        const int64_t grid = fth::ceil_div(a.c.num_seqs * a.c.kv_heads * a.nsplit, 8) * 8 * a.row_tiles;
+        const int64_t grid = fth::ceil_div(a.even ? (int64_t)a.even : (int64_t)a.pairs * a.nsplit, 8) * 8 * a.row_tiles;
         FTH_ARG(grid <= 2147483647LL, "paged_sdpa: too many workgroups for one launch");
         const dim3 blocks((unsigned)grid);
         const bool nt = pl.nt;
         auto go = [&](auto kernel) { kernel<<<blocks, dim3(64 * kWaves), 0, st>>>(a); };
-        if (a.c.page_size % 16 != 0) {
-            if (a.c.head_dim <= 64) go(paged_sdpa_tiles_kernel<T, 64, false, false, true>);
-            else if (a.c.head_dim <= 128) go(paged_sdpa_tiles_kernel<T, 128, false, false, true>);
-            else go(paged_sdpa_tiles_kernel<T, 256, false, false, true>);
-        } else switch (a.c.head_dim) {
-            case 64: go(nt ? paged_sdpa_tiles_kernel<T, 64, true, true, false> : paged_sdpa_tiles_kernel<T, 64, true, false, false>); break;
-            case 128: go(nt ? paged_sdpa_tiles_kernel<T, 128, true, true, false> : paged_sdpa_tiles_kernel<T, 128, true, false, false>); break;
-            case 256: go(nt ? paged_sdpa_tiles_kernel<T, 256, true, true, false> : paged_sdpa_tiles_kernel<T, 256, true, false, false>); break;
-            default:
-                if (a.c.head_dim < 64) go(paged_sdpa_tiles_kernel<T, 64, false, false, false>);
-                else if (a.c.head_dim < 128) go(paged_sdpa_tiles_kernel<T, 128, false, false, false>);
-                else go(paged_sdpa_tiles_kernel<T, 256, false, false, false>);
-        }
+        auto pick = [&](auto even) {
+            constexpr bool E = decltype(even)::value;
+            if (a.c.page_size % 16 != 0) {
+                if (a.c.head_dim <= 64) go(paged_sdpa_tiles_kernel<T, 64, false, false, true, E>);
+                else if (a.c.head_dim <= 128) go(paged_sdpa_tiles_kernel<T, 128, false, false, true, E>);
+                else go(paged_sdpa_tiles_kernel<T, 256, false, false, true, E>);
+            } else switch (a.c.head_dim) {
+                case 64: go(nt ? paged_sdpa_tiles_kernel<T, 64, true, true, false, E> : paged_sdpa_tiles_kernel<T, 64, true, false, false, E>); break;
+                case 128: go(nt ? paged_sdpa_tiles_kernel<T, 128, true, true, false, E> : paged_sdpa_tiles_kernel<T, 128, true, false, false, E>); break;
+                case 256: go(nt ? paged_sdpa_tiles_kernel<T, 256, true, true, false, E> : paged_sdpa_tiles_kernel<T, 256, true, false, false, E>); break;
+                default:
+                    if (a.c.head_dim < 64) go(paged_sdpa_tiles_kernel<T, 64, false, false, false, E>);
+                    else if (a.c.head_dim < 128) go(paged_sdpa_tiles_kernel<T, 128, false, false, false, E>);
+                    else go(paged_sdpa_tiles_kernel<T, 256, false, false, false, E>);
+            }
+        };
+        if (a.even) pick(std::true_type());
+        else pick(std::false_type());
     } else {
         FTH_ARG(pl.rows * a.nsplit <= 2147483647LL, "paged_sdpa: too many rows for one launch");
         paged_sdpa_rows_kernel<T><<<dim3((unsigned)(pl.rows * a.nsplit)), dim3(64), 0, st>>>(a);
     }
     FTH_CHECK_LAUNCH("paged_sdpa");
-    if (a.nsplit > 1) {
+    if (a.even || a.nsplit > 1) {
         const int items = (int)(pl.rows * (a.pitch / 4));  // at most 2^24 rows of 64 groups
         // (us, 1 / 4 / 16 / 64 lanes: 2048 rows of up to 16 shares 5.9 / 5.1 / 11.8 / 41; 32 rows of 256 shares 44 / 15 / 9.6 / 6.3)
-        const int lanes = a.nsplit <= 4 ? 1 : a.nsplit <= 16 ? 4 : a.nsplit <= 64 ? 16 : 64;
+        // (even shares, about one or two a pair, 1 / 4 lanes: 512 pairs level, 2048 pairs 222 / 225 in all)
+        const int lanes = a.even || a.nsplit <= 4 ? 1 : a.nsplit <= 16 ? 4 : a.nsplit <= 64 ? 16 : 64;
         const dim3 blocks((unsigned)fth::ceil_div((int64_t)items * lanes, 256));
-        if (lanes == 1) paged_sdpa_join_kernel<1><<<blocks, dim3(256), 0, st>>>(a, items);
-        else if (lanes == 4) paged_sdpa_join_kernel<4><<<blocks, dim3(256), 0, st>>>(a, items);
-        else if (lanes == 16) paged_sdpa_join_kernel<16><<<blocks, dim3(256), 0, st>>>(a, items);
-        else paged_sdpa_join_kernel<64><<<blocks, dim3(256), 0, st>>>(a, items);
+        auto go = [&](auto kernel) { kernel<<<blocks, dim3(256), 0, st>>>(a, items); };
+        if (a.even) go(paged_sdpa_join_kernel<1, true>);
+        else if (lanes == 1) go(paged_sdpa_join_kernel<1, false>);
+        else if (lanes == 4) go(paged_sdpa_join_kernel<4, false>);
+        else if (lanes == 16) go(paged_sdpa_join_kernel<16, false>);
+        else go(paged_sdpa_join_kernel<64, false>);
         FTH_CHECK_LAUNCH("paged_sdpa_join");
     }
     return FTH_OK;
@@ -785,7 +906,7 @@ template <typename T> int32_t launch(PagedArgs &a, const Plan &pl, bool tiles, h
 extern "C" {
 
 size_t fth_dev_paged_sdpa_workspace_bytes(const fth_paged_cache *c, const fth_paged_sdpa_desc *d) {
-    return check(c, d) == FTH_OK ? workspace_bytes_of(plan(*c, *d)) : 0;
+    return check(c, d) == FTH_OK ? workspace_bytes_of(plan(*c, *d), *c) : 0;
 }
 
 int32_t fth_dev_paged_sdpa_f32(const fth_paged_cache *c, const fth_paged_sdpa_desc *d, float scale, const float *q, const void *k_cache, const void *v_cache,
@@ -794,7 +915,7 @@ int32_t fth_dev_paged_sdpa_f32(const fth_paged_cache *c, const fth_paged_sdpa_de
     if (int32_t rc = check(c, d)) return rc;
     FTH_ARG(c->num_seqs == 0 || (q && lens && out && (block_table || c->max_pages == 0) && ((k_cache && v_cache) || c->num_pages == 0)), "paged_sdpa: NULL operand");
     const Plan pl = plan(*c, *d);
-    const size_t need = workspace_bytes_of(pl);
+    const size_t need = workspace_bytes_of(pl, *c);
     FTH_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15u) == 0), "paged_sdpa: needs a workspace of %zu bytes, 16-byte aligned", need);
     FTH_REQUIRE_DEVICE();
     hipStream_t st = fth::resolve_stream(s);
@@ -808,21 +929,28 @@ int32_t fth_dev_paged_sdpa_f32(const fth_paged_cache *c, const fth_paged_sdpa_de
     a.d = *d;
     a.q = q; a.k = k_cache; a.v = v_cache; a.table = block_table; a.lens = lens; a.out = out; a.bad = bad_index;
     a.part_o = static_cast<float *>(workspace);
-    a.part_ml = need ? a.part_o + pl.rows * pl.nsplit * pl.pitch : nullptr;
+    const bool tiles = pl.tiles && (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15u) == 0;
+    const int64_t slots = slots_of(pl, *c, tiles);
+    a.part_ml = a.part_o + slots * pl.pitch;
+    a.starts = reinterpret_cast<int32_t *>(a.part_ml + 2 * slots);
     a.scale2 = scale * kLog2e;
-    a.most = c->max_pages * c->page_size < d->max_len ? c->max_pages * c->page_size : d->max_len;
+    a.most = pl.most;
     a.group = (int)(d->q_heads / c->kv_heads);
-    a.row_tiles = (int)fth::ceil_div((int64_t)a.group * d->new_tokens, 16);
+    a.rows = a.group * (int)d->new_tokens;
+    a.row_tiles = (int)pl.row_tiles;
     a.nsplit = pl.nsplit; a.share = pl.share; a.pitch = pl.pitch;
+    a.even = tiles ? pl.even : 0; a.step_log2 = pl.step_log2;
+    a.seqs_a_lane = (int)fth::ceil_div(c->num_seqs, 64);
     a.pairs = (int)(c->num_seqs * c->kv_heads);
     a.by_page = fth::Divisor((uint32_t)c->page_size);
     a.by_tiles = fth::Divisor((uint32_t)a.row_tiles);
     a.by_pairs = fth::Divisor((uint32_t)a.pairs);
+    a.by_even = fth::Divisor((uint32_t)(a.even ? a.even : 1));
     a.by_heads = fth::Divisor((uint32_t)c->kv_heads);
     a.by_new = fth::Divisor((uint32_t)d->new_tokens);
     a.by_q_heads = fth::Divisor((uint32_t)d->q_heads);
+    a.by_group = fth::Divisor((uint32_t)a.group);
     a.by_group4 = fth::Divisor((uint32_t)(a.pitch / 4));
-    const bool tiles = pl.tiles && (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15u) == 0;
     switch (c->dtype) {
         case FTH_DTYPE_F32: return launch<float>(a, pl, tiles, st);
         case FTH_DTYPE_F16: return launch<fth::f16>(a, pl, tiles, st);

@@ -478,7 +478,8 @@ int32_t fth_dev_paged_append_f32(const fth_paged_cache *c, const fth_paged_appen
  * sequence with lens[s] outside [0, min(max_len, max_pages * page_size)] or with a page that does not exist has NaN in all its
  * outputs, and bad_index (device, may be NULL) receives the lowest such s, or -1.
  * The workspace (device memory, contents ignored and overwritten) holds the partial results of shares of the keys, which are
- * joined in a fixed order. */
+ * joined in a fixed order. Where the keys are cut may depend on all lengths of the batch: repeated calls are bitwise identical, a
+ * sequence in another batch is so within rounding. */
 typedef struct fth_paged_sdpa_desc {
     int64_t q_heads, new_tokens, max_len;
     int64_t q_seq_stride, q_row_stride, q_head_stride, o_seq_stride, o_row_stride, o_head_stride;
