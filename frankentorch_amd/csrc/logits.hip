@@ -14,7 +14,7 @@
 //     11.1 -> 9.5, and the argmax after it as fast as before in all: 27 us; 8 rows lose 1.2 of 22 us with the argmax).
 //
 // Measured: 200 rows of 131071, a bias each, a mask, up to 8000 tokens before 60 us (318 MB, 5.3 TB/s; one entry a thread and
-// stretches of 4096: 143); 64 rows of 50257, one bias, a mask 9.5 us (27 MB; 17.3); one row 4.6 us.
+// stretches of 4096: 143); 64 rows of 50257, one bias, a mask 7.9 us (27 MB; 17.3); one row 4.6 us.
 
 #include <type_traits>
 
