@@ -102,6 +102,19 @@ def test_every_step_alone_and_any_stride(hip, use, shared, pad, lead):
     assert np.array_equal(run(hip, m, use, shared, pad=pad, lead=lead), plain(m, use, np.float32, shared))
 
 
+@pytest.mark.parametrize("vocab", [1, 2, 3, 4, 5, 29, 30, 61, 4093, 4094, 4095, 4096, 4097, 8189, 8192, 8195])
+@pytest.mark.parametrize("pad,lead", [(0, 0), (0, 1), (1, 2), (2, 3), (4, 0), (3, 1)])
+def test_rows_that_start_anywhere(hip, vocab, pad, lead):
+    m = make(45, 6, vocab, 50)
+    want = plain(m, ALL, np.float32)
+    assert np.array_equal(run(hip, m, ALL, pad=pad, lead=lead), want)
+    assert np.array_equal(run(hip, m, ALL, pad=pad, lead=lead, in_place=True), want)
+    m["history"][3, 0], m["hlen"][3] = -1 - lead, max(m["hlen"][3], 1)  # just before the row
+    bad = DeviceBuffer((1,), np.int64)
+    got = run(hip, m, ALL, pad=pad, lead=lead, bad=bad)
+    assert bad.to_host()[0] == 3 and np.all(got[3] == 7.0) and np.array_equal(np.delete(got, 3, 0), np.delete(want, 3, 0))
+
+
 def test_values_that_are_not_finite(hip):
     """A masked place is -inf whatever was there; NaN and infinities elsewhere go through the steps."""
     m = make(43, 3, 500, 60)
