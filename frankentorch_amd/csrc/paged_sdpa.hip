@@ -4,8 +4,8 @@
 //
 // Bound by reading the cache once. The keys of a sequence are cut into shares; a workgroup takes one share of one K/V head for up to
 // 16 of the query rows that read it (query heads of the group x new tokens), so K and V are read once for all of them. Shares
-// have one length, or, in large batches, are cut from the keys of the whole batch end to end, so that the chip does not wait for
-// long sequences (see steps_of). The four wavefronts of a workgroup walk a share in tiles of 32 keys, each on its own (running
+// have one length, or, in large batches of long sequences, are cut from the keys of the whole batch end to end, so that the chip does
+// not wait for the longest ones (see steps_of). The four wavefronts of a workgroup walk a share in tiles of 32 keys, each on its own (running
 // maximum and sum per row in fp32, no barrier), and are joined through LDS at the end; a second small kernel joins the shares of a
 // row in order.
 //   * S^T[key, row] = K . Q^T with a key row and a query row per lane (16 x 16 tiles); the lane that gets scores of row lr holds
@@ -58,7 +58,7 @@ struct PagedArgs {
     int group, rows, row_tiles, pitch;                    // rows: queries that read a K/V head, group * new_tokens
     int pairs;                                            // of a sequence and a K/V head
     int nsplit, share;                                    // shares of `share` keys from the first key of a pair on, nsplit of the longest
-    int even, step_log2, seqs_a_lane;                     // or this many even shares (0: the former)
+    int even, enough, step_log2, seqs_a_lane;             // or this many even shares, if the keys make `enough` steps (0: the former)
     fth::Divisor by_page, by_tiles, by_pairs, by_heads;   // by page_size, row_tiles, pairs, kv_heads
     fth::Divisor by_new, by_q_heads, by_group, by_group4, by_even;  // by new_tokens, q_heads, group, pitch / 4, even
 };
@@ -653,17 +653,9 @@ template <typename T, int DP, bool FULL, bool NT, bool ANY, bool EVEN> __global_
     const int block8 = (int)(blockIdx.x >> 3), item8 = (int)p.by_tiles((uint32_t)block8), rt = block8 - item8 * p.row_tiles;
     const int item = item8 * 8 + (int)(blockIdx.x & 7), heads = (int)p.c.kv_heads;
     const Const lens = constant(p.lens);
-    if constexpr (!EVEN) {
-        const int split = (int)p.by_pairs((uint32_t)item);
-        if (split >= p.nsplit) return;
-        const int pair = item - split * p.pairs, seq = (int)p.by_heads((uint32_t)pair), raw = lens[seq], key_lo = split * p.share;
-        const bool bad = raw < 0 || raw > p.most;
-        const int len = bad ? 0 : raw;
-        if (split > 0 && key_lo >= len) return;
-        tiles_segment<T, DP, FULL, NT, ANY>(p, lds_o, lds_ml, seq, pair - seq * heads, rt, len, bad, key_lo, len - key_lo < p.share ? len : key_lo + p.share, len <= p.share,
-                                            ((int64_t)pair * p.nsplit + split) * p.rows);
-    } else {
-        // this workgroup's place in the line
+    int seq = 0, hk = 0, raw = 0, split = 0, pos = 0, end = 0, within = 0;
+    bool line = false;  // even shares
+    if constexpr (EVEN) {
         const int lane = threadIdx.x & 63, first = lane * p.seqs_a_lane, num_seqs = (int)p.c.num_seqs;
         const int last = num_seqs - first < p.seqs_a_lane ? num_seqs : first + p.seqs_a_lane;
         int mine = 0;
@@ -675,42 +667,66 @@ template <typename T, int DP, bool FULL, bool NT, bool ANY, bool EVEN> __global_
             upto += lane >= d ? x : 0;
         }
         const int total = __builtin_amdgcn_readlane(upto, 63), share = (int)p.by_even((uint32_t)(total + p.even - 1));
+        line = total - p.pairs >= p.enough;
         if (blockIdx.x == 0 && threadIdx.x < 64) {
             int at = upto - mine;
             for (int j = first; j < last; ++j) {
                 p.starts[j] = at;
                 at += heads * (steps_of(p, lens[j]) + 1);
             }
-            if (lane == 0) p.starts[num_seqs] = share;
+            if (lane == 0) p.starts[num_seqs] = line ? share : 0;
         }
-        int pos = item * share;
-        if (pos >= total) return;
-        const int end = total - pos < share ? total : pos + share, in_lane = __builtin_ctzll(__ballot(upto > pos));
-        int at = __builtin_amdgcn_readlane(upto - mine, in_lane), seq = in_lane * p.seqs_a_lane, raw;
-        for (;;) {
-            raw = lens[seq];
-            const int behind = at + heads * (steps_of(p, raw) + 1);
-            if (pos < behind) break;
-            at = behind;
-            ++seq;
-        }
-        int hk = (pos - at) / (steps_of(p, raw) + 1), within = pos - at - hk * (steps_of(p, raw) + 1);
-        for (;;) {
-            const bool bad = raw < 0 || raw > p.most;
-            const int len = bad ? 0 : raw, steps = steps_of(p, raw), stop = steps + 1 - within < end - pos ? steps + 1 : within + end - pos;
-            const int key_lo = (within > 1 ? within - 1 : 0) << p.step_log2, key_hi = stop > steps ? len : (stop - 1) << p.step_log2;
-            if (key_lo < key_hi || len == 0)
-                tiles_segment<T, DP, FULL, NT, ANY>(p, lds_o, lds_ml, seq, hk, rt, len, bad, key_lo, key_hi, key_lo == 0 && key_hi == len,
-                                                    (int64_t)(2 * item + (within == 0)) * p.rows);
-            pos += stop - within;
-            if (pos >= end) break;
-            within = 0;
-            if (++hk == heads) {
-                hk = 0;
-                raw = lens[++seq];
+        if (line) {  // this workgroup's place in the line
+            pos = item * share;
+            if (item >= p.even || pos >= total) return;
+            end = total - pos < share ? total : pos + share;
+            const int in_lane = __builtin_ctzll(__ballot(upto > pos));
+            int at = __builtin_amdgcn_readlane(upto - mine, in_lane);
+            seq = in_lane * p.seqs_a_lane;
+            for (;;) {
+                raw = lens[seq];
+                const int behind = at + heads * (steps_of(p, raw) + 1);
+                if (pos < behind) break;
+                at = behind;
+                ++seq;
             }
-            __syncthreads();  // lds_o and lds_ml have been read
+            hk = (pos - at) / (steps_of(p, raw) + 1);
+            within = pos - at - hk * (steps_of(p, raw) + 1);
         }
+    }
+    if (!line) {
+        split = (int)p.by_pairs((uint32_t)item);
+        if (split >= p.nsplit) return;
+        const int pair = item - split * p.pairs;
+        seq = (int)p.by_heads((uint32_t)pair);
+        hk = pair - seq * heads;
+        raw = lens[seq];
+    }
+    for (;;) {
+        const bool bad = raw < 0 || raw > p.most;
+        const int len = bad ? 0 : raw, steps = steps_of(p, raw), stop = steps + 1 - within < end - pos ? steps + 1 : within + end - pos;
+        int key_lo, key_hi;
+        int64_t slot;
+        if (EVEN && line) {
+            key_lo = (within > 1 ? within - 1 : 0) << p.step_log2;
+            key_hi = stop > steps ? len : (stop - 1) << p.step_log2;
+            slot = 2 * item + (within == 0);
+        } else {
+            key_lo = split * p.share;
+            key_hi = len - key_lo < p.share ? len : key_lo + p.share;
+            slot = ((int64_t)seq * heads + hk) * p.nsplit + split;
+        }
+        if (key_lo < key_hi || (len == 0 && key_lo == 0))
+            tiles_segment<T, DP, FULL, NT, ANY>(p, lds_o, lds_ml, seq, hk, rt, len, bad, key_lo, key_hi, key_lo == 0 && key_hi == len, slot * p.rows);
+        if (!EVEN || !line) break;
+        pos += stop - within;
+        if (pos >= end) break;
+        within = 0;
+        if (++hk == heads) {
+            hk = 0;
+            raw = lens[++seq];
+        }
+        __syncthreads();  // lds_o and lds_ml have been read
     }
 }
 
@@ -734,12 +750,13 @@ template <int SL, bool EVEN> __global__ __launch_bounds__(256) void paged_sdpa_j
     // are written; so are those of an invalid length.
     int shares = 0;
     int64_t slot0, apart, first = 0;
-    if constexpr (!EVEN) {
+    const int share = EVEN ? p.starts[p.c.num_seqs] : 0;
+    if (!EVEN || share == 0) {
         if (there && len > p.share && len <= p.most) shares = (len - 1) / p.share + 1;
         apart = p.rows;
         slot0 = (seq * p.c.kv_heads + hk) * p.nsplit * apart + in_pair;
     } else {
-        const int steps = steps_of(p, len), share = p.starts[p.c.num_seqs];
+        const int steps = steps_of(p, len);
         const int begin = p.starts[seq] + hk * (steps + 1) + 1, from = begin / share, to = (begin + steps - 1) / share;
         if (there && steps > 0 && to > from) shares = to - from + 1;
         apart = 2 * p.rows;
@@ -784,7 +801,7 @@ template <int SL, bool EVEN> __global__ __launch_bounds__(256) void paged_sdpa_j
 struct Plan {
     bool tiles;  // head size and strides that the 128-bit loads take (the pointers' alignment is looked at later)
     bool nt;     // loads that leave no trace in the caches
-    int even, step_log2, nsplit, share, pitch;
+    int even, enough, step_log2, nsplit, share, pitch;
     int64_t rows, row_tiles, most;
 };
 
@@ -802,25 +819,32 @@ Plan plan(const fth_paged_cache &c, const fth_paged_sdpa_desc &d) {
     // Shares of one length: about 256 workgroups, of 256 keys at least. A join costs 4 to 5 us, so nothing is cut that fills the chip whole (32
     // sequences of 1000 keys: 18.6 us in one share, 23.6 in two) or has 512 keys (8 K/V heads of 128: 10.5 / 12.0). 128 keys where 256
     // would not make 128 workgroups (12 heads of 64, 1024 keys: 10.6 / 12.4; 8 of 128, 4096 keys: 13.4 / 14.7).
+    // In a batch that fills the chip, shares of 512 KB where a sequence has more than 1 MB: the chip does not wait for the longest one
+    // (64 of up to 8191 keys, bf16: 244 us in one share each, 224 in shares of 1 MB, 218 of 512 KB, 227 of 256 KB; 64 of up to 4000,
+    // fp32: 255, 232, 225, 234; 32 of up to 1000, fp32: 39 in one, 45 in 512 KB).
     const int64_t step = kTile * kWaves, least = units * fth::ceil_div(most, 256) <= 128 ? 128 : 256;
+    static_assert(step == 1 << 7, "a step is a tile of every wavefront");
+    const bool large = units >= 256 && most * key_bytes > (1 << 20);
     int64_t share = fth::ceil_div(most, units > 0 && units < 256 ? 256 / units : 1);
+    if (large) share = share < (512 << 10) / key_bytes ? share : (512 << 10) / key_bytes;
     share = share < least ? least : share;
     if (p.tiles && most <= 512) share = most;
     p.share = (int)(fth::ceil_div(share > 0 ? share : 1, step) * step);
     p.nsplit = (int)fth::ceil_div(most, p.share);
     if (p.nsplit < 1) p.nsplit = 1;
-    // Even shares in a batch that fills the chip and whose sequences may have more than 1 MB (us, shares of 512 KB / even ones: 64 of up
-    // to 8191, bf16: 225 / 204; 64 of up to 4000, fp32: 225 / 202; 64 on 12 heads of 64 of up to 5000, bf16: 117 / 103; 128 on heads
-    // of 256 of up to 1500, bf16: 198 / 165; 32 sequences of 1000 keys take 18.6 in one share each, 23 in even ones). One workgroup a
-    // compute unit, two where their tiles would not keep enough bytes on the way (the first of these: 204 / 209, the second 202 / 210,
-    // heads of 64, bf16: 108 / 103).
-    p.even = 0;
+    // There even shares are better for up to 256 sequences that turn out to have 576 KB each on average, at one workgroup a compute unit
+    // (us, shares of 512 KB / even ones: 64 of up to 8191, bf16: 225 / 204; 64 of up to 4000, fp32: 225 / 202; 64 on 12 heads of 64 of
+    // up to 5000, bf16: 117 / 103; 128 on heads of 256 of up to 1500, bf16: 198 / 165; 512 of 1000 on one head: 51 / 56, 1024 of 20 keys:
+    // 19 / 33, where beginning a pair costs more than waiting for one), two where their tiles would not keep enough bytes on the way (the first
+    // of these: 204 / 209, the second 202 / 210, heads of 64, bf16: 108 / 103).
+    p.even = p.enough = 0;
     p.step_log2 = 7;
-    static_assert(kTile * kWaves == 1 << 7, "a step is a tile of every wavefront");
-    if (p.tiles && units >= 256 && most * key_bytes > (1 << 20)) {
+    if (p.tiles && large && c.num_seqs <= 256) {
         p.even = (int)((key_bytes < 512 ? 512 : 256) / p.row_tiles / 8 * 8);
         p.even = p.even < 8 ? 8 : p.even;
         while (pairs * ((most >> p.step_log2) + 2) > (1 << 30)) ++p.step_log2;  // places in the line are 32-bit numbers
+        const int64_t enough = pairs * fth::ceil_div((int64_t)(576 << 10) / key_bytes, (int64_t)1 << p.step_log2);
+        p.enough = (int)(enough < 2147483647LL ? enough : 2147483647LL);
     }
     // Nontemporal loads for what the 256 MB last-level cache cannot hold until the next call, if sequences are half of max_len on
     // average, and that is read once (us, with / without: one sequence of 131071, bf16 87 / 99, fp32 180 / 196; 64 of up to 8191,
@@ -831,12 +855,11 @@ Plan plan(const fth_paged_cache &c, const fth_paged_sdpa_desc &d) {
 
 // Partial results: of the shares of every row, or of two pairs a share.
 int64_t slots_of(const Plan &p, const fth_paged_cache &c, bool tiles) {
-    if (tiles && p.even) return 2 * p.even * (p.rows / (c.num_seqs * c.kv_heads));
-    return p.nsplit > 1 ? p.rows * p.nsplit : 0;
+    const int64_t one = p.nsplit > 1 ? p.rows * p.nsplit : 0, even = tiles && p.even ? 2 * p.even * (p.rows / (c.num_seqs * c.kv_heads)) : 0;
+    return even > one ? even : one;
 }
 size_t workspace_bytes_of(const Plan &p, const fth_paged_cache &c) {
-    const int64_t even = slots_of(p, c, true), other = slots_of(p, c, false);
-    return (size_t)(even > other ? even : other) * (p.pitch + 2) * sizeof(float) + (p.even ? (size_t)(c.num_seqs + 1) * sizeof(int32_t) : 0);
+    return (size_t)slots_of(p, c, true) * (p.pitch + 2) * sizeof(float) + (p.even ? (size_t)(c.num_seqs + 1) * sizeof(int32_t) : 0);
 }
 
 int32_t check(const fth_paged_cache *c, const fth_paged_sdpa_desc *d) {
@@ -856,7 +879,7 @@ int32_t check(const fth_paged_cache *c, const fth_paged_sdpa_desc *d) {
 
 template <typename T> int32_t launch(PagedArgs &a, const Plan &pl, bool tiles, hipStream_t st) {
     if (tiles) {
-        const int64_t grid = fth::ceil_div(a.even ? (int64_t)a.even : (int64_t)a.pairs * a.nsplit, 8) * 8 * a.row_tiles;
+        const int64_t cut = (int64_t)a.pairs * a.nsplit, grid = fth::ceil_div(cut > a.even ? cut : a.even, 8) * 8 * a.row_tiles;
         FTH_ARG(grid <= 2147483647LL, "paged_sdpa: too many workgroups for one launch");
         const dim3 blocks((unsigned)grid);
         const bool nt = pl.nt;
@@ -887,11 +910,11 @@ template <typename T> int32_t launch(PagedArgs &a, const Plan &pl, bool tiles, h
     if (a.even || a.nsplit > 1) {
         const int items = (int)(pl.rows * (a.pitch / 4));  // at most 2^24 rows of 64 groups
         // (us, 1 / 4 / 16 / 64 lanes: 2048 rows of up to 16 shares 5.9 / 5.1 / 11.8 / 41; 32 rows of 256 shares 44 / 15 / 9.6 / 6.3)
-        // (even shares, about one or two a pair, 1 / 4 lanes: 512 pairs level, 2048 pairs 222 / 225 in all)
-        const int lanes = a.even || a.nsplit <= 4 ? 1 : a.nsplit <= 16 ? 4 : a.nsplit <= 64 ? 16 : 64;
+        // (in a batch that fills the chip a row has about one share, though the longest have more)
+        const int lanes = a.nsplit <= 4 ? 1 : a.nsplit <= 16 || a.even ? 4 : a.nsplit <= 64 ? 16 : 64;
         const dim3 blocks((unsigned)fth::ceil_div((int64_t)items * lanes, 256));
         auto go = [&](auto kernel) { kernel<<<blocks, dim3(256), 0, st>>>(a, items); };
-        if (a.even) go(paged_sdpa_join_kernel<1, true>);
+        if (a.even) go(lanes == 1 ? paged_sdpa_join_kernel<1, true> : paged_sdpa_join_kernel<4, true>);
         else if (lanes == 1) go(paged_sdpa_join_kernel<1, false>);
         else if (lanes == 4) go(paged_sdpa_join_kernel<4, false>);
         else if (lanes == 16) go(paged_sdpa_join_kernel<16, false>);
@@ -939,7 +962,7 @@ int32_t fth_dev_paged_sdpa_f32(const fth_paged_cache *c, const fth_paged_sdpa_de
     a.rows = a.group * (int)d->new_tokens;
     a.row_tiles = (int)pl.row_tiles;
     a.nsplit = pl.nsplit; a.share = pl.share; a.pitch = pl.pitch;
-    a.even = tiles ? pl.even : 0; a.step_log2 = pl.step_log2;
+    a.even = tiles ? pl.even : 0; a.enough = pl.enough; a.step_log2 = pl.step_log2;
     a.seqs_a_lane = (int)fth::ceil_div(c->num_seqs, 64);
     a.pairs = (int)(c->num_seqs * c->kv_heads);
     a.by_page = fth::Divisor((uint32_t)c->page_size);

@@ -1,5 +1,6 @@
-"""Attention over a paged cache for batches that fill the chip, where the keys of all sequences are shared out end to end: cuts
-anywhere, sequences of very different lengths among them, against the definition in 64 bits."""
+"""Attention over a paged cache for batches that fill the chip, where the keys of all sequences are shared out end to end if there are
+enough of them, and cut by sequence if not: cuts anywhere, sequences of very different lengths among them, against the definition
+in 64 bits."""
 import numpy as np
 import pytest
 
@@ -48,6 +49,64 @@ def test_even_and_uneven_batches(hip, lens):
     got, ref = run(hip, p, q, 0.1, max_len=2200), attention(q, p.k, p.v, 0.1, lens)
     for s in range(64):
         assert rel_err(got[s], ref[s]) <= TOL_GEMM_F32 if lens[s] else not got[s].any()
+
+
+# (sequences, hq, hkv, new, d, page, dtype, longest): long enough on average to be shared out end to end
+LONG = [(32, 128, 1, 1, 128, 16, "bf16", 3500), (34, 32, 2, 8, 64, 16, "f32", 2700), (16, 256, 1, 1, 256, 16, "bf16", 2000), (32, 120, 1, 1, 72, 8, "f32", 3000),
+        (32, 64, 1, 2, 64, 32, "f16", 6500), (100, 36, 1, 1, 128, 16, "f16", 3000), (70, 8, 4, 1, 128, 16, "bf16", 3000)]
+
+
+def long_lengths(seed, num, longest, new):
+    x = [0, new, 128, 129, longest, longest, 127, 1] + (longest * (0.35 + 0.65 * synth.uniform(seed, "lens", (num,)))).astype(int).tolist()
+    return [x[i] for i in np.argsort(synth.uniform(seed, "order", (num,)))]
+
+
+@pytest.mark.parametrize("case", LONG, ids=str)
+def test_long_batches(hip, case):
+    num, hq, hkv, new, d, page, dtype, longest = case
+    p = Paged(36, long_lengths(36, num, longest, new), hkv, d, page, dtype)
+    q, bad = queries(p, hq, new), DeviceBuffer((1,), np.int64)
+    got = run(hip, p, q, 0.1, bad=bad)
+    assert bad.to_host()[0] == -1
+    ref = attention(q, p.k, p.v, 0.1, p.lens)
+    for s in range(num):
+        assert rel_err(got[s], ref[s]) <= TOL_GEMM_F32 if ref[s].any() else not got[s].any(), p.lens[s]
+    assert np.array_equal(got.view(np.uint32), run(hip, p, q, 0.1).view(np.uint32))
+    # two sequences that are not there: the others stay as they are, though the cuts move
+    told, table = list(p.lens), p.table.copy()
+    first, second = p.lens.index(longest), p.lens.index(128)
+    told[second], table[first, (longest - 1) // page // 2] = longest + 5000, -3
+    got = run(hip, p, q, 0.1, lens=told, table=table, bad=bad)
+    assert bad.to_host()[0] == min(first, second) and np.all(np.isnan(got[[first, second]]))
+    fine = [s for s in range(num) if s not in (first, second)]
+    assert rel_err(got[fine], ref[fine]) <= TOL_GEMM_F32
+
+
+def test_a_graph_serves_long_and_short_batches(hip):
+    from test_gpu_stream_scratch import Graph
+
+    lens = long_lengths(37, 32, 3500, 1)
+    p = Paged(37, lens, 1, 128, 16, "bf16")
+    q = queries(p, 128, 1)
+    kc, vc = p.upload()
+    home, side = Stream(), Stream()
+    desc, dq = hip.paged_sdpa_desc(p.cache, 128, 1, 3500), DeviceBuffer.from_host(q)
+    dl, out = DeviceBuffer.from_host(np.array(lens, np.int32)), DeviceBuffer(q.shape)
+    ws = hip.paged_sdpa_workspace(p.cache, desc)
+    call = lambda stream: hip.paged_sdpa(p.cache, desc, 0.1, dq, kc, vc, p.dev_table, dl, out, workspace=ws, stream=stream)
+    call(home.handle)
+    home.synchronize()
+    graph = Graph(home, call)
+    for step in ([n // 4 for n in lens], lens, [min(n, 3) for n in lens], lens, [0] * 32, [n // 3 for n in lens], lens):
+        _lib.load().fth_memcpy_h2d(dl.ptr, np.array(step, np.int32).ctypes.data, 128)
+        graph.replay(side)
+        hip.synchronize()
+        got = out.to_host()
+        assert rel_err(got, attention(q, p.k, p.v, 0.1, step)) <= TOL_GEMM_F32
+        call(home.handle)
+        hip.synchronize()
+        assert np.array_equal(got.view(np.uint32), out.to_host().view(np.uint32))
+    graph.free()
 
 
 def test_invalid_sequences_are_reported(hip):
