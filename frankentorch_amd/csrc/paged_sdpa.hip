@@ -656,6 +656,10 @@ template <typename T, int DP, bool FULL, bool NT, bool ANY, bool EVEN> __global_
     int seq = 0, hk = 0, raw = 0, split = 0, pos = 0, end = 0, within = 0;
     bool line = false;  // even shares
     if constexpr (EVEN) {
+        if (item >= p.even) {  // nothing to do either way? (most workgroups, where max_len is far above the lengths)
+            const int at = (int)p.by_pairs((uint32_t)item), len = lens[p.by_heads((uint32_t)(item - at * p.pairs))];
+            if (at >= p.nsplit || (at > 0 && (len <= at * p.share || len > p.most))) return;
+        }
         const int lane = threadIdx.x & 63, first = lane * p.seqs_a_lane, num_seqs = (int)p.c.num_seqs;
         const int last = num_seqs - first < p.seqs_a_lane ? num_seqs : first + p.seqs_a_lane;
         int mine = 0;
@@ -821,12 +825,16 @@ Plan plan(const fth_paged_cache &c, const fth_paged_sdpa_desc &d) {
     // would not make 128 workgroups (12 heads of 64, 1024 keys: 10.6 / 12.4; 8 of 128, 4096 keys: 13.4 / 14.7).
     // In a batch that fills the chip, shares of 512 KB where a sequence has more than 1 MB: the chip does not wait for the longest one
     // (64 of up to 8191 keys, bf16: 244 us in one share each, 224 in shares of 1 MB, 218 of 512 KB, 227 of 256 KB; 64 of up to 4000,
-    // fp32: 255, 232, 225, 234; 32 of up to 1000, fp32: 39 in one, 45 in 512 KB).
+    // fp32: 255, 232, 225, 234; 32 of up to 1000, fp32: 39 in one, 45 in 512 KB). At most 16 of the longest: where max_len is far
+    // above the lengths, workgroups without keys take the time (256 sequences of 300 keys, max_len 131072: 248 us in 128 shares, 96).
     const int64_t step = kTile * kWaves, least = units * fth::ceil_div(most, 256) <= 128 ? 128 : 256;
     static_assert(step == 1 << 7, "a step is a tile of every wavefront");
     const bool large = units >= 256 && most * key_bytes > (1 << 20);
     int64_t share = fth::ceil_div(most, units > 0 && units < 256 ? 256 / units : 1);
-    if (large) share = share < (512 << 10) / key_bytes ? share : (512 << 10) / key_bytes;
+    if (large) {
+        const int64_t part = fth::ceil_div(most, 16), cut = (512 << 10) / key_bytes > part ? (512 << 10) / key_bytes : part;
+        share = share < cut ? share : cut;
+    }
     share = share < least ? least : share;
     if (p.tiles && most <= 512) share = most;
     p.share = (int)(fth::ceil_div(share > 0 ? share : 1, step) * step);

@@ -166,3 +166,12 @@ def test_a_graph_serves_every_batch(hip):
         assert np.array_equal(got.view(np.uint32), eager.to_host().view(np.uint32))
         assert rel_err(got, attention(q, p.k, p.v, 0.1, step)) <= TOL_GEMM_F32
     graph.free()
+
+
+@pytest.mark.parametrize("lens", [[5, 300, 0, 131] * 16, [40] * 63 + [3000], [700] * 64], ids=lambda x: str(x[-1]))
+def test_a_bound_far_above_the_lengths(hip, lens):
+    p = Paged(38, lens, 4, 128, 16, "bf16", room=4096)
+    q = queries(p, 8, 1)
+    got, ref = run(hip, p, q, 0.1, max_len=65536), attention(q, p.k, p.v, 0.1, lens)
+    for s, n in enumerate(lens):
+        assert rel_err(got[s], ref[s]) <= TOL_GEMM_F32 if n else not got[s].any()
