@@ -153,6 +153,8 @@ class PagedDecoder:
         n = len(prompt)
         if n == 0 or self.length[seq]:
             raise ValueError("a prompt has at least one token and starts an empty sequence")
+        if n > self.max_len:  # (whole pages may hold more positions than the tables have)
+            raise ValueError("a prompt of %d tokens is longer than max_len, %d" % (n, self.max_len))
         self.kv.reserve(seq, n)
         desc = device.sdpa_desc_gqa(1, self.heads, self.kv_heads, n, n, self.hd, self.hd, True)
         for name, pitch in (("q", self.qkv), ("k", self.qkv), ("v", self.qkv), ("o", self.d)):

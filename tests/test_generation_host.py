@@ -1,0 +1,76 @@
+"""What generation decides on the host: which prompts, tokens and sequences it takes, and what it holds after an error. The device
+is left out: buffers are host arrays, the forward is a stand-in that gives logits of zeros."""
+import numpy as np
+import pytest
+
+from frankentorch_amd import device, generate
+from frankentorch_amd.generate import PagedDecoder
+
+VOCAB, D, HEADS, FFN = 50, 32, 2, 64
+
+
+class HostBuffer:
+    def __init__(self, shape, dtype=np.float32):
+        self.array = np.zeros(shape, dtype)
+        self.shape, self.dtype, self.size, self.nbytes, self.ptr = self.array.shape, self.array.dtype, self.array.size, self.array.nbytes, 64
+
+    @classmethod
+    def from_host(cls, array):
+        buf = cls(np.shape(array), np.asarray(array).dtype)
+        buf.array[...] = array
+        return buf
+
+    def to_host(self):
+        return self.array.copy()
+
+    def view(self, offset):
+        return self
+
+
+def put(buf, array):
+    array = np.ascontiguousarray(array, buf.dtype)
+    buf.array.reshape(-1)[:array.size] = array.reshape(-1)
+    return buf
+
+
+@pytest.fixture
+def make(monkeypatch):
+    """make(max_seqs, num_pages, max_len, rotation): a decoder whose forward notes its tokens in `seen`."""
+    monkeypatch.setattr(generate, "DeviceBuffer", HostBuffer)
+    monkeypatch.setattr(generate, "_put", put)
+    monkeypatch.setattr(device, "synchronize", lambda: None)
+    monkeypatch.setattr(device, "logits_process", lambda *a, **k: None)
+    monkeypatch.setattr(device, "argmax", lambda x, m, vocab, inner, best: best.array.fill(7))
+
+    def make(max_seqs=3, num_pages=12, max_len=20, rotation=False):
+        z = lambda *s: np.zeros(s, np.float32)
+        layer = dict(ln1_w=z(D), ln1_b=z(D), wq=z(D, D), bq=z(D), wk=z(D, D), bk=z(D), wv=z(D, D), bv=z(D), wo=z(D, D), bo=z(D), ln2_w=z(D), ln2_b=z(D), w1=z(FFN, D),
+                     b1=z(FFN), w2=z(D, FFN), b2=z(D))
+        model = PagedDecoder(z(VOCAB, D), None if rotation else z(max_len, D), [layer], z(D), z(D), HEADS, max_seqs, num_pages, max_len=max_len)
+        model.seen = []
+
+        def forward(ids, seqs, positions, attend, prompt=False):
+            model.seen.append((np.asarray(ids).tolist(), list(seqs), np.asarray(positions).tolist()))
+            return HostBuffer((max(len(ids), 1), D))
+
+        model._forward, model._gemm = forward, lambda *a, **k: None
+        return model
+
+    return make
+
+
+def state(model):
+    return len(model.kv.free), model.length.tolist(), model.kv.rows.tolist()
+
+
+@pytest.mark.parametrize("rotation", [False, True])
+@pytest.mark.parametrize("length", [21, 25, 32, 33, 40])
+def test_prompts_longer_than_max_len_are_refused(make, length, rotation):
+    """max_len is no multiple of the page: the pages would hold 32 positions, the positions' table has 20."""
+    model = make(max_len=20, rotation=rotation)
+    before = state(model)
+    with pytest.raises(ValueError):
+        model.prefill(0, [1] * length)
+    assert state(model) == before and not model.seen
+    model.prefill(0, [1] * 20)
+    assert model.length[0] == 20
