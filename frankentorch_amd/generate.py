@@ -148,6 +148,15 @@ class PagedDecoder:
         device.layer_norm(x, *self.lnf, h, t, d, self.eps)
         return h
 
+    def _tokens(self, tokens: Sequence[int]) -> np.ndarray:
+        """The ids of tokens, each of which has a row in the embedding."""
+        ids = np.asarray(tokens, np.float64)
+        with np.errstate(invalid="ignore"):
+            wrong = ~((ids >= 0) & (ids < self.vocab) & (ids == np.floor(ids)))
+        if wrong.any():
+            raise ValueError("token %s is outside the vocabulary of %d" % (ids[wrong][0], self.vocab))
+        return ids
+
     def prefill(self, seq: int, prompt: Sequence[int]) -> DeviceBuffer:
         """A whole prompt into the cache of an empty sequence; the logits [1, vocab] after its last token (a buffer of this object's)."""
         n = len(prompt)
@@ -155,6 +164,7 @@ class PagedDecoder:
             raise ValueError("a prompt has at least one token and starts an empty sequence")
         if n > self.max_len:  # (whole pages may hold more positions than the tables have)
             raise ValueError("a prompt of %d tokens is longer than max_len, %d" % (n, self.max_len))
+        ids = self._tokens(prompt)
         self.kv.reserve(seq, n)
         desc = device.sdpa_desc_gqa(1, self.heads, self.kv_heads, n, n, self.hd, self.hd, True)
         for name, pitch in (("q", self.qkv), ("k", self.qkv), ("v", self.qkv), ("o", self.d)):
@@ -166,7 +176,7 @@ class PagedDecoder:
         def attend(layer, qkv, out):
             device.sdpa_forward(desc, device.default_scale(self.hd), qkv.view(0), qkv.view(k_at), qkv.view(v_at), out)
 
-        hidden = self._forward(prompt, [seq] * n, np.arange(n), attend, prompt=True)
+        hidden = self._forward(ids, [seq] * n, np.arange(n), attend, prompt=True)
         self.length[seq] = n
         logits = self._buffer("prompt_logits", (1, self.vocab))
         self._gemm(hidden.view((n - 1) * self.d), self.wte, logits, 1, self.vocab, self.d)
@@ -179,6 +189,7 @@ class PagedDecoder:
             raise ValueError("a step takes different sequences, each after its prompt")
         if any(self.length[s] >= self.max_len for s in where):
             raise ValueError("a sequence is at max_len")
+        ids = self._tokens(tokens)
         for s in where:
             self.kv.reserve(s, int(self.length[s]) + 1)
         positions = self.length[where]
@@ -197,7 +208,7 @@ class PagedDecoder:
         def attend(layer, qkv, out):
             device.paged_sdpa(cache, desc, device.default_scale(self.hd), qkv, self.kv.k[layer], self.kv.v[layer], table, lens, out, workspace=work)
 
-        hidden = self._forward(tokens, where, positions, attend)
+        hidden = self._forward(ids, where, positions, attend)
         logits = self._buffer("logits", (n, self.vocab))
         self._gemm(hidden, self.wte, logits, n, self.vocab, self.d)
         return logits

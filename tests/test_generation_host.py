@@ -74,3 +74,23 @@ def test_prompts_longer_than_max_len_are_refused(make, length, rotation):
     assert state(model) == before and not model.seen
     model.prefill(0, [1] * 20)
     assert model.length[0] == 20
+
+
+@pytest.mark.parametrize("bad", [-1, VOCAB, VOCAB + 1000, -2 ** 40, 2 ** 40, 1.5, float("nan"), float("inf")], ids=str)
+def test_tokens_outside_the_vocabulary_are_refused(make, bad):
+    model = make()
+    before = state(model)
+    for prompt in ([bad], [1, 2, bad], [bad, 3]):
+        with pytest.raises(ValueError):
+            model.prefill(0, prompt)
+    assert state(model) == before and not model.seen
+    model.prefill(0, [0, VOCAB - 1])
+    model.prefill(1, [5.0])
+    before = state(model)
+    for tokens in ([bad, 1], [1, bad]):
+        with pytest.raises(ValueError):
+            model.step([0, 1], tokens)
+    assert state(model) == before and len(model.seen) == 2
+    model.step([0, 1], [VOCAB - 1, 0])
+    with pytest.raises(ValueError):
+        make().generate([[1], [2, bad]], 3)
