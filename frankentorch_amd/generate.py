@@ -159,7 +159,7 @@ class PagedDecoder:
 
     def prefill(self, seq: int, prompt: Sequence[int]) -> DeviceBuffer:
         """A whole prompt into the cache of an empty sequence; the logits [1, vocab] after its last token (a buffer of this object's)."""
-        n = len(prompt)
+        n, seq = len(prompt), range(len(self.length))[seq]  # (the kernels count from the front alone)
         if n == 0 or self.length[seq]:
             raise ValueError("a prompt has at least one token and starts an empty sequence")
         if n > self.max_len:  # (whole pages may hold more positions than the tables have)
@@ -184,12 +184,14 @@ class PagedDecoder:
 
     def step(self, seqs: Sequence[int], tokens: Sequence[int]) -> DeviceBuffer:
         """One more token of each of `seqs`; the logits [len(seqs), vocab] after them, in that order (a buffer of this object's)."""
-        n, where = len(seqs), list(seqs)
+        n, where = len(seqs), [range(len(self.length))[s] for s in seqs]
         if len(set(where)) != n or any(self.length[s] == 0 for s in where):
             raise ValueError("a step takes different sequences, each after its prompt")
         if any(self.length[s] >= self.max_len for s in where):
             raise ValueError("a sequence is at max_len")
         ids = self._tokens(tokens)
+        if ids.shape != (n,):
+            raise ValueError("%d sequences take one token each, not tokens of shape %s" % (n, ids.shape))
         for s in where:
             self.kv.reserve(s, int(self.length[s]) + 1)
         positions = self.length[where]

@@ -94,3 +94,25 @@ def test_tokens_outside_the_vocabulary_are_refused(make, bad):
     model.step([0, 1], [VOCAB - 1, 0])
     with pytest.raises(ValueError):
         make().generate([[1], [2, bad]], 3)
+
+
+@pytest.mark.parametrize("seqs,tokens", [([0, 1], [3]), ([0], [3, 4]), ([0, 1], []), ([0, 1], [[3, 4]]), ([0, -3], [3, 4]), ([-1, 2], [3, 4]), ([0, 3], [3, 4]), ([0, -4], [3, 4])], ids=str)
+def test_steps_of_sequences_and_tokens_that_do_not_pair_up(make, seqs, tokens):
+    """A token for every sequence; no sequence twice, whichever end of the batch its number counts from; none that is not there."""
+    model = make(max_seqs=3)
+    for s in range(3):
+        model.prefill(s, [s + 1])
+    before = state(model)
+    with pytest.raises((ValueError, IndexError)):
+        model.step(seqs, tokens)
+    assert state(model) == before and len(model.seen) == 3
+
+
+def test_a_sequence_counted_from_the_end_is_the_same_one(make):
+    model = make(max_seqs=3)
+    model.prefill(-1, [1, 2])
+    model.step([-1], [3])
+    model.step([2], [4])
+    assert model.length.tolist() == [0, 0, 4] and model.seen[1][1] == [2] and model.seen[2][2] == [3]
+    with pytest.raises(IndexError):
+        model.prefill(3, [1])
