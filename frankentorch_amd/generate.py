@@ -176,10 +176,14 @@ class PagedDecoder:
         def attend(layer, qkv, out):
             device.sdpa_forward(desc, device.default_scale(self.hd), qkv.view(0), qkv.view(k_at), qkv.view(v_at), out)
 
-        hidden = self._forward(ids, [seq] * n, np.arange(n), attend, prompt=True)
+        try:
+            hidden = self._forward(ids, [seq] * n, np.arange(n), attend, prompt=True)
+            logits = self._buffer("prompt_logits", (1, self.vocab))
+            self._gemm(hidden.view((n - 1) * self.d), self.wte, logits, 1, self.vocab, self.d)
+        except BaseException:
+            self.kv.release(seq)
+            raise
         self.length[seq] = n
-        logits = self._buffer("prompt_logits", (1, self.vocab))
-        self._gemm(hidden.view((n - 1) * self.d), self.wte, logits, 1, self.vocab, self.d)
         return logits
 
     def step(self, seqs: Sequence[int], tokens: Sequence[int]) -> DeviceBuffer:
@@ -223,8 +227,11 @@ class PagedDecoder:
                  allowed: Optional[Callable] = None, stop: Optional[int] = None):
         """Greedy continuations of the prompts, one list a prompt. repetition, frequency and presence are as in
         device.logits_process; bias [vocab] or None; allowed(prompt number, tokens so far) gives the tokens that may follow (a
-        bool array over the vocabulary) or None for all; a sequence ends with the token `stop`, after `new_tokens`, or at max_len."""
+        bool array over the vocabulary) or None for all; a sequence ends with the token `stop`, after `new_tokens`, or at max_len.
+        Uses the sequences 0 .. len(prompts) - 1, which have to be empty, and gives them back, after an error too."""
         n = len(prompts)
+        if n > len(self.length):
+            raise ValueError("%d prompts are more than max_seqs, %d" % (n, len(self.length)))
         tokens = [list(p) for p in prompts]
         done = [[] for _ in prompts]
         width = max(len(p) for p in prompts) + new_tokens
@@ -260,16 +267,19 @@ class PagedDecoder:
                 tokens[r].append(int(t))
                 done[r].append(int(t))
 
-        if new_tokens > 0:
-            for r, p in enumerate(prompts):
-                note([r], choose([r], self.prefill(r, p)))
-        for _ in range(new_tokens - 1):
-            rows = [r for r in range(n) if done[r][-1] != stop and self.length[r] < self.max_len]
-            if not rows:
-                break
-            note(rows, choose(rows, self.step(rows, [tokens[r][-1] for r in rows])))
-        for r in range(n):
-            if self.length[r]:
+        started = []
+        try:
+            for r, p in enumerate(prompts if new_tokens > 0 else []):
+                logits = self.prefill(r, p)
+                started.append(r)
+                note([r], choose([r], logits))
+            for _ in range(new_tokens - 1):
+                rows = [r for r in range(n) if done[r][-1] != stop and self.length[r] < self.max_len]
+                if not rows:
+                    break
+                note(rows, choose(rows, self.step(rows, [tokens[r][-1] for r in rows])))
+        finally:
+            for r in started:
                 self.release(r)
         return done
 

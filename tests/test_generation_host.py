@@ -116,3 +116,55 @@ def test_a_sequence_counted_from_the_end_is_the_same_one(make):
     assert model.length.tolist() == [0, 0, 4] and model.seen[1][1] == [2] and model.seen[2][2] == [3]
     with pytest.raises(IndexError):
         model.prefill(3, [1])
+
+
+def test_generate_gives_back_what_it_took(make):
+    """After an error in the middle the pages are free and the next call goes through."""
+    model = make(max_seqs=3, num_pages=5, max_len=64)
+    empty = state(model)
+    with pytest.raises(MemoryError):  # three prompts fit, their growth does not
+        model.generate([[1] * 16, [2] * 16, [3] * 32], 30)
+    assert state(model) == empty
+    with pytest.raises(MemoryError):  # the third prompt does not fit
+        model.generate([[1] * 30, [2] * 30, [3] * 33], 2)
+    assert state(model) == empty
+
+    def allowed(r, tokens):
+        if len(tokens) == 6:
+            raise KeyError("a grammar's own error")
+        return None
+
+    with pytest.raises(KeyError):
+        model.generate([[1] * 3, [2] * 4], 9, allowed=allowed)
+    assert state(model) == empty
+    with pytest.raises(ValueError):
+        model.generate([[1], [2] * 65], 2)
+    assert state(model) == empty
+    with pytest.raises(ValueError):  # more than max_seqs
+        model.generate([[1]] * 4, 2)
+    assert state(model) == empty
+    assert model.generate([[1] * 16, [2]], 3) == [[7] * 3] * 2 and state(model) == empty
+
+
+def test_generate_leaves_sequences_that_others_hold(make):
+    model = make(max_seqs=3)
+    model.prefill(1, [4] * 17)
+    held = state(model)
+    assert model.generate([[1], [2]], 0) == [[], []] and state(model) == held
+    with pytest.raises(ValueError):
+        model.generate([[1], [2]], 3)
+    assert state(model) == held
+    assert model.generate([[1]], 3) == [[7] * 3] and state(model) == held
+
+
+def test_a_prompt_whose_forward_fails_leaves_nothing(make):
+    model = make()
+    empty = state(model)
+
+    def forward(*a, **k):
+        raise MemoryError("no room for the activations")
+
+    model._forward = forward
+    with pytest.raises(MemoryError):
+        model.prefill(1, [1] * 18)
+    assert state(model) == empty
