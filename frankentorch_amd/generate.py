@@ -199,13 +199,12 @@ class PagedDecoder:
         for s in where:
             self.kv.reserve(s, int(self.length[s]) + 1)
         positions = self.length[where]
-        self.length[where] += 1
         # the rows of the batch are its sequences: their rows of the block table, their lengths
         cache = _lib.PagedCache.from_buffer_copy(self.kv.cache)
         cache.num_seqs = n
         table = _put(self._buffer("rows", (n, cache.max_pages), np.int32), self.kv.rows[where])
-        lens = _put(self._buffer("lens", (n,), np.int32), self.length[where])
-        longest = -(-int(self.length[where].max()) // 128) * 128
+        lens = _put(self._buffer("lens", (n,), np.int32), positions + 1)
+        longest = -(-(int(positions.max()) + 1) // 128) * 128
         desc = device.paged_sdpa_desc(cache, self.heads, 1, min(longest, cache.max_pages * cache.page_size))
         desc.q_seq_stride = desc.q_row_stride = self.qkv
         need = _lib.load().fth_dev_paged_sdpa_workspace_bytes(C.byref(cache), C.byref(desc))
@@ -217,6 +216,7 @@ class PagedDecoder:
         hidden = self._forward(ids, where, positions, attend)
         logits = self._buffer("logits", (n, self.vocab))
         self._gemm(hidden, self.wte, logits, n, self.vocab, self.d)
+        self.length[where] += 1
         return logits
 
     def release(self, seq: int) -> None:
@@ -230,7 +230,7 @@ class PagedDecoder:
         bool array over the vocabulary) or None for all; a sequence ends with the token `stop`, after `new_tokens`, or at max_len.
         Uses the sequences 0 .. len(prompts) - 1, which have to be empty, and gives them back, after an error too."""
         n = len(prompts)
-        if n > len(self.length):
+        if new_tokens > 0 and n > len(self.length):
             raise ValueError("%d prompts are more than max_seqs, %d" % (n, len(self.length)))
         tokens = [list(p) for p in prompts]
         done = [[] for _ in prompts]

@@ -168,3 +168,25 @@ def test_a_prompt_whose_forward_fails_leaves_nothing(make):
     with pytest.raises(MemoryError):
         model.prefill(1, [1] * 18)
     assert state(model) == empty
+
+
+def test_a_step_that_fails_adds_no_position(make):
+    """Neither a pool that runs dry nor an error on the way to the kernels counts a position whose keys were never stored."""
+    model = make(max_seqs=2, num_pages=3)
+    model.prefill(0, [1] * 16)
+    model.prefill(1, [2] * 16)
+    with pytest.raises(MemoryError):
+        model.step([0, 1], [3, 4])
+    assert model.length.tolist() == [16, 16]
+    forward = model._forward
+
+    def fails(*a, **k):
+        raise RuntimeError("no launch")
+
+    model._forward = fails
+    with pytest.raises(RuntimeError):
+        model.step([0], [3])
+    assert model.length.tolist() == [16, 16]
+    model._forward = forward
+    model.step([0], [3])
+    assert model.length.tolist() == [17, 16] and model.seen[-1] == ([3], [0], [16])
