@@ -253,6 +253,8 @@ class PagedDecoder:
                 may = None if allowed is None else allowed(r, tokens[r])
                 if may is not None:
                     bits[i, :self.vocab] = np.asarray(may, bool)
+                    if not bits[i, :self.vocab].any():
+                        raise ValueError("no token may follow prompt %d and the %d tokens after it" % (r, len(done[r])))
             _put(history, past)
             _put(counts, [len(tokens[r]) for r in rows])
             _put(given, [len(prompts[r]) for r in rows])

@@ -190,3 +190,16 @@ def test_a_step_that_fails_adds_no_position(make):
     model._forward = forward
     model.step([0], [3])
     assert model.length.tolist() == [17, 16] and model.seen[-1] == ([3], [0], [16])
+
+
+def test_a_mask_that_allows_no_token_is_an_error(make):
+    """There is no token to choose: all logits are minus infinity and the argmax would give token 0."""
+    model = make()
+    empty = state(model)
+    for after in (2, 4):
+        with pytest.raises(ValueError, match="prompt 1"):
+            model.generate([[1, 2], [3, 4]], 5, allowed=lambda r, tokens: np.full(VOCAB, r == 0 or len(tokens) != after))
+        assert state(model) == empty
+    one = np.zeros(VOCAB, bool)
+    one[VOCAB - 1] = True
+    assert len(model.generate([[1, 2]], 5, allowed=lambda r, tokens: one)[0]) == 5
