@@ -29,10 +29,10 @@ inline int32_t check_paged_cache(const fth_paged_cache *c, const char *who, int6
     FTH_ARG(c->head_dim >= 1 && c->head_dim <= 256, "%s: head_dim %lld is outside 1..256", who, (long long)c->head_dim);
     FTH_ARG(c->page_stride >= c->head_dim && c->head_stride >= c->head_dim && c->row_stride >= c->head_dim, "%s: a stride of the cache is below head_dim", who);
     FTH_ARG(c->table_stride >= c->max_pages, "%s: table_stride is below max_pages", who);
-    // page numbers, positions, sequences and heads are 32-bit numbers in the kernels
+    // page numbers, positions, sequences and heads are 32-bit numbers in the kernels, and so is the divisor of positions
     const int64_t most = 2147483647LL;
     int64_t positions = 0, pages = 0, heads = 0, rows = 0, table = 0;
-    bool over = c->num_pages > most || c->num_seqs > most || c->kv_heads > most || __builtin_mul_overflow(c->max_pages, c->page_size, &positions) || positions > most;
+    bool over = c->num_pages > most || c->num_seqs > most || c->kv_heads > most || c->page_size > most || __builtin_mul_overflow(c->max_pages, c->page_size, &positions) || positions > most;
     over = over || __builtin_mul_overflow(c->num_pages, c->page_stride, &pages) || __builtin_mul_overflow(c->kv_heads, c->head_stride, &heads) ||
            __builtin_mul_overflow(c->page_size, c->row_stride, &rows) || __builtin_mul_overflow(c->num_seqs, c->table_stride, &table);
     const int64_t half = (int64_t)1 << 58;  // bytes of every offset fit 62 bits
