@@ -277,7 +277,7 @@ int32_t fth_dev_paged_append_f32(const fth_paged_cache *c, const fth_paged_appen
     FTH_ARG(d->rotary_dim == 0 || d->max_pos >= 0, "paged_append: negative max_pos");
     for (int64_t x : {d->q_row_stride, d->q_head_stride, d->k_row_stride, d->k_head_stride, d->v_row_stride, d->v_head_stride, d->out_row_stride, d->out_head_stride})
         FTH_ARG(fth::stride_in_range(x), "paged_append: a stride is negative or over 2^40");
-    if (d->q_heads + c->kv_heads > (1 << 20) || d->tokens > 2147483647LL) return fth::set_error(FTH_ERR_SIZE_OVERFLOW, "paged_append: extents overflow");
+    if (d->q_heads > (1 << 20) || d->q_heads + c->kv_heads > (1 << 20) || d->tokens > 2147483647LL) return fth::set_error(FTH_ERR_SIZE_OVERFLOW, "paged_append: extents overflow");
     if (d->tokens > 0) {
         FTH_ARG(positions && (k != nullptr) == (v != nullptr) && (k || d->q_heads > 0), "paged_append: NULL operand");
         FTH_ARG(!k || (seq_ids && (block_table || c->max_pages == 0) && ((k_cache && v_cache) || c->num_pages == 0)), "paged_append: NULL cache, table or sequences");

@@ -21,3 +21,11 @@ def test_pages_longer_than_any_position(page_size, rows):
     assert lib.fth_dev_paged_sdpa_workspace_bytes(C.byref(c), C.byref(device.paged_sdpa_desc(c, 4))) == 0
     kw["page_size"] = (1 << 31) - 1
     assert attend(cache(**kw), 0) in OK
+
+
+@pytest.mark.parametrize("q_heads", [(1 << 63) - 1, (1 << 63) - 2, (1 << 62), (1 << 20) + 1, 1 << 20])
+def test_heads_whose_sum_overflows(q_heads):
+    """Queries and K/V heads together are at most 2^20, also where their sum is no 64-bit number."""
+    for tokens in (0, 1):
+        assert append(cache(), tokens, q_heads=q_heads) == OVERFLOW
+    assert append(cache(), 0, q_heads=(1 << 20) - 2) in OK
