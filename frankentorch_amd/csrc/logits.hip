@@ -95,13 +95,14 @@ template <bool NTB, bool NTS> __global__ __launch_bounds__(kThreads) void logits
                     else atomicAdd(&seen[at], 1u);
                 }
             };
-            for (int i = (int)threadIdx.x * 4; i < count; i += kThreads * 4) {
-                if (i + 4 <= count) {
+            // (unsigned: the step past the end of 2^31 - 1 tokens is a number too)
+            for (uint32_t i = threadIdx.x * 4; i < (uint32_t)count; i += kThreads * 4) {
+                if (i + 4 <= (uint32_t)count) {
                     const I4u ids = *reinterpret_cast<const I4u *>(history + i);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) note(ids[e], i + e);
+                    for (int e = 0; e < 4; ++e) note(ids[e], (int)i + e);
                 } else {
-                    for (int e = i; e < count; ++e) note(history[e], e);
+                    for (int e = (int)i; e < count; ++e) note(history[e], e);
                 }
             }
         }
