@@ -197,19 +197,22 @@ template <> struct Chunk<float> {
 // lies in [2^kTop, 2^(kTop + 1)), and cut into parts of the keys' type whose sum it is (bf16: 3 x 8 bits; f16: 2 x 11 bits, off by
 // 2^-22 of an element or 2^-39 of the largest).
 template <typename T> struct Parts {  // fp32 keys and values: none
-    static constexpr int kParts = 0, kArray = 1, kTop = 0, kWeight = 0;
+    static constexpr int kParts = 0, kArray = 1, kTop = 0;
+    static constexpr float kScale = 1.f;  // of the weights that are cut
     using Vec = __attribute__((ext_vector_type(8))) _Float16;
     static __device__ __forceinline__ F4 mfma(const U4 &, const U4 &, F4 c) { return c; }
 };
 template <> struct Parts<fth::bf16> {
-    static constexpr int kParts = 3, kArray = 3, kTop = 0, kWeight = 64;
+    static constexpr int kParts = 3, kArray = 3, kTop = 0;
+    static constexpr float kScale = 0x1p64f;
     using Vec = __attribute__((ext_vector_type(8))) __bf16;
     static __device__ __forceinline__ F4 mfma(const U4 &a, const U4 &b, F4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Vec, a), __builtin_bit_cast(Vec, b), c, 0, 0, 0);
     }
 };
 template <> struct Parts<fth::f16> {
-    static constexpr int kParts = 2, kArray = 2, kTop = 14, kWeight = 14;
+    static constexpr int kParts = 2, kArray = 2, kTop = 14;
+    static constexpr float kScale = 0x1p14f;
     using Vec = __attribute__((ext_vector_type(8))) _Float16;
     static __device__ __forceinline__ F4 mfma(const U4 &a, const U4 &b, F4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(Vec, a), __builtin_bit_cast(Vec, b), c, 0, 0, 0);
@@ -474,8 +477,9 @@ __device__ __forceinline__ void tiles_segment(const PagedArgs &p, float *lds_o, 
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[e][r] *= alpha;
         }
-        // nothing visible so far: every weight is exp(-inf) = 0
-        const float ref = (m_run == -__builtin_inff() ? 0.f : m_run) - (parts ? (float)Parts<T>::kWeight : 0.f);
+        // nothing visible so far: every weight is exp(-inf) = 0. The power of two that parts are scaled by is a factor, not a part of the
+        // exponent, which would be rounded by it (64 more: weights off by 22 units of 2^-24).
+        const float ref = m_run == -__builtin_inff() ? 0.f : m_run;
         float w[8];
 #pragma unroll
         for (int s = 0; s < 2; ++s)
@@ -483,6 +487,7 @@ __device__ __forceinline__ void tiles_segment(const PagedArgs &p, float *lds_o, 
             for (int r = 0; r < 4; ++r) {
                 w[4 * s + r] = __builtin_amdgcn_exp2f(sc[s][r] - ref);
                 l_run += w[4 * s + r];
+                if constexpr (parts) w[4 * s + r] *= Parts<T>::kScale;
             }
         if constexpr (!more) {  // weight 0 times what an unused row holds would be NaN
             if (key0 + kTile > key_hi) {
@@ -564,23 +569,22 @@ __device__ __forceinline__ void tiles_segment(const PagedArgs &p, float *lds_o, 
         for (; t + kWaves < tiles; t += kWaves) step(t, Yes(), parts);
         step(t, No(), parts);
     };
-    float weight = 0.f;  // the exponent of two in the weights
     if (wave < tiles) {
         if constexpr (kParts == 0) {
             walk(No());
         } else {
             walk(Yes());
-            weight = (float)Parts<T>::kWeight;
             float check = 0.f;
 #pragma unroll
             for (int e = 0; e < NE; ++e)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) check = __builtin_fmaf(o[e][r] * 0x1p28f, 0.f, check);
+                for (int r = 0; r < 4; ++r) {
+                    check = __builtin_fmaf(o[e][r], 0.f, check);
+                    o[e][r] *= 1.f / Parts<T>::kScale;
+                }
             // What is not finite in V meets the parts of a weight, not the weight, and large values times the scaled weights
-            // may overflow (here or when shares are added up) where they do not: from 2^100 on once more on fp32 units, unless
-            // the query row gives NaN anyway.
+            // may overflow where they do not: once more on fp32 units, unless the query row gives NaN anyway.
             if (__any(!(check == 0.f) && finite)) {
-                weight = 0.f;
                 m_run = -__builtin_inff();
                 l_run = 0.f;
 #pragma unroll
@@ -602,7 +606,7 @@ __device__ __forceinline__ void tiles_segment(const PagedArgs &p, float *lds_o, 
     const float l_wave = rows_reduce(l_run, AddOp());
     if constexpr (ANY) bad = __any(bad);
     if (g == 0) {
-        lds_ml[(wave * 16 + lr) * 2] = m_run - weight;  // weights times 2^k relative to m are weights relative to m - k
+        lds_ml[(wave * 16 + lr) * 2] = m_run;
         lds_ml[(wave * 16 + lr) * 2 + 1] = bad ? __builtin_nanf("") : l_wave;
     }
 #pragma unroll
