@@ -44,3 +44,46 @@ def test_two_weights(hip, dtype, i, j, n):
     got, ref = run(hip, p, q, 1.0), attention(q, p.k, p.v, 1.0, p.lens)
     assert np.all(got[ref == 0] == 0)
     assert np.max(np.abs(got - ref)[ref != 0] / ref[ref != 0]) <= 10.25 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype,page,d", [("f32", 16, 64), ("f16", 16, 64), ("bf16", 16, 64), ("f16", 5, 64), ("f16", 16, 128), ("f16", 16, 256), ("f16", 16, 40), ("f16", 16, 7)])
+@pytest.mark.parametrize("n", [2, 33, 512, 1500])
+def test_values_under_small_weights(hip, dtype, page, d, n):
+    """One key has nearly all the weight and zeros in V: the outputs are those of the keys 5 to 80 nats below it, relative to themselves as
+    exact as any."""
+    depths = [5, 12, 16, 20, 25, 28, 40, 60, 80]
+    for heavy in {0, n // 2, n - 1}:
+        scores = -np.array(depths, np.float64)[:, None] + synth.uniform(42, "s", (len(depths), n), -1.0, 1.0)
+        scores[:, heavy] = 0
+        values = synth.normal(42, "v", (len(depths), n, d))
+        values[:, heavy] = 0
+        p = scored(42, [n] * len(depths), scores, d, page, dtype, values)
+        q = np.zeros((len(depths), 2, 3, d), np.float32)
+        q[..., 0] = np.array([1, 0.5, 0.75], np.float32)
+        if heavy == n - 1:
+            q[:, 0] = 0  # the first of the two tokens does not see the key
+        got, ref = run(hip, p, q, 1.0), attention(q, p.k, p.v, 1.0, p.lens)
+        for s, depth in enumerate(depths):
+            for h in range(3):
+                size = np.abs(ref[s, 1, h]).max()
+                assert np.abs(got - ref)[s, 1, h].max() <= TOL_GEMM_F32 * size, (heavy, depth, h)
+
+
+@pytest.mark.parametrize("dtype,d", [("f32", 64), ("f16", 64), ("bf16", 64), ("f16", 128), ("f16", 256)])
+@pytest.mark.parametrize("n", [64, 700])
+@pytest.mark.parametrize("order", ["mixed", "rising", "falling"])
+def test_weights_of_every_size(hip, dtype, d, n, order):
+    """Scores from 0 down to -80; column c of V is zero under all keys above -80 c / d and positive under the others: it is decided by weights of
+    one size, which differs from column to column."""
+    scores = -80.0 * synth.uniform(43, "s", (3, n))
+    if order != "mixed":
+        scores = np.sort(scores, 1) if order == "rising" else -np.sort(-scores, 1)
+    scores = from_storage(to_storage(scores.astype(np.float32), dtype), dtype).astype(np.float64)
+    values = 0.5 + synth.uniform(43, "v", (3, n, d))
+    values[scores[:, :, None] > -80.0 * np.arange(d) / d] = 0
+    p = scored(43, [n] * 3, scores, d, 16, dtype, values)
+    q = np.zeros((3, 1, 2, d), np.float32)
+    q[..., 0] = 1
+    got, ref = run(hip, p, q, 1.0), attention(q, p.k, p.v, 1.0, p.lens)
+    assert np.all(got[ref == 0] == 0)
+    assert np.max(np.abs(got - ref)[ref != 0] / ref[ref != 0]) <= TOL_GEMM_F32
