@@ -4,6 +4,7 @@ import pytest
 
 from frankentorch_amd import _lib
 from frankentorch_amd.device import DeviceBuffer
+from test_gpu_logits import ALL, make, plain, run
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +35,31 @@ def test_a_history_of_as_many_tokens_as_a_length_can_say(hip, n):
     want[3] = np.float32(-0.5) * np.float32(n - 3) - np.float32(0.25)  # counts are rounded to fp32
     want[[6, 1]] = -0.75
     assert np.array_equal(out.to_host()[0], want)
+
+
+@pytest.mark.parametrize("rows,vocab,width", [(130, 65537, 900), (260, 32769, 300), (1030, 4097, 40), (700, 8195, 0), (40, 65537, 500), (2048, 1000, 20), (2048, 1024, 33)])
+@pytest.mark.parametrize("shared", [False, True])
+def test_two_steps_a_stretch_and_outputs_past_the_caches(hip, rows, vocab, width, shared):
+    """From 2048 steps of 4096 logits on a workgroup takes two of them, and from 2^21 logits on outputs go past the caches."""
+    m = make(61, rows, vocab, width)
+    edge = np.array([0, 4095, 4096, 8191, 8192, vocab - 1], np.int32)
+    m["history"][:, :6] = edge[edge < vocab][np.arange(min(6, width)) % len(edge[edge < vocab])] if width else 0
+    bad = DeviceBuffer((1,), np.int64)
+    want = plain(m, ALL, np.float32, shared)
+    assert np.array_equal(run(hip, m, ALL, shared, bad=bad), want) and bad.to_host()[0] == -1
+    assert np.array_equal(run(hip, m, ALL, shared, in_place=True), want)
+    assert np.array_equal(run(hip, m, ALL, shared, pad=3, lead=1), want)
+    use = ("bias", "mask")  # no history: one step a stretch
+    assert np.array_equal(run(hip, m, use, shared), plain(m, use, np.float32, shared))
+
+
+def test_invalid_rows_among_many(hip):
+    m = make(62, 130, 65537, 64)
+    m["hlen"][:], m["plen"][:] = 64, 20
+    m["history"][7, 63], m["history"][99, 0], m["hlen"][129] = 65537, -1, 65
+    want = plain({**m, "history": np.clip(m["history"], 0, 65536), "hlen": np.minimum(m["hlen"], 64)}, ALL, np.float32)
+    bad = DeviceBuffer((1,), np.int64)
+    got = run(hip, m, ALL, bad=bad)
+    hurt = [7, 99, 129]
+    assert bad.to_host()[0] == 7 and np.all(got[hurt] == 7.0)
+    assert np.array_equal(np.delete(got, hurt, 0), np.delete(want, hurt, 0))
