@@ -20,8 +20,7 @@ __device__ __forceinline__ void report_bad_entry(int64_t *bad, int64_t at) {
     if (bad) atomicMin(reinterpret_cast<unsigned long long *>(bad), (unsigned long long)at);
 }
 
-// The descriptor of a cache; on return *elements is the index past its last element.
-inline int32_t check_paged_cache(const fth_paged_cache *c, const char *who, int64_t *elements) {
+inline int32_t check_paged_cache(const fth_paged_cache *c, const char *who) {
     FTH_ARG(c, "%s: NULL cache descriptor", who);
     FTH_ARG(c->dtype == FTH_DTYPE_F32 || c->dtype == FTH_DTYPE_F16 || c->dtype == FTH_DTYPE_BF16, "%s: a cache holds F32, F16 or BF16, not dtype %d", who, c->dtype);
     FTH_ARG(c->num_pages >= 0 && c->num_seqs >= 0 && c->max_pages >= 0, "%s: negative extent", who);
@@ -37,7 +36,6 @@ inline int32_t check_paged_cache(const fth_paged_cache *c, const char *who, int6
            __builtin_mul_overflow(c->page_size, c->row_stride, &rows) || __builtin_mul_overflow(c->num_seqs, c->table_stride, &table);
     const int64_t half = (int64_t)1 << 58;  // bytes of every offset fit 62 bits
     if (over || pages > half || heads > half || rows > half || table > half) return set_error(FTH_ERR_SIZE_OVERFLOW, "%s: the cache's extents overflow", who);
-    if (elements) *elements = pages + heads + rows;
     return FTH_OK;
 }
 

@@ -269,7 +269,7 @@ void fth_dev_paged_cache_contiguous(fth_paged_cache *c, int64_t num_pages, int64
 int32_t fth_dev_paged_append_f32(const fth_paged_cache *c, const fth_paged_append_desc *d, const float *q, const float *k, const float *v, const float *cosines,
                                  const float *sines, const int32_t *block_table, const int32_t *seq_ids, const int32_t *positions, float *q_out, void *k_cache,
                                  void *v_cache, int64_t *bad_index, fth_stream s) {
-    if (int32_t rc = fth::check_paged_cache(c, "paged_append", nullptr)) return rc;
+    if (int32_t rc = fth::check_paged_cache(c, "paged_append")) return rc;
     FTH_ARG(d, "paged_append: NULL descriptor");
     FTH_ARG(d->tokens >= 0 && d->q_heads >= 0, "paged_append: negative extent");
     FTH_ARG(d->rotary_dim >= 0 && d->rotary_dim % 2 == 0 && d->rotary_dim <= c->head_dim, "paged_append: rotary_dim %lld is odd or outside 0..head_dim",

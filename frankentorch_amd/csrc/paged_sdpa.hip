@@ -925,7 +925,7 @@ size_t workspace_bytes_of(const Plan &p, const fth_paged_cache &c) {
 }
 
 int32_t check(const fth_paged_cache *c, const fth_paged_sdpa_desc *d) {
-    if (int32_t rc = fth::check_paged_cache(c, "paged_sdpa", nullptr)) return rc;
+    if (int32_t rc = fth::check_paged_cache(c, "paged_sdpa")) return rc;
     FTH_ARG(d, "paged_sdpa: NULL descriptor");
     if (d->q_heads > (1 << 24)) return fth::set_error(FTH_ERR_SIZE_OVERFLOW, "paged_sdpa: more than 2^24 query heads");
     FTH_ARG(d->q_heads >= 1 && d->q_heads % c->kv_heads == 0, "paged_sdpa: %lld query heads on %lld K/V heads", (long long)d->q_heads, (long long)c->kv_heads);
