@@ -13,8 +13,8 @@
 //     (64 rows of 50257: 9.9 us, past the caches 11.5). Outputs over 8 MiB are stored past them (200 rows 72 -> 60 us; 64 rows
 //     11.1 -> 9.5, and the argmax after it as fast as before in all: 27 us; 8 rows lose 1.2 of 22 us with the argmax).
 //
-// Measured: 200 rows of 131071, a bias each, a mask, up to 8000 tokens before 60 us (318 MB, 5.3 TB/s; one entry a thread and
-// stretches of 4096: 143); 64 rows of 50257, one bias, a mask 7.9 us (27 MB; 17.3); one row 4.6 us.
+// Measured: 200 rows of 131071, a bias each, a mask, up to 8000 tokens before 57 us (322 MB, 5.6 TB/s; one entry a thread and
+// stretches of 4096: 143); 64 rows of 50257, one bias, a mask 7.7 us (27 MB; 17.3); one row 4.0 us.
 
 #include <type_traits>
 

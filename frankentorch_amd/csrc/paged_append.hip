@@ -5,9 +5,9 @@
 // two threads touch one element. -ffp-contract=off rounds a c, b s and their difference one by one.
 // What 128-bit accesses cannot take goes element by element.
 //
-// Measured: three prompts of up to 7001 tokens, 32 query and 8 K/V heads of 128, f16 (712 MB) 112 us, 6.3 TB/s, what a copy of that
-// size reaches (through the caches 134; element by element 447); eight of up to 1024 tokens, 12 heads of 64, fp32 (68 MB) 13.6 us
-// (50); a step of 64 sequences 3.7 us. Four tokens a workgroup where it holds all heads of one are slower (22 us for the eight
+// Measured: three prompts of up to 7001 tokens, 32 query and 8 K/V heads of 128, f16 (712 MB) 109 us, 6.5 TB/s, what a copy of that
+// size reaches (through the caches 134; element by element 447); eight of up to 1024 tokens, 12 heads of 64, fp32 (68 MB) 13 us
+// (50); a step of 64 sequences 3.8 us. Four tokens a workgroup where it holds all heads of one are slower (22 us for the eight
 // prompts: registers), and so is a workgroup that looks the next token up while this one's rows are on their way (145 us for the three).
 
 #include <type_traits>

@@ -3,16 +3,18 @@
 //   out[s, i, h] = sum_j w_j v_j / sum_j w_j,   w_j = exp(x_j - max x),   x_j = scale q . k_j,   j < lens[s] - new_tokens + i + 1
 //
 // Bound by reading the cache once. The keys of a sequence are cut into shares; a workgroup takes one share of one K/V head for up to
-// 16 of the query rows that read it (query heads of the group x new tokens), so K and V are read once for all of them. Shares
-// have one length, or, in large batches of long sequences, are cut from the keys of the whole batch end to end, so that the chip does
+// 16 of the query rows that read it (query heads of the group x new tokens), so K and V are read once for all of them. Every 16 rows
+// more walk the share again, from the L2 that the first 16 have filled, and pay its products, loads and unpacking again (32 sequences of up to 3967 keys,
+// 8 K/V heads of 128, bf16, 304 MB: 8 rows a K/V head 67 us, 16 70, 32 90, 64 144). Shares have one length, or, in large batches of long sequences, are cut from the keys of the whole batch end to end, so that the chip does
 // not wait for the longest ones (see steps_of). The four wavefronts of a workgroup walk a share in tiles of 32 keys, each on its own (running
 // maximum and sum per row in fp32, no barrier), and are joined through LDS at the end; a second small kernel joins the shares of a
 // row in order.
 //   * S^T[key, row] = K . Q^T with a key row and a query row per lane (16 x 16 tiles); the lane that gets scores of row lr holds
 //     them as it needs them for O^T[d, row] += V^T . P^T, so P never moves; V rows are read whole (16 lanes side by side).
 //   * 16-bit caches: both products run on the 16-bit matrix units against the bits as they are stored. The fp32 side is cut into
-//     parts of the storage type whose sum it is (struct Parts), so that the result is that of fp32 arithmetic; what parts cannot
-//     do (values that are not finite) is found and computed again. fp32 caches: fp32 matrix units, 16 times slower a product.
+//     parts of the storage type whose sum it is (struct Parts), so that the result is that of fp32 arithmetic but for queries against f16
+//     keys (22 bits of an element, or 2^-39 of the row's largest); what parts cannot do (values that are not finite) is found
+//     and computed again, small weights of f16 caches are cut more than once. fp32 caches: fp32 matrix units, 16 times slower a product.
 //   * The loads of the next tile's K go out when the scores have consumed this one's, those of V after the outputs have, with
 //     nothing conditional in between: the waits are then for K or V alone, never for both.
 // Pages: with a page size that is a multiple of 16 each half tile lies in one page, whose number is a scalar load one tile
@@ -21,8 +23,8 @@
 //
 // Measured: 64 sequences of 1024 to 8191 keys, 32 query heads on 8 K/V heads of 128, bf16 (1.22 GB): 7.6 ms on one wavefront a
 // row, 283 us with both products on fp32 units, 235 with the scores on 16-bit ones (MFMA-busy 0.31, wavefronts waiting to
-// issue), 212 + 5 with both in shares of 512 KB, 194 + 5 in even ones (6.3 TB/s; a kernel that only reads pages of 4 KB in random
-// order reaches 5.9, with nontemporal loads 6.7). One sequence of 131071: 85 + 5 us (6.3 TB/s). Joining the shares in the last workgroup to arrive instead of a
+// issue), 212 + 5 with both in shares of 512 KB, 192 + 5 in even ones (6.4 TB/s; a kernel that only reads pages of 4 KB in random
+// order reaches 5.9, with nontemporal loads 6.7). One sequence of 131071: 80 + 5 us (6.7 TB/s). Joining the shares in the last workgroup to arrive instead of a
 // second launch was slower in every case (release and acquire across the XCDs): 90 -> 109 us.
 
 #include <type_traits>
@@ -193,6 +195,8 @@ template <> struct Chunk<float> {
     static __device__ __forceinline__ float get(const U4 &v, int e) { return __uint_as_float(v[e]); }
 };
 
+// (Registers: the fp32 instances for heads of 256 spill 10 to 56 of them, those with even shares the most.)
+//
 // Scores against 16-bit keys go to the 16-bit matrix units: a query row is scaled by a power of two so that its largest element
 // lies in [2^kTop, 2^(kTop + 1)), and cut into parts of the keys' type whose sum it is (bf16: 3 x 8 bits; f16: 2 x 11 bits, off by
 // 2^-22 of an element or 2^-39 of the largest). Weights, of which the smallest may be all that V lets through, are cut into as many
@@ -876,7 +880,9 @@ Plan plan(const fth_paged_cache &c, const fth_paged_sdpa_desc &d) {
     const int64_t key_bytes = 2 * c.head_dim * (c.dtype == FTH_DTYPE_F32 ? 4 : 2);
     // Shares of one length: about 256 workgroups, of 256 keys at least. A join costs 4 to 5 us, so nothing is cut that fills the chip whole (32
     // sequences of 1000 keys: 18.6 us in one share, 23.6 in two) or has 512 keys (8 K/V heads of 128: 10.5 / 12.0). 128 keys where 256
-    // would not make 128 workgroups (12 heads of 64, 1024 keys: 10.6 / 12.4; 8 of 128, 4096 keys: 13.4 / 14.7).
+    // would not make 128 workgroups (12 heads of 64, 1024 keys: 10.6 / 12.4; 8 of 128, 4096 keys: 13.4 / 14.7). From 129 workgroups on one
+    // share each (8 heads of 128, up to 4000 keys, bf16, one / two shares: 24 sequences 57 / 63.5, 31 64 / 69, fp32 24 123 / 136, up to 1000 keys 15.3 / 20;
+    // 17 sequences 51.5 / 42.7).
     // In a batch that fills the chip, shares of 512 KB where a sequence has more than 1 MB: the chip does not wait for the longest one
     // (64 of up to 8191 keys, bf16: 244 us in one share each, 224 in shares of 1 MB, 218 of 512 KB, 227 of 256 KB; 64 of up to 4000,
     // fp32: 255, 232, 225, 234; 32 of up to 1000, fp32: 39 in one, 45 in 512 KB). At most 16 of the longest: where max_len is far
@@ -910,7 +916,9 @@ Plan plan(const fth_paged_cache &c, const fth_paged_sdpa_desc &d) {
     }
     // Nontemporal loads for what the 256 MB last-level cache cannot hold until the next call, if sequences are half of max_len on
     // average, and that is read once (us, with / without: one sequence of 131071, bf16 87 / 99, fp32 180 / 196; 64 of up to 8191,
-    // bf16 217 / 229 in shares of 512 KB; 16 of up to 3967, four queries, f16, 260 MB 38.5 / 36.3, fp32, 520 MB 79 / 72).
+    // bf16 217 / 229 in shares of 512 KB; 16 of up to 3967, four queries, f16, 260 MB 38.5 / 36.3, fp32, 520 MB 79 / 72; by the even
+    // shares of today 196 / 220). The host knows the bound alone: where it is far above the lengths, calls that read one cache again and
+    // again lose (under 131072: 4 sequences of 3000 keys 47.5 / 34, 16 of 1000 22.4 / 17.2, 64 of 300 or 600 level).
     p.nt = p.row_tiles == 1 && 2.0 * (double)c.num_seqs * (double)most * (double)c.kv_heads * (double)c.head_dim * (c.dtype == FTH_DTYPE_F32 ? 4 : 2) > 500.0 * (1 << 20);
     return p;
 }

@@ -438,9 +438,10 @@ int32_t fth_dev_sdpa_forward_masked_f64(const fth_sdpa_desc *d, double scale, co
  * + (p % page_size) * row_stride + c]. Any page may belong to several sequences (a shared prompt), in any order. Entries of a
  * sequence's row of the table past its last page are not read. dtype is the storage type (FTH_DTYPE_F32, F16 or BF16; stores
  * round to nearest even, and what is over the largest F16 becomes infinite); queries, new keys and values, and outputs are
- * fp32, and so is all arithmetic. The reference has no cache: its decoder recomputes every position. */
+ * fp32, and so is all arithmetic, with one exception: against an F16 cache each element of a query counts with 22 bits, or to 2^-39 of the
+ * largest element of its row. The reference has no cache: its decoder recomputes every position. */
 typedef struct fth_paged_cache {
-    int64_t num_pages, page_size, kv_heads, head_dim; /* head_dim <= 256 */
+    int64_t num_pages, page_size, kv_heads, head_dim; /* head_dim <= 256, the others and max_pages * page_size below 2^31 */
     int64_t page_stride, head_stride, row_stride;     /* elements, each >= head_dim */
     int64_t num_seqs, max_pages, table_stride;        /* rows, usable columns and row pitch of block_table (int32) */
     int32_t dtype;
