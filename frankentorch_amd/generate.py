@@ -148,9 +148,12 @@ class PagedDecoder:
         device.layer_norm(x, *self.lnf, h, t, d, self.eps)
         return h
 
-    def _tokens(self, tokens: Sequence[int]) -> np.ndarray:
-        """The ids of tokens, each of which has a row in the embedding."""
+    def _tokens(self, tokens: Sequence[int], n: int) -> np.ndarray:
+        """The ids of n tokens, each of which has a row in the embedding."""
         ids = np.asarray(tokens, np.float64)
+        if len(ids) != n or ids.size != n:
+            raise ValueError("%d tokens are asked for, not an array of %s" % (n, ids.shape))
+        ids = ids.reshape(-1)
         with np.errstate(invalid="ignore"):
             wrong = ~((ids >= 0) & (ids < self.vocab) & (ids == np.floor(ids)))
         if wrong.any():
@@ -164,7 +167,7 @@ class PagedDecoder:
             raise ValueError("a prompt has at least one token and starts an empty sequence")
         if n > self.max_len:  # (whole pages may hold more positions than the tables have)
             raise ValueError("a prompt of %d tokens is longer than max_len, %d" % (n, self.max_len))
-        ids = self._tokens(prompt)
+        ids = self._tokens(prompt, n)
         self.kv.reserve(seq, n)
         desc = device.sdpa_desc_gqa(1, self.heads, self.kv_heads, n, n, self.hd, self.hd, True)
         for name, pitch in (("q", self.qkv), ("k", self.qkv), ("v", self.qkv), ("o", self.d)):
@@ -193,9 +196,7 @@ class PagedDecoder:
             raise ValueError("a step takes different sequences, each after its prompt")
         if any(self.length[s] >= self.max_len for s in where):
             raise ValueError("a sequence is at max_len")
-        ids = self._tokens(tokens)
-        if ids.shape != (n,):
-            raise ValueError("%d sequences take one token each, not tokens of shape %s" % (n, ids.shape))
+        ids = self._tokens(tokens, n)
         for s in where:
             self.kv.reserve(s, int(self.length[s]) + 1)
         positions = self.length[where]

@@ -203,3 +203,18 @@ def test_a_mask_that_allows_no_token_is_an_error(make):
     one = np.zeros(VOCAB, bool)
     one[VOCAB - 1] = True
     assert len(model.generate([[1, 2]], 5, allowed=lambda r, tokens: one)[0]) == 5
+
+
+def test_columns_of_tokens(make):
+    """An array with one token a row is those tokens; more than one a row are not."""
+    model = make()
+    model.prefill(0, np.array([[4], [5], [6]]))
+    model.prefill(1, np.array([7]))
+    model.step([0, 1], np.array([[8], [9]], np.int32))
+    assert model.length.tolist() == [4, 2, 0] and [s[0] for s in model.seen] == [[4, 5, 6], [7], [8, 9]]
+    for wrong in ([[1, 2], [3, 4]], [[1, 2]]):
+        with pytest.raises(ValueError):
+            model.prefill(2, np.array(wrong))
+        with pytest.raises(ValueError):
+            model.step([0, 1], np.array(wrong))
+    assert model.length.tolist() == [4, 2, 0]
