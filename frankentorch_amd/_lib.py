@@ -90,8 +90,16 @@ class PagedSdpaDesc(C.Structure):
                                          "o_seq_stride", "o_row_stride", "o_head_stride")]
 
 
+class PagedScales(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("block", "page_stride", "head_stride")]
+
+
 class LogitsDesc(C.Structure):
     _fields_ = [(n, C.c_int64) for n in ("rows", "vocab", "logits_stride", "out_stride", "history_stride", "bias_stride", "mask_stride")]
+
+
+class SampleDesc(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("rows", "vocab", "logits_stride")]
 
 
 class LayerWeights(C.Structure):

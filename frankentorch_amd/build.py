@@ -38,7 +38,12 @@ HIP_SOURCES = [
     "int8ops.hip",
     "paged_append.hip",
     "paged_sdpa.hip",
+    "paged_append_scaled.hip",
+    "paged_sdpa_scaled.hip",
+    "paged_sdpa_e4m3.hip",
+    "paged_sdpa_i8.hip",
     "logits.hip",
+    "sample.hip",
     "host_api.hip",
     "resident.hip",
 ]

@@ -247,6 +247,33 @@ template <typename T> int32_t launch(const AppendArgs &a, hipStream_t st) {
 
 }  // namespace
 
+namespace fth {
+
+int32_t check_paged_append(const fth_paged_cache *c, const fth_paged_append_desc *d, const float *q, const float *k, const float *v, const float *cosines, const float *sines,
+                           const int32_t *block_table, const int32_t *seq_ids, const int32_t *positions, const float *q_out, const void *k_cache, const void *v_cache,
+                           const char *who) {
+    if (int32_t rc = check_paged_cache(c, who)) return rc;
+    FTH_ARG(d, "%s: NULL descriptor", who);
+    FTH_ARG(d->tokens >= 0 && d->q_heads >= 0, "%s: negative extent", who);
+    FTH_ARG(d->rotary_dim >= 0 && d->rotary_dim % 2 == 0 && d->rotary_dim <= c->head_dim, "%s: rotary_dim %lld is odd or outside 0..head_dim", who,
+            (long long)d->rotary_dim);
+    FTH_ARG(d->rotary_dim == 0 || d->max_pos >= 0, "%s: negative max_pos", who);
+    for (int64_t x : {d->q_row_stride, d->q_head_stride, d->k_row_stride, d->k_head_stride, d->v_row_stride, d->v_head_stride, d->out_row_stride, d->out_head_stride})
+        FTH_ARG(stride_in_range(x), "%s: a stride is negative or over 2^40", who);
+    if (d->q_heads > (1 << 20) || d->q_heads + c->kv_heads > (1 << 20) || d->tokens > 2147483647LL) return set_error(FTH_ERR_SIZE_OVERFLOW, "%s: extents overflow", who);
+    if (d->tokens > 0) {
+        FTH_ARG(positions && (k != nullptr) == (v != nullptr) && (k || d->q_heads > 0), "%s: NULL operand", who);
+        FTH_ARG(!k || (seq_ids && (block_table || c->max_pages == 0) && ((k_cache && v_cache) || c->num_pages == 0)), "%s: NULL cache, table or sequences", who);
+        FTH_ARG(d->q_heads == 0 || (q && q_out), "%s: NULL queries", who);
+        FTH_ARG(d->rotary_dim == 0 || (cosines && sines), "%s: NULL rotation tables", who);
+        FTH_ARG(q != q_out || d->q_heads == 0 || (d->q_row_stride == d->out_row_stride && d->q_head_stride == d->out_head_stride),
+                "%s: queries rotated in place need the strides they have", who);
+    }
+    return FTH_OK;
+}
+
+}  // namespace fth
+
 extern "C" {
 
 void fth_dev_paged_cache_contiguous(fth_paged_cache *c, int64_t num_pages, int64_t page_size, int64_t kv_heads, int64_t head_dim, int64_t num_seqs, int64_t max_pages,
@@ -269,23 +296,7 @@ void fth_dev_paged_cache_contiguous(fth_paged_cache *c, int64_t num_pages, int64
 int32_t fth_dev_paged_append_f32(const fth_paged_cache *c, const fth_paged_append_desc *d, const float *q, const float *k, const float *v, const float *cosines,
                                  const float *sines, const int32_t *block_table, const int32_t *seq_ids, const int32_t *positions, float *q_out, void *k_cache,
                                  void *v_cache, int64_t *bad_index, fth_stream s) {
-    if (int32_t rc = fth::check_paged_cache(c, "paged_append")) return rc;
-    FTH_ARG(d, "paged_append: NULL descriptor");
-    FTH_ARG(d->tokens >= 0 && d->q_heads >= 0, "paged_append: negative extent");
-    FTH_ARG(d->rotary_dim >= 0 && d->rotary_dim % 2 == 0 && d->rotary_dim <= c->head_dim, "paged_append: rotary_dim %lld is odd or outside 0..head_dim",
-            (long long)d->rotary_dim);
-    FTH_ARG(d->rotary_dim == 0 || d->max_pos >= 0, "paged_append: negative max_pos");
-    for (int64_t x : {d->q_row_stride, d->q_head_stride, d->k_row_stride, d->k_head_stride, d->v_row_stride, d->v_head_stride, d->out_row_stride, d->out_head_stride})
-        FTH_ARG(fth::stride_in_range(x), "paged_append: a stride is negative or over 2^40");
-    if (d->q_heads > (1 << 20) || d->q_heads + c->kv_heads > (1 << 20) || d->tokens > 2147483647LL) return fth::set_error(FTH_ERR_SIZE_OVERFLOW, "paged_append: extents overflow");
-    if (d->tokens > 0) {
-        FTH_ARG(positions && (k != nullptr) == (v != nullptr) && (k || d->q_heads > 0), "paged_append: NULL operand");
-        FTH_ARG(!k || (seq_ids && (block_table || c->max_pages == 0) && ((k_cache && v_cache) || c->num_pages == 0)), "paged_append: NULL cache, table or sequences");
-        FTH_ARG(d->q_heads == 0 || (q && q_out), "paged_append: NULL queries");
-        FTH_ARG(d->rotary_dim == 0 || (cosines && sines), "paged_append: NULL rotation tables");
-        FTH_ARG(q != q_out || d->q_heads == 0 || (d->q_row_stride == d->out_row_stride && d->q_head_stride == d->out_head_stride),
-                "paged_append: queries rotated in place need the strides they have");
-    }
+    if (int32_t rc = fth::check_paged_append(c, d, q, k, v, cosines, sines, block_table, seq_ids, positions, q_out, k_cache, v_cache, "paged_append")) return rc;
     FTH_REQUIRE_DEVICE();
     hipStream_t st = fth::resolve_stream(s);
     if (bad_index) {

@@ -27,154 +27,11 @@
 // order reaches 5.9, with nontemporal loads 6.7). One sequence of 131071: 80 + 5 us (6.7 TB/s). Joining the shares in the last workgroup to arrive instead of a
 // second launch was slower in every case (release and acquire across the XCDs): 90 -> 109 us.
 
-#include <type_traits>
-
-#include "paged.hpp"
+#include "paged_sdpa.hpp"
 
 namespace {
 
-using F4 = float __attribute__((ext_vector_type(4)));
-using U4 = uint32_t __attribute__((ext_vector_type(4)));
-using U2 = uint32_t __attribute__((ext_vector_type(2)));
-
-// What no kernel here writes: such loads stay scalar ones also behind stores.
-using Const = const int32_t __attribute__((address_space(4))) *;
-__device__ __forceinline__ Const constant(const int32_t *x) { return (Const)(uintptr_t)x; }
-
-constexpr float kLog2e = 1.44269502162933349609375f;
-constexpr int kTile = 32, kWaves = 4;
-
-struct PagedArgs {
-    fth_paged_cache c;
-    fth_paged_sdpa_desc d;
-    const float *q;
-    const void *k, *v;
-    const int32_t *table, *lens;
-    float *out;
-    int64_t *bad;
-    float *part_o;    // [slot][pitch] unnormalised outputs of the shares (rows with more than one)
-    float *part_ml;   // [slot][2] their maxima (of scores times log2 e) and sums
-    int32_t *starts;  // even shares: where each sequence begins in the line of steps; behind the last one the length of a share
-    float scale2;     // scale * log2(e)
-    int64_t most;     // the longest valid sequence
-    int group, rows, row_tiles, pitch;                    // rows: queries that read a K/V head, group * new_tokens
-    int pairs;                                            // of a sequence and a K/V head
-    int nsplit, share;                                    // shares of `share` keys from the first key of a pair on, nsplit of the longest
-    int even, enough, step_log2, seqs_a_lane;             // or this many even shares, if the keys make `enough` steps (0: the former)
-    fth::Divisor by_page, by_tiles, by_pairs, by_heads;   // by page_size, row_tiles, pairs, kv_heads
-    fth::Divisor by_new, by_q_heads, by_group, by_group4, by_even;  // by new_tokens, q_heads, group, pitch / 4, even
-};
-
-// Even shares: all pairs of a sequence and a K/V head stand in one line, each as one step for beginning it and the steps of
-// 2^step_log2 keys that it has, and every workgroup takes the same stretch of that line. A stretch has at most two pairs in part, its
-// first and its last, so a workgroup has two groups of `rows` slots.
-__device__ __forceinline__ int steps_of(const PagedArgs &p, int len) { return len < 0 || len > p.most ? 0 : (int)(((uint32_t)len + (1u << p.step_log2) - 1) >> p.step_log2); }
-
-// All lines of the arguments at once: the compiler reads them as it needs them, in several round trips one after the other (8
-// sequences of up to 1024 keys, 12 heads of 64: 10.8 + 3.8 -> 10.3 + 3.1 us).
-__device__ __forceinline__ void fetch_arguments() {
-    const auto a = (const uint32_t __attribute__((address_space(4))) *)__builtin_amdgcn_kernarg_segment_ptr();
-    uint32_t any = 0;
-#pragma unroll
-    for (unsigned i = 0; i < sizeof(PagedArgs) / 4; i += 16) any |= a[i];
-    asm volatile("" ::"s"(any));
-}
-
-struct MaxOp { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
-struct AddOp { __device__ float operator()(float a, float b) const { return a + b; } };
-template <typename F> __device__ __forceinline__ float wave_reduce(float x, F op) {
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) x = op(x, __shfl_xor(x, m));
-    return x;
-}
-// over the four 16-lane rows of a wavefront, the result in every lane
-template <typename F> __device__ __forceinline__ float rows_reduce(float x, F op) {
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
-// Where a row (sequence, new token, query head) of the output lies.
-__device__ __forceinline__ float *out_row(const PagedArgs &p, int64_t seq, int i, int h) {
-    return p.out + seq * p.d.o_seq_stride + i * p.d.o_row_stride + h * p.d.o_head_stride;
-}
-
-// ---- one wavefront a row and share: any page size, head size, stride and alignment ----------------------------------------
-
-template <typename T> __global__ __launch_bounds__(64) void paged_sdpa_rows_kernel(const PagedArgs p) {
-    __shared__ float qs[256], ps[64];
-    __shared__ int64_t at[64];
-    const int lane = threadIdx.x, hd = (int)p.c.head_dim, page_size = (int)p.c.page_size;
-    const int split = (int)(blockIdx.x % (unsigned)p.nsplit), row32 = (int)(blockIdx.x / (unsigned)p.nsplit);
-    const int token = (int)p.by_q_heads((uint32_t)row32), h = row32 - token * (int)p.d.q_heads;
-    const int seq32 = (int)p.by_new((uint32_t)token), i = token - seq32 * (int)p.d.new_tokens;
-    const int64_t seq = seq32, hk = p.by_group((uint32_t)h);
-    const T *K = static_cast<const T *>(p.k) + hk * p.c.head_stride, *V = static_cast<const T *>(p.v) + hk * p.c.head_stride;
-    int len = p.lens[seq];
-    bool bad = len < 0 || len > p.most;
-    if (bad) len = 0;
-    const int key_lo = split * p.share;
-    if (split > 0 && key_lo >= len) return;
-    const bool alone = len <= p.share;  // no other share of this row
-    const int end = len - key_lo < p.share ? len : key_lo + p.share;
-    const int sees = len - (int)p.d.new_tokens + i + 1, key_hi = sees < end ? sees : end;  // pages are looked at up to `end`, so that all rows of a sequence find a bad one
-    const float *q = p.q + seq * p.d.q_seq_stride + i * p.d.q_row_stride + h * p.d.q_head_stride;
-    for (int c = lane; c < hd; c += 64) qs[c] = q[c];
-    __syncthreads();
-    float o[4] = {0.f, 0.f, 0.f, 0.f}, m = -__builtin_inff(), l = 0.f;
-    for (int key0 = key_lo; key0 < end; key0 += 64) {
-        const int key = key0 + lane, n = key_hi - key0 < 64 ? key_hi - key0 : 64;
-        float x = -__builtin_inff();
-        if (key < end) {
-            const int index = (int)p.by_page((uint32_t)key);
-            int page = p.table[seq * p.c.table_stride + index];
-            if (page < 0 || page >= p.c.num_pages) {
-                bad = true;
-                page = -1;
-            }
-            const int64_t off = page < 0 ? -1 : (int64_t)page * p.c.page_stride + (int64_t)(key - index * page_size) * p.c.row_stride;
-            at[lane] = off;
-            if (page >= 0 && lane < n) {
-                float dot[4] = {0.f, 0.f, 0.f, 0.f};  // short chains of roundings
-                for (int c = 0; c < hd; ++c) dot[c & 3] = __builtin_fmaf(qs[c], fth::to_f32(K[off + c]), dot[c & 3]);
-                x = ((dot[0] + dot[1]) + (dot[2] + dot[3])) * p.scale2;
-            }
-        }
-        const float m_new = fmaxf(m, wave_reduce(x, MaxOp()));
-        const float ref = m_new == -__builtin_inff() ? 0.f : m_new;
-        const float alpha = __builtin_amdgcn_exp2f(m - ref), w = lane < n ? __builtin_amdgcn_exp2f(x - ref) : 0.f;
-        m = m_new;
-        l = l * alpha + wave_reduce(w, AddOp());
-        ps[lane] = w;
-        __syncthreads();
-        for (int j = 0; j < 4; ++j) {
-            const int c = lane + 64 * j;
-            if (c >= hd) break;
-            float acc = 0.f;
-            for (int r = 0; r < n; ++r)
-                if (at[r] >= 0) acc = __builtin_fmaf(ps[r], fth::to_f32(V[at[r] + c]), acc);
-            o[j] = o[j] * alpha + acc;
-        }
-        __syncthreads();
-    }
-    bad = __any(bad);
-    if (bad && lane == 0) fth::report_bad_entry(p.bad, seq);
-    if (bad) l = __builtin_nanf("");
-    float *dst = out_row(p, seq, i, h);
-    if (!alone) {
-        const int64_t slot = ((seq * p.c.kv_heads + hk) * p.nsplit + split) * p.rows + (h - hk * p.group) * p.d.new_tokens + i;
-        dst = p.part_o + slot * p.pitch;
-        if (lane == 0) {
-            p.part_ml[2 * slot] = m;
-            p.part_ml[2 * slot + 1] = l;
-        }
-    }
-    for (int j = 0; j < 4; ++j) {
-        const int c = lane + 64 * j;
-        if (c < hd) dst[c] = !alone ? o[j] : sees <= 0 && !bad ? 0.f : o[j] / l;
-    }
-}
+using namespace fth::paged;
 
 // ---- tiles of 32 keys on the matrix units ---------------------------------------------------------------------------------
 
@@ -705,91 +562,10 @@ __device__ __forceinline__ void tiles_segment(const PagedArgs &p, float *lds_o, 
 template <typename T, int DP, bool FULL, bool NT, bool ANY, bool EVEN> __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void paged_sdpa_tiles_kernel(const PagedArgs p) {
     __shared__ __attribute__((aligned(16))) float lds_o[kWaves * 16 * (DP + 4)];
     __shared__ float lds_ml[kWaves * 16 * 2];
-    fetch_arguments();
-    // Workgroup ids go round the 8 XCDs: the row tiles of one share of a K/V head come 8 apart, so that they find its K and V in
-    // one L2 (16 sequences of up to 3967 keys, 64 query heads on 8 of 128: four queries, bf16 64.6 -> 57.3 us; eight, fp32 202 -> 155).
-    const int block8 = (int)(blockIdx.x >> 3), item8 = (int)p.by_tiles((uint32_t)block8), rt = block8 - item8 * p.row_tiles;
-    const int item = item8 * 8 + (int)(blockIdx.x & 7), heads = (int)p.c.kv_heads;
-    const Const lens = constant(p.lens);
-    int seq = 0, hk = 0, raw = 0, split = 0, pos = 0, end = 0, within = 0;
-    bool line = false;  // even shares
-    if constexpr (EVEN) {
-        if (item >= p.even) {  // nothing to do either way? (most workgroups, where max_len is far above the lengths)
-            const int at = (int)p.by_pairs((uint32_t)item), len = lens[p.by_heads((uint32_t)(item - at * p.pairs))];
-            if (at >= p.nsplit || (at > 0 && (len <= at * p.share || len > p.most))) return;
-        }
-        const int lane = threadIdx.x & 63, first = lane * p.seqs_a_lane, num_seqs = (int)p.c.num_seqs;
-        const int last = num_seqs - first < p.seqs_a_lane ? num_seqs : first + p.seqs_a_lane;
-        int mine = 0;
-        for (int j = first; j < last; ++j) mine += heads * (steps_of(p, lens[j]) + 1);
-        int upto = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int x = __shfl_up(upto, d);
-            upto += lane >= d ? x : 0;
-        }
-        const int total = __builtin_amdgcn_readlane(upto, 63), share = (int)p.by_even((uint32_t)(total + p.even - 1));
-        line = total - p.pairs >= p.enough;
-        if (blockIdx.x == 0 && threadIdx.x < 64) {
-            int at = upto - mine;
-            for (int j = first; j < last; ++j) {
-                p.starts[j] = at;
-                at += heads * (steps_of(p, lens[j]) + 1);
-            }
-            if (lane == 0) p.starts[num_seqs] = line ? share : 0;
-        }
-        if (line) {  // this workgroup's place in the line
-            pos = item * share;
-            if (item >= p.even || pos >= total) return;
-            end = total - pos < share ? total : pos + share;
-            const int in_lane = __builtin_ctzll(__ballot(upto > pos));
-            int at = __builtin_amdgcn_readlane(upto - mine, in_lane);
-            seq = in_lane * p.seqs_a_lane;
-            for (;;) {
-                raw = lens[seq];
-                const int behind = at + heads * (steps_of(p, raw) + 1);
-                if (pos < behind) break;
-                at = behind;
-                ++seq;
-            }
-            hk = (pos - at) / (steps_of(p, raw) + 1);
-            within = pos - at - hk * (steps_of(p, raw) + 1);
-        }
-    }
-    if (!line) {
-        split = (int)p.by_pairs((uint32_t)item);
-        if (split >= p.nsplit) return;
-        const int pair = item - split * p.pairs;
-        seq = (int)p.by_heads((uint32_t)pair);
-        hk = pair - seq * heads;
-        raw = lens[seq];
-    }
-    for (;;) {
-        const bool bad = raw < 0 || raw > p.most;
-        const int len = bad ? 0 : raw, steps = steps_of(p, raw), stop = steps + 1 - within < end - pos ? steps + 1 : within + end - pos;
-        int key_lo, key_hi;
-        int64_t slot;
-        if (EVEN && line) {
-            key_lo = (within > 1 ? within - 1 : 0) << p.step_log2;
-            key_hi = stop > steps ? len : (stop - 1) << p.step_log2;
-            slot = 2 * item + (within == 0);
-        } else {
-            key_lo = split * p.share;
-            key_hi = len - key_lo < p.share ? len : key_lo + p.share;
-            slot = ((int64_t)seq * heads + hk) * p.nsplit + split;
-        }
-        if (key_lo < key_hi || (len == 0 && key_lo == 0))
-            tiles_segment<T, DP, FULL, NT, ANY>(p, lds_o, lds_ml, seq, hk, rt, len, bad, key_lo, key_hi, key_lo == 0 && key_hi == len, slot * p.rows);
-        if (!EVEN || !line) break;
-        pos += stop - within;
-        if (pos >= end) break;
-        within = 0;
-        if (++hk == heads) {
-            hk = 0;
-            raw = lens[++seq];
-        }
-        __syncthreads();  // lds_o and lds_ml have been read
-    }
+    fetch_arguments<PagedArgs>();
+    walk_shares<EVEN>(p, [&](int seq, int hk, int rt, int len, bool bad, int key_lo, int key_hi, bool alone, int64_t slot) __attribute__((always_inline)) {
+        tiles_segment<T, DP, FULL, NT, ANY>(p, lds_o, lds_ml, seq, hk, rt, len, bad, key_lo, key_hi, alone, slot);
+    });
 }
 
 // ---- shares joined in their order -----------------------------------------------------------------------------------------
@@ -799,7 +575,7 @@ template <typename T, int DP, bool FULL, bool NT, bool ANY, bool EVEN> __global_
 // has more than a few loads to wait for.
 template <int SL, bool EVEN> __global__ __launch_bounds__(256) void paged_sdpa_join_kernel(const PagedArgs p, int items) {
     constexpr int CL = 64 / SL;
-    fetch_arguments();
+    fetch_arguments<PagedArgs>();
     const int item = (int)((blockIdx.x * 4 + (threadIdx.x >> 6)) * CL + (threadIdx.x & (CL - 1)));
     const int lane_s = (threadIdx.x & 63) / CL;
     const bool there = item < items;
@@ -856,20 +632,16 @@ template <int SL, bool EVEN> __global__ __launch_bounds__(256) void paged_sdpa_j
     for (int j = 0; j < 4; ++j)
         if (c + j < p.c.head_dim) dst[j] = acc[j] / l;
 }
-
 // ---- host -------------------------------------------------------------------------------------------------------------------
 
-// How a call is cut: the same for its workspace and its launch.
-struct Plan {
-    bool tiles;  // head size and strides that the 128-bit loads take (the pointers' alignment is looked at later)
-    bool nt;     // loads that leave no trace in the caches
-    int even, enough, step_log2, nsplit, share, pitch;
-    int64_t rows, row_tiles, most;
-};
+}  // namespace
+
+namespace fth {
+namespace paged {
 
 Plan plan(const fth_paged_cache &c, const fth_paged_sdpa_desc &d) {
     Plan p;
-    const int64_t ch = c.dtype == FTH_DTYPE_F32 ? 4 : 8;
+    const int64_t size = fth::element_size(c.dtype), ch = 16 / size;
     p.rows = c.num_seqs * d.new_tokens * d.q_heads;
     p.tiles = c.head_dim % ch == 0 && c.row_stride % ch == 0 && c.head_stride % ch == 0 && c.page_stride % ch == 0 &&
               c.row_stride <= ((int64_t)1 << 24) && c.num_pages > 0;
@@ -877,7 +649,7 @@ Plan plan(const fth_paged_cache &c, const fth_paged_sdpa_desc &d) {
     const int64_t most = p.most = c.max_pages * c.page_size < d.max_len ? c.max_pages * c.page_size : d.max_len;
     p.row_tiles = fth::ceil_div(d.q_heads / c.kv_heads * d.new_tokens, 16);
     const int64_t pairs = c.num_seqs * c.kv_heads, units = p.tiles ? pairs * p.row_tiles : p.rows;
-    const int64_t key_bytes = 2 * c.head_dim * (c.dtype == FTH_DTYPE_F32 ? 4 : 2);
+    const int64_t key_bytes = 2 * c.head_dim * size;
     // Shares of one length: about 256 workgroups, of 256 keys at least. A join costs 4 to 5 us, so nothing is cut that fills the chip whole (32
     // sequences of 1000 keys: 18.6 us in one share, 23.6 in two) or has 512 keys (8 K/V heads of 128: 10.5 / 12.0). 128 keys where 256
     // would not make 128 workgroups (12 heads of 64, 1024 keys: 10.6 / 12.4; 8 of 128, 4096 keys: 13.4 / 14.7). From 129 workgroups on one
@@ -919,12 +691,12 @@ Plan plan(const fth_paged_cache &c, const fth_paged_sdpa_desc &d) {
     // bf16 217 / 229 in shares of 512 KB; 16 of up to 3967, four queries, f16, 260 MB 38.5 / 36.3, fp32, 520 MB 79 / 72; by the even
     // shares of today 196 / 220). The host knows the bound alone: where it is far above the lengths, calls that read one cache again and
     // again lose (under 131072: 4 sequences of 3000 keys 47.5 / 34, 16 of 1000 22.4 / 17.2, 64 of 300 or 600 level).
-    p.nt = p.row_tiles == 1 && 2.0 * (double)c.num_seqs * (double)most * (double)c.kv_heads * (double)c.head_dim * (c.dtype == FTH_DTYPE_F32 ? 4 : 2) > 500.0 * (1 << 20);
+    p.nt = p.row_tiles == 1 && 2.0 * (double)c.num_seqs * (double)most * (double)c.kv_heads * (double)c.head_dim * (double)size > 500.0 * (1 << 20);
     return p;
 }
 
 // Partial results: of the shares of every row, or of two pairs a share.
-int64_t slots_of(const Plan &p, const fth_paged_cache &c, bool tiles) {
+static int64_t slots_of(const Plan &p, const fth_paged_cache &c, bool tiles) {
     const int64_t one = p.nsplit > 1 ? p.rows * p.nsplit : 0, even = tiles && p.even ? 2 * p.even * (p.rows / (c.num_seqs * c.kv_heads)) : 0;
     return even > one ? even : one;
 }
@@ -932,8 +704,8 @@ size_t workspace_bytes_of(const Plan &p, const fth_paged_cache &c) {
     return (size_t)slots_of(p, c, true) * (p.pitch + 2) * sizeof(float) + (p.even ? (size_t)(c.num_seqs + 1) * sizeof(int32_t) : 0);
 }
 
-int32_t check(const fth_paged_cache *c, const fth_paged_sdpa_desc *d) {
-    if (int32_t rc = fth::check_paged_cache(c, "paged_sdpa")) return rc;
+int32_t check(const fth_paged_cache *c, const fth_paged_sdpa_desc *d, bool scaled) {
+    if (int32_t rc = fth::check_paged_cache(c, "paged_sdpa", scaled)) return rc;
     FTH_ARG(d, "paged_sdpa: NULL descriptor");
     if (d->q_heads > (1 << 24)) return fth::set_error(FTH_ERR_SIZE_OVERFLOW, "paged_sdpa: more than 2^24 query heads");
     FTH_ARG(d->q_heads >= 1 && d->q_heads % c->kv_heads == 0, "paged_sdpa: %lld query heads on %lld K/V heads", (long long)d->q_heads, (long long)c->kv_heads);
@@ -947,9 +719,68 @@ int32_t check(const fth_paged_cache *c, const fth_paged_sdpa_desc *d) {
     return FTH_OK;
 }
 
-template <typename T> int32_t launch(PagedArgs &a, const Plan &pl, bool tiles, hipStream_t st) {
+bool fill_args(PagedArgs &a, const fth_paged_cache &c, const fth_paged_sdpa_desc &d, const Plan &pl, float scale, const float *q, const void *k_cache, const void *v_cache,
+               const int32_t *block_table, const int32_t *lens, float *out, int64_t *bad_index, void *workspace) {
+    a.c = c;
+    a.d = d;
+    a.q = q; a.k = k_cache; a.v = v_cache; a.table = block_table; a.lens = lens; a.out = out; a.bad = bad_index;
+    a.part_o = static_cast<float *>(workspace);
+    const bool tiles = pl.tiles && (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15u) == 0;
+    const int64_t slots = slots_of(pl, c, tiles);
+    a.part_ml = a.part_o + slots * pl.pitch;
+    a.starts = reinterpret_cast<int32_t *>(a.part_ml + 2 * slots);
+    a.scale2 = scale * kLog2e;
+    a.most = pl.most;
+    a.group = (int)(d.q_heads / c.kv_heads);
+    a.rows = a.group * (int)d.new_tokens;
+    a.row_tiles = (int)pl.row_tiles;
+    a.nsplit = pl.nsplit; a.share = pl.share; a.pitch = pl.pitch;
+    a.even = tiles ? pl.even : 0; a.enough = pl.enough; a.step_log2 = pl.step_log2;
+    a.seqs_a_lane = (int)fth::ceil_div(c.num_seqs, 64);
+    a.pairs = (int)(c.num_seqs * c.kv_heads);
+    a.by_page = fth::Divisor((uint32_t)c.page_size);
+    a.by_tiles = fth::Divisor((uint32_t)a.row_tiles);
+    a.by_pairs = fth::Divisor((uint32_t)a.pairs);
+    a.by_even = fth::Divisor((uint32_t)(a.even ? a.even : 1));
+    a.by_heads = fth::Divisor((uint32_t)c.kv_heads);
+    a.by_new = fth::Divisor((uint32_t)d.new_tokens);
+    a.by_q_heads = fth::Divisor((uint32_t)d.q_heads);
+    a.by_group = fth::Divisor((uint32_t)a.group);
+    a.by_group4 = fth::Divisor((uint32_t)(a.pitch / 4));
+    return tiles;
+}
+
+int64_t tiles_grid(const PagedArgs &a) {
+    const int64_t cut = (int64_t)a.pairs * a.nsplit;
+    return fth::ceil_div(cut > a.even ? cut : a.even, 8) * 8 * a.row_tiles;
+}
+
+int32_t launch_join(const PagedArgs &a, const Plan &pl, hipStream_t st) {
+    if (a.even || a.nsplit > 1) {
+        const int items = (int)(pl.rows * (a.pitch / 4));  // at most 2^24 rows of 64 groups
+        // (us, 1 / 4 / 16 / 64 lanes: 2048 rows of up to 16 shares 5.9 / 5.1 / 11.8 / 41; 32 rows of 256 shares 44 / 15 / 9.6 / 6.3)
+        // (in a batch that fills the chip a row has about one share, though the longest have more)
+        const int lanes = a.nsplit <= 4 ? 1 : a.nsplit <= 16 || a.even ? 4 : a.nsplit <= 64 ? 16 : 64;
+        const dim3 blocks((unsigned)fth::ceil_div((int64_t)items * lanes, 256));
+        auto go = [&](auto kernel) { kernel<<<blocks, dim3(256), 0, st>>>(a, items); };
+        if (a.even) go(lanes == 1 ? paged_sdpa_join_kernel<1, true> : paged_sdpa_join_kernel<4, true>);
+        else if (lanes == 1) go(paged_sdpa_join_kernel<1, false>);
+        else if (lanes == 4) go(paged_sdpa_join_kernel<4, false>);
+        else if (lanes == 16) go(paged_sdpa_join_kernel<16, false>);
+        else go(paged_sdpa_join_kernel<64, false>);
+        FTH_CHECK_LAUNCH("paged_sdpa_join");
+    }
+    return FTH_OK;
+}
+
+}  // namespace paged
+}  // namespace fth
+
+namespace {
+
+template <typename T> int32_t launch(const PagedArgs &a, const Plan &pl, bool tiles, hipStream_t st) {
     if (tiles) {
-        const int64_t cut = (int64_t)a.pairs * a.nsplit, grid = fth::ceil_div(cut > a.even ? cut : a.even, 8) * 8 * a.row_tiles;
+        const int64_t grid = tiles_grid(a);
         FTH_ARG(grid <= 2147483647LL, "paged_sdpa: too many workgroups for one launch");
         const dim3 blocks((unsigned)grid);
         const bool nt = pl.nt;
@@ -974,24 +805,10 @@ template <typename T> int32_t launch(PagedArgs &a, const Plan &pl, bool tiles, h
         else pick(std::false_type());
     } else {
         FTH_ARG(pl.rows * a.nsplit <= 2147483647LL, "paged_sdpa: too many rows for one launch");
-        paged_sdpa_rows_kernel<T><<<dim3((unsigned)(pl.rows * a.nsplit)), dim3(64), 0, st>>>(a);
+        paged_sdpa_rows_kernel<T, PagedArgs><<<dim3((unsigned)(pl.rows * a.nsplit)), dim3(64), 0, st>>>(a);
     }
     FTH_CHECK_LAUNCH("paged_sdpa");
-    if (a.even || a.nsplit > 1) {
-        const int items = (int)(pl.rows * (a.pitch / 4));  // at most 2^24 rows of 64 groups
-        // (us, 1 / 4 / 16 / 64 lanes: 2048 rows of up to 16 shares 5.9 / 5.1 / 11.8 / 41; 32 rows of 256 shares 44 / 15 / 9.6 / 6.3)
-        // (in a batch that fills the chip a row has about one share, though the longest have more)
-        const int lanes = a.nsplit <= 4 ? 1 : a.nsplit <= 16 || a.even ? 4 : a.nsplit <= 64 ? 16 : 64;
-        const dim3 blocks((unsigned)fth::ceil_div((int64_t)items * lanes, 256));
-        auto go = [&](auto kernel) { kernel<<<blocks, dim3(256), 0, st>>>(a, items); };
-        if (a.even) go(lanes == 1 ? paged_sdpa_join_kernel<1, true> : paged_sdpa_join_kernel<4, true>);
-        else if (lanes == 1) go(paged_sdpa_join_kernel<1, false>);
-        else if (lanes == 4) go(paged_sdpa_join_kernel<4, false>);
-        else if (lanes == 16) go(paged_sdpa_join_kernel<16, false>);
-        else go(paged_sdpa_join_kernel<64, false>);
-        FTH_CHECK_LAUNCH("paged_sdpa_join");
-    }
-    return FTH_OK;
+    return launch_join(a, pl, st);
 }
 
 }  // namespace
@@ -1018,32 +835,7 @@ int32_t fth_dev_paged_sdpa_f32(const fth_paged_cache *c, const fth_paged_sdpa_de
     }
     if (c->num_seqs == 0) return FTH_OK;
     PagedArgs a;
-    a.c = *c;
-    a.d = *d;
-    a.q = q; a.k = k_cache; a.v = v_cache; a.table = block_table; a.lens = lens; a.out = out; a.bad = bad_index;
-    a.part_o = static_cast<float *>(workspace);
-    const bool tiles = pl.tiles && (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15u) == 0;
-    const int64_t slots = slots_of(pl, *c, tiles);
-    a.part_ml = a.part_o + slots * pl.pitch;
-    a.starts = reinterpret_cast<int32_t *>(a.part_ml + 2 * slots);
-    a.scale2 = scale * kLog2e;
-    a.most = pl.most;
-    a.group = (int)(d->q_heads / c->kv_heads);
-    a.rows = a.group * (int)d->new_tokens;
-    a.row_tiles = (int)pl.row_tiles;
-    a.nsplit = pl.nsplit; a.share = pl.share; a.pitch = pl.pitch;
-    a.even = tiles ? pl.even : 0; a.enough = pl.enough; a.step_log2 = pl.step_log2;
-    a.seqs_a_lane = (int)fth::ceil_div(c->num_seqs, 64);
-    a.pairs = (int)(c->num_seqs * c->kv_heads);
-    a.by_page = fth::Divisor((uint32_t)c->page_size);
-    a.by_tiles = fth::Divisor((uint32_t)a.row_tiles);
-    a.by_pairs = fth::Divisor((uint32_t)a.pairs);
-    a.by_even = fth::Divisor((uint32_t)(a.even ? a.even : 1));
-    a.by_heads = fth::Divisor((uint32_t)c->kv_heads);
-    a.by_new = fth::Divisor((uint32_t)d->new_tokens);
-    a.by_q_heads = fth::Divisor((uint32_t)d->q_heads);
-    a.by_group = fth::Divisor((uint32_t)a.group);
-    a.by_group4 = fth::Divisor((uint32_t)(a.pitch / 4));
+    const bool tiles = fill_args(a, *c, *d, pl, scale, q, k_cache, v_cache, block_table, lens, out, bad_index, workspace);
     switch (c->dtype) {
         case FTH_DTYPE_F32: return launch<float>(a, pl, tiles, st);
         case FTH_DTYPE_F16: return launch<fth::f16>(a, pl, tiles, st);

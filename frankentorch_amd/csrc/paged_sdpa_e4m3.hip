@@ -1,0 +1,11 @@
+// Attention over a paged cache of scaled 8-bit numbers: the kernels for e4m3.
+
+#include "paged_sdpa_scaled.hpp"
+
+namespace fth {
+namespace paged {
+
+int32_t launch_e4m3(ScaledArgs &a, const Plan &pl, bool tiles, hipStream_t st) { return launch_scaled<fth::e4m3>(a, pl, tiles, st); }
+
+}  // namespace paged
+}  // namespace fth

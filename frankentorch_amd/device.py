@@ -463,13 +463,13 @@ def linear_int8_dynamic(x, m, k, w_i8, w_scales, n, bias, out, workspace=None, s
     return workspace
 
 
-DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 1, 2, 3
-_STORAGE = {"f32": DTYPE_F32, "f16": DTYPE_F16, "bf16": DTYPE_BF16}
+DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_I8, DTYPE_E4M3 = 1, 2, 3, 16, 17
+_STORAGE = {"f32": DTYPE_F32, "f16": DTYPE_F16, "bf16": DTYPE_BF16, "i8": DTYPE_I8, "e4m3": DTYPE_E4M3}
 
 
 def paged_cache(num_pages, page_size, kv_heads, head_dim, num_seqs, max_pages, dtype="f32") -> _lib.PagedCache:
-    """Contiguous [num_pages, kv_heads, page_size, head_dim] K and V arrays of type "f32", "f16" or "bf16", and a
-    [num_seqs, max_pages] int32 block table. Other layouts: set the strides of the result."""
+    """Contiguous [num_pages, kv_heads, page_size, head_dim] K and V arrays of type "f32", "f16" or "bf16" (or "i8" or "e4m3", for the
+    calls that take scales), and a [num_seqs, max_pages] int32 block table. Other layouts: set the strides of the result."""
     c = _lib.PagedCache()
     _lib.load().fth_dev_paged_cache_contiguous(C.byref(c), num_pages, page_size, kv_heads, head_dim, num_seqs, max_pages, _STORAGE[dtype])
     return c
@@ -523,6 +523,35 @@ def paged_sdpa(cache, desc, scale, q, k_cache, v_cache, block_table, lens, out, 
     return workspace
 
 
+def paged_scales(cache, block) -> _lib.PagedScales:
+    """Contiguous fp32 [num_pages, kv_heads, page_size / block] scales of an "i8" or "e4m3" cache: one for each block of positions and head."""
+    sc = _lib.PagedScales()
+    _lib.load().fth_dev_paged_scales_contiguous(C.byref(sc), C.byref(cache), block)
+    return sc
+
+
+def paged_append_scaled(cache, scales, desc, q, k, v, cosines, sines, block_table, seq_ids, positions, q_out, k_cache, v_cache, k_scales, v_scales, bad_index=None,
+                        stream=None):
+    """paged_append into a cache of 8 bits: elements are rounded to multiples of their block's scale, which grows to what the block's
+    largest element needs. Tokens of one block stand one after the other, positions ascending."""
+    check(_lib.load().fth_dev_paged_append_scaled_f32(C.byref(cache), C.byref(scales), C.byref(desc), _ptr(q), _ptr(k), _ptr(v), _ptr(cosines), _ptr(sines),
+                                                      _ptr(block_table), _ptr(seq_ids), _ptr(positions), _ptr(q_out), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales),
+                                                      _ptr(v_scales), _ptr(bad_index), stream))
+
+
+def paged_sdpa_scaled_workspace(cache, scales, desc) -> DeviceBuffer:
+    """A workspace for paged_sdpa_scaled calls with these descriptors."""
+    return _workspace(_lib.load().fth_dev_paged_sdpa_scaled_workspace_bytes(C.byref(cache), C.byref(scales), C.byref(desc)), None)
+
+
+def paged_sdpa_scaled(cache, scales, desc, scale, q, k_cache, v_cache, k_scales, v_scales, block_table, lens, out, bad_index=None, workspace=None, stream=None):
+    """paged_sdpa over a cache of 8 bits with a scale for each block of positions and head; returns the workspace for the next call."""
+    workspace = paged_sdpa_scaled_workspace(cache, scales, desc) if workspace is None else workspace
+    check(_lib.load().fth_dev_paged_sdpa_scaled_f32(C.byref(cache), C.byref(scales), C.byref(desc), scale, _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales),
+                                                    _ptr(v_scales), _ptr(block_table), _ptr(lens), _ptr(out), _ptr(bad_index), workspace.ptr, workspace.nbytes, stream))
+    return workspace
+
+
 def logits_desc(rows, vocab, history_stride=0, shared_bias=False) -> _lib.LogitsDesc:
     """Contiguous logits, out and bias [rows, vocab] (shared_bias: bias [vocab]), history [rows, history_stride], mask [rows, words of 32 bits]."""
     d = _lib.LogitsDesc()
@@ -535,6 +564,27 @@ def logits_process(desc, logits, history, history_len, prompt_len, repetition, f
     """Penalties for repeated tokens, a bias and a mask of allowed tokens on the logits of a step; each of them may be None."""
     check(_lib.load().fth_dev_logits_process_f32(C.byref(desc), _ptr(logits), _ptr(history), _ptr(history_len), _ptr(prompt_len), _ptr(repetition),
                                                  _ptr(frequency), _ptr(presence), _ptr(bias), _ptr(mask), _ptr(out), _ptr(bad_index), stream))
+
+
+def sample_desc(rows, vocab) -> _lib.SampleDesc:
+    """Contiguous logits [rows, vocab]."""
+    d = _lib.SampleDesc()
+    d.rows, d.vocab, d.logits_stride = rows, vocab, vocab
+    return d
+
+
+def sample_workspace(desc) -> DeviceBuffer:
+    """A workspace for sample calls with this descriptor."""
+    return _workspace(_lib.load().fth_dev_sample_workspace_bytes(C.byref(desc)), None)
+
+
+def sample(desc, logits, temperature, top_k, top_p, min_p, uniform, tokens, logprobs=None, bad_index=None, workspace=None, stream=None):
+    """The next token (int32) of each row from its float64 number in [0, 1), and the logarithm of its probability; temperature, top_p,
+    min_p (float32) and top_k (int32, 0: all) hold one value a row and may each be None. Returns the workspace for the next call."""
+    workspace = sample_workspace(desc) if workspace is None else workspace
+    check(_lib.load().fth_dev_sample_f32(C.byref(desc), _ptr(logits), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(uniform), _ptr(tokens),
+                                         _ptr(logprobs), _ptr(bad_index), workspace.ptr, workspace.nbytes, stream))
+    return workspace
 
 
 def default_scale(head_dim: int) -> float:

@@ -71,6 +71,7 @@ enum {
  * 4123-4308 narrows F16/BF16 above the kernels). */
 enum { FTH_DTYPE_F64 = 0, FTH_DTYPE_F32 = 1, FTH_DTYPE_F16 = 2, FTH_DTYPE_BF16 = 3 }; /* the kernels compute in the first two;
                                                                                        the other two are storage types of a weight file */
+enum { FTH_DTYPE_I8 = 16, FTH_DTYPE_E4M3 = 17 }; /* of a paged K/V cache with scales alone */
 enum { FTH_DEVICE_CPU = 0, FTH_DEVICE_CUDA = 1, FTH_DEVICE_HIP = 2 };
 
 #define FTH_MAX_DIMS 8
@@ -490,6 +491,36 @@ size_t fth_dev_paged_sdpa_workspace_bytes(const fth_paged_cache *c, const fth_pa
 int32_t fth_dev_paged_sdpa_f32(const fth_paged_cache *c, const fth_paged_sdpa_desc *d, float scale, const float *q, const void *k_cache,
                                const void *v_cache, const int32_t *block_table, const int32_t *lens, float *out, int64_t *bad_index,
                                void *workspace, size_t workspace_bytes, fth_stream s);
+/* The same cache in 8 bits: dtype is FTH_DTYPE_I8 (whole numbers, -127 .. 127) or FTH_DTYPE_E4M3 (OCP e4m3, largest 448), and each
+ * `block` positions of a page have one fp32 scale a head in k_scales (v_scales): an element of K at row r = p % page_size of a page
+ * stands for k_cache[...] * k_scales[page * page_stride + h * head_stride + r / block]. block divides page_size. Strides in
+ * elements. */
+typedef struct fth_paged_scales {
+    int64_t block, page_stride, head_stride;
+} fth_paged_scales;
+/* Fills the strides for contiguous [num_pages, kv_heads, page_size / block] arrays. */
+void fth_dev_paged_scales_contiguous(fth_paged_scales *sc, const fth_paged_cache *c, int64_t block);
+/* fth_dev_paged_append_f32 into such a cache: places, rotation, queries, skipped and reported tokens are as there. A scale is 0
+ * for a block of zeros, else a power of two (2^-126 at least), the smallest whose 127 (448) multiples reach the largest element
+ * that the block was given since its first position was written; NaN if one of those was not finite, and then all of the
+ * block is NaN to whoever reads it. Elements are rounded to nearest even multiples. Where tokens raise the scale of a block, what
+ * the block holds before them is rounded to the new scale (e4m3: exact but for what becomes subnormal). A prompt gets the scales
+ * that its tokens one by one would get. What a block holds at and behind the positions written counts as gone: a
+ * sequence that is cut back goes on from there, and a token at the first position of a block starts it anew.
+ * Tokens of one block stand one after the other in the call, positions ascending by one; one that follows a token of its block
+ * without being at the next position is left out and reported like one without a place. Tokens of one block in two places of the list
+ * leave that block unspecified (nothing else). */
+int32_t fth_dev_paged_append_scaled_f32(const fth_paged_cache *c, const fth_paged_scales *sc, const fth_paged_append_desc *d, const float *q, const float *k,
+                                        const float *v, const float *cosines, const float *sines, const int32_t *block_table, const int32_t *seq_ids,
+                                        const int32_t *positions, float *q_out, void *k_cache, void *v_cache, float *k_scales, float *v_scales,
+                                        int64_t *bad_index, fth_stream s);
+/* fth_dev_paged_sdpa_f32 over such a cache: the attention, in fp32 arithmetic, over the values that the cache stands for, except that each
+ * element of a query counts with 22 bits, or to 2^-39 of the largest element of its row. Scales may be any numbers, those of one block each by itself; one that is
+ * not finite, and NaN codes of e4m3, make what sees them NaN. Scales of blocks past a sequence's length are not used. */
+size_t fth_dev_paged_sdpa_scaled_workspace_bytes(const fth_paged_cache *c, const fth_paged_scales *sc, const fth_paged_sdpa_desc *d);
+int32_t fth_dev_paged_sdpa_scaled_f32(const fth_paged_cache *c, const fth_paged_scales *sc, const fth_paged_sdpa_desc *d, float scale, const float *q,
+                                      const void *k_cache, const void *v_cache, const float *k_scales, const float *v_scales, const int32_t *block_table,
+                                      const int32_t *lens, float *out, int64_t *bad_index, void *workspace, size_t workspace_bytes, fth_stream s);
 /* The logits of a step made ready for the choice of a token. Row r has the tokens so far in history[r * history_stride ...],
  * history_len[r] of them, the first prompt_len[r] given and the others generated. For every v < vocab, in this order:
  *   seen anywhere in the history:                   x = x > 0 ? x / repetition[r] : x * repetition[r]
@@ -509,6 +540,27 @@ typedef struct fth_logits_desc {
 int32_t fth_dev_logits_process_f32(const fth_logits_desc *d, const float *logits, const int32_t *history, const int32_t *history_len,
                                    const int32_t *prompt_len, const float *repetition, const float *frequency, const float *presence,
                                    const float *bias, const uint32_t *mask, float *out, int64_t *bad_index, fth_stream s);
+/* The next token of each row of logits, drawn with a given number uniform[r] in [0, 1) (fp64: 24 bits are too few for a large
+ * vocabulary). Tokens are ordered by their logits, largest first, the lower index first among equals; w[v] = exp((x[v] - max x) /
+ * temperature[r]). Kept are, one filter after the other:
+ *   top_k[r] > 0:  the first top_k[r] tokens of the order
+ *   top_p[r] < 1:  of those the fewest from the first on whose w reach top_p[r] of the sum over all of those; one at least
+ *   min_p[r] > 0:  of those the tokens with w >= min_p[r]
+ * tokens[r] is the smallest v for which the sum of w over the kept tokens up to v exceeds uniform[r] times the sum over all kept, and
+ * logprobs[r] (may be NULL) the logarithm of its share of the latter. temperature 0 takes the first token of the order (logprob 0).
+ * temperature, top_k, top_p and min_p may each be NULL (temperature 1, that filter left out). Logits of -inf are never chosen. A
+ * row that holds NaN or +inf or nothing above -inf, or whose settings are out of range (temperature negative or not finite,
+ * top_k < 0, top_p or min_p NaN or negative, min_p > 1, uniform outside [0, 1)) gets token -1 and logprob NaN, and bad_index (device, may be NULL)
+ * receives the lowest such row, or -1. Exponentials are fp64, since which side of a border a number lies on decides the token, and w
+ * counts as a whole multiple of 2^-45 of the largest (2^-44 above 2^17 tokens, a bit less for each doubling): sums are exact, so runs repeat bit for
+ * bit, and rows do not depend on each other. The workspace's contents are ignored and overwritten. */
+typedef struct fth_sample_desc {
+    int64_t rows, vocab, logits_stride; /* elements, >= vocab */
+} fth_sample_desc;
+size_t fth_dev_sample_workspace_bytes(const fth_sample_desc *d);
+int32_t fth_dev_sample_f32(const fth_sample_desc *d, const float *logits, const float *temperature, const int32_t *top_k, const float *top_p,
+                           const float *min_p, const double *uniform, int32_t *tokens, float *logprobs, int64_t *bad_index, void *workspace,
+                           size_t workspace_bytes, fth_stream s);
 
 /* ------------------------------------------------------------------------------------------ */
 /* Tier A: host slices in, host buffer out (the ft_kernel_cpu surface)                        */

@@ -37,6 +37,8 @@ pub const FTH_DTYPE_F64: i32 = 0;
 pub const FTH_DTYPE_F32: i32 = 1;
 pub const FTH_DTYPE_F16: i32 = 2;
 pub const FTH_DTYPE_BF16: i32 = 3;
+pub const FTH_DTYPE_I8: i32 = 16;
+pub const FTH_DTYPE_E4M3: i32 = 17;
 pub const FTH_DEVICE_CPU: i32 = 0;
 pub const FTH_DEVICE_CUDA: i32 = 1;
 pub const FTH_DEVICE_HIP: i32 = 2;
@@ -172,6 +174,14 @@ pub struct fth_paged_sdpa_desc {
 
 #[repr(C)]
 #[derive(Debug, Clone, Copy)]
+pub struct fth_paged_scales {
+    pub block: i64,
+    pub page_stride: i64,
+    pub head_stride: i64,
+}
+
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
 pub struct fth_logits_desc {
     pub rows: i64,
     pub vocab: i64,
@@ -180,6 +190,14 @@ pub struct fth_logits_desc {
     pub history_stride: i64,
     pub bias_stride: i64,
     pub mask_stride: i64,
+}
+
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct fth_sample_desc {
+    pub rows: i64,
+    pub vocab: i64,
+    pub logits_stride: i64,
 }
 
 #[repr(C)]
@@ -344,7 +362,13 @@ extern "C" {
     pub fn fth_dev_paged_append_f32(c: *const fth_paged_cache, d: *const fth_paged_append_desc, q: *const f32, k: *const f32, v: *const f32, cosines: *const f32, sines: *const f32, block_table: *const i32, seq_ids: *const i32, positions: *const i32, q_out: *mut f32, k_cache: *mut c_void, v_cache: *mut c_void, bad_index: *mut i64, s: fth_stream) -> i32;
     pub fn fth_dev_paged_sdpa_workspace_bytes(c: *const fth_paged_cache, d: *const fth_paged_sdpa_desc) -> usize;
     pub fn fth_dev_paged_sdpa_f32(c: *const fth_paged_cache, d: *const fth_paged_sdpa_desc, scale: f32, q: *const f32, k_cache: *const c_void, v_cache: *const c_void, block_table: *const i32, lens: *const i32, out: *mut f32, bad_index: *mut i64, workspace: *mut c_void, workspace_bytes: usize, s: fth_stream) -> i32;
+    pub fn fth_dev_paged_scales_contiguous(sc: *mut fth_paged_scales, c: *const fth_paged_cache, block: i64);
+    pub fn fth_dev_paged_append_scaled_f32(c: *const fth_paged_cache, sc: *const fth_paged_scales, d: *const fth_paged_append_desc, q: *const f32, k: *const f32, v: *const f32, cosines: *const f32, sines: *const f32, block_table: *const i32, seq_ids: *const i32, positions: *const i32, q_out: *mut f32, k_cache: *mut c_void, v_cache: *mut c_void, k_scales: *mut f32, v_scales: *mut f32, bad_index: *mut i64, s: fth_stream) -> i32;
+    pub fn fth_dev_paged_sdpa_scaled_workspace_bytes(c: *const fth_paged_cache, sc: *const fth_paged_scales, d: *const fth_paged_sdpa_desc) -> usize;
+    pub fn fth_dev_paged_sdpa_scaled_f32(c: *const fth_paged_cache, sc: *const fth_paged_scales, d: *const fth_paged_sdpa_desc, scale: f32, q: *const f32, k_cache: *const c_void, v_cache: *const c_void, k_scales: *const f32, v_scales: *const f32, block_table: *const i32, lens: *const i32, out: *mut f32, bad_index: *mut i64, workspace: *mut c_void, workspace_bytes: usize, s: fth_stream) -> i32;
     pub fn fth_dev_logits_process_f32(d: *const fth_logits_desc, logits: *const f32, history: *const i32, history_len: *const i32, prompt_len: *const i32, repetition: *const f32, frequency: *const f32, presence: *const f32, bias: *const f32, mask: *const u32, out: *mut f32, bad_index: *mut i64, s: fth_stream) -> i32;
+    pub fn fth_dev_sample_workspace_bytes(d: *const fth_sample_desc) -> usize;
+    pub fn fth_dev_sample_f32(d: *const fth_sample_desc, logits: *const f32, temperature: *const f32, top_k: *const i32, top_p: *const f32, min_p: *const f32, uniform: *const f64, tokens: *mut i32, logprobs: *mut f32, bad_index: *mut i64, workspace: *mut c_void, workspace_bytes: usize, s: fth_stream) -> i32;
     pub fn fth_matmul_tensor_contiguous_f32(lhs: *const f32, lhs_len: usize, rhs: *const f32, rhs_len: usize, lhs_meta: *const fth_meta, rhs_meta: *const fth_meta, out: *mut f32, out_cap: usize, out_len: *mut usize) -> i32;
     pub fn fth_matmul_tensor_contiguous_f64(lhs: *const f64, lhs_len: usize, rhs: *const f64, rhs_len: usize, lhs_meta: *const fth_meta, rhs_meta: *const fth_meta, out: *mut f64, out_cap: usize, out_len: *mut usize) -> i32;
     pub fn fth_bmm_tensor_contiguous_f32(lhs: *const f32, lhs_len: usize, rhs: *const f32, rhs_len: usize, lhs_meta: *const fth_meta, rhs_meta: *const fth_meta, out: *mut f32, out_cap: usize, out_len: *mut usize) -> i32;
