@@ -81,11 +81,6 @@ template <> struct Parts<fth::f16> {
     }
 };
 
-template <bool NT> __device__ __forceinline__ U4 load128(const void *p) {
-    const U4 *v = static_cast<const U4 *>(p);
-    return NT ? __builtin_nontemporal_load(v) : *v;
-}
-
 // v[0..7] as kParts vectors of the storage type whose sum they are (up to the last part's rounding).
 template <typename T> __device__ __forceinline__ void split_parts(float *v, U4 (&parts)[Parts<T>::kArray]) {
     using V8 = typename Parts<T>::Vec;
@@ -127,13 +122,8 @@ __device__ __forceinline__ void tiles_segment(const PagedArgs &p, float *lds_o, 
     const Const table = constant(p.table) + seq * p.c.table_stride;
     const int rs = (int)p.c.row_stride, num_pages = (int)p.c.num_pages;
 
-    const int stored = rows - rt * 16 < 16 ? rows - rt * 16 : 16;
     if (len == 0) {
-        if (bad && threadIdx.x == 0) fth::report_bad_entry(p.bad, seq);
-        for (int x = threadIdx.x; x < stored * hd; x += 64 * kWaves) {
-            const int row = rt * 16 + x / hd;
-            out_row(p, seq, row % new_tokens, hk * p.group + row / new_tokens)[x % hd] = bad ? __builtin_nanf("") : 0.f;
-        }
+        store_empty(p, seq, hk, rt, bad);
         return;
     }
 
@@ -512,51 +502,10 @@ __device__ __forceinline__ void tiles_segment(const PagedArgs &p, float *lds_o, 
         }
     }
 
-    // join the wavefronts: MFMA row 4 g + r of column tile e is output column ((e / CV) * 16 + 4 g + r) * CV + e % CV
-    constexpr int P = DP + 4;
-    const float l_wave = rows_reduce(l_run, AddOp());
     if constexpr (ANY) bad = __any(bad);
-    if (g == 0) {
-        lds_ml[(wave * 16 + lr) * 2] = m_run;
-        lds_ml[(wave * 16 + lr) * 2 + 1] = bad ? __builtin_nanf("") : l_wave;
-    }
-#pragma unroll
-    for (int e = 0; e < NE; ++e)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) lds_o[(wave * 16 + lr) * P + ((e / CV) * 16 + 4 * g + r) * CV + e % CV] = o[e][r];
-    if (bad && lane == 0) fth::report_bad_entry(p.bad, seq);
-    __syncthreads();
-    for (int x = threadIdx.x; x < stored * (DP / 4); x += 64 * kWaves) {
-        const int row = x / (DP / 4), c = x % (DP / 4) * 4;
-        if (c >= hd) continue;
-        float m = -__builtin_inff(), l = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) m = fmaxf(m, lds_ml[(w * 16 + row) * 2]);
-        const float ref = m == -__builtin_inff() ? 0.f : m;
-        F4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const float weight = __builtin_amdgcn_exp2f(lds_ml[(w * 16 + row) * 2] - ref);
-            l += lds_ml[(w * 16 + row) * 2 + 1] * weight;
-            const F4 part = *reinterpret_cast<const F4 *>(&lds_o[(w * 16 + row) * P + c]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[j] += part[j] * weight;
-        }
-        const int head = (int)p.by_new((uint32_t)(rt * 16 + row)), ri = rt * 16 + row - head * new_tokens, rh = hk * p.group + head;
-        if (alone) {
-            float *dst = out_row(p, seq, ri, rh);
-            const bool nothing = !(l != l) && len - new_tokens + 1 + ri <= 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) dst[c + j] = nothing ? 0.f : acc[j] / l;
-        } else {
-            const int64_t slot = slot0 + rt * 16 + row;
-            *reinterpret_cast<F4 *>(p.part_o + slot * p.pitch + c) = acc;
-            if (c == 0) {
-                p.part_ml[2 * slot] = m;
-                p.part_ml[2 * slot + 1] = l;
-            }
-        }
-    }
+    // MFMA row 4 g + r of column tile e is output column ((e / CV) * 16 + 4 g + r) * CV + e % CV
+    join_wavefronts<DP>(p, lds_o, lds_ml, seq, hk, rt, len, bad, alone, slot0, o, m_run, l_run,
+                        [&](int e, int r) __attribute__((always_inline)) { return ((e / CV) * 16 + 4 * g + r) * CV + e % CV; });
 }
 
 template <typename T, int DP, bool FULL, bool NT, bool ANY, bool EVEN> __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void paged_sdpa_tiles_kernel(const PagedArgs p) {

@@ -169,6 +169,70 @@ template <typename T, typename Args> __global__ __launch_bounds__(64) void paged
     }
 }
 
+// ---- what every kernel of tiles ends with ------------------------------------------------------------------------------------
+
+// A pair without keys: row tile rt of its queries gives zeros, or NaN for a sequence that is invalid.
+__device__ __forceinline__ void store_empty(const PagedArgs &p, int64_t seq, int hk, int rt, bool bad) {
+    const int hd = (int)p.c.head_dim, new_tokens = (int)p.d.new_tokens, stored = p.rows - rt * 16 < 16 ? p.rows - rt * 16 : 16;
+    if (bad && threadIdx.x == 0) fth::report_bad_entry(p.bad, seq);
+    for (int x = threadIdx.x; x < stored * hd; x += 64 * kWaves) {
+        const int row = rt * 16 + x / hd;
+        out_row(p, seq, row % new_tokens, hk * p.group + row / new_tokens)[x % hd] = bad ? __builtin_nanf("") : 0.f;
+    }
+}
+
+// The wavefronts of a workgroup joined through LDS, and the result written: to the outputs (`alone`) or to the slots from slot0 on. A lane
+// holds o[e][r], column(e, r) of query row lane % 16, its maximum, and the sum over its own keys.
+template <int DP, int NE, typename F>
+__device__ __forceinline__ void join_wavefronts(const PagedArgs &p, float *lds_o, float *lds_ml, int64_t seq, int hk, int rt, int len, bool bad, bool alone, int64_t slot0, const F4 (&o)[NE],
+                                                float m_run, float l_run, F column) {
+    constexpr int P = DP + 4;
+    const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int hd = (int)p.c.head_dim, new_tokens = (int)p.d.new_tokens, stored = p.rows - rt * 16 < 16 ? p.rows - rt * 16 : 16;
+    const float l_wave = rows_reduce(l_run, AddOp());
+    if (g == 0) {
+        lds_ml[(wave * 16 + lr) * 2] = m_run;
+        lds_ml[(wave * 16 + lr) * 2 + 1] = bad ? __builtin_nanf("") : l_wave;
+    }
+#pragma unroll
+    for (int e = 0; e < NE; ++e)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) lds_o[(wave * 16 + lr) * P + column(e, r)] = o[e][r];
+    if (bad && lane == 0) fth::report_bad_entry(p.bad, seq);
+    __syncthreads();
+    for (int x = threadIdx.x; x < stored * (DP / 4); x += 64 * kWaves) {
+        const int row = x / (DP / 4), c = x % (DP / 4) * 4;
+        if (c >= hd) continue;
+        float m = -__builtin_inff(), l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) m = fmaxf(m, lds_ml[(w * 16 + row) * 2]);
+        const float ref = m == -__builtin_inff() ? 0.f : m;
+        F4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float weight = __builtin_amdgcn_exp2f(lds_ml[(w * 16 + row) * 2] - ref);
+            l += lds_ml[(w * 16 + row) * 2 + 1] * weight;
+            const F4 part = *reinterpret_cast<const F4 *>(&lds_o[(w * 16 + row) * P + c]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] += part[j] * weight;
+        }
+        const int head = (int)p.by_new((uint32_t)(rt * 16 + row)), ri = rt * 16 + row - head * new_tokens, rh = hk * p.group + head;
+        if (alone) {
+            float *dst = out_row(p, seq, ri, rh);
+            const bool nothing = !(l != l) && len - new_tokens + 1 + ri <= 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) dst[c + j] = nothing ? 0.f : acc[j] / l;
+        } else {
+            const int64_t slot = slot0 + rt * 16 + row;
+            *reinterpret_cast<F4 *>(p.part_o + slot * p.pitch + c) = acc;
+            if (c == 0) {
+                p.part_ml[2 * slot] = m;
+                p.part_ml[2 * slot + 1] = l;
+            }
+        }
+    }
+}
+
 // ---- shares -----------------------------------------------------------------------------------------------------------------
 
 // The shares of a workgroup one after the other: segment(seq, hk, rt, len, bad, key_lo, key_hi, alone, slot) attends to keys key_lo .. key_hi - 1
@@ -258,6 +322,11 @@ template <bool EVEN, typename F> __device__ __forceinline__ void walk_shares(con
         }
         __syncthreads();  // the segment's LDS has been read
     }
+}
+
+template <bool NT> __device__ __forceinline__ U4 load128(const void *p) {
+    const U4 *v = static_cast<const U4 *>(p);
+    return NT ? __builtin_nontemporal_load(v) : *v;
 }
 
 // ---- how a call is cut, and the join --------------------------------------------------------------------------------------

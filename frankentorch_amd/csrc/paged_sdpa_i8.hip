@@ -5,7 +5,7 @@
 namespace fth {
 namespace paged {
 
-int32_t launch_i8(ScaledArgs &a, const Plan &pl, bool tiles, hipStream_t st) { return launch_scaled<fth::i8>(a, pl, tiles, st); }
+int32_t launch_i8(const ScaledArgs &a, const Plan &pl, bool tiles, hipStream_t st) { return launch_scaled<fth::i8>(a, pl, tiles, st); }
 
 }  // namespace paged
 }  // namespace fth

@@ -1,4 +1,16 @@
-// Attention over a paged cache of 8-bit numbers, each block of positions and head with a scale.
+// Attention of the last one to eight tokens of every sequence over a paged K/V cache of 8-bit numbers, each block of positions and
+// head with a scale.
+//
+//   out = sum_j w_j s'_j v_j / sum_j w_j,   w_j = exp(x_j - max x),   x_j = scale s_j (q . k_j),   k, v codes, s, s' the scales of the key's blocks
+//
+// Bound by reading the cache once. Shares, tiles of 32 keys and the way keys and query rows lie in the lanes are those of the kernels
+// for 16-bit caches; both products run on the 16-bit matrix units against codes turned into numbers of 16 bits, which hold them exactly:
+//   * K as f16, against a query row scaled by a power of two and cut into two parts of f16 (22 bits of an element, or 2^-39 of the row's largest). A
+//     score meets the scale of its key's block in fp32 afterwards.
+//   * V as bf16, against weights that have met the scale of their key's block in fp32 and are cut into three parts of bf16, whose sum they
+//     are. They carry a factor of 2^40, which keeps the third part of every weight an output of fp32 can show above the smallest bf16; where that
+//     overflows (scales of V beyond 2^70) the share is walked again with 2^-24.
+// e4m3 becomes either type two at a time by one instruction of gfx950; whole numbers become f16 by the bits of 1024 + 128 + x, bf16 through fp32.
 #pragma once
 
 #include "paged_sdpa.hpp"
@@ -13,16 +25,402 @@ struct ScaledArgs : PagedArgs {
     fth::Divisor by_block;
 };
 
-template <typename T> int32_t launch_scaled(ScaledArgs &a, const Plan &pl, bool tiles, hipStream_t st) {
-    a.even = 0;
-    FTH_ARG(pl.rows * a.nsplit <= 2147483647LL, "paged_sdpa_scaled: too many rows for one launch");
-    paged_sdpa_rows_kernel<T, ScaledArgs><<<dim3((unsigned)(pl.rows * a.nsplit)), dim3(64), 0, st>>>(a);
+using H2 = _Float16 __attribute__((ext_vector_type(2)));
+using H8 = _Float16 __attribute__((ext_vector_type(8)));
+using B2 = __bf16 __attribute__((ext_vector_type(2)));
+using B8 = __bf16 __attribute__((ext_vector_type(8)));
+using ConstF = const float __attribute__((address_space(4))) *;
+
+// Where the scales of a tile's keys come from: one for each half tile (blocks and pages are multiples of 16: scalar loads); a load for each
+// key, the rows found from the half tile's first (pages are multiples of 16); a load for each key, whose page every lane looks up (any pages).
+enum class ScaleOf { half, key, any };
+
+// 8 codes (two words) as f16.
+template <typename T> __device__ __forceinline__ H8 to_f16(uint32_t a, uint32_t b) {
+    H2 x[4];
+    const uint32_t w[2] = {a, b};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if constexpr (std::is_same<T, fth::e4m3>::value) {
+            x[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w[i], 1.f, false);
+            x[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w[i], 1.f, true);
+        } else {  // 0x6400 + u is the f16 1024 + u; u = 128 + the number
+            const uint32_t u = w[i] ^ 0x80808080u;
+            const H2 bias = {(_Float16)1152.f, (_Float16)1152.f};
+            x[2 * i] = __builtin_bit_cast(H2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias;
+            x[2 * i + 1] = __builtin_bit_cast(H2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias;
+        }
+    }
+    return H8{x[0][0], x[0][1], x[1][0], x[1][1], x[2][0], x[2][1], x[3][0], x[3][1]};
+}
+
+// Byte b (a constant) of two words as two bf16.
+template <typename T> __device__ __forceinline__ uint32_t to_bf16(uint32_t first, uint32_t second, int b) {
+    if constexpr (std::is_same<T, fth::e4m3>::value) {
+        const uint32_t pairs = __builtin_amdgcn_perm(second, first, b < 2 ? 0x05010400u : 0x07030602u);  // bytes 0 and 1 (2 and 3) of both
+        return __builtin_bit_cast(uint32_t, (b & 1) ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)pairs, 1.f, true)
+                                                    : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)pairs, 1.f, false));
+    } else {  // 8 bits: the upper halves of fp32
+        const float x = (float)(int8_t)(first >> (8 * b)), y = (float)(int8_t)(second >> (8 * b));
+        return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+    }
+}
+
+// Bit 7 of every byte that is a NaN of e4m3.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// One segment: keys key_lo .. key_hi - 1 of a pair of `len` keys, with row tile rt of its queries. FULL: head_dim == DP; otherwise what lies past
+// head_dim counts as zero. NT: K and V leave no trace in the caches.
+template <typename T, int DP, bool FULL, bool NT, ScaleOf OF>
+__device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o, float *lds_ml, int seq32, int hk, int rt, int len, bool bad, int key_lo, int key_hi, bool alone, int64_t slot0) {
+    constexpr bool ANY = OF == ScaleOf::any, HALF = OF == ScaleOf::half, kNan = std::is_same<T, fth::e4m3>::value;
+    constexpr int NK = DP / 64;   // 128-bit loads of a lane's quarter of a K row
+    constexpr int NE = DP / 16;   // output columns of a lane, consecutive ones
+    constexpr int NV = NE / 4;    // words of its part of a V row
+    constexpr int NS = HALF ? 1 : 4;
+    const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t seq = seq32;
+    const int hd = (int)p.c.head_dim, new_tokens = (int)p.d.new_tokens, rows = p.rows;
+    const int tiles = (key_hi - key_lo + kTile - 1) / kTile, last16 = (key_hi - 1) >> 4;
+    const uint8_t *K = static_cast<const uint8_t *>(p.k) + hk * p.c.head_stride, *V = static_cast<const uint8_t *>(p.v) + hk * p.c.head_stride;
+    const float *KS = p.k_scales + hk * p.sc.head_stride, *VS = p.v_scales + hk * p.sc.head_stride;
+    const Const table = constant(p.table) + seq * p.c.table_stride;
+    const int rs = (int)p.c.row_stride, num_pages = (int)p.c.num_pages;
+    if (len == 0) {
+        store_empty(p, seq, hk, rt, bad);
+        return;
+    }
+
+    // this lane's query row (rows past the last repeat it and are never stored) and how many keys it sees
+    int rr = rt * 16 + lr;
+    rr = rr < rows ? rr : rows - 1;
+    const int in_group = (int)p.by_new((uint32_t)rr), qi = rr - in_group * new_tokens, qh = hk * p.group + in_group;
+    const int sees = len - new_tokens + 1 + qi;
+    const float *qr = p.q + seq * p.d.q_seq_stride + qi * p.d.q_row_stride + qh * p.d.q_head_stride;
+    float q[2 * NK][8];
+#pragma unroll
+    for (int i = 0; i < 2 * NK; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int c = (4 * (i / 2) + g) * 16 + 8 * (i % 2) + e;
+            q[i][e] = FULL || c < hd ? qr[c] : 0.f;
+        }
+
+    // The 16 keys number t16 (of the sequence): the page and the row in it of the first (ANY: of this lane's); half tiles past the
+    // end repeat the last one (ANY: keys past the end repeat the last one).
+    auto page_of = [&](int t16) __attribute__((always_inline)) {
+        int key;
+        if constexpr (ANY) {
+            key = (t16 << 4) + lr;
+            key = key < len ? key : len - 1;
+        } else {
+            key = (t16 < last16 ? t16 : last16) << 4;
+        }
+        const int index = (int)p.by_page((uint32_t)key);
+        return make_int2(table[index], key - index * (int)p.c.page_size);
+    };
+    struct Place {
+        int64_t row;   // the offset of the row
+        int64_t page;  // of the page's scales
+        int in_page;   // the row in its page
+    };
+    auto place_of = [&](int2 page) __attribute__((always_inline)) {
+        const bool there = page.x >= 0 && page.x < num_pages;
+        bad = bad || !there;
+        Place at;
+        at.row = (int64_t)(there ? page.x : 0) * p.c.page_stride + (int64_t)page.y * rs;
+        at.page = (int64_t)(there ? page.x : 0) * p.sc.page_stride;
+        at.in_page = page.y;
+        if constexpr (!ANY) {  // one for all lanes
+            at.row = (int64_t)__builtin_amdgcn_readfirstlane((int)(at.row >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)at.row);
+            at.page = (int64_t)__builtin_amdgcn_readfirstlane((int)(at.page >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)at.page);
+            at.in_page = __builtin_amdgcn_readfirstlane(at.in_page);
+        }
+        return at;
+    };
+    // the offset of row `row` of a half tile
+    auto row_offset = [&](const Place &at, int row) __attribute__((always_inline)) {
+        if constexpr (ANY) return (int64_t)__shfl((int)(at.row >> 32), row) << 32 | (uint32_t)__shfl((int)at.row, row);
+        return at.row + row * rs;
+    };
+    U4 kf[2][NK];
+    uint32_t vf[2][4][NV];
+    float ks[2][NS], vs[2][NS];  // of the half tile, or of this lane's keys 4 g + r
+    const uint32_t k_lane = (uint32_t)((ANY ? 0 : lr * rs) + g * 16);
+    uint32_t v_lane[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v_lane[r] = (uint32_t)((ANY ? 0 : (4 * g + r) * rs) + lr * NE);
+    auto load_scales = [&](float (&s)[2][NS], const float *from, const Place (&at)[2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if constexpr (HALF) {
+                s[h][0] = ((ConstF)(uintptr_t)from)[at[h].page + p.by_block((uint32_t)at[h].in_page)];
+            } else if constexpr (ANY) {
+                const float mine = from[at[h].page + p.by_block((uint32_t)at[h].in_page)];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[h][r] = __shfl(mine, 4 * g + r);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[h][r] = from[at[h].page + p.by_block((uint32_t)(at[h].in_page + 4 * g + r))];
+            }
+        }
+    };
+    auto load_k = [&](const Place (&at)[2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const uint8_t *base = K + at[s].row;
+#pragma unroll
+            for (int i = 0; i < NK; ++i) {
+                if (!FULL) kf[s][i] = U4{0u, 0u, 0u, 0u};
+                if (FULL || (4 * i + g) * 16 < hd) kf[s][i] = load128<NT>(base + k_lane + 64 * i);
+            }
+        }
+        load_scales(ks, KS, at);
+    };
+    auto load_v = [&](const Place (&at)[2]) __attribute__((always_inline)) {
+        using Row = uint32_t __attribute__((ext_vector_type(NV)));
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const uint8_t *base = V + at[s].row;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if constexpr (ANY) base = V + row_offset(at[s], 4 * g + r);
+                if (!FULL)
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) vf[s][r][i] = 0u;
+                if (FULL || lr * NE < hd) {
+                    const Row *src = reinterpret_cast<const Row *>(base + v_lane[r]);
+                    const Row w = NT ? __builtin_nontemporal_load(src) : *src;
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) vf[s][r][i] = w[i];
+                }
+            }
+        }
+        load_scales(vs, VS, at);
+    };
+
+    const int t16_lo = key_lo >> 4;
+    Place off[2];
+    int2 ahead[2];
+    auto begin = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            off[s] = place_of(page_of(t16_lo + 2 * wave + s));
+            ahead[s] = page_of(t16_lo + 2 * (wave + kWaves) + s);
+        }
+        load_k(off);  // (a wavefront without a tile reads the last one)
+        load_v(off);
+    };
+    begin();
+    __builtin_amdgcn_sched_barrier(0);
+
+    // The query row times a power of two that brings its largest element to [2^14, 2^15), in two parts (one that is not finite gives NaN).
+    H8 qp[2][2 * NK];
+    float big = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2 * NK; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(q[i][e]));
+    big = rows_reduce(big, MaxOp());
+    const int up = big > 0.f && big < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(big) : 0;
+    const float down = __builtin_ldexpf(1.f, -up);
+#pragma unroll
+    for (int i = 0; i < 2 * NK; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float x = __builtin_ldexpf(q[i][e], up);
+            qp[0][i][e] = (_Float16)x;
+            qp[1][i][e] = (_Float16)(x - (float)qp[0][i][e]);
+        }
+
+    F4 o[NE];
+    float m_run, l_run;  // the sum: this lane's keys only
+    const int limit = sees < key_hi ? sees : key_hi;
+
+    // One tile of 32 keys. `more` (a constant): another one of this wavefront follows, whose loads go out on the way (what a query
+    // may not see lies in the last two tiles of the sequence, which are the last ones of their wavefronts). `unit`: the factor of the weights.
+    auto step = [&](int t, float unit, auto more) __attribute__((always_inline)) {
+        const int key0 = key_lo + t * kTile;
+        F4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, low[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int i = 0; i < 2 * NK; ++i)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const H8 k8 = to_f16<T>(kf[s][i / 2][2 * (i % 2)], kf[s][i / 2][2 * (i % 2) + 1]);
+                low[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qp[1][i], low[s], 0, 0, 0);
+                sc[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qp[0][i], sc[s], 0, 0, 0);
+            }
+        float by[2][NS];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int r = 0; r < NS; ++r) by[s][r] = (ks[s][r] * down) * p.scale2;
+        Place next[2];
+        if constexpr (more) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                next[s] = place_of(ahead[s]);
+                ahead[s] = page_of(t16_lo + 2 * (t + 2 * kWaves) + s);
+            }
+            load_k(next);
+        }
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float x = (sc[s][r] + low[s][r]) * by[s][HALF ? 0 : r];
+                sc[s][r] = more || key0 + 16 * s + 4 * g + r < limit ? x : -__builtin_inff();
+                mx = fmaxf(mx, sc[s][r]);
+            }
+        mx = rows_reduce(mx, MaxOp());
+        if (__any(mx > m_run)) {
+            const float m_new = fmaxf(m_run, mx);
+            const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -__builtin_inff() ? 0.f : m_new));
+            m_run = m_new;
+            l_run *= alpha;
+#pragma unroll
+            for (int e = 0; e < NE; ++e)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[e][r] *= alpha;
+        }
+        // nothing visible so far: every weight is exp(-inf) = 0; a key that is not seen has weight 0 whatever its scale is
+        const float ref = m_run == -__builtin_inff() ? 0.f : m_run;
+        float w[8];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float e = __builtin_amdgcn_exp2f(sc[s][r] - ref);
+                l_run += e;
+                w[4 * s + r] = more || key0 + 16 * s + 4 * g + r < limit ? e * (vs[s][HALF ? 0 : r] * unit) : 0.f;
+            }
+        // A NaN code under a weight of 0 would be NaN: what lies past the keys counts as zero, and so does, in keys that only the later of the new
+        // tokens see, a NaN, which is added below to the rows that see it.
+        const int partly = len - new_tokens + 1;
+        bool held = false;
+        if constexpr (kNan && !more) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int key = key0 + 16 * s + 4 * g + r;
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) {
+                        const uint32_t nan = key >= partly && key < key_hi ? nan_bytes(vf[s][r][i]) : 0u;
+                        held |= nan != 0u;
+                        vf[s][r][i] = key >= key_hi ? 0u : vf[s][r][i] & ~((nan >> 7) * 255u);
+                    }
+                }
+        }
+        // The weights in three parts of bf16, and the products with the columns of V.
+        B8 wp[3];
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                wp[j][e] = (__bf16)w[e];
+                w[e] -= (float)wp[j][e];
+            }
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+            U4 column;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) column[j] = to_bf16<T>(vf[j >> 1][2 * (j & 1)][e / 4], vf[j >> 1][2 * (j & 1) + 1][e / 4], e % 4);
+#pragma unroll
+            for (int j = 2; j >= 0; --j) o[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(B8, column), wp[j], o[e], 0, 0, 0);
+        }
+        if constexpr (kNan && !more) {
+            if (__any(held)) {
+                const int from = partly > key0 ? partly : key0, to = key_hi < key0 + kTile ? key_hi : key0 + kTile;
+                for (int key = from; key < to; ++key) {
+                    const uint8_t *vr = V + row_offset(off[(key - key0) >> 4], (key - key0) & 15);
+#pragma unroll
+                    for (int e = 0; e < NE; ++e)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int c = (4 * g + r) * NE + e;
+                            if (key < sees && (FULL || c < hd) && (vr[c] & 127) == 127) o[e][r] = __builtin_nanf("");
+                        }
+                }
+            }
+        }
+        if constexpr (more) {
+            load_v(next);
+            off[0] = next[0];
+            off[1] = next[1];
+        }
+    };
+    for (float unit = 0x1p40f;; unit = 0x1p-24f) {
+        m_run = -__builtin_inff();
+        l_run = 0.f;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) o[e] = F4{0.f, 0.f, 0.f, 0.f};
+        if (wave >= tiles) break;
+        int t = wave;
+        for (; t + kWaves < tiles; t += kWaves) step(t, unit, std::true_type());
+        step(t, unit, std::false_type());
+        float check = 0.f;
+#pragma unroll
+        for (int e = 0; e < NE; ++e)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                check = __builtin_fmaf(o[e][r], 0.f, check);
+                o[e][r] *= unit > 1.f ? 0x1p-40f : 0x1p24f;
+            }
+        if (unit < 1.f || !__any(!(check == 0.f))) break;
+        begin();
+    }
+
+    if constexpr (ANY) bad = __any(bad);
+    join_wavefronts<DP>(p, lds_o, lds_ml, seq, hk, rt, len, bad, alone, slot0, o, m_run, l_run,
+                        [&](int e, int r) __attribute__((always_inline)) { return (4 * g + r) * NE + e; });
+}
+
+template <typename T, int DP, bool FULL, bool NT, ScaleOf OF, bool EVEN>
+__global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void paged_sdpa_scaled_kernel(const ScaledArgs p) {
+    __shared__ __attribute__((aligned(16))) float lds_o[kWaves * 16 * (DP + 4)];
+    __shared__ float lds_ml[kWaves * 16 * 2];
+    fetch_arguments<ScaledArgs>();
+    walk_shares<EVEN>(p, [&](int seq, int hk, int rt, int len, bool bad, int key_lo, int key_hi, bool alone, int64_t slot) __attribute__((always_inline)) {
+        scaled_segment<T, DP, FULL, NT, OF>(p, lds_o, lds_ml, seq, hk, rt, len, bad, key_lo, key_hi, alone, slot);
+    });
+}
+
+template <typename T> int32_t launch_scaled(const ScaledArgs &a, const Plan &pl, bool tiles, hipStream_t st) {
+    if (tiles) {
+        const int64_t grid = tiles_grid(a);
+        FTH_ARG(grid <= 2147483647LL, "paged_sdpa_scaled: too many workgroups for one launch");
+        auto go = [&](auto kernel) { kernel<<<dim3((unsigned)grid), dim3(64 * kWaves), 0, st>>>(a); };
+        const bool nt = pl.nt, full = a.c.head_dim == 64 || a.c.head_dim == 128 || a.c.head_dim == 256;
+        const bool half = a.c.page_size % 16 == 0 && a.sc.block % 16 == 0, key = a.c.page_size % 16 == 0 && full;
+        auto pick = [&](auto even) {
+            constexpr bool E = decltype(even)::value;
+            constexpr ScaleOf H = ScaleOf::half, K = ScaleOf::key, A = ScaleOf::any;
+            auto size = [&](auto dp) {
+                constexpr int DP = decltype(dp)::value;
+                if (half && full) go(nt ? paged_sdpa_scaled_kernel<T, DP, true, true, H, E> : paged_sdpa_scaled_kernel<T, DP, true, false, H, E>);
+                else if (half) go(paged_sdpa_scaled_kernel<T, DP, false, false, H, E>);
+                else if (key) go(nt ? paged_sdpa_scaled_kernel<T, DP, true, true, K, E> : paged_sdpa_scaled_kernel<T, DP, true, false, K, E>);
+                else go(paged_sdpa_scaled_kernel<T, DP, false, false, A, E>);
+            };
+            if (a.c.head_dim <= 64) size(std::integral_constant<int, 64>());
+            else if (a.c.head_dim <= 128) size(std::integral_constant<int, 128>());
+            else size(std::integral_constant<int, 256>());
+        };
+        if (a.even) pick(std::true_type());
+        else pick(std::false_type());
+    } else {
+        FTH_ARG(pl.rows * a.nsplit <= 2147483647LL, "paged_sdpa_scaled: too many rows for one launch");
+        paged_sdpa_rows_kernel<T, ScaledArgs><<<dim3((unsigned)(pl.rows * a.nsplit)), dim3(64), 0, st>>>(a);
+    }
     FTH_CHECK_LAUNCH("paged_sdpa_scaled");
     return launch_join(a, pl, st);
 }
 
-int32_t launch_e4m3(ScaledArgs &a, const Plan &pl, bool tiles, hipStream_t st);
-int32_t launch_i8(ScaledArgs &a, const Plan &pl, bool tiles, hipStream_t st);
+int32_t launch_e4m3(const ScaledArgs &a, const Plan &pl, bool tiles, hipStream_t st);
+int32_t launch_i8(const ScaledArgs &a, const Plan &pl, bool tiles, hipStream_t st);
 
 }  // namespace paged
 }  // namespace fth
