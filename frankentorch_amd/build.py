@@ -37,6 +37,7 @@ HIP_SOURCES = [
     "ingest.hip",
     "int8ops.hip",
     "paged_append.hip",
+    "paged_sdpa_shares.hip",
     "paged_sdpa.hip",
     "paged_append_scaled.hip",
     "paged_sdpa_scaled.hip",

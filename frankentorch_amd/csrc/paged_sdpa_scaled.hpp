@@ -31,9 +31,10 @@ using B2 = __bf16 __attribute__((ext_vector_type(2)));
 using B8 = __bf16 __attribute__((ext_vector_type(8)));
 using ConstF = const float __attribute__((address_space(4))) *;
 
-// Where the scales of a tile's keys come from: one for each half tile (blocks and pages are multiples of 16: scalar loads); a load for each
-// key, the rows found from the half tile's first (pages are multiples of 16); a load for each key, whose page every lane looks up (any pages).
-enum class ScaleOf { half, key, any };
+// Where the scales of 16 keys come from: one number (blocks and pages are multiples of 16: a scalar load); one for each four (blocks are
+// multiples of 4, pages of 16); one for each key, four in a 128-bit load (blocks of one, pages of 16); one for each key, whose page every
+// lane looks up (any pages and blocks).
+enum class ScaleOf { sixteen, four, one, any };
 
 // 8 codes (two words) as f16.
 template <typename T> __device__ __forceinline__ H8 to_f16(uint32_t a, uint32_t b) {
@@ -69,23 +70,28 @@ template <typename T> __device__ __forceinline__ uint32_t to_bf16(uint32_t first
 // Bit 7 of every byte that is a NaN of e4m3.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
+// 16 keys so many times make a tile of a wavefront.
+template <int DP, ScaleOf OF> constexpr int sixteens() { return 2; }
+
 // One segment: keys key_lo .. key_hi - 1 of a pair of `len` keys, with row tile rt of its queries. FULL: head_dim == DP; otherwise what lies past
 // head_dim counts as zero. NT: K and V leave no trace in the caches.
 template <typename T, int DP, bool FULL, bool NT, ScaleOf OF>
 __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o, float *lds_ml, int seq32, int hk, int rt, int len, bool bad, int key_lo, int key_hi, bool alone, int64_t slot0) {
-    constexpr bool ANY = OF == ScaleOf::any, HALF = OF == ScaleOf::half, kNan = std::is_same<T, fth::e4m3>::value;
+    constexpr bool ANY = OF == ScaleOf::any, SIXTEEN = OF == ScaleOf::sixteen, FOUR = OF == ScaleOf::four, kNan = std::is_same<T, fth::e4m3>::value;
     constexpr int NK = DP / 64;   // 128-bit loads of a lane's quarter of a K row
     constexpr int NE = DP / 16;   // output columns of a lane, consecutive ones
     constexpr int NV = NE / 4;    // words of its part of a V row
-    constexpr int NS = HALF ? 1 : 4;
+    constexpr int NS = SIXTEEN || FOUR ? 1 : 4;
+    constexpr int H = sixteens<DP, OF>(), kKeys = 16 * H;
     const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t seq = seq32;
     const int hd = (int)p.c.head_dim, new_tokens = (int)p.d.new_tokens, rows = p.rows;
-    const int tiles = (key_hi - key_lo + kTile - 1) / kTile, last16 = (key_hi - 1) >> 4;
+    const int tiles = (key_hi - key_lo + kKeys - 1) / kKeys, last16 = (key_hi - 1) >> 4;
     const uint8_t *K = static_cast<const uint8_t *>(p.k) + hk * p.c.head_stride, *V = static_cast<const uint8_t *>(p.v) + hk * p.c.head_stride;
     const float *KS = p.k_scales + hk * p.sc.head_stride, *VS = p.v_scales + hk * p.sc.head_stride;
     const Const table = constant(p.table) + seq * p.c.table_stride;
+    const int t16_lo = key_lo >> 4;
     const int rs = (int)p.c.row_stride, num_pages = (int)p.c.num_pages;
     if (len == 0) {
         store_empty(p, seq, hk, rt, bad);
@@ -128,14 +134,34 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
     auto place_of = [&](int2 page) __attribute__((always_inline)) {
         const bool there = page.x >= 0 && page.x < num_pages;
         bad = bad || !there;
-        Place at;
-        at.row = (int64_t)(there ? page.x : 0) * p.c.page_stride + (int64_t)page.y * rs;
-        at.page = (int64_t)(there ? page.x : 0) * p.sc.page_stride;
-        at.in_page = page.y;
-        if constexpr (!ANY) {  // one for all lanes
-            at.row = (int64_t)__builtin_amdgcn_readfirstlane((int)(at.row >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)at.row);
-            at.page = (int64_t)__builtin_amdgcn_readfirstlane((int)(at.page >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)at.page);
-            at.in_page = __builtin_amdgcn_readfirstlane(at.in_page);
+        return Place{(int64_t)(there ? page.x : 0) * p.c.page_stride + (int64_t)page.y * rs, (int64_t)(there ? page.x : 0) * p.sc.page_stride, page.y};
+    };
+    // Where the next 64 of this wavefront's half tiles are, one a lane (a half tile costs some 60 scalar instructions by itself, as many
+    // as half of its products take): half tile j is number t16_lo + H wave + s + H kWaves (j / H), s = j % H.
+    Place mine;
+    float my_ks = 0.f, my_vs = 0.f;  // SIXTEEN: the scales
+    auto page_ahead = [&](int j0) __attribute__((always_inline)) {
+        const int j = j0 + lane, t16 = t16_lo + H * wave + j % H + H * kWaves * (j / H), key = (t16 < last16 ? t16 : last16) << 4, index = (int)p.by_page((uint32_t)key);
+        return make_int2(p.table[seq * p.c.table_stride + index], key - index * (int)p.c.page_size);
+    };
+    int2 ahead64;
+    auto look_ahead = [&](int j0) __attribute__((always_inline)) {
+        mine = place_of(ahead64);
+        if constexpr (SIXTEEN) {
+            const int64_t at = mine.page + p.by_block((uint32_t)mine.in_page);
+            my_ks = KS[at];
+            my_vs = VS[at];
+        }
+        ahead64 = page_ahead(j0 + 64);
+    };
+    auto one_of = [&](int64_t x, int j) __attribute__((always_inline)) {
+        return (int64_t)__builtin_amdgcn_readlane((int)(x >> 32), j) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, j);
+    };
+    auto half_tile = [&](int j) __attribute__((always_inline)) {
+        Place at = {one_of(mine.row, j & 63), 0, 0};
+        if constexpr (!SIXTEEN) {
+            at.page = one_of(mine.page, j & 63);
+            at.in_page = __builtin_amdgcn_readlane(mine.in_page, j & 63);
         }
         return at;
     };
@@ -144,31 +170,33 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
         if constexpr (ANY) return (int64_t)__shfl((int)(at.row >> 32), row) << 32 | (uint32_t)__shfl((int)at.row, row);
         return at.row + row * rs;
     };
-    U4 kf[2][NK];
-    uint32_t vf[2][4][NV];
-    float ks[2][NS], vs[2][NS];  // of the half tile, or of this lane's keys 4 g + r
+    U4 kf[H][NK];
+    uint32_t vf[H][4][NV];
+    float ks[H][NS], vs[H][NS];  // of 16 keys, of this lane's keys 4 g .. 4 g + 3, or of each of them
     const uint32_t k_lane = (uint32_t)((ANY ? 0 : lr * rs) + g * 16);
     uint32_t v_lane[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) v_lane[r] = (uint32_t)((ANY ? 0 : (4 * g + r) * rs) + lr * NE);
-    auto load_scales = [&](float (&s)[2][NS], const float *from, const Place (&at)[2]) __attribute__((always_inline)) {
+    auto load_scales = [&](float (&s)[H][NS], const float *from, const Place (&at)[H]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if constexpr (HALF) {
-                s[h][0] = ((ConstF)(uintptr_t)from)[at[h].page + p.by_block((uint32_t)at[h].in_page)];
+        for (int h = 0; h < H; ++h) {
+            if constexpr (SIXTEEN) {  // in the lanes, see above
             } else if constexpr (ANY) {
-                const float mine = from[at[h].page + p.by_block((uint32_t)at[h].in_page)];
+                const float of_row = from[at[h].page + p.by_block((uint32_t)at[h].in_page)];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[h][r] = __shfl(mine, 4 * g + r);
+                for (int r = 0; r < 4; ++r) s[h][r] = __shfl(of_row, 4 * g + r);
+            } else if constexpr (FOUR) {
+                s[h][0] = from[at[h].page + p.by_block((uint32_t)(at[h].in_page + 4 * g))];
             } else {
+                const F4 x = *reinterpret_cast<const F4 *>(from + at[h].page + at[h].in_page + 4 * g);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[h][r] = from[at[h].page + p.by_block((uint32_t)(at[h].in_page + 4 * g + r))];
+                for (int r = 0; r < 4; ++r) s[h][r] = x[r];
             }
         }
     };
-    auto load_k = [&](const Place (&at)[2]) __attribute__((always_inline)) {
+    auto load_k = [&](const Place (&at)[H]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < H; ++s) {
             const uint8_t *base = K + at[s].row;
 #pragma unroll
             for (int i = 0; i < NK; ++i) {
@@ -178,10 +206,10 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
         }
         load_scales(ks, KS, at);
     };
-    auto load_v = [&](const Place (&at)[2]) __attribute__((always_inline)) {
+    auto load_v = [&](const Place (&at)[H]) __attribute__((always_inline)) {
         using Row = uint32_t __attribute__((ext_vector_type(NV)));
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < H; ++s) {
             const uint8_t *base = V + at[s].row;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -200,17 +228,27 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
         load_scales(vs, VS, at);
     };
 
-    const int t16_lo = key_lo >> 4;
-    Place off[2];
-    int2 ahead[2];
+    int2 ahead[H];  // ANY: of the next tile
     auto begin = [&]() __attribute__((always_inline)) {
+        Place at[H];
+        if constexpr (ANY) {
+            int2 now[H];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            off[s] = place_of(page_of(t16_lo + 2 * wave + s));
-            ahead[s] = page_of(t16_lo + 2 * (wave + kWaves) + s);
+            for (int s = 0; s < H; ++s) {
+                now[s] = page_of(t16_lo + H * wave + s);
+                ahead[s] = page_of(t16_lo + H * (wave + kWaves) + s);
+            }
+#pragma unroll
+            for (int s = 0; s < H; ++s) at[s] = place_of(now[s]);
+        } else {
+            ahead64 = page_ahead(0);
+            look_ahead(0);
+            __builtin_amdgcn_sched_barrier(0);  // the scales before K and V: who waits for them would wait for V
+#pragma unroll
+            for (int s = 0; s < H; ++s) at[s] = half_tile(s);
         }
-        load_k(off);  // (a wavefront without a tile reads the last one)
-        load_v(off);
+        load_k(at);  // (a wavefront without a tile reads the last one)
+        load_v(at);
     };
     begin();
     __builtin_amdgcn_sched_barrier(0);
@@ -238,39 +276,54 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
     float m_run, l_run;  // the sum: this lane's keys only
     const int limit = sees < key_hi ? sees : key_hi;
 
-    // One tile of 32 keys. `more` (a constant): another one of this wavefront follows, whose loads go out on the way (what a query
+    // One tile. `more` (a constant): another one of this wavefront follows, whose loads go out on the way (what a query
     // may not see lies in the last two tiles of the sequence, which are the last ones of their wavefronts). `unit`: the factor of the weights.
     auto step = [&](int t, float unit, auto more) __attribute__((always_inline)) {
-        const int key0 = key_lo + t * kTile;
-        F4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, low[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        const int key0 = key_lo + t * kKeys;
+        F4 sc[H], low[H];
+#pragma unroll
+        for (int s = 0; s < H; ++s) sc[s] = low[s] = F4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < 2 * NK; ++i)
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
+            for (int s = 0; s < H; ++s) {
                 const H8 k8 = to_f16<T>(kf[s][i / 2][2 * (i % 2)], kf[s][i / 2][2 * (i % 2) + 1]);
                 low[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qp[1][i], low[s], 0, 0, 0);
                 sc[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qp[0][i], sc[s], 0, 0, 0);
             }
-        float by[2][NS];
+        float by[H][NS];
+        const int j = H * (t - wave) / kWaves;
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < H; ++s)
 #pragma unroll
-            for (int r = 0; r < NS; ++r) by[s][r] = (ks[s][r] * down) * p.scale2;
-        Place next[2];
+            for (int r = 0; r < NS; ++r) {
+                if constexpr (SIXTEEN) {
+                    ks[s][r] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_ks), (j + s) & 63));
+                    vs[s][r] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_vs), (j + s) & 63));
+                }
+                by[s][r] = (ks[s][r] * down) * p.scale2;
+            }
+        Place next[H];
         if constexpr (more) {
+            if constexpr (ANY) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                next[s] = place_of(ahead[s]);
-                ahead[s] = page_of(t16_lo + 2 * (t + 2 * kWaves) + s);
+                for (int s = 0; s < H; ++s) {
+                    next[s] = place_of(ahead[s]);
+                    ahead[s] = page_of(t16_lo + H * (t + 2 * kWaves) + s);
+                }
+            } else {
+                if (((j + H) & 63) == 0) look_ahead(j + H);
+#pragma unroll
+                for (int s = 0; s < H; ++s) next[s] = half_tile(j + H + s);
             }
             load_k(next);
         }
         float mx = -__builtin_inff();
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < H; ++s)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float x = (sc[s][r] + low[s][r]) * by[s][HALF ? 0 : r];
+                const float x = (sc[s][r] + low[s][r]) * by[s][NS == 1 ? 0 : r];
                 sc[s][r] = more || key0 + 16 * s + 4 * g + r < limit ? x : -__builtin_inff();
                 mx = fmaxf(mx, sc[s][r]);
             }
@@ -287,14 +340,14 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
         }
         // nothing visible so far: every weight is exp(-inf) = 0; a key that is not seen has weight 0 whatever its scale is
         const float ref = m_run == -__builtin_inff() ? 0.f : m_run;
-        float w[8];
+        float w[H][4];
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < H; ++s)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float e = __builtin_amdgcn_exp2f(sc[s][r] - ref);
                 l_run += e;
-                w[4 * s + r] = more || key0 + 16 * s + 4 * g + r < limit ? e * (vs[s][HALF ? 0 : r] * unit) : 0.f;
+                w[s][r] = more || key0 + 16 * s + 4 * g + r < limit ? e * (vs[s][NS == 1 ? 0 : r] * unit) : 0.f;
             }
         // A NaN code under a weight of 0 would be NaN: what lies past the keys counts as zero, and so does, in keys that only the later of the new
         // tokens see, a NaN, which is added below to the rows that see it.
@@ -302,7 +355,7 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
         bool held = false;
         if constexpr (kNan && !more) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
+            for (int s = 0; s < H; ++s)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int key = key0 + 16 * s + 4 * g + r;
@@ -314,28 +367,33 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
                     }
                 }
         }
-        // The weights in three parts of bf16, and the products with the columns of V.
-        B8 wp[3];
+        // The weights in three parts of bf16, and the products with the columns of V, 32 keys at a time.
 #pragma unroll
-        for (int j = 0; j < 3; ++j)
+        for (int two = 0; two < H; two += 2) {
+            B8 wp[3];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                wp[j][e] = (__bf16)w[e];
-                w[e] -= (float)wp[j][e];
+            for (int j = 0; j < 3; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float &x = w[two + (e >> 2)][e & 3];
+                    wp[j][e] = (__bf16)x;
+                    x -= (float)wp[j][e];
+                }
+#pragma unroll
+            for (int e = 0; e < NE; ++e) {
+                U4 column;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) column[j] = to_bf16<T>(vf[two + (j >> 1)][2 * (j & 1)][e / 4], vf[two + (j >> 1)][2 * (j & 1) + 1][e / 4], e % 4);
+#pragma unroll
+                for (int j = 2; j >= 0; --j) o[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(B8, column), wp[j], o[e], 0, 0, 0);
             }
-#pragma unroll
-        for (int e = 0; e < NE; ++e) {
-            U4 column;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) column[j] = to_bf16<T>(vf[j >> 1][2 * (j & 1)][e / 4], vf[j >> 1][2 * (j & 1) + 1][e / 4], e % 4);
-#pragma unroll
-            for (int j = 2; j >= 0; --j) o[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(B8, column), wp[j], o[e], 0, 0, 0);
         }
         if constexpr (kNan && !more) {
             if (__any(held)) {
-                const int from = partly > key0 ? partly : key0, to = key_hi < key0 + kTile ? key_hi : key0 + kTile;
+                const int from = partly > key0 ? partly : key0, to = key_hi < key0 + kKeys ? key_hi : key0 + kKeys;
                 for (int key = from; key < to; ++key) {
-                    const uint8_t *vr = V + row_offset(off[(key - key0) >> 4], (key - key0) & 15);
+                    const Place place = place_of(page_of(key >> 4));
+                    const uint8_t *vr = V + row_offset(place, key & 15);
 #pragma unroll
                     for (int e = 0; e < NE; ++e)
 #pragma unroll
@@ -348,8 +406,6 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
         }
         if constexpr (more) {
             load_v(next);
-            off[0] = next[0];
-            off[1] = next[1];
         }
     };
     for (float unit = 0x1p40f;; unit = 0x1p-24f) {
@@ -373,7 +429,7 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
         begin();
     }
 
-    if constexpr (ANY) bad = __any(bad);
+    bad = __any(bad);
     join_wavefronts<DP>(p, lds_o, lds_ml, seq, hk, rt, len, bad, alone, slot0, o, m_run, l_run,
                         [&](int e, int r) __attribute__((always_inline)) { return (4 * g + r) * NE + e; });
 }
@@ -394,16 +450,17 @@ template <typename T> int32_t launch_scaled(const ScaledArgs &a, const Plan &pl,
         FTH_ARG(grid <= 2147483647LL, "paged_sdpa_scaled: too many workgroups for one launch");
         auto go = [&](auto kernel) { kernel<<<dim3((unsigned)grid), dim3(64 * kWaves), 0, st>>>(a); };
         const bool nt = pl.nt, full = a.c.head_dim == 64 || a.c.head_dim == 128 || a.c.head_dim == 256;
-        const bool half = a.c.page_size % 16 == 0 && a.sc.block % 16 == 0, key = a.c.page_size % 16 == 0 && full;
+        const bool pages = a.c.page_size % 16 == 0, sixteen = pages && a.sc.block % 16 == 0, four = pages && full && a.sc.block % 4 == 0;
+        const bool one = pages && full && a.sc.block == 1 && ((uintptr_t)a.k_scales % 16 | (uintptr_t)a.v_scales % 16 | a.sc.page_stride % 4 | a.sc.head_stride % 4) == 0;
         auto pick = [&](auto even) {
             constexpr bool E = decltype(even)::value;
-            constexpr ScaleOf H = ScaleOf::half, K = ScaleOf::key, A = ScaleOf::any;
             auto size = [&](auto dp) {
                 constexpr int DP = decltype(dp)::value;
-                if (half && full) go(nt ? paged_sdpa_scaled_kernel<T, DP, true, true, H, E> : paged_sdpa_scaled_kernel<T, DP, true, false, H, E>);
-                else if (half) go(paged_sdpa_scaled_kernel<T, DP, false, false, H, E>);
-                else if (key) go(nt ? paged_sdpa_scaled_kernel<T, DP, true, true, K, E> : paged_sdpa_scaled_kernel<T, DP, true, false, K, E>);
-                else go(paged_sdpa_scaled_kernel<T, DP, false, false, A, E>);
+                if (sixteen && full) go(nt ? paged_sdpa_scaled_kernel<T, DP, true, true, ScaleOf::sixteen, E> : paged_sdpa_scaled_kernel<T, DP, true, false, ScaleOf::sixteen, E>);
+                else if (sixteen) go(paged_sdpa_scaled_kernel<T, DP, false, false, ScaleOf::sixteen, E>);
+                else if (one) go(nt ? paged_sdpa_scaled_kernel<T, DP, true, true, ScaleOf::one, E> : paged_sdpa_scaled_kernel<T, DP, true, false, ScaleOf::one, E>);
+                else if (four) go(paged_sdpa_scaled_kernel<T, DP, true, false, ScaleOf::four, E>);
+                else go(paged_sdpa_scaled_kernel<T, DP, false, false, ScaleOf::any, E>);
             };
             if (a.c.head_dim <= 64) size(std::integral_constant<int, 64>());
             else if (a.c.head_dim <= 128) size(std::integral_constant<int, 128>());
