@@ -3,7 +3,7 @@
 // Tokens are ordered by a code of 64 bits, the complement of the logit's ordered bits above the index: smaller codes come first. Every
 // filter keeps a prefix of that order, so the kept tokens are those up to a last code (and above min-p). Weights are fp64 exponentials; where sums of
 // them are collected by atomics they are whole numbers W = round(2^S w), whose sums do not depend on the order. Two launches:
-//   * pieces: one wavefront for 1024 logits, which it holds. It finds their maximum; where all of the row count (no top-k) the sum of their
+//   * pieces: one wavefront for 2048 logits, which it holds. It finds their maximum; where all of the row count (no top-k) the sum of their
 //     weights relative to that maximum; and where there is a filter it writes down the largest of them, in the order of the vocabulary: at least
 //     `want`, by a bisection of the lanes' maxima, which costs a comparison of one register a step.
 //   * choice: one workgroup for a row. Without a filter the sums of the pieces give the piece, and its logits the token. With one, the
@@ -15,8 +15,9 @@
 
 namespace {
 
-constexpr int kPiece = 1024, kEntries = 64, kWaves = 4;          // logits of a piece, candidates that it may write down, pieces of a workgroup
-constexpr int kThreads = 1024, kBins = 2048, kList = 8192, kFew = 1024;  // the choice: bins, candidates in LDS, members of a bin that are ranked
+constexpr int kPiece = 2048, kEntries = 128, kWaves = 4;         // logits of a piece, candidates that it may write down, pieces of a workgroup
+constexpr int kThreads = 1024, kBins = 2048, kList = 7168, kFew = 1024;   // the choice: bins, candidates in LDS, members of a bin that are ranked
+constexpr int kPlaces = 512, kAhead = 4;                            // pieces of a row whose candidates are listed; of a wavefront, fetched at once
 
 struct Piece {
     float max, limit;  // of what is not written down, every logit is below `limit` (-inf: all is written down)
@@ -39,11 +40,13 @@ struct SampleArgs {
     Piece *pieces;
     Entry *entries;
     int per_row;  // pieces of a row
-    int want_p;   // candidates of a piece for top-p and min-p
+    int want_p;   // lanes of a piece that write something down for top-p and min-p
     double magic; // 1.5 * 2^(52 - S): added to a weight in [0, 1], leaves round(2^S weight) in the low bits
     double unit;  // 2^S
+    fth::Divisor by_pieces;  // by per_row
 };
 
+constexpr int kVecs = kPiece / 256;
 using F4u = float __attribute__((ext_vector_type(4), aligned(4)));  // rows start anywhere
 
 // A row's settings as they are used.
@@ -72,108 +75,148 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 }
 __device__ __forceinline__ uint64_t code_of(float x, uint32_t v) { return (uint64_t)order_of(x) << 32 | v; }
 
-template <typename T, typename F> __device__ __forceinline__ T wave_reduce(T x, F op) {
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) x = op(x, (T)__shfl_xor(x, m));
-    return x;
+// Across a wavefront by data-parallel moves (a shuffle through LDS costs five times as much): a lane without a source gets `old`.
+template <int CTRL, int ROWS, typename T> __device__ __forceinline__ T moved(T old, T x) {
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, old), __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
+    } else {
+        const uint64_t o = __builtin_bit_cast(uint64_t, old), v = __builtin_bit_cast(uint64_t, x);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp((int)o, (int)v, CTRL, ROWS, 0xf, false);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp((int)(o >> 32), (int)(v >> 32), CTRL, ROWS, 0xf, false);
+        return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
+    }
+}
+template <typename T> __device__ __forceinline__ T lane_value(T x, int lane) {
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
+    } else {
+        const uint64_t v = __builtin_bit_cast(uint64_t, x);
+        return __builtin_bit_cast(T, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane));
+    }
+}
+// op over the lanes up to each one: within rows of 16, then the last of a row into the next, then of the first half into the second. NEUTRAL is
+// its neutral element.
+template <typename T, typename F> __device__ __forceinline__ T wave_scan(T x, T neutral, F op) {
+    x = op(moved<0x111, 0xf>(neutral, x), x);
+    x = op(moved<0x112, 0xf>(neutral, x), x);
+    x = op(moved<0x114, 0xf>(neutral, x), x);
+    x = op(moved<0x118, 0xf>(neutral, x), x);
+    x = op(moved<0x142, 0xa>(neutral, x), x);
+    return op(moved<0x143, 0xc>(neutral, x), x);
 }
 struct MaxOp { template <typename T> __device__ T operator()(T a, T b) const { return a > b ? a : b; } };
 struct AddOp { template <typename T> __device__ T operator()(T a, T b) const { return a + b; } };
+template <typename T> __device__ __forceinline__ T wave_sum(T x) { return lane_value(wave_scan(x, (T)0, AddOp()), 63); }
+__device__ __forceinline__ float wave_max(float x) { return lane_value(wave_scan(x, -__builtin_inff(), MaxOp()), 63); }
 
 // ---- pieces -----------------------------------------------------------------------------------------------------------------
 
 __global__ __launch_bounds__(64 * kWaves) void sample_pieces_kernel(const SampleArgs p) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int64_t piece = (int64_t)blockIdx.x * kWaves + wave;
-    const int64_t r = piece / p.per_row;
+    const int piece32 = (int)blockIdx.x * kWaves + wave, row32 = (int)p.by_pieces((uint32_t)piece32);
+    const int64_t piece = piece32, r = row32;
     if (r >= p.d.rows) return;
-    const int64_t v0 = (piece - r * p.per_row) * kPiece;
+    const int64_t v0 = (int64_t)(piece32 - row32 * p.per_row) * kPiece;
     const int n = (int)(p.d.vocab - v0 < kPiece ? p.d.vocab - v0 : kPiece);
     const float *x = p.logits + r * p.d.logits_stride + v0;
-    F4u z[4];
+    F4u z[kVecs];  // logit 256 s + 4 lane + e of the piece
+    if (n == kPiece) {
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        const int i = 256 * s + 4 * lane;
-        z[s] = F4u{-__builtin_inff(), -__builtin_inff(), -__builtin_inff(), -__builtin_inff()};
-        if (i + 4 <= n) z[s] = *reinterpret_cast<const F4u *>(x + i);
-        else
+        for (int s = 0; s < kVecs; ++s) z[s] = *reinterpret_cast<const F4u *>(x + 256 * s + 4 * lane);
+    } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (i + e < n) z[s][e] = x[i + e];
+        for (int s = 0; s < kVecs; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[s][e] = 256 * s + 4 * lane + e < n ? x[256 * s + 4 * lane + e] : -__builtin_inff();
     }
     const Settings set(p, r);
     float mine = -__builtin_inff();
-    bool bad = false;
+    int up = 0;          // +inf and positive NaN are the largest numbers as signed integers,
+    uint32_t down = 0u;  // negative NaN as unsigned ones
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+    for (int s = 0; s < kVecs; ++s)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            bad |= !(z[s][e] < __builtin_inff());
+            const uint32_t bits = __float_as_uint(z[s][e]);
             mine = fmaxf(mine, z[s][e]);
+            up = (int)bits > up ? (int)bits : up;
+            down = bits > down ? bits : down;
         }
-    bad = __any(bad);
-    Piece out = {wave_reduce(mine, MaxOp()), -__builtin_inff(), 0u, bad ? 1u : 0u, 0.0};
+    const bool bad = __any(up >= 0x7f800000 || down > 0xff800000u);
+    Piece out = {wave_max(mine), -__builtin_inff(), 0u, bad ? 1u : 0u, 0.0};
     if (!bad && !set.bad && out.max > -__builtin_inff()) {
         if (set.top_k == 0) {
             double sum = 0.0;
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
+            for (int s = 0; s < kVecs; ++s)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum += fth::exp2_softmax(((double)z[s][e] - (double)out.max) * set.rate);
-            out.sum = wave_reduce(sum, AddOp());
+            out.sum = wave_sum(sum);
         }
         if (set.filters()) {
-            // The largest power-of-two-spaced number that `want` lanes reach; fewer where they would write down too much.
+            // How many lanes shall write something down (tokens of a vocabulary in order of frequency have their largest logits side by side),
+            // and what cannot be kept, as far as the piece by itself can tell (no more than a hint: `limit` says what was left out).
             int want = p.want_p;
+            float hint = -3.402823466e38f;
             if (set.top_k > 0) {
-                const int share = 2 * ((set.top_k + p.per_row - 1) / p.per_row) + 14;
-                want = share < 40 ? share : 40;
+                const int share = 2 * (int)p.by_pieces((uint32_t)((set.top_k < 1 << 30 ? set.top_k : 1 << 30) + p.per_row - 1)) + 14;
+                want = share < 36 ? 36 : share < 52 ? share : 52;
                 want = want < set.top_k ? want : set.top_k;
+            } else {
+                const float part = set.top_p < 1.f ? (1.f - set.top_p) * (float)out.sum * (1.f / kPiece) : 0.f, far = fmaxf(part, set.min_p * 0.999f);
+                if (far > 0.f) hint = fmaxf(hint, out.max + __builtin_amdgcn_logf(far) / (float)set.rate);
             }
             const uint32_t key = order_of(mine);
             Entry *to = p.entries + piece * kEntries;
-            for (; want > 0; want >>= 1) {
-                // the smallest c (16 bits) for which `want` lanes have key < (c + 1) << 16
-                uint32_t c = 0;
+            // Written down is what reaches `least`: all that the hint leaves, if few lanes have any of it; else what reaches the number of 16 bits that
+            // `want` lanes reach, or fewer lanes where that would be too much.
+            float least = hint;
+            if (least > -3.402823466e38f) out.limit = least;
+            bool first = __popcll(__ballot(mine >= least)) > want;
+            for (;;) {
+                if (!first) {
+                    uint64_t in[4 * kVecs];
+                    uint32_t n_in = 0;
+#pragma unroll
+                    for (int i = 0; i < 4 * kVecs; ++i) {
+                        in[i] = __ballot(z[i >> 2][i & 3] >= least);
+                        n_in += __popcll(in[i]);
+                    }
+                    if (n_in <= kEntries) {
+                        out.count = n_in;
+                        uint32_t at = 0;
+#pragma unroll
+                        for (int s = 0; s < kVecs; ++s) {
+                            uint32_t before = at;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                before = __builtin_amdgcn_mbcnt_hi((uint32_t)(in[4 * s + e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in[4 * s + e], before));
+                                at += __popcll(in[4 * s + e]);
+                            }
+                            if (!(in[4 * s] | in[4 * s + 1] | in[4 * s + 2] | in[4 * s + 3])) continue;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (z[s][e] >= least) to[before++] = Entry{z[s][e], (uint32_t)(v0 + 256 * s + 4 * lane + e)};
+                        }
+                        break;
+                    }
+                    if (want == 0) {
+                        out.limit = __builtin_inff();
+                        break;
+                    }
+                }
+                first = false;
+                uint32_t c = 0;  // the smallest for which `want` lanes have key < (c + 1) << 16
 #pragma unroll
                 for (int b = 15; b >= 0; --b) {
                     const uint32_t c1 = c | (1u << b);
                     if (__popcll(__ballot(key < c1 << 16)) < want) c = c1;
                 }
-                const uint32_t end = c << 16 | 0xffffu;  // written down: what has an order up to `end`
-                uint32_t at = 0;
-#pragma unroll
-                for (int s = 0; s < 4; ++s)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) at += __popcll(__ballot(order_of(z[s][e]) <= end && z[s][e] > -__builtin_inff()));
-                if (at > kEntries) continue;
-                out.count = at;
-                at = 0;
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    uint64_t in[4];
-                    uint32_t before = at;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        in[e] = __ballot(order_of(z[s][e]) <= end && z[s][e] > -__builtin_inff());
-                        before += __builtin_amdgcn_mbcnt_hi((uint32_t)(in[e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in[e], 0));
-                        at += __popcll(in[e]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (in[e] >> lane & 1) to[before++] = Entry{z[s][e], (uint32_t)(v0 + 256 * s + 4 * lane + e)};
-                }
-                // the number whose order is `end`: what is left is below it
-                out.limit = end == ~0u ? -__builtin_inff() : __uint_as_float((end & 0x80000000u) ? end : end ^ 0x7fffffffu);
-                bool left = false;
-#pragma unroll
-                for (int s = 0; s < 4; ++s)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) left |= order_of(z[s][e]) > end && z[s][e] > -__builtin_inff();
-                if (!__any(left)) out.limit = -__builtin_inff();
-                break;
+                const uint32_t end = c << 16 | 0xffffu;  // the order of `least`
+                const float reached = __uint_as_float((end & 0x80000000u) ? end : end ^ 0x7fffffffu);
+                if (reached > least) least = out.limit = reached;  // (else fewer lanes than that have anything)
+                want >>= 1;
             }
-            if (want == 0) out.limit = __builtin_inff();
         }
     }
     if (lane == 0) p.pieces[piece] = out;
@@ -181,47 +224,40 @@ __global__ __launch_bounds__(64 * kWaves) void sample_pieces_kernel(const Sample
 
 // ---- the choice ---------------------------------------------------------------------------------------------------------------
 
+struct Member {
+    uint64_t code, weight;
+};
 struct Shared {
-    uint64_t sums[kThreads / 64];
-    uint64_t ranges[256];
-    uint64_t weight[kBins];
+    uint64_t weight[kBins];  // of the bins
     uint32_t count[kBins];
-    Entry list[kList];
-    Entry few[kFew];
-    float maxima[kThreads / 64];
+    Entry list[kList];       // the candidates, in the order of the vocabulary
+    uint64_t whole[kList];   // their weights
+    Member few[kFew];
+    uint64_t sums[2][kThreads / 64];
     uint64_t found, above;
+    uint32_t places[kPlaces + 1];  // where the candidates of each piece stand in the list
     uint32_t members;
     int at;
 };
 
-template <typename T, typename F> __device__ __forceinline__ T block_reduce(T x, T *lds, F op) {
-    x = wave_reduce(x, op);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
-    __syncthreads();
-    x = lds[0];
-    for (int w = 1; w < kThreads / 64; ++w) x = op(x, lds[w]);
-    return x;
-}
-// The sum over the threads before this one; *total: over all.
-template <typename T> __device__ __forceinline__ T block_scan(T x, T *lds, T *total) {
+// The sums over the threads before this one of two numbers at once, and over all.
+__device__ __forceinline__ void block_scan(uint64_t &x, uint64_t &y, uint64_t (&lds)[2][kThreads / 64], uint64_t *all_x, uint64_t *all_y) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    T upto = x;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const T other = (T)__shfl_up(upto, m);
-        upto += lane >= m ? other : (T)0;
+    const uint64_t upto_x = wave_scan(x, (uint64_t)0, AddOp()), upto_y = wave_scan(y, (uint64_t)0, AddOp());
+    __syncthreads();
+    if (lane == 63) {
+        lds[0][wave] = upto_x;
+        lds[1][wave] = upto_y;
     }
     __syncthreads();
-    if (lane == 63) lds[wave] = upto;
-    __syncthreads();
-    T before = 0, all = 0;
-    for (int w = 0; w < kThreads / 64; ++w) {
-        if (w < wave) before += lds[w];
-        all += lds[w];
-    }
-    *total = all;
-    return before + upto - x;
+    uint64_t tx = lds[0][lane & 15], ty = lds[1][lane & 15];  // 16 wavefronts: a row of lanes
+    tx = wave_scan(tx, (uint64_t)0, AddOp());
+    ty = wave_scan(ty, (uint64_t)0, AddOp());
+    *all_x = lane_value(tx, 15);
+    *all_y = lane_value(ty, 15);
+    const int w = __builtin_amdgcn_readfirstlane(wave);
+    x = upto_x - x + (w ? lane_value(tx, w ? w - 1 : 0) : 0);
+    y = upto_y - y + (w ? lane_value(ty, w ? w - 1 : 0) : 0);
 }
 
 struct Row {
@@ -246,48 +282,61 @@ struct Row {
         const int b = (int)(__float_as_uint(big - z) >> 17) - ((127 - 16) << 6);
         return b < 0 ? 0 : b >= kBins ? kBins - 1 : b;
     }
+    // f(logit, token, weight) of every candidate (of the row: of every token that is allowed), by this workgroup's threads.
     template <bool LIST, typename F> __device__ __forceinline__ void each(int n, F f) const {
         for (int i = threadIdx.x; i < n; i += kThreads) {
-            if constexpr (LIST) f(s.list[i].x, s.list[i].v);
-            else f(x[i], (uint32_t)i);
+            if constexpr (LIST) {
+                f(s.list[i].x, s.list[i].v, s.whole[i]);
+            } else {
+                const float z = x[i];
+                if (z > -__builtin_inff()) f(z, (uint32_t)i, whole(z));
+            }
         }
     }
     __device__ __forceinline__ void write(int token, double share) const {
         p.tokens[r] = token;
         if (p.logprobs) p.logprobs[r] = (float)log(share);
     }
-
-    // The smallest code for which the tokens up to it are `k` at least (k > 0) or weigh `need`, among those up to `last` of the n of the list
-    // (of the row); all ones if there is none. *weight: what they weigh (k > 0). Bins first, then ranks in one of them; where a bin has
-    // too many members (ties) digit by digit.
-    template <bool LIST> __device__ __forceinline__ uint64_t boundary(int n, uint64_t last, uint32_t k, uint64_t need, uint64_t *weight) const {
-        const int t = threadIdx.x;
-        __syncthreads();
-        for (int b = t; b < kBins; b += kThreads) {
+    __device__ __forceinline__ void clear_bins() const {
+        for (int b = threadIdx.x; b < kBins; b += kThreads) {
             s.weight[b] = 0;
             s.count[b] = 0;
         }
+    }
+    __device__ __forceinline__ void to_bin(float z, uint64_t w) const {
+        const int b = bin_of(z);
+        atomicAdd(&s.count[b], 1u);
+        if (w) atomicAdd(reinterpret_cast<unsigned long long *>(&s.weight[b]), (unsigned long long)w);
+    }
+
+    // What comes before each of a thread's two bins.
+    struct Prefix {
+        uint64_t count, weight;
+    };
+    __device__ __forceinline__ Prefix scan_bins(uint64_t *all) const {
+        const int t = threadIdx.x;
+        Prefix at = {(uint64_t)s.count[2 * t] + s.count[2 * t + 1], s.weight[2 * t] + s.weight[2 * t + 1]};
+        uint64_t unused;
+        block_scan(at.count, at.weight, s.sums, &unused, all);
+        return at;
+    }
+
+    // The smallest code for which the tokens up to it are `k` at least (k > 0) or weigh `need`, by the bins: the bin, then the ranks of its
+    // members; where it has too many (ties) digit by digit. All ones if there is none. *weight: what they weigh.
+    template <bool LIST> __device__ __forceinline__ uint64_t boundary(int n, const Prefix &at, uint32_t k, uint64_t need, uint64_t *weight) const {
+        const int t = threadIdx.x;
+        __syncthreads();
         if (t == 0) {
             s.members = 0;
             s.at = -1;
         }
         __syncthreads();
-        each<LIST>(n, [&](float z, uint32_t v) {
-            if (!(z > -__builtin_inff()) || code_of(z, v) > last) return;
-            const int b = bin_of(z);
-            const uint64_t w = whole(z);
-            atomicAdd(&s.count[b], 1u);
-            if (w) atomicAdd(reinterpret_cast<unsigned long long *>(&s.weight[b]), (unsigned long long)w);
-        });
-        __syncthreads();
-        uint64_t total;
-        const uint64_t c0 = s.count[2 * t], c1 = s.count[2 * t + 1], w0 = s.weight[2 * t], w1 = s.weight[2 * t + 1];
-        const uint64_t wb = block_scan(w0 + w1, s.sums, &total), cb = block_scan(c0 + c1, s.sums, &total);
-        const uint64_t goal = k ? k : need, b0 = k ? cb : wb, m0 = b0 + (k ? c0 : w0), e0 = m0 + (k ? c1 : w1);
+        const uint64_t goal = k ? k : need, c0 = s.count[2 * t], w0 = s.weight[2 * t];
+        const uint64_t b0 = k ? at.count : at.weight, m0 = b0 + (k ? c0 : w0), e0 = m0 + (k ? (uint64_t)s.count[2 * t + 1] : s.weight[2 * t + 1]);
         if (b0 < goal && e0 >= goal) {
             const bool second = m0 < goal;
             s.at = 2 * t + second;
-            s.found = wb + (second ? w0 : 0);
+            s.found = at.weight + (second ? w0 : 0);
             s.above = second ? m0 : b0;
         }
         __syncthreads();
@@ -296,91 +345,149 @@ struct Row {
         uint64_t weighs = s.found, had = s.above;
         const uint32_t members = s.count[bin];
         if (members <= kFew) {
-            each<LIST>(n, [&](float z, uint32_t v) {
-                if (z > -__builtin_inff() && code_of(z, v) <= last && bin_of(z) == bin) s.few[atomicAdd(&s.members, 1u)] = Entry{z, v};
+            each<LIST>(n, [&](float z, uint32_t v, uint64_t w) {
+                if (bin_of(z) == bin) s.few[atomicAdd(&s.members, 1u)] = Member{code_of(z, v), w};
             });
             __syncthreads();
             if (t < (int)members) {  // ranks: in whatever order the members stand
-                const uint64_t mine = code_of(s.few[t].x, s.few[t].v);
+                const Member mine = s.few[t];
                 uint64_t count = 0, sum = 0;
+#pragma unroll 4
                 for (uint32_t i = 0; i < members; ++i) {
-                    const bool before = code_of(s.few[i].x, s.few[i].v) < mine;
+                    const Member other = s.few[i];
+                    const bool before = other.code < mine.code;
                     count += before;
-                    if (before) sum += whole(s.few[i].x);
+                    sum += before ? other.weight : 0;
                 }
-                const uint64_t w = whole(s.few[t].x), upto = had + (k ? count : sum), here = k ? 1 : w;
+                const uint64_t upto = had + (k ? count : sum), here = k ? 1 : mine.weight;
                 if (upto < goal && upto + here >= goal) {
-                    s.found = mine;
-                    s.above = weighs + sum + w;
+                    s.found = mine.code;
+                    s.above = weighs + sum + mine.weight;
                 }
             }
             __syncthreads();
             *weight = s.above;
             return s.found;
         }
+        // (the bins of digits stand where the members would)
+        uint64_t *digit_weight = &s.few[0].code;
+        uint32_t *digit_count = reinterpret_cast<uint32_t *>(&s.few[kFew / 2]);
         uint64_t prefix = 0;
         for (int shift = 56; shift >= 0; shift -= 8) {
             __syncthreads();
             if (t < 256) {
-                s.weight[t] = 0;
-                s.count[t] = 0;
+                digit_weight[t] = 0;
+                digit_count[t] = 0;
             }
             __syncthreads();
-            each<LIST>(n, [&](float z, uint32_t v) {
+            each<LIST>(n, [&](float z, uint32_t v, uint64_t w) {
                 const uint64_t c = code_of(z, v);
-                if (!(z > -__builtin_inff()) || c > last || bin_of(z) != bin || (shift < 56 && c >> (shift + 8) != prefix)) return;
-                const int at = (int)(c >> shift) & 255;
-                atomicAdd(&s.count[at], 1u);
-                atomicAdd(reinterpret_cast<unsigned long long *>(&s.weight[at]), (unsigned long long)whole(z));
+                if (bin_of(z) != bin || (shift < 56 && c >> (shift + 8) != prefix)) return;
+                const int at_digit = (int)(c >> shift) & 255;
+                atomicAdd(&digit_count[at_digit], 1u);
+                atomicAdd(reinterpret_cast<unsigned long long *>(&digit_weight[at_digit]), (unsigned long long)w);
             });
             __syncthreads();
             if (t == 0) {
-                int at = 0;
-                for (;; ++at) {
-                    const uint64_t here = k ? s.count[at] : s.weight[at];
-                    if (had + here >= goal || at == 255) break;
+                int d = 0;
+                for (;; ++d) {
+                    const uint64_t here = k ? digit_count[d] : digit_weight[d];
+                    if (had + here >= goal || d == 255) break;
                     had += here;
-                    weighs += s.weight[at];
+                    weighs += digit_weight[d];
                 }
-                s.found = prefix << 8 | at;
+                s.found = prefix << 8 | d;
                 s.above = had;
-                s.sums[0] = weighs + s.weight[at];
-                s.sums[1] = weighs;
+                s.sums[0][0] = weighs + digit_weight[d];
+                s.sums[0][1] = weighs;
             }
             __syncthreads();
             prefix = s.found;
             had = s.above;
-            *weight = s.sums[0];
-            weighs = s.sums[1];
+            *weight = s.sums[0][0];
+            weighs = s.sums[0][1];
         }
         return prefix;
     }
 
-    // The token among those up to `last` and above min-p, from the n of the list (of the row), which stand in the order of the vocabulary: they
-    // are cut into 256 ranges; the sums of all give the range, the wavefront that has it the token.
-    template <bool LIST> __device__ __forceinline__ void draw(int n, uint64_t last) const {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, length = ((n + 255) / 256 + 63) & ~63;  // of a range
-        auto weigh = [&](int64_t i, uint32_t *v) {
-            if (i >= n) return (uint64_t)0;
-            const float z = LIST ? s.list[i].x : x[i];
-            *v = LIST ? s.list[i].v : (uint32_t)i;
-            if (!(z > -__builtin_inff()) || code_of(z, *v) > last) return (uint64_t)0;
+    // The last code that the filters keep; 0: the candidates do not say. `limit`: what is not among them is below it. `sum`: of all
+    // weights. The bins hold all candidates.
+    template <bool LIST> __device__ __forceinline__ uint64_t filter(int n, double sum, float limit) const {
+        const bool whole_row = !LIST || limit == -__builtin_inff();
+        // whether nothing that was left out could stand before a code
+        auto sure = [&](uint64_t code) { return whole_row || (code != ~0ull && (uint32_t)(code >> 32) <= order_of(limit)); };
+        // whether min-p leaves out what was left out, and so all that other filters are not sure of
+        const bool below = !whole_row && set.min_p > 0.f && fth::exp2_softmax(((double)limit - (double)big) * set.rate) < (double)set.min_p;
+        uint64_t last = ~0ull, weight = 0, all = 0;
+        if (set.top_k == 0 && !(set.top_p < 1.f)) return whole_row || below ? last : 0;
+        const Prefix at = scan_bins(&all);
+        if (set.top_k > 0) {
+            last = boundary<LIST>(n, at, (uint32_t)set.top_k, 0, &weight);
+            if (!sure(last) && (set.top_p < 1.f || !below)) return 0;
+            sum = (double)(last == ~0ull ? all : weight);  // (fewer tokens are allowed)
+        }
+        if (set.top_p < 1.f) {
+            const double need = __builtin_ceil(sum * (double)set.top_p);
+            const uint64_t code = boundary<LIST>(n, at, 0, need < 1.0 ? 1 : (uint64_t)need, &weight);
+            if (code < last) last = code;  // (none: rounded weights fall short of it, or the candidates do)
+            if (!sure(last) && (set.top_k > 0 || !below)) return 0;
+        }
+        return last;
+    }
+
+    // The token among the candidates up to `last` and above min-p.
+    __device__ __forceinline__ void draw_list(int n, uint64_t last) const {
+        const int t = threadIdx.x, each_has = (n + kThreads - 1) / kThreads, from = t * each_has, to = from + each_has < n ? from + each_has : n;
+        auto kept = [&](int i) -> uint64_t {
+            if (code_of(s.list[i].x, s.list[i].v) > last) return 0;
+            if (set.min_p > 0.f) {
+                double w;
+                whole(s.list[i].x, &w);
+                if (w < (double)set.min_p) return 0;
+            }
+            return s.whole[i];
+        };
+        uint64_t before = 0, unused = 0, total, none;
+        for (int i = from; i < to; ++i) before += kept(i);
+        const uint64_t mine = before;
+        block_scan(before, unused, s.sums, &total, &none);
+        uint64_t target = (uint64_t)((double)total * u);
+        target = target < total ? target : total - 1;
+        if (mine == 0 || before > target || before + mine <= target) return;
+        for (int i = from; i < to; ++i) {
+            const uint64_t w = kept(i);
+            if (before + w > target) {
+                write((int)s.list[i].v, (double)w / (double)total);
+                return;
+            }
+            before += w;
+        }
+    }
+
+    // The same from the whole row: cut into 256 ranges, whose sums give the range; a wavefront finds the token in it.
+    __device__ __forceinline__ void draw_row(int n, uint64_t last) const {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, length = ((n + 255) / 256 + 63) & ~63;
+        uint64_t *ranges = &s.few[0].code;
+        auto kept = [&](int64_t i) -> uint64_t {
+            if (i >= n) return 0;
+            const float z = x[i];
+            if (!(z > -__builtin_inff()) || code_of(z, (uint32_t)i) > last) return 0;
             double w;
             const uint64_t all = whole(z, &w);
-            return w >= (double)set.min_p ? all : (uint64_t)0;
+            return w >= (double)set.min_p ? all : 0;
         };
-        uint32_t v;
         __syncthreads();
         for (int g = wave; g < 256; g += kThreads / 64) {
             uint64_t sum = 0;
             if (g * (int64_t)length < n)
-                for (int i = lane; i < length; i += 64) sum += weigh((int64_t)g * length + i, &v);
-            sum = wave_reduce(sum, AddOp());
-            if (lane == 0) s.ranges[g] = sum;
+                for (int i = lane; i < length; i += 64) sum += kept((int64_t)g * length + i);
+            sum = wave_sum(sum);
+            if (lane == 0) ranges[g] = sum;
         }
         __syncthreads();
-        uint64_t total;
-        const uint64_t mine = threadIdx.x < 256 ? s.ranges[threadIdx.x] : 0, before = block_scan(mine, s.sums, &total);
+        const uint64_t mine = threadIdx.x < 256 ? ranges[threadIdx.x] : 0;
+        uint64_t before = mine, unused = 0, total, none;
+        block_scan(before, unused, s.sums, &total, &none);
         uint64_t target = (uint64_t)((double)total * u);
         target = target < total ? target : total - 1;
         if (mine > 0 && before <= target && before + mine > target) {
@@ -392,70 +499,72 @@ struct Row {
         uint64_t left = s.found;
         const int g = s.at;
         for (int i0 = 0; i0 < length; i0 += 64) {
-            const uint64_t here = i0 + lane < length ? weigh((int64_t)g * length + i0 + lane, &v) : 0;
-            uint64_t upto = here;
-#pragma unroll
-            for (int m = 1; m < 64; m <<= 1) {
-                const uint64_t other = __shfl_up(upto, m);
-                upto += lane >= m ? other : 0;
-            }
-            if (here > 0 && upto > left && upto - here <= left) write((int)v, (double)here / (double)total);
-            const uint64_t all = __shfl(upto, 63);
+            const uint64_t here = i0 + lane < length ? kept((int64_t)g * length + i0 + lane) : 0, upto = wave_scan(here, (uint64_t)0, AddOp());
+            if (here > 0 && upto > left && upto - here <= left) write(g * length + i0 + lane, (double)here / (double)total);
+            const uint64_t all = lane_value(upto, 63);
             if (all > left) return;
             left -= all;
         }
     }
 
-    // The last code that the filters keep; 0: the candidates do not say. `limit`: what is not among them is below it. `sum`: of all weights.
-    template <bool LIST> __device__ __forceinline__ uint64_t filter(int n, double sum, float limit) const {
-        const bool whole_row = !LIST || limit == -__builtin_inff();
-        // whether nothing that was left out could stand before a code
-        auto sure = [&](uint64_t code) { return whole_row || (code != ~0ull && (uint32_t)(code >> 32) <= order_of(limit)); };
-        // whether min-p leaves out what was left out, and so all that other filters are not sure of
-        const bool below = !whole_row && set.min_p > 0.f && fth::exp2_softmax(((double)limit - (double)big) * set.rate) < (double)set.min_p;
-        uint64_t last = ~0ull, weight = 0;
-        if (set.top_k > 0) {
-            last = boundary<LIST>(n, last, (uint32_t)set.top_k, 0, &weight);
-            if (!sure(last) && (set.top_p < 1.f || !below)) return 0;
-            if (last == ~0ull) {  // fewer tokens are allowed
-                uint64_t all = 0;
-                each<LIST>(n, [&](float z, uint32_t) { all += whole(z); });
-                weight = block_reduce(all, s.sums, AddOp());
+    // Without a filter: the token that `left` of the weight before it leads to, in piece `at`; one wavefront. Where rounding leads past the
+    // piece's end, its last.
+    __device__ __forceinline__ void draw_piece(int at, double left, double total) const {
+        const int lane = threadIdx.x & 63;
+        const int64_t v0 = (int64_t)at * kPiece;
+        float z[kPiece / 64];
+#pragma unroll
+        for (int i = 0; i < kPiece / 64; ++i) z[i] = v0 + 64 * i + lane < p.d.vocab ? x[v0 + 64 * i + lane] : -__builtin_inff();
+        int token = -1;
+        double share = 0.0;
+        bool found = false;
+#pragma unroll
+        for (int i = 0; i < kPiece / 64; ++i) {
+            if (found) continue;
+            const double w = z[i] > -__builtin_inff() ? fth::exp2_softmax(((double)z[i] - (double)big) * set.rate) : 0.0;
+            const double upto = wave_scan(w, 0.0, AddOp());
+            const uint64_t over = __ballot(w > 0.0 && upto > left), some = __ballot(w > 0.0);
+            if (some) {
+                const int which = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
+                token = (int)v0 + 64 * i + which;
+                share = lane_value(w, which);
             }
-            sum = (double)weight;
+            found = over != 0;
+            left -= lane_value(upto, 63);
         }
-        if (set.top_p < 1.f) {
-            const double need = __builtin_ceil(sum * (double)set.top_p);
-            const uint64_t code = boundary<LIST>(n, last, 0, need < 1.0 ? 1 : (uint64_t)need, &weight);
-            if (code != ~0ull) last = code;  // (else rounded weights fall short of it, or the candidates do)
-            if (!sure(last) && (set.top_k > 0 || !below)) return 0;
-        } else if (set.top_k == 0 && !whole_row && !below) {
-            return 0;
-        }
-        return last;
+        if (lane == 0) write(token, share / total);
     }
 };
 
 __global__ __launch_bounds__(kThreads) void sample_choice_kernel(const SampleArgs p) {
     __shared__ Shared s;
     const int64_t r = blockIdx.x;
-    const int t = threadIdx.x;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const Piece *pieces = p.pieces + r * p.per_row;
+    // The candidates of the first pieces, before it is known how many there are.
+    Entry ahead[kAhead][kEntries / 64];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+        const int i = wave + j * (kThreads / 64);
+#pragma unroll
+        for (int h = 0; h < kEntries / 64; ++h) ahead[j][h] = p.entries[(r * p.per_row + (i < p.per_row ? i : 0)) * kEntries + 64 * h + lane];
+    }
     const Settings set(p, r);
     const double u = p.uniform[r];
-    const Piece *pieces = p.pieces + r * p.per_row;
+    // Every wavefront looks at all pieces, a lane at neighbouring ones, so that nothing has to be handed round.
+    const int each = (p.per_row + 63) / 64, from = lane * each, to = from + each < p.per_row ? from + each : p.per_row;
     bool bad = set.bad || !(u >= 0.0 && u < 1.0);
     float big = -__builtin_inff(), limit = -__builtin_inff();
     uint32_t count = 0;
-    for (int i = t; i < p.per_row; i += kThreads) {
+    for (int i = from; i < to; ++i) {
         const Piece one = pieces[i];
         bad |= one.bad != 0;
         big = fmaxf(big, one.max);
         limit = fmaxf(limit, one.limit);
         count += one.count;
     }
-    bad = __syncthreads_or(bad);
-    big = block_reduce(big, s.maxima, MaxOp());
-    if (bad || big == -__builtin_inff()) {
+    big = wave_max(big) + 0.f;  // (0 - -0 is 0, -0 - 0 would be -0)
+    if (__any(bad) || big == -__builtin_inff()) {
         if (t == 0) {
             p.tokens[r] = -1;
             if (p.logprobs) p.logprobs[r] = __builtin_nanf("");
@@ -464,106 +573,84 @@ __global__ __launch_bounds__(kThreads) void sample_choice_kernel(const SampleArg
         return;
     }
     const Row row = {p, set, s, p.logits + r * p.d.logits_stride, big, u, r};
-    // the sums of the pieces, in their order: a thread has neighbouring ones
-    const int each = (p.per_row + kThreads - 1) / kThreads, from = t * each, to = from + each < p.per_row ? from + each : p.per_row;
     auto sum_of = [&](int i) {  // (0 where the weights of its tokens could be)
-        const double t = ((double)pieces[i].max - (double)big) * set.rate;
-        return t > -1000.0 ? pieces[i].sum * fth::exp2_softmax(t) : 0.0;
+        const double far = ((double)pieces[i].max - (double)big) * set.rate;
+        return far > -1000.0 ? pieces[i].sum * fth::exp2_softmax(far) : 0.0;
     };
-    double mine = 0.0, total = 0.0, before = 0.0;
+    double mine = 0.0, upto = 0.0, total = 0.0;
     if (set.top_k == 0) {
         for (int i = from; i < to; ++i) mine += sum_of(i);
-        before = block_scan(mine, reinterpret_cast<double *>(s.sums), &total);
+        upto = wave_scan(mine, 0.0, AddOp());
+        total = lane_value(upto, 63);
     }
     if (!set.filters()) {
+        if (wave != 0) return;
+        // the first lane over the number (none, by rounding at the very end: the last that has something)
         const double target = total * u;
-        if (t == 0) s.at = -1;
-        __syncthreads();
-        // (several threads, where rounding lets their stretches overlap: the first; none at the very end: the last that has something)
-        if (mine > 0.0 && before + mine > target) atomicMin(reinterpret_cast<unsigned *>(&s.at), (unsigned)t);
-        __syncthreads();
-        int who = s.at;
-        if (who < 0) {
-            __syncthreads();
-            if (mine > 0.0) atomicMax(&s.at, t);
-            __syncthreads();
-            who = s.at;
+        const uint64_t over = __ballot(mine > 0.0 && upto > target), some = __ballot(mine > 0.0);
+        const int who = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
+        int at = from, last = from;
+        double left = target - (upto - mine);
+        for (; at < to; ++at) {
+            const double here = sum_of(at);
+            if (here > left) break;
+            if (here > 0.0) last = at;
+            left -= here;
         }
-        if (t != who && (t >> 6) != (who >> 6)) return;
-        // the wavefront of that thread: its piece, and the token in it
-        int at = 0;
-        double left = 0.0;
-        if (t == who) {
-            left = target - before;
-            int last = from;
-            for (at = from; at < to; ++at) {
-                const double here = sum_of(at);
-                if (here > left) break;
-                if (here > 0.0) last = at;
-                left -= here;
-            }
-            if (at == to) {
-                at = last;
-                left = 1e300;
-            }
+        if (at == to) {
+            at = last;
+            left = 1e300;
         }
-        at = __shfl(at, who & 63);
-        left = __shfl(left, who & 63);
-        const int lane = t & 63, n = (int)(p.d.vocab - (int64_t)at * kPiece < kPiece ? p.d.vocab - (int64_t)at * kPiece : kPiece);
-        int token = -1;
-        double share = 0.0;
-        for (int i0 = 0; i0 < n; i0 += 64) {
-            const float z = i0 + lane < n ? row.x[(int64_t)at * kPiece + i0 + lane] : -__builtin_inff();
-            const double w = z > -__builtin_inff() ? fth::exp2_softmax(((double)z - (double)big) * set.rate) : 0.0;
-            double upto = w;
-#pragma unroll
-            for (int m = 1; m < 64; m <<= 1) {
-                const double other = __shfl_up(upto, m);
-                upto += lane >= m ? other : 0.0;
-            }
-            const uint64_t over = __ballot(w > 0.0 && upto > left), some = __ballot(w > 0.0);
-            if (some) {  // the first that is over, else the last so far
-                const int lane_of = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
-                token = at * kPiece + i0 + lane_of;
-                share = __shfl(w, lane_of);
-            }
-            if (over) break;
-            left -= __shfl(upto, 63);
-        }
-        if (lane == 0) row.write(token, share / total);
+        row.draw_piece(lane_value(at, who), lane_value(left, who), total);
         return;
     }
 
-    limit = block_reduce(limit, s.maxima, MaxOp());
-    count = 0;
-    for (int i = from; i < to; ++i) count += pieces[i].count;
-    uint32_t listed;
-    uint32_t place = block_scan(count, reinterpret_cast<uint32_t *>(s.sums), &listed);
+    limit = wave_max(limit);
+    const uint32_t upto_count = wave_scan(count, 0u, AddOp()), listed = lane_value(upto_count, 63);
     uint64_t last = 0;
-    if (listed <= kList) {
-        __syncthreads();
-        if (p.per_row <= kThreads) {  // a wavefront for a piece
-            s.count[t] = count;
-            s.members = 0;
-            reinterpret_cast<uint32_t *>(s.weight)[t] = place;
-            __syncthreads();
-#pragma unroll 4
-            for (int i = t >> 6; i < p.per_row; i += kThreads / 64)
-                if ((uint32_t)(t & 63) < s.count[i]) s.list[reinterpret_cast<uint32_t *>(s.weight)[i] + (t & 63)] = p.entries[(r * p.per_row + i) * kEntries + (t & 63)];
-        } else {
-            for (int i = from; i < to; ++i)
-                for (uint32_t e = 0; e < pieces[i].count; ++e) s.list[place++] = p.entries[(r * p.per_row + i) * kEntries + e];
+    row.clear_bins();
+    if (listed <= kList && p.per_row <= kPlaces) {
+        if (wave == 0) {
+            uint32_t place = upto_count - count;
+            for (int i = from; i < to; ++i) {
+                s.places[i] = place;
+                place += pieces[i].count;
+            }
+            if (lane == 0) s.places[p.per_row] = listed;
         }
         __syncthreads();
+        auto put = [&](int i, int h, Entry one) {
+            const uint32_t place = s.places[i] + 64 * h;
+            if (place + lane >= s.places[i + 1]) return;
+            const uint64_t w = row.whole(one.x);
+            s.list[place + lane] = one;
+            s.whole[place + lane] = w;
+            row.to_bin(one.x, w);
+        };
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (wave + j * (kThreads / 64) < p.per_row)
+#pragma unroll
+                for (int h = 0; h < kEntries / 64; ++h) put(wave + j * (kThreads / 64), h, ahead[j][h]);
+        for (int i = wave + kAhead * (kThreads / 64); i < p.per_row; i += kThreads / 64)
+            for (int h = 0; h < kEntries / 64; ++h) put(i, h, p.entries[(r * p.per_row + i) * kEntries + 64 * h + lane]);
+        __syncthreads();
         last = row.filter<true>((int)listed, total * p.unit, limit);
+        if (last) {
+            row.draw_list((int)listed, last);
+            return;
+        }
+        __syncthreads();
+        row.clear_bins();
     }
-    if (last) {
-        row.draw<true>((int)listed, last);
-    } else {
-        last = row.filter<false>((int)p.d.vocab, total * p.unit, limit);
-        row.draw<false>((int)p.d.vocab, last);
-    }
+    __syncthreads();
+    row.each<false>((int)p.d.vocab, [&](float z, uint32_t, uint64_t w) { row.to_bin(z, w); });
+    __syncthreads();
+    last = row.filter<false>((int)p.d.vocab, total * p.unit, limit);
+    row.draw_row((int)p.d.vocab, last);
 }
+
+int64_t pieces_of(const fth_sample_desc &d) { return d.rows * fth::ceil_div(d.vocab, kPiece); }
 
 int32_t check(const fth_sample_desc *d) {
     FTH_ARG(d, "sample: NULL descriptor");
@@ -571,10 +658,9 @@ int32_t check(const fth_sample_desc *d) {
     FTH_ARG(d->logits_stride >= d->vocab, "sample: the row stride is below the vocabulary");
     if (d->logits_stride > ((int64_t)1 << 40) || d->vocab > 2147483647LL || d->rows > ((int64_t)1 << 20)) return fth::set_error(FTH_ERR_SIZE_OVERFLOW, "sample: extents overflow");
     FTH_ARG(d->rows == 0 || d->vocab > 0, "sample: no token to choose from");
+    if (pieces_of(*d) > 2147483640LL) return fth::set_error(FTH_ERR_SIZE_OVERFLOW, "sample: more than 2^42 logits");
     return FTH_OK;
 }
-
-int64_t pieces_of(const fth_sample_desc &d) { return d.rows * fth::ceil_div(d.vocab, kPiece); }
 
 }  // namespace
 
@@ -603,14 +689,14 @@ int32_t fth_dev_sample_f32(const fth_sample_desc *d, const float *logits, const 
     a.pieces = static_cast<Piece *>(workspace);
     a.entries = reinterpret_cast<Entry *>(a.pieces + pieces);
     a.per_row = (int)fth::ceil_div(d->vocab, kPiece);
-    a.want_p = 32;
+    a.by_pieces = fth::Divisor((uint32_t)a.per_row);
+    a.want_p = 48;
     int bits = 0;
     while (((int64_t)1 << bits) < d->vocab) ++bits;
     const int s_bits = 62 - bits < 45 ? 62 - bits : 45;
     a.magic = __builtin_ldexp(1.5, 52 - s_bits);
     a.unit = __builtin_ldexp(1.0, s_bits);
     const int64_t blocks = fth::ceil_div(pieces, kWaves);
-    FTH_ARG(blocks <= 2147483647LL, "sample: too many rows for one launch");
     sample_pieces_kernel<<<dim3((unsigned)blocks), dim3(64 * kWaves), 0, st>>>(a);
     FTH_CHECK_LAUNCH("sample_pieces");
     sample_choice_kernel<<<dim3((unsigned)d->rows), dim3(kThreads), 0, st>>>(a);
