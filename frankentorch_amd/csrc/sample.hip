@@ -17,7 +17,7 @@ namespace {
 
 constexpr int kPiece = 2048, kEntries = 128, kWaves = 4;         // logits of a piece, candidates that it may write down, pieces of a workgroup
 constexpr int kThreads = 1024, kBins = 2048, kList = 7168, kFew = 1024;   // the choice: bins, candidates in LDS, members of a bin that are ranked
-constexpr int kPlaces = 512, kAhead = 4;                            // pieces of a row whose candidates are listed; of a wavefront, fetched at once
+constexpr int kPlaces = 512, kAhead = 4, kGroups = kPiece / kThreads;                            // pieces of a row whose candidates are listed; of a wavefront, fetched at once
 
 struct Piece {
     float max, limit;  // of what is not written down, every logit is below `limit` (-inf: all is written down)
@@ -150,7 +150,10 @@ __global__ __launch_bounds__(64 * kWaves) void sample_pieces_kernel(const Sample
 #pragma unroll
             for (int s = 0; s < kVecs; ++s)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum += fth::exp2_softmax(((double)z[s][e] - (double)out.max) * set.rate);
+                for (int e = 0; e < 4; ++e) {
+                    sum += fth::exp2_softmax(((double)z[s][e] - (double)out.max) * set.rate);
+                    if (e & 1) __builtin_amdgcn_sched_barrier(0);  // two at a time, for the registers' sake
+                }
             out.sum = wave_sum(sum);
         }
         if (set.filters()) {
@@ -175,29 +178,25 @@ __global__ __launch_bounds__(64 * kWaves) void sample_pieces_kernel(const Sample
             bool first = __popcll(__ballot(mine >= least)) > want;
             for (;;) {
                 if (!first) {
-                    uint64_t in[4 * kVecs];
-                    uint32_t n_in = 0;
+                    uint32_t at = 0;
 #pragma unroll
-                    for (int i = 0; i < 4 * kVecs; ++i) {
-                        in[i] = __ballot(z[i >> 2][i & 3] >= least);
-                        n_in += __popcll(in[i]);
-                    }
-                    if (n_in <= kEntries) {
-                        out.count = n_in;
-                        uint32_t at = 0;
+                    for (int s = 0; s < kVecs; ++s) {
+                        uint32_t before = at;
+                        uint64_t in[4];
 #pragma unroll
-                        for (int s = 0; s < kVecs; ++s) {
-                            uint32_t before = at;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                before = __builtin_amdgcn_mbcnt_hi((uint32_t)(in[4 * s + e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in[4 * s + e], before));
-                                at += __popcll(in[4 * s + e]);
-                            }
-                            if (!(in[4 * s] | in[4 * s + 1] | in[4 * s + 2] | in[4 * s + 3])) continue;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (z[s][e] >= least) to[before++] = Entry{z[s][e], (uint32_t)(v0 + 256 * s + 4 * lane + e)};
+                        for (int e = 0; e < 4; ++e) {
+                            in[e] = __ballot(z[s][e] >= least);
+                            before = __builtin_amdgcn_mbcnt_hi((uint32_t)(in[e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in[e], before));
+                            at += __popcll(in[e]);
                         }
+                        if (at > kEntries) continue;  // too many: once more with fewer
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (z[s][e] >= least) to[before++] = Entry{z[s][e], (uint32_t)(v0 + 256 * s + 4 * lane + e)};
+                        __builtin_amdgcn_sched_barrier(0);  // for the registers' sake
+                    }
+                    if (at <= kEntries) {
+                        out.count = at;
                         break;
                     }
                     if (want == 0) {
@@ -507,32 +506,35 @@ struct Row {
         }
     }
 
-    // Without a filter: the token that `left` of the weight before it leads to, in piece `at`; one wavefront. Where rounding leads past the
-    // piece's end, its last.
+    // Without a filter: the token that `left` of the weight before it leads to, in piece `at`. Where rounding leads past the piece's end, its
+    // last. Each wavefront has two groups of 64 neighbouring tokens.
     __device__ __forceinline__ void draw_piece(int at, double left, double total) const {
-        const int lane = threadIdx.x & 63;
-        const int64_t v0 = (int64_t)at * kPiece;
-        float z[kPiece / 64];
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int64_t v0 = (int64_t)at * kPiece + kGroups * 64 * wave;
+        double *sums = reinterpret_cast<double *>(s.sums);
+        double w[kGroups], upto[kGroups];
 #pragma unroll
-        for (int i = 0; i < kPiece / 64; ++i) z[i] = v0 + 64 * i + lane < p.d.vocab ? x[v0 + 64 * i + lane] : -__builtin_inff();
-        int token = -1;
-        double share = 0.0;
-        bool found = false;
-#pragma unroll
-        for (int i = 0; i < kPiece / 64; ++i) {
-            if (found) continue;
-            const double w = z[i] > -__builtin_inff() ? fth::exp2_softmax(((double)z[i] - (double)big) * set.rate) : 0.0;
-            const double upto = wave_scan(w, 0.0, AddOp());
-            const uint64_t over = __ballot(w > 0.0 && upto > left), some = __ballot(w > 0.0);
-            if (some) {
-                const int which = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
-                token = (int)v0 + 64 * i + which;
-                share = lane_value(w, which);
-            }
-            found = over != 0;
-            left -= lane_value(upto, 63);
+        for (int g = 0; g < kGroups; ++g) {
+            const float z = v0 + 64 * g + lane < p.d.vocab ? x[v0 + 64 * g + lane] : -__builtin_inff();
+            w[g] = z > -__builtin_inff() ? fth::exp2_softmax(((double)z - (double)big) * set.rate) : 0.0;
+            upto[g] = wave_scan(w[g], 0.0, AddOp());
+            if (lane == 63) sums[kGroups * wave + g] = upto[g];
         }
-        if (lane == 0) write(token, share / total);
+        __syncthreads();
+        static_assert(kPiece == 64 * kGroups * (kThreads / 64) && kPiece / 64 <= 64, "a lane for each group");
+        const double here = lane < kPiece / 64 ? sums[lane] : 0.0, through = wave_scan(here, 0.0, AddOp());
+        const uint64_t over = __ballot(here > 0.0 && through > left), some = __ballot(here > 0.0);
+        if (!some) return;
+        const int group = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
+        if (group / kGroups != wave) return;
+        left -= lane_value(through - here, group);
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            if (g != group % kGroups) continue;
+            const uint64_t past = __ballot(w[g] > 0.0 && upto[g] > left), any = __ballot(w[g] > 0.0);
+            const int which = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(any);
+            if (lane == which) write((int)v0 + 64 * g + lane, w[g] / total);
+        }
     }
 };
 
@@ -584,7 +586,6 @@ __global__ __launch_bounds__(kThreads) void sample_choice_kernel(const SampleArg
         total = lane_value(upto, 63);
     }
     if (!set.filters()) {
-        if (wave != 0) return;
         // the first lane over the number (none, by rounding at the very end: the last that has something)
         const double target = total * u;
         const uint64_t over = __ballot(mine > 0.0 && upto > target), some = __ballot(mine > 0.0);
