@@ -274,49 +274,77 @@ __device__ __forceinline__ uint32_t largest_of(F4 x, F4 y, uint32_t so_far) {
     return so_far;
 }
 
-constexpr int kWaves = 4, kHeld = 4;
+constexpr int kWaves = 4;
 
-// One wavefront a run and head: 64 / (head_dim / 8) rows side by side, kHeld times of them in registers; longer runs are read twice.
-template <typename T, bool INTER, bool NT> __device__ __forceinline__ void store_run(const Args &p, const Run &run, int64_t t, int item) {
+// `tokens` tokens from t on, all of one block from position `pos` of sequence `seq` on: one wavefront (TEAM: the workgroup) for their rows of one head, 64 /
+// (head_dim / 8) of them side by side, kHeld times as many in registers; longer runs are read twice. The rows are asked for before it is
+// known where they go.
+constexpr int kHeld = 4;
+struct Team {
+    uint32_t largest[kWaves];
+    float had;
+};
+template <typename T, bool INTER, bool NT, bool TEAM> __device__ __forceinline__ void store_run(const Args &p, int64_t t, int tokens, int pos, int seq, int item, Team &team) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, hd = (int)p.c.head_dim, hkv = (int)p.c.kv_heads, per_row = hd / 8, abreast = 64 / per_row;
-    const int slot = lane / per_row, i = lane % per_row;
+    const int slot = lane / per_row, i = lane % per_row, held = kHeld * abreast;
+    const int from = TEAM ? wave * held : 0, step = TEAM ? kWaves * held : held;  // this wavefront's rows
     const bool keys = item < hkv, there = slot < abreast;
     const int64_t h = keys ? item : item - hkv, pitch = keys ? p.d.k_row_stride : p.d.v_row_stride;
     const float *src = keys ? p.k + t * pitch + h * p.d.k_head_stride : p.v + t * pitch + h * p.d.v_head_stride;
-    uint8_t *dst = static_cast<uint8_t *>(keys ? p.k_cache : p.v_cache) + run.page * p.c.page_stride + h * p.c.head_stride;
-    float *scale = (keys ? p.k_scales : p.v_scales) + run.page * p.sc.page_stride + h * p.sc.head_stride + (int)p.by_block((uint32_t)run.first);
     const bool turns = keys && p.d.rotary_dim > 0;
     const Chunks at = chunks_of<INTER>(i, hd, (int)p.d.rotary_dim, turns);
-    const float had = run.row > run.first ? *scale : 0.f;
     F4 x[kHeld], y[kHeld];
     auto fetch = [&](int row0) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < kHeld; ++j) {
             const int row = row0 + j * abreast + slot;
             x[j] = y[j] = F4{0.f, 0.f, 0.f, 0.f};
-            if (there && row < run.tokens) {
+            if (there && row < tokens) {
                 x[j] = load4<NT>(src + row * pitch + at.a);
                 y[j] = load4<NT>(src + row * pitch + at.b);
             }
         }
-        if (turns) {
-            Angles g[kHeld];
-#pragma unroll
-            for (int j = 0; j < kHeld; ++j) {
-                const int row = row0 + j * abreast + slot;
-                if (there && row < run.tokens) g[j] = angles_at<INTER>(p, run.pos + row, i, at);
-            }
-#pragma unroll
-            for (int j = 0; j < kHeld; ++j) {
-                const int row = row0 + j * abreast + slot;
-                if (there && row < run.tokens) turn<INTER>(x[j], y[j], g[j], at);
-            }
-        }
     };
+    auto turn_all = [&](int row0) __attribute__((always_inline)) {
+        if (!turns) return;
+        Angles g[kHeld];
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            const int row = row0 + j * abreast + slot;
+            if (there && row < tokens) g[j] = angles_at<INTER>(p, pos + row, i, at);
+        }
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j)
+            if (there && row0 + j * abreast + slot < tokens) turn<INTER>(x[j], y[j], g[j], at);
+    };
+    // (a position without an angle has no place either; and then nothing is stored)
+    const bool angles = !turns || (pos >= 0 && pos < p.d.max_pos);
+    fetch(from);
+    int page = 0, row = 0;
+    const bool placed = find_row(p, seq, pos, &page, &row);
+    const int first = placed ? (int)p.by_block((uint32_t)row) * (int)p.sc.block : 0;
+    float *scale = (keys ? p.k_scales : p.v_scales) + (placed ? page : 0) * p.sc.page_stride + h * p.sc.head_stride + (int)p.by_block((uint32_t)first);
+    float had = placed && row > first && (!TEAM || wave == 0) ? *scale : 0.f;
+    if (angles) turn_all(from);
+    if (!placed) {
+        if (item == 0 && threadIdx.x % (TEAM ? 64 * kWaves : 64) == 0) fth::report_bad_entry(p.bad, t);
+        return;
+    }
+    if (p.d.rotary_dim > 0 && pos + (int64_t)tokens > p.d.max_pos) {  // its last tokens have no place
+        const int rest = (int)(p.d.max_pos - pos);
+        if (item == 0 && threadIdx.x % (TEAM ? 64 * kWaves : 64) == 0) fth::report_bad_entry(p.bad, t + rest);
+        tokens = rest;
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j)
+            if (from + j * abreast + slot >= tokens) x[j] = y[j] = F4{0.f, 0.f, 0.f, 0.f};
+    }
     uint32_t largest = 0;
-    const int held = kHeld * abreast;
-    for (int row0 = 0; row0 < run.tokens; row0 += held) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) largest = largest_of(x[j], y[j], largest);
+    for (int row0 = from + step; row0 < tokens; row0 += step) {
         fetch(row0);
+        turn_all(row0);
 #pragma unroll
         for (int j = 0; j < kHeld; ++j) largest = largest_of(x[j], y[j], largest);
     }
@@ -325,83 +353,170 @@ template <typename T, bool INTER, bool NT> __device__ __forceinline__ void store
         const uint32_t other = __shfl_xor(largest, m);
         largest = other > largest ? other : largest;
     }
+    if constexpr (TEAM) {
+        __syncthreads();  // what an earlier run left has been read
+        if (lane == 0) {
+            team.largest[wave] = largest;
+            if (wave == 0) team.had = had;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) largest = team.largest[w] > largest ? team.largest[w] : largest;
+        had = team.had;
+    }
     const float now = larger_scale(had, scale_for<T>(__uint_as_float(largest))), per = per_scale(now);
-    if (run.row == run.first || now != had) {
+    uint8_t *dst = static_cast<uint8_t *>(keys ? p.k_cache : p.v_cache) + page * p.c.page_stride + h * p.c.head_stride;
+    if (row == first || now != had) {
         const float shrink = had * per;
-        for (int row = run.first + slot; there && row < run.row; row += abreast) {
-            uint32_t *w = reinterpret_cast<uint32_t *>(dst + row * p.c.row_stride + 8 * i);
+        for (int old = first + slot + (TEAM ? wave * abreast : 0); there && old < row; old += abreast * (TEAM ? kWaves : 1)) {
+            uint32_t *w = reinterpret_cast<uint32_t *>(dst + old * p.c.row_stride + 8 * i);
             const uint32_t u = w[0], v = w[1];
             w[0] = now == now ? codes4<T>(values4<T>(u) * shrink) : 0u;
             w[1] = now == now ? codes4<T>(values4<T>(v) * shrink) : 0u;
         }
-        if (lane == 0) *scale = now;
+        if (lane == 0 && (!TEAM || wave == 0)) *scale = now;
     }
-    for (int row0 = 0; row0 < run.tokens; row0 += held) {
-        if (run.tokens > held) fetch(row0);
+    for (int row0 = from; row0 < tokens; row0 += step) {
+        if (tokens > step) {
+            fetch(row0);
+            turn_all(row0);
+        }
 #pragma unroll
         for (int j = 0; j < kHeld; ++j) {
-            const int row = row0 + j * abreast + slot;
-            if (!there || row >= run.tokens) continue;
-            uint8_t *to = dst + (run.row + row) * p.c.row_stride;
+            const int in_run = row0 + j * abreast + slot;
+            if (!there || in_run >= tokens) continue;
+            uint8_t *to = dst + (row + in_run) * p.c.row_stride;
             *reinterpret_cast<uint32_t *>(to + at.a) = now == now ? codes4<T>(x[j] * per) : 0u;
             *reinterpret_cast<uint32_t *>(to + at.b) = now == now ? codes4<T>(y[j] * per) : 0u;
         }
     }
 }
 
-// `chunk` tokens for a wavefront, of which it does the runs that begin there; behind those the queries, 4 kHeld rows of a token for a wavefront.
-template <typename T, bool INTER, bool NT> __global__ __launch_bounds__(64 * kWaves) void append_scaled_vec_kernel(const Args p, int chunk, int64_t kv_items, int q_parts) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hkv = (int)p.c.kv_heads;
-    const int64_t work = (int64_t)blockIdx.x * kWaves + wave;
-    if (work < kv_items) {
-        const int item = (int)(work % (2 * hkv));
-        const int64_t t0 = work / (2 * hkv) * chunk, end = t0 + chunk < p.d.tokens ? t0 + chunk : p.d.tokens;
-        uint64_t begins = 1;
-        if (chunk > 1) {  // not those that go on from the token before them
-            const int64_t t = t0 + lane;
-            bool first = t < end && p.positions[t] != -1;
-            if (first && t > 0 && p.seq_ids[t] == p.seq_ids[t - 1] && p.positions[t] == p.positions[t - 1] + 1)
-                first = (uint32_t)p.positions[t] == p.by_block((uint32_t)p.positions[t]) * (uint32_t)p.sc.block;  // (pages are whole blocks)
-            begins = __ballot(first);
-        }
-        for (; begins; begins &= begins - 1) {
-            const int64_t t = t0 + __builtin_ctzll(begins);
-            const Run run = run_at(p, t, item == 0);
-            if (run.tokens) store_run<T, INTER, NT>(p, run, t, item);
-        }
-        return;
-    }
-    const int64_t rest = work - kv_items, t = rest / q_parts;
-    if (t >= p.d.tokens) return;
-    const int pos = p.positions[t];
-    int page, row;
-    if (pos == -1 || !find_row(p, p.seq_ids[t], pos, &page, &row)) return;
-    const int hd = (int)p.c.head_dim, per_row = hd / 8, abreast = 64 / per_row, slot = lane / per_row, i = lane % per_row;
-    if (slot >= abreast) return;
-    const Chunks at = chunks_of<INTER>(i, hd, (int)p.d.rotary_dim, p.d.rotary_dim > 0);
-    const int h0 = (int)(rest % q_parts) * kHeld * abreast + slot, hq = (int)p.d.q_heads;
-    F4 x[kHeld], y[kHeld];
+// The rows of one token: its queries, and with blocks of one position (ONE) its keys and values, each row with a scale of its own.
+template <typename T, bool INTER, bool NT, bool ONE> __device__ __forceinline__ void store_token(const Args &p, int64_t t, int part) {
+    constexpr int HELD = 4;
+    const int lane = threadIdx.x & 63, hd = (int)p.c.head_dim, hq = (int)p.d.q_heads, hkv = ONE ? (int)p.c.kv_heads : 0, per_row = hd / 8, abreast = 64 / per_row;
+    const int slot = lane / per_row, i = lane % per_row, h0 = part * HELD * abreast + slot, rows = hq + 2 * hkv;
+    const int pos = p.positions[t], seq = p.seq_ids[t];
+    const bool there = slot < abreast;
+    const Chunks turned_at = chunks_of<INTER>(i, hd, (int)p.d.rotary_dim, p.d.rotary_dim > 0), plain_at = chunks_of<INTER>(i, hd, 0, false);
+    F4 x[HELD], y[HELD];
 #pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
+    for (int j = 0; j < HELD; ++j) {
         const int h = h0 + j * abreast;
-        if (h >= hq) continue;
-        const float *src = p.q + t * p.d.q_row_stride + h * p.d.q_head_stride;
+        x[j] = y[j] = F4{0.f, 0.f, 0.f, 0.f};
+        if (!there || h >= rows) continue;
+        const float *src = h < hq ? p.q + t * p.d.q_row_stride + h * p.d.q_head_stride
+                           : h < hq + hkv ? p.k + t * p.d.k_row_stride + (h - hq) * p.d.k_head_stride
+                                          : p.v + t * p.d.v_row_stride + (h - hq - hkv) * p.d.v_head_stride;
+        const Chunks &at = h < hq + hkv ? turned_at : plain_at;
         x[j] = load4<NT>(src + at.a);
         y[j] = load4<NT>(src + at.b);
     }
-    const Angles g = angles_at<INTER>(p, pos, i, at);
+    if (pos == -1) return;
+    int page = 0, row = 0;
+    if (!find_row(p, seq, pos, &page, &row)) {
+        if (ONE && part == 0 && lane == 0) fth::report_bad_entry(p.bad, t);
+        return;
+    }
+    const bool again = ONE && t > 0 && p.positions[t - 1] == pos && p.seq_ids[t - 1] == seq;  // once more the same place
+    if (again && part == 0 && lane == 0) fth::report_bad_entry(p.bad, t);
+    if (p.d.rotary_dim > 0) {
+        const Angles g = angles_at<INTER>(p, pos, i, turned_at);
 #pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
+        for (int j = 0; j < HELD; ++j)
+            if (h0 + j * abreast < hq + hkv) turn<INTER>(x[j], y[j], g, turned_at);
+    }
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
         const int h = h0 + j * abreast;
-        if (h >= hq) continue;
-        if (p.d.rotary_dim > 0) turn<INTER>(x[j], y[j], g, at);
-        float *dst = p.q_out + t * p.d.out_row_stride + h * p.d.out_head_stride;
-        if constexpr (NT) {
-            __builtin_nontemporal_store(x[j], reinterpret_cast<F4 *>(dst + at.a));
-            __builtin_nontemporal_store(y[j], reinterpret_cast<F4 *>(dst + at.b));
-        } else {
-            *reinterpret_cast<F4 *>(dst + at.a) = x[j];
-            *reinterpret_cast<F4 *>(dst + at.b) = y[j];
+        const bool mine = there && h < rows;
+        if (mine && h < hq) {
+            float *dst = p.q_out + t * p.d.out_row_stride + h * p.d.out_head_stride;
+            if constexpr (NT) {
+                __builtin_nontemporal_store(x[j], reinterpret_cast<F4 *>(dst + turned_at.a));
+                __builtin_nontemporal_store(y[j], reinterpret_cast<F4 *>(dst + turned_at.b));
+            } else {
+                *reinterpret_cast<F4 *>(dst + turned_at.a) = x[j];
+                *reinterpret_cast<F4 *>(dst + turned_at.b) = y[j];
+            }
+        }
+        if constexpr (ONE) {
+            uint32_t largest = largest_of(x[j], y[j], 0);
+#pragma unroll
+            for (int m = 16; m > 0; m >>= 1) {  // to the first lane of the row, which need not be a power of two long
+                const uint32_t other = __shfl_down(largest, m);
+                largest = i + m < per_row && other > largest ? other : largest;
+            }
+            largest = __shfl(largest, slot * per_row);
+            if (!mine || h < hq || again) continue;
+            const bool keys = h < hq + hkv;
+            const int64_t hk = keys ? h - hq : h - hq - hkv;
+            const Chunks &at = keys ? turned_at : plain_at;
+            const float now = scale_for<T>(__uint_as_float(largest)), per = per_scale(now);
+            uint8_t *to = static_cast<uint8_t *>(keys ? p.k_cache : p.v_cache) + page * p.c.page_stride + hk * p.c.head_stride + row * p.c.row_stride;
+            *reinterpret_cast<uint32_t *>(to + at.a) = now == now ? codes4<T>(x[j] * per) : 0u;
+            *reinterpret_cast<uint32_t *>(to + at.b) = now == now ? codes4<T>(y[j] * per) : 0u;
+            if (i == 0) (keys ? p.k_scales : p.v_scales)[page * p.sc.page_stride + hk * p.sc.head_stride + row] = now;
+        }
+    }
+}
+
+// What a wavefront takes: one token's rows alone (RUNS none, blocks of one position); or the runs that begin in `chunk` tokens, for one head (one), and so
+// all wavefronts of the workgroup together (team). Workgroups with rows of tokens stand between those with runs, which wait for loads that depend on each
+// other.
+enum class Runs { none, one, team };
+
+struct Cut {
+    uint32_t share;      // of the first b workgroups, b share / 2^32 have runs (0: all)
+    int chunk, runs;     // tokens; items of a chunk and a head
+    int parts;           // wavefronts for the rows of a token
+    fth::Divisor by_heads, by_parts;
+};
+
+template <typename T, bool INTER, bool NT, Runs RUNS> __global__ __launch_bounds__(64 * kWaves, 4) void append_scaled_vec_kernel(const Args p, const Cut cut) {
+    constexpr bool TEAM = RUNS == Runs::team;
+    __shared__ Team team;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), heads = 2 * (int)p.c.kv_heads;
+    auto with_runs = [&](uint32_t b) { return RUNS == Runs::none ? 0 : cut.share ? (int)__umulhi(b, cut.share) : (int)b; };
+    const int before = with_runs(blockIdx.x), upto = with_runs(blockIdx.x + 1);
+    if (before == upto) {
+        const int work = ((int)blockIdx.x - before) * kWaves + wave, t = (int)cut.by_parts((uint32_t)work);
+        if (t < p.d.tokens) store_token<T, INTER, NT, RUNS == Runs::none>(p, t, work - t * cut.parts);
+        return;
+    }
+    if constexpr (RUNS != Runs::none) {
+        const int work = TEAM ? before : before * kWaves + wave;
+        if (work >= cut.runs) return;
+        const int group = (int)cut.by_heads((uint32_t)work), item = work - group * heads, chunk = cut.chunk, block = (int)p.sc.block;
+        const int64_t t0 = (int64_t)group * chunk, t = t0 + lane;
+        const bool there = t < p.d.tokens;
+        const int pos = there ? p.positions[t] : -1, seq = there ? p.seq_ids[t] : -1;
+        int pos_before = __shfl_up(pos, 1), seq_before = __shfl_up(seq, 1);
+        if (lane == 0 && t0 > 0) pos_before = p.positions[t0 - 1], seq_before = p.seq_ids[t0 - 1];
+        const bool known = t > 0 && pos >= 0 && pos_before >= 0 && seq == seq_before;
+        const int start = pos >= 0 ? (int)p.by_block((uint32_t)pos) * block : 0;  // of its block (pages are whole blocks)
+        const bool inside = known && pos_before >= start && pos_before - start < block, goes_on = inside && pos_before == pos - 1;
+        const uint64_t on = __ballot(goes_on);
+        if (item == 0 && lane < chunk && inside && !goes_on) fth::report_bad_entry(p.bad, t);
+        for (uint64_t begins = __ballot(lane < chunk && there && pos != -1 && !inside); begins; begins &= begins - 1) {
+            const int at = __builtin_ctzll(begins);
+            const int first_pos = __builtin_amdgcn_readlane(pos, at), first_seq = __builtin_amdgcn_readlane(seq, at);
+            const uint64_t others = ~(at < 63 ? on >> (at + 1) : 0);
+            int n = 1 + (others ? __builtin_ctzll(others) : 64);
+            // (a block that reaches past these 64 tokens)
+            if (at + n >= 64) {
+                n = 64 - at;
+                const int most = first_pos < 0 ? n : block - (first_pos - (int)p.by_block((uint32_t)first_pos) * block);
+                for (;;) {
+                    const int64_t next = t0 + at + n + lane;
+                    const bool more = n + lane < most && next < p.d.tokens && p.positions[next] == first_pos + n + lane && p.seq_ids[next] == first_seq;
+                    const uint64_t every = __ballot(more);
+                    n += ~every ? __builtin_ctzll(~every) : 64;
+                    if (~every) break;
+                }
+            }
+            store_run<T, INTER, NT, TEAM>(p, t0 + at, n, first_pos, first_seq, item, team);
         }
     }
 }
@@ -419,14 +534,28 @@ bool takes_vectors(const Args &a) {
 template <typename T> int32_t launch(const Args &a, hipStream_t st) {
     if (takes_vectors(a)) {
         const int64_t heads = 2 * a.c.kv_heads, abreast = 64 / (a.c.head_dim / 8);
-        const int chunk = a.d.tokens * heads <= 8192 ? 1 : (int)(a.sc.block < 64 ? a.sc.block : 64);
-        const int64_t kv_items = fth::ceil_div(a.d.tokens, chunk) * heads, q_parts = fth::ceil_div(a.d.q_heads, abreast * kHeld);
-        const int64_t blocks = fth::ceil_div(kv_items + a.d.tokens * q_parts, kWaves);
-        FTH_ARG(blocks <= 2147483647LL, "paged_append_scaled: too many tokens for one launch");
+        const bool one = a.sc.block == 1;
+        const int chunk = a.d.tokens * heads <= 8192 ? 1 : (int)(a.sc.block < 32 ? a.sc.block : 32);
+        const int64_t run_items = one ? 0 : fth::ceil_div(a.d.tokens, chunk) * heads, parts = fth::ceil_div(a.d.q_heads + (one ? heads : 0), abreast * 4);
+        const bool team = a.sc.block > kHeld * abreast && chunk > 1;
+        const int64_t run_blocks = team ? run_items : fth::ceil_div(run_items, kWaves), blocks = run_blocks + fth::ceil_div(a.d.tokens * parts, kWaves);
+        FTH_ARG(run_items <= 2147483600LL && a.d.tokens * parts <= 2147483600LL && blocks <= 2147483647LL, "paged_append_scaled: too many tokens for one launch");
         const bool nt = (double)a.d.tokens * a.c.head_dim * (8.0 * a.d.q_heads + 10.0 * a.c.kv_heads) > 0x1p28;
-        auto go = [&](auto kernel) { kernel<<<dim3((unsigned)blocks), dim3(64 * kWaves), 0, st>>>(a, chunk, kv_items, (int)(q_parts ? q_parts : 1)); };
-        if (a.d.interleaved && a.d.rotary_dim > 0) go(nt ? append_scaled_vec_kernel<T, true, true> : append_scaled_vec_kernel<T, true, false>);
-        else go(nt ? append_scaled_vec_kernel<T, false, true> : append_scaled_vec_kernel<T, false, false>);
+        Cut cut;
+        cut.chunk = chunk; cut.runs = (int)run_items; cut.parts = (int)(parts ? parts : 1);
+        cut.share = run_blocks == blocks ? 0u : (uint32_t)((((uint64_t)run_blocks << 32) + (uint64_t)blocks - 1) / (uint64_t)blocks);  // rounded up: of all, run_blocks have them
+        cut.by_heads = fth::Divisor((uint32_t)heads);
+        cut.by_parts = fth::Divisor((uint32_t)cut.parts);
+        auto go = [&](auto kernel) { kernel<<<dim3((unsigned)blocks), dim3(64 * kWaves), 0, st>>>(a, cut); };
+        auto pick = [&](auto inter, auto past) {
+            constexpr bool I = decltype(inter)::value, N = decltype(past)::value;
+            if (one) go(append_scaled_vec_kernel<T, I, N, Runs::none>);
+            else if (team) go(append_scaled_vec_kernel<T, I, N, Runs::team>);
+            else go(append_scaled_vec_kernel<T, I, N, Runs::one>);
+        };
+        const bool inter = a.d.interleaved && a.d.rotary_dim > 0;
+        if (inter) nt ? pick(std::true_type(), std::true_type()) : pick(std::true_type(), std::false_type());
+        else nt ? pick(std::false_type(), std::true_type()) : pick(std::false_type(), std::false_type());
         FTH_CHECK_LAUNCH("paged_append_scaled");
         return FTH_OK;
     }
