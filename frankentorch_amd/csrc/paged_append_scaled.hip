@@ -308,15 +308,20 @@ template <typename T, bool INTER, bool NT, bool TEAM> __device__ __forceinline__
     };
     auto turn_all = [&](int row0) __attribute__((always_inline)) {
         if (!turns) return;
-        Angles g[kHeld];
+        constexpr int AT_ONCE = INTER ? kHeld / 2 : kHeld;  // (registers)
 #pragma unroll
-        for (int j = 0; j < kHeld; ++j) {
-            const int row = row0 + j * abreast + slot;
-            if (there && row < tokens) g[j] = angles_at<INTER>(p, pos + row, i, at);
+        for (int j0 = 0; j0 < kHeld; j0 += AT_ONCE) {
+            Angles g[AT_ONCE];
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j) {
+                const int row = row0 + (j0 + j) * abreast + slot;
+                if (there && row < tokens) g[j] = angles_at<INTER>(p, pos + row, i, at);
+            }
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j)
+                if (there && row0 + (j0 + j) * abreast + slot < tokens) turn<INTER>(x[j0 + j], y[j0 + j], g[j], at);
+            if (INTER) __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int j = 0; j < kHeld; ++j)
-            if (there && row0 + j * abreast + slot < tokens) turn<INTER>(x[j], y[j], g[j], at);
     };
     // (a position without an angle has no place either; and then nothing is stored)
     const bool angles = !turns || (pos >= 0 && pos < p.d.max_pos);
