@@ -277,27 +277,27 @@ __device__ __forceinline__ uint32_t largest_of(F4 x, F4 y, uint32_t so_far) {
 constexpr int kWaves = 4;
 
 // `tokens` tokens from t on, all of one block from position `pos` of sequence `seq` on: one wavefront (TEAM: the workgroup) for their rows of one head, 64 /
-// (head_dim / 8) of them side by side, kHeld times as many in registers; longer runs are read twice. The rows are asked for before it is
+// (head_dim / 8) of them side by side, HELD times as many in registers; longer runs are read twice. The rows are asked for before it is
 // known where they go.
-constexpr int kHeld = 4;
+constexpr int kHeld = 4;  // at most
 struct Team {
     uint32_t largest[kWaves];
     float had;
 };
-template <typename T, bool INTER, bool NT, bool TEAM> __device__ __forceinline__ void store_run(const Args &p, int64_t t, int tokens, int pos, int seq, int item, Team &team) {
+template <typename T, bool INTER, bool NT, bool TEAM, int HELD> __device__ __forceinline__ void store_run(const Args &p, int64_t t, int tokens, int pos, int seq, int item, Team &team) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, hd = (int)p.c.head_dim, hkv = (int)p.c.kv_heads, per_row = hd / 8, abreast = 64 / per_row;
-    const int slot = lane / per_row, i = lane % per_row, held = kHeld * abreast;
+    const int slot = lane / per_row, i = lane % per_row, held = HELD * abreast;
     const int from = TEAM ? wave * held : 0, step = TEAM ? kWaves * held : held;  // this wavefront's rows
     const bool keys = item < hkv, there = slot < abreast;
     const int64_t h = keys ? item : item - hkv, pitch = keys ? p.d.k_row_stride : p.d.v_row_stride;
     const float *src = keys ? p.k + t * pitch + h * p.d.k_head_stride : p.v + t * pitch + h * p.d.v_head_stride;
     const bool turns = keys && p.d.rotary_dim > 0;
     const Chunks at = chunks_of<INTER>(i, hd, (int)p.d.rotary_dim, turns);
-    F4 x[kHeld], y[kHeld];
+    F4 x[HELD], y[HELD];
     auto fetch = [&](int row0) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < kHeld; ++j) {
+        for (int j = 0; j < HELD; ++j) {
             const int row = row0 + j * abreast + slot;
             x[j] = y[j] = F4{0.f, 0.f, 0.f, 0.f};
             if (there && row < tokens) {
@@ -308,9 +308,9 @@ template <typename T, bool INTER, bool NT, bool TEAM> __device__ __forceinline__
     };
     auto turn_all = [&](int row0) __attribute__((always_inline)) {
         if (!turns) return;
-        constexpr int AT_ONCE = INTER ? kHeld / 2 : kHeld;  // (registers)
+        constexpr int AT_ONCE = INTER ? HELD / 2 : HELD;  // (registers)
 #pragma unroll
-        for (int j0 = 0; j0 < kHeld; j0 += AT_ONCE) {
+        for (int j0 = 0; j0 < HELD; j0 += AT_ONCE) {
             Angles g[AT_ONCE];
 #pragma unroll
             for (int j = 0; j < AT_ONCE; ++j) {
@@ -341,17 +341,17 @@ template <typename T, bool INTER, bool NT, bool TEAM> __device__ __forceinline__
         if (item == 0 && threadIdx.x % (TEAM ? 64 * kWaves : 64) == 0) fth::report_bad_entry(p.bad, t + rest);
         tokens = rest;
 #pragma unroll
-        for (int j = 0; j < kHeld; ++j)
+        for (int j = 0; j < HELD; ++j)
             if (from + j * abreast + slot >= tokens) x[j] = y[j] = F4{0.f, 0.f, 0.f, 0.f};
     }
     uint32_t largest = 0;
 #pragma unroll
-    for (int j = 0; j < kHeld; ++j) largest = largest_of(x[j], y[j], largest);
+    for (int j = 0; j < HELD; ++j) largest = largest_of(x[j], y[j], largest);
     for (int row0 = from + step; row0 < tokens; row0 += step) {
         fetch(row0);
         turn_all(row0);
 #pragma unroll
-        for (int j = 0; j < kHeld; ++j) largest = largest_of(x[j], y[j], largest);
+        for (int j = 0; j < HELD; ++j) largest = largest_of(x[j], y[j], largest);
     }
 #pragma unroll
     for (int m = 32; m > 0; m >>= 1) {
@@ -387,7 +387,7 @@ template <typename T, bool INTER, bool NT, bool TEAM> __device__ __forceinline__
             turn_all(row0);
         }
 #pragma unroll
-        for (int j = 0; j < kHeld; ++j) {
+        for (int j = 0; j < HELD; ++j) {
             const int in_run = row0 + j * abreast + slot;
             if (!there || in_run >= tokens) continue;
             uint8_t *to = dst + (row + in_run) * p.c.row_stride;
@@ -479,7 +479,7 @@ struct Cut {
     fth::Divisor by_heads, by_parts;
 };
 
-template <typename T, bool INTER, bool NT, Runs RUNS> __global__ __launch_bounds__(64 * kWaves, 4) void append_scaled_vec_kernel(const Args p, const Cut cut) {
+template <typename T, bool INTER, bool NT, Runs RUNS, int HELD> __global__ __launch_bounds__(64 * kWaves, HELD == 2 ? 5 : 4) void append_scaled_vec_kernel(const Args p, const Cut cut) {
     constexpr bool TEAM = RUNS == Runs::team;
     __shared__ Team team;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), heads = 2 * (int)p.c.kv_heads;
@@ -521,7 +521,7 @@ template <typename T, bool INTER, bool NT, Runs RUNS> __global__ __launch_bounds
                     if (~every) break;
                 }
             }
-            store_run<T, INTER, NT, TEAM>(p, t0 + at, n, first_pos, first_seq, item, team);
+            store_run<T, INTER, NT, TEAM, HELD>(p, t0 + at, n, first_pos, first_seq, item, team);
         }
     }
 }
@@ -554,9 +554,10 @@ template <typename T> int32_t launch(const Args &a, hipStream_t st) {
         auto go = [&](auto kernel) { kernel<<<dim3((unsigned)blocks), dim3(64 * kWaves), 0, st>>>(a, cut); };
         auto pick = [&](auto inter, auto past) {
             constexpr bool I = decltype(inter)::value, N = decltype(past)::value;
-            if (one) go(append_scaled_vec_kernel<T, I, N, Runs::none>);
-            else if (team) go(append_scaled_vec_kernel<T, I, N, Runs::team>);
-            else go(append_scaled_vec_kernel<T, I, N, Runs::one>);
+            if (one) go(append_scaled_vec_kernel<T, I, N, Runs::none, kHeld>);
+            else if (team) go(append_scaled_vec_kernel<T, I, N, Runs::team, kHeld>);
+            else if (a.sc.block > 2 * abreast) go(append_scaled_vec_kernel<T, I, N, Runs::one, kHeld>);
+            else go(append_scaled_vec_kernel<T, I, N, Runs::one, 2>);
         };
         const bool inter = a.d.interleaved && a.d.rotary_dim > 0;
         if (inter) nt ? pick(std::true_type(), std::true_type()) : pick(std::true_type(), std::false_type());
