@@ -4,13 +4,16 @@
 blocks, tied head) that keeps keys and values there, so that a new token costs one pass over the weights and one over the
 cache instead of a forward over all positions. Prompts run through the dense causal attention and are appended on the way;
 after that every step appends one token per sequence, attends over the pages, and readies the logits (penalties, bias, a mask of
-allowed tokens) for the argmax. Positions are a learned table (`wpe`) or, without one, a rotation of queries and keys. K/V heads
-may be fewer than query heads (rows of `wk`, `wv`).
+allowed tokens) for the argmax or for sampling. Positions are a learned table (`wpe`) or, without one, a rotation of queries and keys. K/V heads
+may be fewer than query heads (rows of `wk`, `wv`). The cache holds fp32, 16 bits, or 8 bits with a scale for each block of
+positions and head.
 
     python -m frankentorch_amd.generate        # a GPT-2-small-shaped decoder with random weights, a few sequences
+    python -m frankentorch_amd.generate --cache e4m3 --temperature 0.8 --top-k 50 --top-p 0.95
 """
 from __future__ import annotations
 
+import argparse
 import ctypes as C
 from typing import Callable, Optional, Sequence
 
@@ -33,13 +36,24 @@ def _put(buf: DeviceBuffer, array) -> DeviceBuffer:
 
 class PagedKVCache:
     """Pages of one pool for up to `max_seqs` sequences of up to `max_len` positions, in every layer alike. `cache` is the
-    descriptor, `table` the block table on the device (kept in line with `rows` by `sync`)."""
+    descriptor, `table` the block table on the device (kept in line with `rows` by `sync`). With `dtype` "i8" or "e4m3" every `scale_block`
+    positions of a page (default: all of it) have a scale a head, and `scales` is their descriptor (None otherwise)."""
 
-    def __init__(self, layers: int, num_pages: int, page_size: int, kv_heads: int, head_dim: int, max_seqs: int, max_len: int, dtype: str = "f32"):
+    def __init__(self, layers: int, num_pages: int, page_size: int, kv_heads: int, head_dim: int, max_seqs: int, max_len: int, dtype: str = "f32",
+                 scale_block: Optional[int] = None):
         width = -(-max_len // page_size)
         self.cache = device.paged_cache(num_pages, page_size, kv_heads, head_dim, max_seqs, width, dtype)
-        store = np.float32 if dtype == "f32" else np.uint16
+        store = {"f32": np.float32, "f16": np.uint16, "bf16": np.uint16}.get(dtype, np.uint8)
         self.k, self.v = ([DeviceBuffer((num_pages * kv_heads * page_size * head_dim,), store) for _ in range(layers)] for _ in range(2))
+        self.scales = None
+        if store is np.uint8:
+            block = page_size if scale_block is None else scale_block
+            if block < 1 or page_size % block:
+                raise ValueError("blocks of %d positions do not make up a page of %d" % (block, page_size))
+            self.scales = device.paged_scales(self.cache, block)
+            self.k_scales, self.v_scales = ([DeviceBuffer((num_pages * kv_heads * (page_size // block),)) for _ in range(layers)] for _ in range(2))
+        elif scale_block is not None:
+            raise ValueError("a cache of %s has no scales" % dtype)
         self.rows = np.full((max_seqs, width), -1, np.int32)
         self.table = DeviceBuffer((max_seqs, width), np.int32)
         self.free = list(range(num_pages))[::-1]
@@ -63,6 +77,30 @@ class PagedKVCache:
         self.rows[seq] = -1
         self._dirty = True
 
+    def append(self, layer: int, desc, q, k, v, cosines, sines, table, seq_ids, positions, q_out) -> None:
+        """device.paged_append into a layer's pages, or with k and v None the rotation of queries alone."""
+        kc, vc = (None, None) if k is None else (self.k[layer], self.v[layer])
+        if self.scales is None:
+            device.paged_append(self.cache, desc, q, k, v, cosines, sines, table, seq_ids, positions, q_out, kc, vc)
+            return
+        ks, vs = (None, None) if k is None else (self.k_scales[layer], self.v_scales[layer])
+        device.paged_append_scaled(self.cache, self.scales, desc, q, k, v, cosines, sines, table, seq_ids, positions, q_out, kc, vc, ks, vs)
+
+    def workspace_bytes(self, cache, desc) -> int:
+        """Of `attend` with a descriptor of this cache and one of device.paged_sdpa_desc."""
+        lib = _lib.load()
+        if self.scales is None:
+            return lib.fth_dev_paged_sdpa_workspace_bytes(C.byref(cache), C.byref(desc))
+        return lib.fth_dev_paged_sdpa_scaled_workspace_bytes(C.byref(cache), C.byref(self.scales), C.byref(desc))
+
+    def attend(self, layer: int, cache, desc, scale, q, table, lens, out, workspace) -> None:
+        """device.paged_sdpa over a layer's pages; `cache`: this cache's descriptor, or one with other rows of the table."""
+        if self.scales is None:
+            device.paged_sdpa(cache, desc, scale, q, self.k[layer], self.v[layer], table, lens, out, workspace=workspace)
+        else:
+            device.paged_sdpa_scaled(cache, self.scales, desc, scale, q, self.k[layer], self.v[layer], self.k_scales[layer], self.v_scales[layer], table, lens, out,
+                                     workspace=workspace)
+
     def sync(self) -> DeviceBuffer:
         if self._dirty:
             _put(self.table, self.rows)
@@ -72,8 +110,10 @@ class PagedKVCache:
 
 class PagedDecoder:
     def __init__(self, wte, wpe, layers: Sequence[dict], lnf_w, lnf_b, n_heads: int, max_seqs: int, num_pages: int, page_size: int = 16, max_len: Optional[int] = None,
-                 cache: str = "f32", ln_eps: float = 1e-5, gelu_tanh: bool = True, rotary_dim: Optional[int] = None, interleaved: bool = False, rotary_base: float = 10000.0):
-        """The weights of `fused.Gpt2Hip`; wpe None: positions by rotation of the first `rotary_dim` elements of a head (default: all)."""
+                 cache: str = "f32", ln_eps: float = 1e-5, gelu_tanh: bool = True, rotary_dim: Optional[int] = None, interleaved: bool = False, rotary_base: float = 10000.0,
+                 scale_block: Optional[int] = None):
+        """The weights of `fused.Gpt2Hip`; wpe None: positions by rotation of the first `rotary_dim` elements of a head (default: all).
+        cache, scale_block: the type that keys and values are held in, and the block of a scale, as in PagedKVCache."""
         up = lambda a: DeviceBuffer.from_host(np.ascontiguousarray(a, np.float32))
         self.vocab, self.d = np.shape(wte)
         self.heads, self.hd, self.eps = n_heads, self.d // n_heads, ln_eps
@@ -95,7 +135,7 @@ class PagedDecoder:
             packed["wqkv"] = up(np.concatenate([lw["wq"], lw["wk"], lw["wv"]]))
             packed["bqkv"] = up(np.concatenate([lw["bq"], lw["bk"], lw["bv"]]))
             self.layers.append(packed)
-        self.kv = PagedKVCache(len(layers), num_pages, page_size, self.kv_heads, self.hd, max_seqs, self.max_len, cache)
+        self.kv = PagedKVCache(len(layers), num_pages, page_size, self.kv_heads, self.hd, max_seqs, self.max_len, cache, scale_block)
         self.act = device.EPI_GELU_TANH if gelu_tanh else device.EPI_GELU
         self.length = np.zeros(max_seqs, np.int32)  # positions of each sequence that are in the cache
         self._room = {}
@@ -138,8 +178,8 @@ class PagedDecoder:
             self._gemm(h, lw["wqkv"], qkv, t, self.qkv, d, lw["bqkv"])
             q = qkv.view(0) if append.q_heads else None
             if turn is not append:
-                device.paged_append(self.kv.cache, turn, qkv.view(0), None, None, self.cos, self.sin, None, None, pos, qkv.view(0), None, None)
-            device.paged_append(self.kv.cache, append, q, qkv.view(k_at), qkv.view(v_at), self.cos, self.sin, table, seq_ids, pos, q, self.kv.k[i], self.kv.v[i])
+                self.kv.append(i, turn, qkv.view(0), None, None, self.cos, self.sin, None, None, pos, qkv.view(0))
+            self.kv.append(i, append, q, qkv.view(k_at), qkv.view(v_at), self.cos, self.sin, table, seq_ids, pos, q)
             attend(i, qkv, ctx)
             self._gemm(ctx, lw["wo"], x, t, d, d, lw["bo"], x)
             device.layer_norm(x, lw["ln2_w"], lw["ln2_b"], h, t, d, self.eps)
@@ -208,11 +248,10 @@ class PagedDecoder:
         longest = -(-(int(positions.max()) + 1) // 128) * 128
         desc = device.paged_sdpa_desc(cache, self.heads, 1, min(longest, cache.max_pages * cache.page_size))
         desc.q_seq_stride = desc.q_row_stride = self.qkv
-        need = _lib.load().fth_dev_paged_sdpa_workspace_bytes(C.byref(cache), C.byref(desc))
-        work = self._buffer("attention", (need // 4 + 4,))
+        work = self._buffer("attention", (self.kv.workspace_bytes(cache, desc) // 4 + 4,))
 
         def attend(layer, qkv, out):
-            device.paged_sdpa(cache, desc, device.default_scale(self.hd), qkv, self.kv.k[layer], self.kv.v[layer], table, lens, out, workspace=work)
+            self.kv.attend(layer, cache, desc, device.default_scale(self.hd), qkv, table, lens, out, work)
 
         hidden = self._forward(ids, where, positions, attend)
         logits = self._buffer("logits", (n, self.vocab))
@@ -225,14 +264,22 @@ class PagedDecoder:
         self.length[seq] = 0
 
     def generate(self, prompts: Sequence[Sequence[int]], new_tokens: int, repetition: float = 1.0, frequency: float = 0.0, presence: float = 0.0, bias=None,
-                 allowed: Optional[Callable] = None, stop: Optional[int] = None):
-        """Greedy continuations of the prompts, one list a prompt. repetition, frequency and presence are as in
+                 allowed: Optional[Callable] = None, stop: Optional[int] = None, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, seed: int = 0):
+        """Continuations of the prompts, one list a prompt. repetition, frequency and presence are as in
         device.logits_process; bias [vocab] or None; allowed(prompt number, tokens so far) gives the tokens that may follow (a
         bool array over the vocabulary) or None for all; a sequence ends with the token `stop`, after `new_tokens`, or at max_len.
+        temperature, top_k, top_p and min_p are as in device.sample, one number for all prompts or one for each; where the temperature is 0
+        the choice is greedy. The numbers that a prompt's tokens are drawn with depend on `seed` and the prompt's place alone.
         Uses the sequences 0 .. len(prompts) - 1, which have to be empty, and gives them back, after an error too."""
         n = len(prompts)
         if new_tokens > 0 and n > len(self.length):
             raise ValueError("%d prompts are more than max_seqs, %d" % (n, len(self.length)))
+        settings = [np.broadcast_to(np.asarray(x, t), (n,)) for x, t in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32))]
+        temperatures, top_ks, top_ps, min_ps = settings
+        if not (np.all(np.isfinite(temperatures) & (temperatures >= 0)) and np.all(top_ks >= 0) and np.all(top_ps >= 0) and np.all((min_ps >= 0) & (min_ps <= 1))):
+            raise ValueError("a temperature, top_k or top_p is negative or not a number, or min_p is outside [0, 1]")
+        drawn = bool(np.any(temperatures > 0))
+        numbers = [np.random.default_rng([seed, r]) for r in range(n)]
         tokens = [list(p) for p in prompts]
         done = [[] for _ in prompts]
         width = max(len(p) for p in prompts) + new_tokens
@@ -242,6 +289,10 @@ class PagedDecoder:
         history, counts, given = DeviceBuffer((n, width), np.int32), DeviceBuffer((n,), np.int32), DeviceBuffer((n,), np.int32)
         words = (self.vocab + 31) // 32
         mask, ready, best = DeviceBuffer((n, words), np.uint32), DeviceBuffer((n, self.vocab)), DeviceBuffer((n,))
+        if drawn:
+            choice = [DeviceBuffer((n,), x.dtype) for x in settings]
+            uniform, chosen = DeviceBuffer((n,), np.float64), DeviceBuffer((n,), np.int32)
+            draw_work = device.sample_workspace(device.sample_desc(n, self.vocab))
 
         def choose(rows, logits):
             """The next token of the sequences `rows` from their logits."""
@@ -262,8 +313,17 @@ class PagedDecoder:
             if allowed is not None:
                 _put(mask, np.packbits(bits, axis=1, bitorder="little").view(np.uint32))
             device.logits_process(desc, logits, history, counts, given, *penalties, dev_bias, mask if allowed is not None else None, ready)
-            device.argmax(ready, m, self.vocab, 1, best)
-            return best.to_host()[:m].astype(np.int64)
+            if not drawn:
+                device.argmax(ready, m, self.vocab, 1, best)
+                return best.to_host()[:m].astype(np.int64)
+            for buf, values in zip(choice, settings):
+                _put(buf, values[rows])
+            _put(uniform, [numbers[r].random() for r in rows])
+            device.sample(device.sample_desc(m, self.vocab), ready, *choice, uniform, chosen, workspace=draw_work)
+            got = chosen.to_host()[:m].astype(np.int64)
+            if (got < 0).any():
+                raise ValueError("the logits after prompt %d cannot be sampled: one is not a number or infinite" % rows[int(np.argmax(got < 0))])
+            return got
 
         def note(rows, chosen):
             for r, t in zip(rows, chosen):
@@ -290,6 +350,14 @@ class PagedDecoder:
 def main() -> None:
     import time
 
+    args = argparse.ArgumentParser(prog="python -m frankentorch_amd.generate", description="A GPT-2-small-shaped decoder with random weights, eight sequences.")
+    args.add_argument("--cache", default="bf16", choices=["f32", "f16", "bf16", "i8", "e4m3"], help="the type that keys and values are held in")
+    args.add_argument("--temperature", type=float, default=0.0, help="0: greedy")
+    args.add_argument("--top-k", type=int, default=0, help="0: all")
+    args.add_argument("--top-p", type=float, default=1.0)
+    args.add_argument("--min-p", type=float, default=0.0)
+    args.add_argument("--seed", type=int, default=0)
+    args = args.parse_args()
     rng = np.random.RandomState(0)
     d, heads, layers, vocab, max_pos, ffn = 768, 12, 12, 50257, 1024, 3072
     w = lambda *s: (rng.standard_normal(s) * 0.02).astype(np.float32)
@@ -297,11 +365,11 @@ def main() -> None:
     blocks = [dict(ln1_w=one, ln1_b=zero, wq=w(d, d), bq=zero, wk=w(d, d), bk=zero, wv=w(d, d), bv=zero, wo=w(d, d), bo=zero, ln2_w=one, ln2_b=zero,
                    w1=w(ffn, d), b1=np.zeros(ffn, np.float32), w2=w(d, ffn), b2=zero) for _ in range(layers)]
     batch, new = 8, 64
-    model = PagedDecoder(w(vocab, d), w(max_pos, d), blocks, one, zero, heads, batch, batch * max_pos // 16, cache="bf16")
+    model = PagedDecoder(w(vocab, d), w(max_pos, d), blocks, one, zero, heads, batch, batch * max_pos // 16, cache=args.cache)
     prompts = [rng.randint(0, vocab, 40 + 60 * i).tolist() for i in range(batch)]
     model.generate(prompts, 4)
     start = time.perf_counter()
-    out = model.generate(prompts, new, repetition=1.1, frequency=0.1)
+    out = model.generate(prompts, new, repetition=1.1, frequency=0.1, temperature=args.temperature, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p, seed=args.seed)
     took = time.perf_counter() - start
     print("%d sequences, %d new tokens each: %.2f ms a step (prompts included), first tokens of each: %s" % (batch, new, 1e3 * took / new, [o[:4] for o in out]))
 
