@@ -17,7 +17,7 @@ namespace {
 
 constexpr int kPiece = 2048, kEntries = 128, kWaves = 4;         // logits of a piece, candidates that it may write down, pieces of a workgroup
 constexpr int kThreads = 1024, kBins = 2048, kList = 7168, kFew = 1024;   // the choice: bins, candidates in LDS, members of a bin that are ranked
-constexpr int kPlaces = 512, kAhead = 4, kGroups = kPiece / kThreads;                            // pieces of a row whose candidates are listed; of a wavefront, fetched at once
+constexpr int kPlaces = 512, kAhead = 4, kGroups = kPiece / kThreads, kMyBins = kBins / kThreads;                            // pieces of a row whose candidates are listed; of a wavefront, fetched at once
 
 struct Piece {
     float max, limit;  // of what is not written down, every logit is below `limit` (-inf: all is written down)
@@ -226,37 +226,41 @@ __global__ __launch_bounds__(64 * kWaves) void sample_pieces_kernel(const Sample
 struct Member {
     uint64_t code, weight;
 };
+struct Found {  // what the threads of a boundary() tell each other
+    uint64_t code, weight;
+    uint32_t members;
+    int at;
+};
 struct Shared {
     uint64_t weight[kBins];  // of the bins
     uint32_t count[kBins];
     Entry list[kList];       // the candidates, in the order of the vocabulary
     uint64_t whole[kList];   // their weights
     Member few[kFew];
-    uint64_t sums[2][kThreads / 64];
-    uint64_t found, above;
+    uint64_t sums[2][32];
+    Found finds[2];
     uint32_t places[kPlaces + 1];  // where the candidates of each piece stand in the list
-    uint32_t members;
-    int at;
 };
 
-// The sums over the threads before this one of two numbers at once, and over all.
-__device__ __forceinline__ void block_scan(uint64_t &x, uint64_t &y, uint64_t (&lds)[2][kThreads / 64], uint64_t *all_x, uint64_t *all_y) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint64_t upto_x = wave_scan(x, (uint64_t)0, AddOp()), upto_y = wave_scan(y, (uint64_t)0, AddOp());
+// op over the lanes of a row of 16 up to each one.
+template <typename T, typename F> __device__ __forceinline__ T row_scan(T x, T neutral, F op) {
+    x = op(moved<0x111, 0xf>(neutral, x), x);
+    x = op(moved<0x112, 0xf>(neutral, x), x);
+    x = op(moved<0x114, 0xf>(neutral, x), x);
+    return op(moved<0x118, 0xf>(neutral, x), x);
+}
+// The sum over the threads before this one, and over all. One barrier before `lds` is written, one after.
+template <typename T> __device__ __forceinline__ T block_scan(T x, T *lds, T *all) {
+    constexpr int W = kThreads / 64;
+    static_assert(W == 16, "the wavefronts' sums are a row of lanes");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const T upto = wave_scan(x, (T)0, AddOp());
     __syncthreads();
-    if (lane == 63) {
-        lds[0][wave] = upto_x;
-        lds[1][wave] = upto_y;
-    }
+    if (lane == 63) lds[wave] = upto;
     __syncthreads();
-    uint64_t tx = lds[0][lane & 15], ty = lds[1][lane & 15];  // 16 wavefronts: a row of lanes
-    tx = wave_scan(tx, (uint64_t)0, AddOp());
-    ty = wave_scan(ty, (uint64_t)0, AddOp());
-    *all_x = lane_value(tx, 15);
-    *all_y = lane_value(ty, 15);
-    const int w = __builtin_amdgcn_readfirstlane(wave);
-    x = upto_x - x + (w ? lane_value(tx, w ? w - 1 : 0) : 0);
-    y = upto_y - y + (w ? lane_value(ty, w ? w - 1 : 0) : 0);
+    const T t = row_scan(lds[lane & (W - 1)], (T)0, AddOp());
+    *all = lane_value(t, W - 1);
+    return upto - x + (wave ? lane_value(t, wave ? wave - 1 : 0) : (T)0);
 }
 
 struct Row {
@@ -297,6 +301,7 @@ struct Row {
         if (p.logprobs) p.logprobs[r] = (float)log(share);
     }
     __device__ __forceinline__ void clear_bins() const {
+        if (threadIdx.x < 2) s.finds[threadIdx.x] = Found{0, 0, 0, -1};
         for (int b = threadIdx.x; b < kBins; b += kThreads) {
             s.weight[b] = 0;
             s.count[b] = 0;
@@ -308,48 +313,55 @@ struct Row {
         if (w) atomicAdd(reinterpret_cast<unsigned long long *>(&s.weight[b]), (unsigned long long)w);
     }
 
-    // What comes before each of a thread's two bins.
+    // What comes before a thread's first bin.
     struct Prefix {
-        uint64_t count, weight;
+        uint32_t count;
+        uint64_t weight;
     };
-    __device__ __forceinline__ Prefix scan_bins(uint64_t *all) const {
-        const int t = threadIdx.x;
-        Prefix at = {(uint64_t)s.count[2 * t] + s.count[2 * t + 1], s.weight[2 * t] + s.weight[2 * t + 1]};
-        uint64_t unused;
-        block_scan(at.count, at.weight, s.sums, &unused, all);
+    __device__ __forceinline__ Prefix scan_bins(bool counts, bool weights, uint64_t *all) const {
+        Prefix at = {0, 0};
+#pragma unroll
+        for (int b = 0; b < kMyBins; ++b) {
+            at.count += s.count[kMyBins * threadIdx.x + b];
+            at.weight += s.weight[kMyBins * threadIdx.x + b];
+        }
+        uint32_t unused;
+        if (counts) at.count = block_scan(at.count, reinterpret_cast<uint32_t *>(s.sums[1]), &unused);
+        if (weights) at.weight = block_scan(at.weight, s.sums[0], all);
         return at;
     }
 
     // The smallest code for which the tokens up to it are `k` at least (k > 0) or weigh `need`, by the bins: the bin, then the ranks of its
-    // members; where it has too many (ties) digit by digit. All ones if there is none. *weight: what they weigh.
-    template <bool LIST> __device__ __forceinline__ uint64_t boundary(int n, const Prefix &at, uint32_t k, uint64_t need, uint64_t *weight) const {
+    // members; where it has too many (ties) digit by digit. All ones if there is none. *weight: what they weigh. `call`: 0, then 1.
+    template <bool LIST> __device__ __forceinline__ uint64_t boundary(int n, const Prefix &at, uint32_t k, uint64_t need, int call, uint64_t *weight) const {
         const int t = threadIdx.x;
+        Found &f = s.finds[call];
+        const uint64_t goal = k ? k : need;
+        uint64_t before = k ? (uint64_t)at.count : at.weight, weighed = at.weight;
+        if (before < goal)
+#pragma unroll
+            for (int b = 0; b < kMyBins; ++b) {
+                const uint64_t w = s.weight[kMyBins * t + b], here = k ? (uint64_t)s.count[kMyBins * t + b] : w;
+                if (before < goal && before + here >= goal) {
+                    f.at = kMyBins * t + b;
+                    f.code = weighed;
+                    f.weight = before;
+                }
+                before += here;
+                weighed += w;
+            }
         __syncthreads();
-        if (t == 0) {
-            s.members = 0;
-            s.at = -1;
-        }
-        __syncthreads();
-        const uint64_t goal = k ? k : need, c0 = s.count[2 * t], w0 = s.weight[2 * t];
-        const uint64_t b0 = k ? at.count : at.weight, m0 = b0 + (k ? c0 : w0), e0 = m0 + (k ? (uint64_t)s.count[2 * t + 1] : s.weight[2 * t + 1]);
-        if (b0 < goal && e0 >= goal) {
-            const bool second = m0 < goal;
-            s.at = 2 * t + second;
-            s.found = at.weight + (second ? w0 : 0);
-            s.above = second ? m0 : b0;
-        }
-        __syncthreads();
-        const int bin = s.at;
+        const int bin = f.at;
         if (bin < 0) return ~0ull;
-        uint64_t weighs = s.found, had = s.above;
+        uint64_t weighs = f.code, had = f.weight;
         const uint32_t members = s.count[bin];
         if (members <= kFew) {
             each<LIST>(n, [&](float z, uint32_t v, uint64_t w) {
-                if (bin_of(z) == bin) s.few[atomicAdd(&s.members, 1u)] = Member{code_of(z, v), w};
+                if (bin_of(z) == bin) s.few[atomicAdd(&f.members, 1u)] = Member{code_of(z, v), w};
             });
             __syncthreads();
-            if (t < (int)members) {  // ranks: in whatever order the members stand
-                const Member mine = s.few[t];
+            for (int m = t; m < (int)members; m += kThreads) {  // ranks: in whatever order the members stand
+                const Member mine = s.few[m];
                 uint64_t count = 0, sum = 0;
 #pragma unroll 4
                 for (uint32_t i = 0; i < members; ++i) {
@@ -360,13 +372,13 @@ struct Row {
                 }
                 const uint64_t upto = had + (k ? count : sum), here = k ? 1 : mine.weight;
                 if (upto < goal && upto + here >= goal) {
-                    s.found = mine.code;
-                    s.above = weighs + sum + mine.weight;
+                    f.code = mine.code;
+                    f.weight = weighs + sum + mine.weight;
                 }
             }
             __syncthreads();
-            *weight = s.above;
-            return s.found;
+            *weight = f.weight;
+            return f.code;
         }
         // (the bins of digits stand where the members would)
         uint64_t *digit_weight = &s.few[0].code;
@@ -374,9 +386,9 @@ struct Row {
         uint64_t prefix = 0;
         for (int shift = 56; shift >= 0; shift -= 8) {
             __syncthreads();
-            if (t < 256) {
-                digit_weight[t] = 0;
-                digit_count[t] = 0;
+            for (int d = t; d < 256; d += kThreads) {
+                digit_weight[d] = 0;
+                digit_count[d] = 0;
             }
             __syncthreads();
             each<LIST>(n, [&](float z, uint32_t v, uint64_t w) {
@@ -395,14 +407,14 @@ struct Row {
                     had += here;
                     weighs += digit_weight[d];
                 }
-                s.found = prefix << 8 | d;
-                s.above = had;
+                f.code = prefix << 8 | d;
+                f.weight = had;
                 s.sums[0][0] = weighs + digit_weight[d];
                 s.sums[0][1] = weighs;
             }
             __syncthreads();
-            prefix = s.found;
-            had = s.above;
+            prefix = f.code;
+            had = f.weight;
             *weight = s.sums[0][0];
             weighs = s.sums[0][1];
         }
@@ -419,15 +431,15 @@ struct Row {
         const bool below = !whole_row && set.min_p > 0.f && fth::exp2_softmax(((double)limit - (double)big) * set.rate) < (double)set.min_p;
         uint64_t last = ~0ull, weight = 0, all = 0;
         if (set.top_k == 0 && !(set.top_p < 1.f)) return whole_row || below ? last : 0;
-        const Prefix at = scan_bins(&all);
+        const Prefix at = scan_bins(set.top_k > 0, set.top_p < 1.f, &all);
         if (set.top_k > 0) {
-            last = boundary<LIST>(n, at, (uint32_t)set.top_k, 0, &weight);
+            last = boundary<LIST>(n, at, (uint32_t)set.top_k, 0, 0, &weight);
             if (!sure(last) && (set.top_p < 1.f || !below)) return 0;
             sum = (double)(last == ~0ull ? all : weight);  // (fewer tokens are allowed)
         }
         if (set.top_p < 1.f) {
             const double need = __builtin_ceil(sum * (double)set.top_p);
-            const uint64_t code = boundary<LIST>(n, at, 0, need < 1.0 ? 1 : (uint64_t)need, &weight);
+            const uint64_t code = boundary<LIST>(n, at, 0, need < 1.0 ? 1 : (uint64_t)need, 1, &weight);
             if (code < last) last = code;  // (none: rounded weights fall short of it, or the candidates do)
             if (!sure(last) && (set.top_k > 0 || !below)) return 0;
         }
@@ -446,10 +458,9 @@ struct Row {
             }
             return s.whole[i];
         };
-        uint64_t before = 0, unused = 0, total, none;
-        for (int i = from; i < to; ++i) before += kept(i);
-        const uint64_t mine = before;
-        block_scan(before, unused, s.sums, &total, &none);
+        uint64_t mine = 0, total;
+        for (int i = from; i < to; ++i) mine += kept(i);
+        uint64_t before = block_scan(mine, s.sums[0], &total);
         uint64_t target = (uint64_t)((double)total * u);
         target = target < total ? target : total - 1;
         if (mine == 0 || before > target || before + mine <= target) return;
@@ -484,19 +495,20 @@ struct Row {
             if (lane == 0) ranges[g] = sum;
         }
         __syncthreads();
+        static_assert(kThreads >= 256, "a thread for each range");
         const uint64_t mine = threadIdx.x < 256 ? ranges[threadIdx.x] : 0;
-        uint64_t before = mine, unused = 0, total, none;
-        block_scan(before, unused, s.sums, &total, &none);
+        uint64_t total;
+        const uint64_t before = block_scan(mine, s.sums[0], &total);
         uint64_t target = (uint64_t)((double)total * u);
         target = target < total ? target : total - 1;
         if (mine > 0 && before <= target && before + mine > target) {
-            s.at = threadIdx.x;
-            s.found = target - before;
+            s.finds[0].at = threadIdx.x;
+            s.finds[0].code = target - before;
         }
         __syncthreads();
         if (wave != 0) return;
-        uint64_t left = s.found;
-        const int g = s.at;
+        uint64_t left = s.finds[0].code;
+        const int g = s.finds[0].at;
         for (int i0 = 0; i0 < length; i0 += 64) {
             const uint64_t here = i0 + lane < length ? kept((int64_t)g * length + i0 + lane) : 0, upto = wave_scan(here, (uint64_t)0, AddOp());
             if (here > 0 && upto > left && upto - here <= left) write(g * length + i0 + lane, (double)here / (double)total);
