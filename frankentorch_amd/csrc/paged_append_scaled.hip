@@ -294,6 +294,9 @@ template <typename T, bool INTER, bool NT, bool TEAM, int HELD> __device__ __for
     const float *src = keys ? p.k + t * pitch + h * p.d.k_head_stride : p.v + t * pitch + h * p.d.v_head_stride;
     const bool turns = keys && p.d.rotary_dim > 0;
     const Chunks at = chunks_of<INTER>(i, hd, (int)p.d.rotary_dim, turns);
+    // rows that have an angle (the others have no place either, and are not stored)
+    const int64_t angles = pos < 0 ? 0 : p.d.max_pos - pos;
+    const int to_turn = !turns || angles < 0 ? 0 : angles < tokens ? (int)angles : tokens;
     F4 x[HELD], y[HELD];
     auto fetch = [&](int row0) __attribute__((always_inline)) {
 #pragma unroll
@@ -315,23 +318,21 @@ template <typename T, bool INTER, bool NT, bool TEAM, int HELD> __device__ __for
 #pragma unroll
             for (int j = 0; j < AT_ONCE; ++j) {
                 const int row = row0 + (j0 + j) * abreast + slot;
-                if (there && row < tokens) g[j] = angles_at<INTER>(p, pos + row, i, at);
+                if (there && row < to_turn) g[j] = angles_at<INTER>(p, pos + row, i, at);
             }
 #pragma unroll
             for (int j = 0; j < AT_ONCE; ++j)
-                if (there && row0 + (j0 + j) * abreast + slot < tokens) turn<INTER>(x[j0 + j], y[j0 + j], g[j], at);
+                if (there && row0 + (j0 + j) * abreast + slot < to_turn) turn<INTER>(x[j0 + j], y[j0 + j], g[j], at);
             if (INTER) __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // (a position without an angle has no place either; and then nothing is stored)
-    const bool angles = !turns || (pos >= 0 && pos < p.d.max_pos);
     fetch(from);
     int page = 0, row = 0;
     const bool placed = find_row(p, seq, pos, &page, &row);
     const int first = placed ? (int)p.by_block((uint32_t)row) * (int)p.sc.block : 0;
     float *scale = (keys ? p.k_scales : p.v_scales) + (placed ? page : 0) * p.sc.page_stride + h * p.sc.head_stride + (int)p.by_block((uint32_t)first);
     float had = placed && row > first && (!TEAM || wave == 0) ? *scale : 0.f;
-    if (angles) turn_all(from);
+    turn_all(from);
     if (!placed) {
         if (item == 0 && threadIdx.x % (TEAM ? 64 * kWaves : 64) == 0) fth::report_bad_entry(p.bad, t);
         return;
