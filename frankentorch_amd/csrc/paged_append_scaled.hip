@@ -3,6 +3,10 @@
 // A block's scale s is the smallest power of two whose 127 (448) multiples reach the largest element it was given: x / s is exact, so
 // that an element is rounded once, and a scale that grows by 2^k takes what the block holds to code / 2^k. A run is the tokens of one block that stand
 // one after the other in the call; whoever has its first token does all of it, so that no two workgroups touch one block.
+//
+// Bound by reading the rows and writing the queries once: 3 prompts of up to 7001 tokens, 32 query heads on 8 of 128, e4m3, blocks of 48: 115 us, 5.9
+// TB/s (element by element 473; a wavefront a run that first asks for its place 156). Short calls wait for loads that depend on each
+// other, position -> page -> scale: 5.6 us for a step of 64 sequences, where an empty launch takes 5.
 
 #include <type_traits>
 
@@ -541,11 +545,19 @@ template <typename T> int32_t launch(const Args &a, hipStream_t st) {
     if (takes_vectors(a)) {
         const int64_t heads = 2 * a.c.kv_heads, abreast = 64 / (a.c.head_dim / 8);
         const bool one = a.sc.block == 1;
-        const int chunk = a.d.tokens * heads <= 8192 ? 1 : (int)(a.sc.block < 32 ? a.sc.block : 32);
+        // Tokens that a wavefront looks through for runs (the host does not know whether they make a few long ones or each its own). us for 1 / 4 / 32 of them,
+        // 16 heads of 128: steps of 64 sequences 5.6 / 10.7 / 33, of 256 9.0 / 12.4 / 35, of 700 18.0 / 18.5 / 40, of 2000 43 / 38 / 57; 3 prompts of up to
+        // 150 tokens, blocks of 48, 16.3 / 9.0 / 10.7, of up to 300 19.7 / 11.7 / 12.2, of 1000 37 / 28 / 23, of 7001 184 / 157 / 117; 8 of up
+        // to 1024, 24 heads of 64, 53 / 18.6 / 12.6.
+        const int most = a.d.tokens * heads <= 8192 ? 1 : a.d.tokens * heads <= 32768 ? 4 : 32, chunk = (int)(a.sc.block < most ? a.sc.block : most);
         const int64_t run_items = one ? 0 : fth::ceil_div(a.d.tokens, chunk) * heads, parts = fth::ceil_div(a.d.q_heads + (one ? heads : 0), abreast * 4);
+        // Four wavefronts for a run that one would read twice (us, one / four: 3 prompts of up to 7001, blocks of 32 137 / 124, of 64 156 / 119; against it 8 of up
+        // to 1024, heads of 64, blocks of 64 14.6 / 19).
         const bool team = a.sc.block > kHeld * abreast && chunk > 1;
         const int64_t run_blocks = team ? run_items : fth::ceil_div(run_items, kWaves), blocks = run_blocks + fth::ceil_div(a.d.tokens * parts, kWaves);
         FTH_ARG(run_items <= 2147483600LL && a.d.tokens * parts <= 2147483600LL && blocks <= 2147483647LL, "paged_append_scaled: too many tokens for one launch");
+        // Nontemporal where rows and queries are more than the 256 MB last-level cache has (us, without / with: 3 prompts of up to 7001, 680 MB, 126 / 117, of
+        // 4000 78 / 71, of 3000 61 / 55; of 2000, 190 MB, 42 / 38, but what comes next finds its queries there; 8 of up to 1024 12.6 / 12.9).
         const bool nt = (double)a.d.tokens * a.c.head_dim * (8.0 * a.d.q_heads + 10.0 * a.c.kv_heads) > 0x1p28;
         Cut cut;
         cut.chunk = chunk; cut.runs = (int)run_items; cut.parts = (int)(parts ? parts : 1);
@@ -555,6 +567,8 @@ template <typename T> int32_t launch(const Args &a, hipStream_t st) {
         auto go = [&](auto kernel) { kernel<<<dim3((unsigned)blocks), dim3(64 * kWaves), 0, st>>>(a, cut); };
         auto pick = [&](auto inter, auto past) {
             constexpr bool I = decltype(inter)::value, N = decltype(past)::value;
+            // Rows that blocks do not have cost wavefronts (us, 4 / 2 rows a lane: heads of 64, blocks of 16 14.2 / 12.6, of 8 20.8 / 17.2; heads of 128, of 16 113 / 137, of
+            // 8 121 / 117, of 4 135 / 124).
             if (one) go(append_scaled_vec_kernel<T, I, N, Runs::none, kHeld>);
             else if (team) go(append_scaled_vec_kernel<T, I, N, Runs::team, kHeld>);
             else if (a.sc.block > 2 * abreast) go(append_scaled_vec_kernel<T, I, N, Runs::one, kHeld>);

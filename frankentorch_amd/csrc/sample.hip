@@ -669,7 +669,7 @@ int32_t check(const fth_sample_desc *d) {
     FTH_ARG(d, "sample: NULL descriptor");
     FTH_ARG(d->rows >= 0 && d->vocab >= 0, "sample: negative extent");
     FTH_ARG(d->logits_stride >= d->vocab, "sample: the row stride is below the vocabulary");
-    if (d->logits_stride > ((int64_t)1 << 40) || d->vocab > 2147483647LL || d->rows > ((int64_t)1 << 20)) return fth::set_error(FTH_ERR_SIZE_OVERFLOW, "sample: extents overflow");
+    if (d->logits_stride > ((int64_t)1 << 40) || d->vocab > ((int64_t)1 << 30) || d->rows > ((int64_t)1 << 20)) return fth::set_error(FTH_ERR_SIZE_OVERFLOW, "sample: extents overflow");
     FTH_ARG(d->rows == 0 || d->vocab > 0, "sample: no token to choose from");
     if (pieces_of(*d) > 2147483640LL) return fth::set_error(FTH_ERR_SIZE_OVERFLOW, "sample: more than 2^42 logits");
     return FTH_OK;
