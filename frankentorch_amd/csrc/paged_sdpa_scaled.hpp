@@ -11,6 +11,13 @@
 //     are. They carry a factor of 2^40, which keeps the third part of every weight an output of fp32 can show above the smallest bf16; where that
 //     overflows (scales of V beyond 2^70) the share is walked again with 2^-24.
 // e4m3 becomes either type two at a time by one instruction of gfx950; whole numbers become f16 by the bits of 1024 + 128 + x, bf16 through fp32.
+//
+// Measured: 64 sequences of 1024 to 8191 keys, 32 query heads on 8 of 128, e4m3, blocks of 16 (614 MB): 111 us, 5.6 TB/s (one wavefront a row 3660;
+// a bf16 cache of the same keys, 1.22 GB, 193). One sequence of 131071: 53 us (5.1 TB/s). 16 of up to 3967, four queries, i8: 27. Bound by the loads, of which the
+// two workgroups of a compute unit keep too few bytes on the way: the loop without its products takes 110 / 49 / 26 us. Of two workgroups with equal
+// shares the older one ends at 82 us, the younger at 105; lengthening the shares of the older by 6 to 25 % was level, and so were three workgroups a
+// compute unit, tiles of 64 keys, raised wavefront priorities, and twice or four times as many shares (one sequence: 57 / 58 / 60).
+// Half tiles looked up 64 at a time took the loop from 460 to 330 instructions a tile (134 -> 111 us).
 #pragma once
 
 #include "paged_sdpa.hpp"
@@ -70,9 +77,6 @@ template <typename T> __device__ __forceinline__ uint32_t to_bf16(uint32_t first
 // Bit 7 of every byte that is a NaN of e4m3.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
-// 16 keys so many times make a tile of a wavefront.
-template <int DP, ScaleOf OF> constexpr int sixteens() { return 2; }
-
 // One segment: keys key_lo .. key_hi - 1 of a pair of `len` keys, with row tile rt of its queries. FULL: head_dim == DP; otherwise what lies past
 // head_dim counts as zero. NT: K and V leave no trace in the caches.
 template <typename T, int DP, bool FULL, bool NT, ScaleOf OF>
@@ -82,7 +86,7 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
     constexpr int NE = DP / 16;   // output columns of a lane, consecutive ones
     constexpr int NV = NE / 4;    // words of its part of a V row
     constexpr int NS = SIXTEEN || FOUR ? 1 : 4;
-    constexpr int H = sixteens<DP, OF>(), kKeys = 16 * H;
+    constexpr int H = 2, kKeys = 16 * H;  // 16 keys so many times make a tile of a wavefront
     const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t seq = seq32;
@@ -452,6 +456,7 @@ template <typename T> int32_t launch_scaled(const ScaledArgs &a, const Plan &pl,
         const bool nt = pl.nt, full = a.c.head_dim == 64 || a.c.head_dim == 128 || a.c.head_dim == 256;
         const bool pages = a.c.page_size % 16 == 0, sixteen = pages && a.sc.block % 16 == 0, four = pages && full && a.sc.block % 4 == 0;
         const bool one = pages && full && a.sc.block == 1 && ((uintptr_t)a.k_scales % 16 | (uintptr_t)a.v_scales % 16 | a.sc.page_stride % 4 | a.sc.head_stride % 4) == 0;
+        // (us for 64 sequences of up to 8191 keys, scales by four and by one / looked up by every lane: blocks of 8 129 / 188, of 4 131 / 188, of 1 130 / 190; of 16 124)
         auto pick = [&](auto even) {
             constexpr bool E = decltype(even)::value;
             auto size = [&](auto dp) {

@@ -1,14 +1,21 @@
 // The next token of each row of logits from a given number: temperature, top-k, top-p, min-p.
 //
 // Tokens are ordered by a code of 64 bits, the complement of the logit's ordered bits above the index: smaller codes come first. Every
-// filter keeps a prefix of that order, so the kept tokens are those up to a last code (and above min-p). Weights are fp64 exponentials; where sums of
-// them are collected by atomics they are whole numbers W = round(2^S w), whose sums do not depend on the order. Two launches:
+// filter keeps a prefix of that order, so the kept tokens are those up to a last code (and above min-p). Weights are fp64 exponentials (which side of a
+// border a sum lies on decides the token); where sums of them are collected by atomics they are whole numbers W = round(2^S w), S = 45 up to 2^17 tokens,
+// whose sums are exact and do not depend on the order: a weight under 2^-46 of the largest counts as none there. Two launches:
 //   * pieces: one wavefront for 2048 logits, which it holds. It finds their maximum; where all of the row count (no top-k) the sum of their
 //     weights relative to that maximum; and where there is a filter it writes down the largest of them, in the order of the vocabulary: at least
 //     `want`, by a bisection of the lanes' maxima, which costs a comparison of one register a step.
 //   * choice: one workgroup for a row. Without a filter the sums of the pieces give the piece, and its logits the token. With one, the
 //     candidates of all pieces are gathered in LDS, and a histogram over max - x and the ranks inside one of its bins find the last code. It holds if no piece
 //     has left out what could lie before it; otherwise the same is done over the whole row.
+//
+// Bound by latency, then by the instructions of the pieces (some 390 vector ones and 350 scalar ones a wavefront beside 32 loads of 4 bytes a lane; six
+// wavefronts a SIMD): 200 rows of 131071, top-k, top-p and min-p, 42.4 us = 25.8 for the pieces (4.1 TB/s) + 17.2 for the choice (eight passes of a radix
+// selection a row, the simplest form, took 1171). Without filters 40 us, as each logit needs an fp64 exponential (32 + 8.6). 64 rows of 50257 17.6 (9.5 + 8.7), 16
+// 10.6, 1 13.6. Slower were: pieces of 1024 logits (twice the candidates), wavefronts that take several pieces with the next one's loads ahead, and
+// bounds of 72 or 64 registers, all three by spills (87, 80 and 90 us for the pieces); the choice by 512 threads 20.9, 256 32.3 us.
 
 #include "devmath.hpp"
 #include "paged.hpp"
@@ -157,7 +164,8 @@ __global__ __launch_bounds__(64 * kWaves) void sample_pieces_kernel(const Sample
             out.sum = wave_sum(sum);
         }
         if (set.filters()) {
-            // How many lanes shall write something down (tokens of a vocabulary in order of frequency have their largest logits side by side),
+            // How many lanes shall write something down (tokens of a vocabulary in order of frequency have their largest logits side by side: 36 at
+            // least, though spread evenly 16 would do; us for 200 x 131071, top-k 50, 16 / 36 / 52 of them: level, 25.4 + 12.8 / 12.8 / 14.8),
             // and what cannot be kept, as far as the piece by itself can tell (no more than a hint: `limit` says what was left out).
             int want = p.want_p;
             float hint = -3.402823466e38f;
@@ -703,7 +711,7 @@ int32_t fth_dev_sample_f32(const fth_sample_desc *d, const float *logits, const 
     a.entries = reinterpret_cast<Entry *>(a.pieces + pieces);
     a.per_row = (int)fth::ceil_div(d->vocab, kPiece);
     a.by_pieces = fth::Divisor((uint32_t)a.per_row);
-    a.want_p = 48;
+    a.want_p = 48;  // (us for 200 x 131071, top-p 0.9, 24 / 48 / 63: 37.3 + 11.4 / 38.2 + 13.9 / 40.9 + 12.5; fewer send more rows to the pass over all)
     int bits = 0;
     while (((int64_t)1 << bits) < d->vocab) ++bits;
     const int s_bits = 62 - bits < 45 ? 62 - bits : 45;

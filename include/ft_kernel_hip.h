@@ -508,8 +508,8 @@ void fth_dev_paged_scales_contiguous(fth_paged_scales *sc, const fth_paged_cache
  * that its tokens one by one would get. What a block holds at and behind the positions written counts as gone: a
  * sequence that is cut back goes on from there, and a token at the first position of a block starts it anew.
  * Tokens of one block stand one after the other in the call, positions ascending by one; one that follows a token of its block
- * without being at the next position is left out and reported like one without a place. Tokens of one block in two places of the list
- * leave that block unspecified (nothing else). */
+ * without being at the next position is left out and reported like one without a place, but for its queries, which are rotated.
+ * Tokens of one block in two places of the list leave that block unspecified (nothing else). */
 int32_t fth_dev_paged_append_scaled_f32(const fth_paged_cache *c, const fth_paged_scales *sc, const fth_paged_append_desc *d, const float *q, const float *k,
                                         const float *v, const float *cosines, const float *sines, const int32_t *block_table, const int32_t *seq_ids,
                                         const int32_t *positions, float *q_out, void *k_cache, void *v_cache, float *k_scales, float *v_scales,
@@ -551,9 +551,10 @@ int32_t fth_dev_logits_process_f32(const fth_logits_desc *d, const float *logits
  * temperature, top_k, top_p and min_p may each be NULL (temperature 1, that filter left out). Logits of -inf are never chosen. A
  * row that holds NaN or +inf or nothing above -inf, or whose settings are out of range (temperature negative or not finite,
  * top_k < 0, top_p or min_p NaN or negative, min_p > 1, uniform outside [0, 1)) gets token -1 and logprob NaN, and bad_index (device, may be NULL)
- * receives the lowest such row, or -1. Exponentials are fp64, since which side of a border a number lies on decides the token, and w
- * counts as a whole multiple of 2^-45 of the largest (2^-44 above 2^17 tokens, a bit less for each doubling): sums are exact, so runs repeat bit for
- * bit, and rows do not depend on each other. The workspace's contents are ignored and overwritten. */
+ * receives the lowest such row, or -1. Exponentials and sums are fp64, since which side of a border a number lies on decides the token; in a
+ * row with a filter w counts as a whole multiple of 2^-45 of the largest (2^-44 above 2^17 tokens, a bit less for each doubling), so what is
+ * below half of that is not drawn there. Runs repeat bit for bit, and rows do not depend on each other. The workspace (an eighth of the
+ * logits' bytes and a little) is overwritten; what it holds before does not matter. At most 2^30 tokens, 2^20 rows and 2^42 logits. */
 typedef struct fth_sample_desc {
     int64_t rows, vocab, logits_stride; /* elements, >= vocab */
 } fth_sample_desc;
