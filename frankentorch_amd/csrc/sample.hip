@@ -12,10 +12,12 @@
 //     has left out what could lie before it; otherwise the same is done over the whole row.
 //
 // Bound by latency, then by the instructions of the pieces (some 390 vector ones and 350 scalar ones a wavefront beside 32 loads of 4 bytes a lane; six
-// wavefronts a SIMD): 200 rows of 131071, top-k, top-p and min-p, 42.4 us = 25.8 for the pieces (4.1 TB/s) + 17.2 for the choice (eight passes of a radix
+// wavefronts a SIMD): 200 rows of 131071, top-k 1000 and top-p 0.98, 42.4 us = 25.8 for the pieces (4.1 TB/s) + 17.2 for the choice (eight passes of a radix
 // selection a row, the simplest form, took 1171). Without filters 40 us, as each logit needs an fp64 exponential (32 + 8.6). 64 rows of 50257 17.6 (9.5 + 8.7), 16
 // 10.6, 1 13.6. Slower were: pieces of 1024 logits (twice the candidates), wavefronts that take several pieces with the next one's loads ahead, and
-// bounds of 72 or 64 registers, all three by spills (87, 80 and 90 us for the pieces); the choice by 512 threads 20.9, 256 32.3 us.
+// bounds of 72 or 64 registers, the last three by spills (87, 80 and 90 us for the pieces); the choice by 512 threads 20.9, 256 32.3 us.
+// Rows that the candidates do not decide (a nucleus of tens of thousands, top-k 20000) are read three times more, by one workgroup: 131071 logits 225 us,
+// 50257 88 to 106 (one logit a thread at a time, all members of a bin ranked: 690 and 137 to 154), most of it fp64 exponentials and atomics in LDS.
 
 #include "devmath.hpp"
 #include "paged.hpp"
@@ -23,7 +25,8 @@
 namespace {
 
 constexpr int kPiece = 2048, kEntries = 128, kWaves = 4;         // logits of a piece, candidates that it may write down, pieces of a workgroup
-constexpr int kThreads = 1024, kBins = 2048, kList = 7168, kFew = 1024;   // the choice: bins, candidates in LDS, members of a bin that are ranked
+constexpr int kThreads = 1024, kBins = 2048, kList = 7168, kRanked = 256;   // the choice: bins, candidates in LDS, members of a bin that are ranked
+constexpr int kAtOnce = 8;  // logits that a thread asks for at once in passes over the row (4 / 8 / 16: 501 / 475 / 473 us before members went digit by digit)
 constexpr int kPlaces = 512, kAhead = 4, kGroups = kPiece / kThreads, kMyBins = kBins / kThreads;                            // pieces of a row whose candidates are listed; of a wavefront, fetched at once
 
 struct Piece {
@@ -244,7 +247,7 @@ struct Shared {
     uint32_t count[kBins];
     Entry list[kList];       // the candidates, in the order of the vocabulary
     uint64_t whole[kList];   // their weights
-    Member few[kFew];
+    Member few[kRanked];     // the members of a bin, or bins of digits, or the sums of ranges
     uint64_t sums[2][32];
     Found finds[2];
     uint32_t places[kPlaces + 1];  // where the candidates of each piece stand in the list
@@ -295,12 +298,16 @@ struct Row {
     }
     // f(logit, token, weight) of every candidate (of the row: of every token that is allowed), by this workgroup's threads.
     template <bool LIST, typename F> __device__ __forceinline__ void each(int n, F f) const {
-        for (int i = threadIdx.x; i < n; i += kThreads) {
-            if constexpr (LIST) {
-                f(s.list[i].x, s.list[i].v, s.whole[i]);
-            } else {
-                const float z = x[i];
-                if (z > -__builtin_inff()) f(z, (uint32_t)i, whole(z));
+        if constexpr (LIST) {
+            for (int i = threadIdx.x; i < n; i += kThreads) f(s.list[i].x, s.list[i].v, s.whole[i]);
+        } else {
+            for (int i = threadIdx.x; i < n; i += kAtOnce * kThreads) {
+                float z[kAtOnce];
+#pragma unroll
+                for (int e = 0; e < kAtOnce; ++e) z[e] = i + e * kThreads < n ? x[i + e * kThreads] : -__builtin_inff();
+#pragma unroll
+                for (int e = 0; e < kAtOnce; ++e)
+                    if (z[e] > -__builtin_inff()) f(z[e], (uint32_t)(i + e * kThreads), whole(z[e]));
             }
         }
     }
@@ -340,7 +347,7 @@ struct Row {
     }
 
     // The smallest code for which the tokens up to it are `k` at least (k > 0) or weigh `need`, by the bins: the bin, then the ranks of its
-    // members; where it has too many (ties) digit by digit. All ones if there is none. *weight: what they weigh. `call`: 0, then 1.
+    // members; where it has too many (ties, wide nuclei) digit by digit. All ones if there is none. *weight: what they weigh. `call`: 0, then 1.
     template <bool LIST> __device__ __forceinline__ uint64_t boundary(int n, const Prefix &at, uint32_t k, uint64_t need, int call, uint64_t *weight) const {
         const int t = threadIdx.x;
         Found &f = s.finds[call];
@@ -363,7 +370,7 @@ struct Row {
         if (bin < 0) return ~0ull;
         uint64_t weighs = f.code, had = f.weight;
         const uint32_t members = s.count[bin];
-        if (members <= kFew) {
+        if (members <= kRanked) {
             each<LIST>(n, [&](float z, uint32_t v, uint64_t w) {
                 if (bin_of(z) == bin) s.few[atomicAdd(&f.members, 1u)] = Member{code_of(z, v), w};
             });
@@ -388,13 +395,29 @@ struct Row {
             *weight = f.weight;
             return f.code;
         }
-        // (the bins of digits stand where the members would)
+        // Digit by digit (the bins of digits stand where the members would); of the row the members alone, if the list has room for them.
+        if constexpr (!LIST) {
+            if (members <= kList) {
+                each<false>(n, [&](float z, uint32_t v, uint64_t w) {
+                    if (bin_of(z) != bin) return;
+                    const uint32_t at_member = atomicAdd(&f.members, 1u);
+                    s.list[at_member] = Entry{z, v};
+                    s.whole[at_member] = w;
+                });
+                return digits<true>((int)members, bin, k != 0, goal, had, weighs, f, weight);
+            }
+        }
+        return digits<LIST>(n, bin, k != 0, goal, had, weighs, f, weight);
+    }
+    // Among the candidates in `bin`, before which there are `had` (tokens, or their weights) and the weights `weighs`.
+    template <bool LIST> __device__ __forceinline__ uint64_t digits(int n, int bin, bool counts, uint64_t goal, uint64_t had, uint64_t weighs, Found &f, uint64_t *weight) const {
+        static_assert(kRanked >= 192, "256 weights and 256 counts");
         uint64_t *digit_weight = &s.few[0].code;
-        uint32_t *digit_count = reinterpret_cast<uint32_t *>(&s.few[kFew / 2]);
+        uint32_t *digit_count = reinterpret_cast<uint32_t *>(&s.few[128]);
         uint64_t prefix = 0;
         for (int shift = 56; shift >= 0; shift -= 8) {
             __syncthreads();
-            for (int d = t; d < 256; d += kThreads) {
+            for (int d = threadIdx.x; d < 256; d += kThreads) {
                 digit_weight[d] = 0;
                 digit_count[d] = 0;
             }
@@ -407,18 +430,35 @@ struct Row {
                 atomicAdd(reinterpret_cast<unsigned long long *>(&digit_weight[at_digit]), (unsigned long long)w);
             });
             __syncthreads();
-            if (t == 0) {
-                int d = 0;
-                for (;; ++d) {
-                    const uint64_t here = k ? digit_count[d] : digit_weight[d];
-                    if (had + here >= goal || d == 255) break;
-                    had += here;
-                    weighs += digit_weight[d];
+            if (threadIdx.x < 64) {  // four digits a lane
+                const int lane = threadIdx.x;
+                uint64_t here[4], heavy[4], all = 0, all_heavy = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    heavy[e] = digit_weight[4 * lane + e];
+                    here[e] = counts ? digit_count[4 * lane + e] : heavy[e];
+                    all += here[e];
+                    all_heavy += heavy[e];
                 }
-                f.code = prefix << 8 | d;
-                f.weight = had;
-                s.sums[0][0] = weighs + digit_weight[d];
-                s.sums[0][1] = weighs;
+                const uint64_t upto = wave_scan(all, (uint64_t)0, AddOp()), upto_heavy = wave_scan(all_heavy, (uint64_t)0, AddOp());
+                const uint64_t over = __ballot(had + upto >= goal);
+                if (lane == (over ? __builtin_ctzll(over) : 63)) {
+                    uint64_t before = had + upto - all, before_heavy = weighs + upto_heavy - all_heavy;
+                    bool found = false;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (found) continue;
+                        if (before + here[e] >= goal || e == 3) {
+                            f.code = prefix << 8 | (uint32_t)(4 * lane + e);
+                            f.weight = before;
+                            s.sums[0][0] = before_heavy + heavy[e];
+                            s.sums[0][1] = before_heavy;
+                            found = true;
+                        }
+                        before += here[e];
+                        before_heavy += heavy[e];
+                    }
+                }
             }
             __syncthreads();
             prefix = f.code;
@@ -486,9 +526,8 @@ struct Row {
     __device__ __forceinline__ void draw_row(int n, uint64_t last) const {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, length = ((n + 255) / 256 + 63) & ~63;
         uint64_t *ranges = &s.few[0].code;
-        auto kept = [&](int64_t i) -> uint64_t {
-            if (i >= n) return 0;
-            const float z = x[i];
+        auto logit = [&](int64_t i) { return i < n ? x[i] : -__builtin_inff(); };
+        auto kept = [&](int64_t i, float z) -> uint64_t {
             if (!(z > -__builtin_inff()) || code_of(z, (uint32_t)i) > last) return 0;
             double w;
             const uint64_t all = whole(z, &w);
@@ -497,8 +536,15 @@ struct Row {
         __syncthreads();
         for (int g = wave; g < 256; g += kThreads / 64) {
             uint64_t sum = 0;
-            if (g * (int64_t)length < n)
-                for (int i = lane; i < length; i += 64) sum += kept((int64_t)g * length + i);
+            const int64_t end = (g + 1) * (int64_t)length;
+            if (end - length < n)
+                for (int64_t i = end - length + lane; i < end; i += kAtOnce * 64) {
+                    float z[kAtOnce];
+#pragma unroll
+                    for (int e = 0; e < kAtOnce; ++e) z[e] = i + 64 * e < end ? logit(i + 64 * e) : -__builtin_inff();
+#pragma unroll
+                    for (int e = 0; e < kAtOnce; ++e) sum += kept(i + 64 * e, z[e]);
+                }
             sum = wave_sum(sum);
             if (lane == 0) ranges[g] = sum;
         }
@@ -518,8 +564,9 @@ struct Row {
         uint64_t left = s.finds[0].code;
         const int g = s.finds[0].at;
         for (int i0 = 0; i0 < length; i0 += 64) {
-            const uint64_t here = i0 + lane < length ? kept((int64_t)g * length + i0 + lane) : 0, upto = wave_scan(here, (uint64_t)0, AddOp());
-            if (here > 0 && upto > left && upto - here <= left) write(g * length + i0 + lane, (double)here / (double)total);
+            const int64_t i = (int64_t)g * length + i0 + lane;
+            const uint64_t here = kept(i, logit(i)), upto = wave_scan(here, (uint64_t)0, AddOp());
+            if (here > 0 && upto > left && upto - here <= left) write((int)i, (double)here / (double)total);
             const uint64_t all = lane_value(upto, 63);
             if (all > left) return;
             left -= all;
