@@ -179,7 +179,7 @@ template <typename T> __global__ __launch_bounds__(64) void append_scaled_kernel
     }
     for (int64_t x = lane; x < (int64_t)run.tokens * hd; x += 64) {
         const int i = (int)(x / hd), c = (int)(x % hd);
-        store(run.row + i, c, element(i, c) * per);
+        store(run.row + i, c, now == now ? element(i, c) * per : 0.f);
     }
 }
 
