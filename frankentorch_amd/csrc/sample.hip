@@ -11,11 +11,11 @@
 //     candidates of all pieces are gathered in LDS, and a histogram over max - x and the ranks inside one of its bins find the last code. It holds if no piece
 //     has left out what could lie before it; otherwise the same is done over the whole row.
 //
-// Bound by latency, then by the instructions of the pieces (some 390 vector ones and 350 scalar ones a wavefront beside 32 loads of 4 bytes a lane; six
-// wavefronts a SIMD): 200 rows of 131071, top-k 1000 and top-p 0.98, 42.4 us = 25.8 for the pieces (4.1 TB/s) + 17.2 for the choice (eight passes of a radix
-// selection a row, the simplest form, took 1171). Without filters 40 us, as each logit needs an fp64 exponential (32 + 8.6). 64 rows of 50257 17.6 (9.5 + 8.7), 16
-// 10.6, 1 13.6. Slower were: pieces of 1024 logits (twice the candidates), wavefronts that take several pieces with the next one's loads ahead, and
-// bounds of 72 or 64 registers, the last three by spills (87, 80 and 90 us for the pieces); the choice by 512 threads 20.9, 256 32.3 us.
+// Bound by latency, then by reading: 200 rows of 131071, top-k 1000 and top-p 0.98, 40.3 us = 23.8 for the pieces (4.4 TB/s; reading and the maxima
+// alone 19.8) + 17.1 for the choice (eight passes of a radix selection a row, the simplest form, took 1171). Without filters 40 us, as each logit needs an fp64
+// exponential (31 + 8.3). 64 rows of 50257 17.5 (9.5 + 8.7: 4.4 for reading, 3 for exponentials, 2.4 for the candidates), 16 10.6, 1 13.4. Slower were: pieces of 1024 logits (twice the
+// candidates), wavefronts that take several pieces with the next one's loads ahead and bounds of 72 or 64 registers, the last three by spills (87, 80 and
+// 90 us for the pieces); candidates straight to memory, a branch each (25.9). Level: eight wavefronts a SIMD instead of six. The choice by 512 threads 20.9, 256 32.3 us.
 // Rows that the candidates do not decide (a nucleus of tens of thousands, top-k 20000) are read three times more, by one workgroup: 131071 logits 225 us,
 // 50257 88 to 106 (one logit a thread at a time, all members of a bin ranked: 690 and 137 to 154), most of it fp64 exponentials and atomics in LDS.
 
@@ -122,6 +122,7 @@ __device__ __forceinline__ float wave_max(float x) { return lane_value(wave_scan
 // ---- pieces -----------------------------------------------------------------------------------------------------------------
 
 __global__ __launch_bounds__(64 * kWaves) void sample_pieces_kernel(const SampleArgs p) {
+    __shared__ Entry found[kWaves][kEntries + 64];  // of each wavefront, and a place for each lane that has none to write
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int piece32 = (int)blockIdx.x * kWaves + wave, row32 = (int)p.by_pieces((uint32_t)piece32);
     const int64_t piece = piece32, r = row32;
@@ -168,7 +169,7 @@ __global__ __launch_bounds__(64 * kWaves) void sample_pieces_kernel(const Sample
         }
         if (set.filters()) {
             // How many lanes shall write something down (tokens of a vocabulary in order of frequency have their largest logits side by side: 36 at
-            // least, though spread evenly 16 would do; us for 200 x 131071, top-k 50, 16 / 36 / 52 of them: level, 25.4 + 12.8 / 12.8 / 14.8),
+            // least, though spread evenly 16 would do; us for 200 x 131071, top-k 50, 16 / 36 / 52 of them: the choice 12.8 / 12.8 / 14.8),
             // and what cannot be kept, as far as the piece by itself can tell (no more than a hint: `limit` says what was left out).
             int want = p.want_p;
             float hint = -3.402823466e38f;
@@ -181,7 +182,6 @@ __global__ __launch_bounds__(64 * kWaves) void sample_pieces_kernel(const Sample
                 if (far > 0.f) hint = fmaxf(hint, out.max + __builtin_amdgcn_logf(far) / (float)set.rate);
             }
             const uint32_t key = order_of(mine);
-            Entry *to = p.entries + piece * kEntries;
             // Written down is what reaches `least`: all that the hint leaves, if few lanes have any of it; else what reaches the number of 16 bits that
             // `want` lanes reach, or fewer lanes where that would be too much.
             float least = hint;
@@ -189,7 +189,8 @@ __global__ __launch_bounds__(64 * kWaves) void sample_pieces_kernel(const Sample
             bool first = __popcll(__ballot(mine >= least)) > want;
             for (;;) {
                 if (!first) {
-                    uint32_t at = 0;
+                    uint32_t at = 0, v = (uint32_t)v0 + 4 * lane;
+                    asm volatile("" : "+v"(v));  // (32 token numbers need not stay in registers from here on)
 #pragma unroll
                     for (int s = 0; s < kVecs; ++s) {
                         uint32_t before = at;
@@ -202,12 +203,21 @@ __global__ __launch_bounds__(64 * kWaves) void sample_pieces_kernel(const Sample
                         }
                         if (at > kEntries) continue;  // too many: once more with fewer
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (z[s][e] >= least) to[before++] = Entry{z[s][e], (uint32_t)(v0 + 256 * s + 4 * lane + e)};
+                        for (int e = 0; e < 4; ++e) {
+                            const bool mine = z[s][e] >= least;
+                            Entry &to = found[wave][mine ? before : kEntries + lane];
+                            to.x = z[s][e];
+                            to.v = v + 256 * s + e;
+                            before += mine;
+                        }
                         __builtin_amdgcn_sched_barrier(0);  // for the registers' sake
                     }
                     if (at <= kEntries) {
                         out.count = at;
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+                        for (int h = 0; h < kEntries / 64; ++h)
+                            if (64 * h + lane < (int)at) p.entries[piece * kEntries + 64 * h + lane] = found[wave][64 * h + lane];
                         break;
                     }
                     if (want == 0) {
@@ -758,7 +768,7 @@ int32_t fth_dev_sample_f32(const fth_sample_desc *d, const float *logits, const 
     a.entries = reinterpret_cast<Entry *>(a.pieces + pieces);
     a.per_row = (int)fth::ceil_div(d->vocab, kPiece);
     a.by_pieces = fth::Divisor((uint32_t)a.per_row);
-    a.want_p = 48;  // (us for 200 x 131071, top-p 0.9, 24 / 48 / 63: 37.3 + 11.4 / 38.2 + 13.9 / 40.9 + 12.5; fewer send more rows to the pass over all)
+    a.want_p = 48;  // (us for 200 x 131071, top-p 0.9, 24 / 48 / 63: 37.3 + 11.4 / 38.2 + 13.9 / 40.9 + 12.5 in all; fewer send more rows to the pass over all)
     int bits = 0;
     while (((int64_t)1 << bits) < d->vocab) ++bits;
     const int s_bits = 62 - bits < 45 ? 62 - bits : 45;
