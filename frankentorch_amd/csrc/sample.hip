@@ -19,6 +19,8 @@
 // Rows that the candidates do not decide (a nucleus of tens of thousands, top-k 20000) are read three times more, by one workgroup: 131071 logits 225 us,
 // 50257 88 to 106 (one logit a thread at a time, all members of a bin ranked: 690 and 137 to 154), most of it fp64 exponentials and atomics in LDS.
 
+#include <type_traits>
+
 #include "devmath.hpp"
 #include "paged.hpp"
 
@@ -116,6 +118,17 @@ template <typename T, typename F> __device__ __forceinline__ T wave_scan(T x, T 
 }
 struct MaxOp { template <typename T> __device__ T operator()(T a, T b) const { return a > b ? a : b; } };
 struct AddOp { template <typename T> __device__ T operator()(T a, T b) const { return a + b; } };
+// The sum over 4 or 16 neighbouring lanes, in each of them: pairs and pairs of pairs of a quad, then mirror images.
+template <int N, typename T> __device__ __forceinline__ T neighbours_sum(T x) {
+    static_assert(N == 4 || N == 16, "a quad or a row");
+    x += moved<0xb1, 0xf>(x, x);
+    x += moved<0x4e, 0xf>(x, x);
+    if constexpr (N == 16) {
+        x += moved<0x141, 0xf>(x, x);
+        x += moved<0x140, 0xf>(x, x);
+    }
+    return x;
+}
 template <typename T> __device__ __forceinline__ T wave_sum(T x) { return lane_value(wave_scan(x, (T)0, AddOp()), 63); }
 __device__ __forceinline__ float wave_max(float x) { return lane_value(wave_scan(x, -__builtin_inff(), MaxOp()), 63); }
 
@@ -271,17 +284,27 @@ template <typename T, typename F> __device__ __forceinline__ T row_scan(T x, T n
     return op(moved<0x118, 0xf>(neutral, x), x);
 }
 // The sum over the threads before this one, and over all. One barrier before `lds` is written, one after.
-template <typename T> __device__ __forceinline__ T block_scan(T x, T *lds, T *all) {
-    constexpr int W = kThreads / 64;
+template <typename T> struct BlockScan {
+    static constexpr int W = kThreads / 64;
     static_assert(W == 16, "the wavefronts' sums are a row of lanes");
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const T upto = wave_scan(x, (T)0, AddOp());
+    T x, upto, *lds;
+    int wave;
+    __device__ __forceinline__ BlockScan(T x, T *lds) : x(x), upto(wave_scan(x, (T)0, AddOp())), lds(lds), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {}
+    __device__ __forceinline__ void write() const {
+        if ((threadIdx.x & 63) == 63) lds[wave] = upto;
+    }
+    __device__ __forceinline__ T read(T *all) const {
+        const T t = row_scan(lds[threadIdx.x & (W - 1)], (T)0, AddOp());
+        *all = lane_value(t, W - 1);
+        return upto - x + (wave ? lane_value(t, wave ? wave - 1 : 0) : (T)0);
+    }
+};
+template <typename T> __device__ __forceinline__ T block_scan(T x, T *lds, T *all) {
+    const BlockScan<T> scan(x, lds);
     __syncthreads();
-    if (lane == 63) lds[wave] = upto;
+    scan.write();
     __syncthreads();
-    const T t = row_scan(lds[lane & (W - 1)], (T)0, AddOp());
-    *all = lane_value(t, W - 1);
-    return upto - x + (wave ? lane_value(t, wave ? wave - 1 : 0) : (T)0);
+    return scan.read(all);
 }
 
 struct Row {
@@ -351,6 +374,15 @@ struct Row {
             at.weight += s.weight[kMyBins * threadIdx.x + b];
         }
         uint32_t unused;
+        if (counts && weights) {  // between the same barriers
+            const BlockScan<uint32_t> count(at.count, reinterpret_cast<uint32_t *>(s.sums[1]));
+            const BlockScan<uint64_t> weight(at.weight, s.sums[0]);
+            __syncthreads();
+            count.write();
+            weight.write();
+            __syncthreads();
+            return Prefix{count.read(&unused), weight.read(all)};
+        }
         if (counts) at.count = block_scan(at.count, reinterpret_cast<uint32_t *>(s.sums[1]), &unused);
         if (weights) at.weight = block_scan(at.weight, s.sums[0], all);
         return at;
@@ -385,22 +417,34 @@ struct Row {
                 if (bin_of(z) == bin) s.few[atomicAdd(&f.members, 1u)] = Member{code_of(z, v), w};
             });
             __syncthreads();
-            for (int m = t; m < (int)members; m += kThreads) {  // ranks: in whatever order the members stand
+            // ranks, in whatever order the members stand: PARTS neighbouring threads for one
+            auto rank = [&](auto parts) {
+                constexpr int PARTS = decltype(parts)::value;
+                const int m = t / PARTS;
+                if (m >= (int)members) return;
                 const Member mine = s.few[m];
-                uint64_t count = 0, sum = 0;
+                uint32_t count = 0;
+                uint64_t sum = 0;
 #pragma unroll 4
-                for (uint32_t i = 0; i < members; ++i) {
+                for (uint32_t i = t % PARTS; i < members; i += PARTS) {
                     const Member other = s.few[i];
                     const bool before = other.code < mine.code;
                     count += before;
                     sum += before ? other.weight : 0;
                 }
+                if constexpr (PARTS > 1) {
+                    count = neighbours_sum<PARTS>(count);
+                    sum = neighbours_sum<PARTS>(sum);
+                }
                 const uint64_t upto = had + (k ? count : sum), here = k ? 1 : mine.weight;
-                if (upto < goal && upto + here >= goal) {
+                if (t % PARTS == 0 && upto < goal && upto + here >= goal) {
                     f.code = mine.code;
                     f.weight = weighs + sum + mine.weight;
                 }
-            }
+            };
+            if (members <= 16) rank(std::integral_constant<int, 1>());
+            else if (members <= kThreads / 16) rank(std::integral_constant<int, 16>());
+            else rank(std::integral_constant<int, kThreads / kRanked>());
             __syncthreads();
             *weight = f.weight;
             return f.code;
