@@ -276,8 +276,8 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
             qp[1][i][e] = (_Float16)(x - (float)qp[0][i][e]);
         }
 
-    F4 o[NE];
-    float m_run, l_run;  // the sum: this lane's keys only
+    F4 o[NE], before[NE];          // of the last tiles; of those before them
+    float m_run, l_run, l_before;  // likewise the sums of the weights, of this lane's keys only
     const int limit = sees < key_hi ? sees : key_hi;
 
     // One tile. `more` (a constant): another one of this wavefront follows, whose loads go out on the way (what a query
@@ -337,22 +337,27 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
             const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -__builtin_inff() ? 0.f : m_new));
             m_run = m_new;
             l_run *= alpha;
+            l_before *= alpha;
 #pragma unroll
             for (int e = 0; e < NE; ++e)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) o[e][r] *= alpha;
+                for (int r = 0; r < 4; ++r) {
+                    o[e][r] *= alpha;
+                    before[e][r] *= alpha;
+                }
         }
         // nothing visible so far: every weight is exp(-inf) = 0; a key that is not seen has weight 0 whatever its scale is
         const float ref = m_run == -__builtin_inff() ? 0.f : m_run;
-        float w[H][4];
+        float w[H][4], l_tile = 0.f;
 #pragma unroll
         for (int s = 0; s < H; ++s)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float e = __builtin_amdgcn_exp2f(sc[s][r] - ref);
-                l_run += e;
+                l_tile += e;
                 w[s][r] = more || key0 + 16 * s + 4 * g + r < limit ? e * (vs[s][NS == 1 ? 0 : r] * unit) : 0.f;
             }
+        l_run += l_tile;
         // A NaN code under a weight of 0 would be NaN: what lies past the keys counts as zero, and so does, in keys that only the later of the new
         // tokens see, a NaN, which is added below to the rows that see it.
         const int partly = len - new_tokens + 1;
@@ -410,22 +415,35 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
         }
         if constexpr (more) {
             load_v(next);
+            // Every eighth tile the sums begin anew: a sum over tens of thousands of keys that a few outweigh drops the others' last bits all to one
+            // side (28000 keys in one share: sums of weights were off by up to 200 units of 2^-24), and those of the matrix units err to one side too.
+            if ((j & (8 * H - 1)) == 7 * H) {
+#pragma unroll
+                for (int e = 0; e < NE; ++e) {
+                    before[e] += o[e];
+                    o[e] = F4{0.f, 0.f, 0.f, 0.f};
+                }
+                l_before += l_run;
+                l_run = 0.f;
+            }
         }
     };
     for (float unit = 0x1p40f;; unit = 0x1p-24f) {
         m_run = -__builtin_inff();
-        l_run = 0.f;
+        l_run = l_before = 0.f;
 #pragma unroll
-        for (int e = 0; e < NE; ++e) o[e] = F4{0.f, 0.f, 0.f, 0.f};
+        for (int e = 0; e < NE; ++e) o[e] = before[e] = F4{0.f, 0.f, 0.f, 0.f};
         if (wave >= tiles) break;
         int t = wave;
         for (; t + kWaves < tiles; t += kWaves) step(t, unit, std::true_type());
         step(t, unit, std::false_type());
+        l_run += l_before;
         float check = 0.f;
 #pragma unroll
         for (int e = 0; e < NE; ++e)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
+                o[e][r] += before[e][r];
                 check = __builtin_fmaf(o[e][r], 0.f, check);
                 o[e][r] *= unit > 1.f ? 0x1p-40f : 0x1p24f;
             }

@@ -253,3 +253,21 @@ def test_large_batches_in_even_shares(hip):
                 x = k @ q[s, 0, h].astype(np.float64) * float(np.float32(0.02))
                 w = np.exp(x - x.max())
                 assert rel_err(got[s, 0, h], (w[:, None] * v).sum(0) / w.sum()) <= TOL_GEMM_F32
+
+
+@pytest.mark.parametrize("dtype", ["i8", "e4m3"])
+def test_one_key_above_tens_of_thousands(hip, dtype):
+    """130 heads take one share each: 20000 keys of one weight, 9 to 14 nats below the first, under values of one are one. Sums of weights go over
+    8 keys of a tile, 8 tiles, 20 such groups, 16 lanes and 4 wavefronts: at most 7 + 8 + 20 + 5 roundings of 2^-24 of a sum of positive numbers; the
+    products' over 3 x 8 steps of the matrix units, counted twice, 20 groups and 4 wavefronts."""
+    n, heads, d = 20000, 130, 64
+    p = Scaled(22, 1, heads, d, 64, 64, dtype, -(-n // 64))
+    one = 1 if dtype == "i8" else 0x38
+    p.codes = [np.zeros_like(p.codes[0]), np.full_like(p.codes[1], one)]
+    p.scales = [np.ones_like(x) for x in p.scales]
+    for h in range(heads):
+        at = p.row_at(0, 0, h)
+        p.codes[0][at:at + d] = one
+    q = np.repeat(np.linspace(9.0, 14.0, heads, dtype=np.float32)[None, None, :, None] / d, d, axis=3)
+    got = run(hip, p, q, 1.0, [n])
+    assert np.max(np.abs(got.astype(np.float64) - 1)) <= (40 + 48 + 24) * 2.0 ** -24
