@@ -13,7 +13,7 @@
 // e4m3 becomes either type two at a time by one instruction of gfx950; whole numbers become f16 by the bits of 1024 + 128 + x, bf16 through fp32.
 //
 // Measured: 64 sequences of 1024 to 8191 keys, 32 query heads on 8 of 128, e4m3, blocks of 16 (614 MB): 111 us, 5.6 TB/s (one wavefront a row 3660;
-// a bf16 cache of the same keys, 1.22 GB, 193). One sequence of 131071: 53 us (5.1 TB/s). 16 of up to 3967, four queries, i8: 27. Bound by the loads, of which the
+// a bf16 cache of the same keys, 1.22 GB, 193). One sequence of 131071: 53 us (5.1 TB/s). 16 of up to 3967, four queries, i8: 27.6. Bound by the loads, of which the
 // two workgroups of a compute unit keep too few bytes on the way: the loop without its products takes 110 / 49 / 26 us. Of two workgroups with equal
 // shares the older one ends at 82 us, the younger at 105; lengthening the shares of the older by 6 to 25 % was level, and so were three workgroups a
 // compute unit, tiles of 64 keys, raised wavefront priorities, and twice or four times as many shares (one sequence: 57 / 58 / 60).

@@ -11,11 +11,11 @@
 //     candidates of all pieces are gathered in LDS, and a histogram over max - x and the ranks inside one of its bins find the last code. It holds if no piece
 //     has left out what could lie before it; otherwise the same is done over the whole row.
 //
-// Bound by latency, then by reading: 200 rows of 131071, top-k 1000 and top-p 0.98, 40.3 us = 23.8 for the pieces (4.4 TB/s; reading and the maxima
-// alone 19.8) + 17.1 for the choice (eight passes of a radix selection a row, the simplest form, took 1171). Without filters 40 us, as each logit needs an fp64
-// exponential (31 + 8.3). 64 rows of 50257 17.5 (9.5 + 8.7: 4.4 for reading, 3 for exponentials, 2.4 for the candidates), 16 10.6, 1 13.4. Slower were: pieces of 1024 logits (twice the
+// Bound by latency, then by reading: 200 rows of 131071, top-k 1000 and top-p 0.98, 38.8 us = 23.6 for the pieces (4.4 TB/s; reading and the maxima
+// alone 19.8) + 15.7 for the choice (eight passes of a radix selection a row, the simplest form, took 1171). Without filters 40 us, as each logit needs an fp64
+// exponential (31 + 8.3). 64 rows of 50257 17.4 (9.4 + 8.7: 4.4 for reading, 3 for exponentials, 2.4 for the candidates), 16 10.6, 1 13.3. Slower were: pieces of 1024 logits (twice the
 // candidates), wavefronts that take several pieces with the next one's loads ahead and bounds of 72 or 64 registers, the last three by spills (87, 80 and
-// 90 us for the pieces); candidates straight to memory, a branch each (25.9). Level: eight wavefronts a SIMD instead of six. The choice by 512 threads 20.9, 256 32.3 us.
+// 90 us for the pieces); candidates straight to memory, a branch each (25.9); one thread to rank each member of a bin (the choice 17.1). Level: eight wavefronts a SIMD instead of six. The choice by 512 threads 20.9, 256 32.3 us.
 // Rows that the candidates do not decide (a nucleus of tens of thousands, top-k 20000) are read three times more, by one workgroup: 131071 logits 225 us,
 // 50257 88 to 106 (one logit a thread at a time, all members of a bin ranked: 690 and 137 to 154), most of it fp64 exponentials and atomics in LDS.
 
