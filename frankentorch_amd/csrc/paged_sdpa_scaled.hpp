@@ -85,7 +85,8 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
     constexpr int NK = DP / 64;   // 128-bit loads of a lane's quarter of a K row
     constexpr int NE = DP / 16;   // output columns of a lane, consecutive ones
     constexpr int NV = NE / 4;    // words of its part of a V row
-    constexpr int NS = SIXTEEN || FOUR ? 1 : 4;
+    constexpr int NS = SIXTEEN || FOUR ? 1 : 4;  // scales of a lane's four keys
+    constexpr int NL = ANY ? 1 : NS;             // as they are loaded: ANY has that of this lane's row
     constexpr int H = 2, kKeys = 16 * H;  // 16 keys so many times make a tile of a wavefront
     const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -176,19 +177,17 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
     };
     U4 kf[H][NK];
     uint32_t vf[H][4][NV];
-    float ks[H][NS], vs[H][NS];  // of 16 keys, of this lane's keys 4 g .. 4 g + 3, or of each of them
+    float ks[H][NL], vs[H][NL];  // of 16 keys, of this lane's keys 4 g .. 4 g + 3, or of each of them
     const uint32_t k_lane = (uint32_t)((ANY ? 0 : lr * rs) + g * 16);
     uint32_t v_lane[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) v_lane[r] = (uint32_t)((ANY ? 0 : (4 * g + r) * rs) + lr * NE);
-    auto load_scales = [&](float (&s)[H][NS], const float *from, const Place (&at)[H]) __attribute__((always_inline)) {
+    auto load_scales = [&](float (&s)[H][NL], const float *from, const Place (&at)[H]) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < H; ++h) {
             if constexpr (SIXTEEN) {  // in the lanes, see above
             } else if constexpr (ANY) {
-                const float of_row = from[at[h].page + p.by_block((uint32_t)at[h].in_page)];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) s[h][r] = __shfl(of_row, 4 * g + r);
+                s[h][0] = from[at[h].page + p.by_block((uint32_t)at[h].in_page)];  // (handed round where it is used: it is on its way until then)
             } else if constexpr (FOUR) {
                 s[h][0] = from[at[h].page + p.by_block((uint32_t)(at[h].in_page + 4 * g))];
             } else {
@@ -305,7 +304,7 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
                     ks[s][r] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_ks), (j + s) & 63));
                     vs[s][r] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_vs), (j + s) & 63));
                 }
-                by[s][r] = (ks[s][r] * down) * p.scale2;
+                by[s][r] = ((ANY ? __shfl(ks[s][0], 4 * g + r) : ks[s][r % NL]) * down) * p.scale2;
             }
         Place next[H];
         if constexpr (more) {
@@ -355,7 +354,8 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
             for (int r = 0; r < 4; ++r) {
                 const float e = __builtin_amdgcn_exp2f(sc[s][r] - ref);
                 l_tile += e;
-                w[s][r] = more || key0 + 16 * s + 4 * g + r < limit ? e * (vs[s][NS == 1 ? 0 : r] * unit) : 0.f;
+                const float v_scale = ANY ? __shfl(vs[s][0], 4 * g + r) : vs[s][NS == 1 ? 0 : r % NL];
+                w[s][r] = more || key0 + 16 * s + 4 * g + r < limit ? e * (v_scale * unit) : 0.f;
             }
         l_run += l_tile;
         // A NaN code under a weight of 0 would be NaN: what lies past the keys counts as zero, and so does, in keys that only the later of the new
