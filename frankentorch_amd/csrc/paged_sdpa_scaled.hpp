@@ -474,7 +474,7 @@ template <typename T> int32_t launch_scaled(const ScaledArgs &a, const Plan &pl,
         const bool nt = pl.nt, full = a.c.head_dim == 64 || a.c.head_dim == 128 || a.c.head_dim == 256;
         const bool pages = a.c.page_size % 16 == 0, sixteen = pages && a.sc.block % 16 == 0, four = pages && full && a.sc.block % 4 == 0;
         const bool one = pages && full && a.sc.block == 1 && ((uintptr_t)a.k_scales % 16 | (uintptr_t)a.v_scales % 16 | a.sc.page_stride % 4 | a.sc.head_stride % 4) == 0;
-        // (us for 64 sequences of up to 8191 keys, scales by four and by one / looked up by every lane: blocks of 8 129 / 188, of 4 131 / 188, of 1 130 / 190; of 16 124)
+        // (us for 64 sequences of up to 8191 keys, scales by four and by one / looked up by every lane: blocks of 8 133 / 164, of 4 136 / 163, of 1 136 / 166; of 16 128)
         auto pick = [&](auto even) {
             constexpr bool E = decltype(even)::value;
             auto size = [&](auto dp) {
