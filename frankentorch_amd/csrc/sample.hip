@@ -199,6 +199,7 @@ __global__ __launch_bounds__(64 * kWaves) void sample_pieces_kernel(const Sample
             // `want` lanes reach, or fewer lanes where that would be too much.
             float least = hint;
             if (least > -3.402823466e38f) out.limit = least;
+            int tries = 0;
             bool first = __popcll(__ballot(mine >= least)) > want;
             for (;;) {
                 if (!first) {
@@ -248,7 +249,7 @@ __global__ __launch_bounds__(64 * kWaves) void sample_pieces_kernel(const Sample
                 const uint32_t end = c << 16 | 0xffffu;  // the order of `least`
                 const float reached = __uint_as_float((end & 0x80000000u) ? end : end ^ 0x7fffffffu);
                 if (reached > least) least = out.limit = reached;  // (else fewer lanes than that have anything)
-                want >>= 1;
+                want = tries++ < 3 ? want - want / 8 : want >> 1;  // (the first time it goes down after too many; ties would go down far)
             }
         }
     }
