@@ -629,7 +629,7 @@ struct Row {
     }
 
     // Without a filter: the token that `left` of the weight before it leads to, in piece `at`. Where rounding leads past the piece's end, its
-    // last. Each wavefront has two groups of 64 neighbouring tokens.
+    // last. The piece has weight: its largest token is above 2^-1000 of the row's. Each wavefront has two groups of 64 neighbouring tokens.
     __device__ __forceinline__ void draw_piece(int at, double left, double total) const {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int64_t v0 = (int64_t)at * kPiece + kGroups * 64 * wave;
@@ -646,7 +646,6 @@ struct Row {
         static_assert(kPiece == 64 * kGroups * (kThreads / 64) && kPiece / 64 <= 64, "a lane for each group");
         const double here = lane < kPiece / 64 ? sums[lane] : 0.0, through = wave_scan(here, 0.0, AddOp());
         const uint64_t over = __ballot(here > 0.0 && through > left), some = __ballot(here > 0.0);
-        if (!some) return;
         const int group = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
         if (group / kGroups != wave) return;
         left -= lane_value(through - here, group);
@@ -715,9 +714,11 @@ __global__ __launch_bounds__(kThreads) void sample_choice_kernel(const SampleArg
         int at = from, last = from;
         double left = target - (upto - mine);
         for (; at < to; ++at) {
-            const double here = sum_of(at);
-            if (here > left) break;
-            if (here > 0.0) last = at;
+            const double here = sum_of(at);  // (`left` may be just below 0 by the scan's rounding: a piece without weight is never it)
+            if (here > 0.0) {
+                if (here > left) break;
+                last = at;
+            }
             left -= here;
         }
         if (at == to) {
