@@ -3,7 +3,8 @@
 // Tokens are ordered by a code of 64 bits, the complement of the logit's ordered bits above the index: smaller codes come first. Every
 // filter keeps a prefix of that order, so the kept tokens are those up to a last code (and above min-p). Weights are fp64 exponentials (which side of a
 // border a sum lies on decides the token); where sums of them are collected by atomics they are whole numbers W = round(2^S w), S = 45 up to 2^17 tokens,
-// whose sums are exact and do not depend on the order: a weight under 2^-46 of the largest counts as none there. Two launches:
+// whose sums are exact and do not depend on the order: a weight under 2^-46 of the largest counts as none there. That
+// is so where the border of top-p is looked for; the token is drawn with the fp64 weights, summed in a fixed order. Two launches:
 //   * pieces: one wavefront for 2048 logits, which it holds. It finds their maximum; where all of the row count (no top-k) the sum of their
 //     weights relative to that maximum; and where there is a filter it writes down the largest of them, in the order of the vocabulary: at least
 //     `want`, by a bisection of the lanes' maxima, which costs a comparison of one register a step.
@@ -270,7 +271,7 @@ struct Shared {
     uint64_t weight[kBins];  // of the bins
     uint32_t count[kBins];
     Entry list[kList];       // the candidates, in the order of the vocabulary
-    uint64_t whole[kList];   // their weights
+    double weigh[kList];     // their weights
     Member few[kRanked];     // the members of a bin, or bins of digits, or the sums of ranges
     uint64_t sums[2][32];
     Found finds[2];
@@ -299,6 +300,11 @@ template <typename T> struct BlockScan {
         *all = lane_value(t, W - 1);
         return upto - x + (wave ? lane_value(t, wave ? wave - 1 : 0) : (T)0);
     }
+    __device__ __forceinline__ T read_upto(T *all) const {  // with this thread's
+        const T t = row_scan(lds[threadIdx.x & (W - 1)], (T)0, AddOp());
+        *all = lane_value(t, W - 1);
+        return upto + (wave ? lane_value(t, wave ? wave - 1 : 0) : (T)0);
+    }
 };
 template <typename T> __device__ __forceinline__ T block_scan(T x, T *lds, T *all) {
     const BlockScan<T> scan(x, lds);
@@ -317,13 +323,9 @@ struct Row {
     double u;
     int64_t r;
 
-    __device__ __forceinline__ uint64_t whole(float z, double *w) const {
-        *w = fth::exp2_softmax(((double)z - (double)big) * set.rate);
-        return (uint64_t)__builtin_bit_cast(int64_t, *w + p.magic) - (uint64_t)__builtin_bit_cast(int64_t, p.magic);
-    }
-    __device__ __forceinline__ uint64_t whole(float z) const {
-        double w;
-        return whole(z, &w);
+    __device__ __forceinline__ double weight_of(float z) const { return fth::exp2_softmax(((double)z - (double)big) * set.rate); }
+    __device__ __forceinline__ uint64_t whole(double w) const {
+        return (uint64_t)__builtin_bit_cast(int64_t, w + p.magic) - (uint64_t)__builtin_bit_cast(int64_t, p.magic);
     }
     // Distances from the maximum in steps of 1/64 of their size, from 2^-16 to 2^16: they grow with the order.
     __device__ __forceinline__ int bin_of(float z) const {
@@ -333,7 +335,7 @@ struct Row {
     // f(logit, token, weight) of every candidate (of the row: of every token that is allowed), by this workgroup's threads.
     template <bool LIST, typename F> __device__ __forceinline__ void each(int n, F f) const {
         if constexpr (LIST) {
-            for (int i = threadIdx.x; i < n; i += kThreads) f(s.list[i].x, s.list[i].v, s.whole[i]);
+            for (int i = threadIdx.x; i < n; i += kThreads) f(s.list[i].x, s.list[i].v, s.weigh[i]);
         } else {
             for (int i = threadIdx.x; i < n; i += kAtOnce * kThreads) {
                 float z[kAtOnce];
@@ -341,7 +343,7 @@ struct Row {
                 for (int e = 0; e < kAtOnce; ++e) z[e] = i + e * kThreads < n ? x[i + e * kThreads] : -__builtin_inff();
 #pragma unroll
                 for (int e = 0; e < kAtOnce; ++e)
-                    if (z[e] > -__builtin_inff()) f(z[e], (uint32_t)(i + e * kThreads), whole(z[e]));
+                    if (z[e] > -__builtin_inff()) f(z[e], (uint32_t)(i + e * kThreads), weight_of(z[e]));
             }
         }
     }
@@ -356,8 +358,9 @@ struct Row {
             s.count[b] = 0;
         }
     }
-    __device__ __forceinline__ void to_bin(float z, uint64_t w) const {
+    __device__ __forceinline__ void to_bin(float z, double weight) const {
         const int b = bin_of(z);
+        const uint64_t w = whole(weight);
         atomicAdd(&s.count[b], 1u);
         if (w) atomicAdd(reinterpret_cast<unsigned long long *>(&s.weight[b]), (unsigned long long)w);
     }
@@ -414,8 +417,8 @@ struct Row {
         uint64_t weighs = f.code, had = f.weight;
         const uint32_t members = s.count[bin];
         if (members <= kRanked) {
-            each<LIST>(n, [&](float z, uint32_t v, uint64_t w) {
-                if (bin_of(z) == bin) s.few[atomicAdd(&f.members, 1u)] = Member{code_of(z, v), w};
+            each<LIST>(n, [&](float z, uint32_t v, double w) {
+                if (bin_of(z) == bin) s.few[atomicAdd(&f.members, 1u)] = Member{code_of(z, v), whole(w)};
             });
             __syncthreads();
             // ranks, in whatever order the members stand: PARTS neighbouring threads for one
@@ -453,11 +456,11 @@ struct Row {
         // Digit by digit (the bins of digits stand where the members would); of the row the members alone, if the list has room for them.
         if constexpr (!LIST) {
             if (members <= kList) {
-                each<false>(n, [&](float z, uint32_t v, uint64_t w) {
+                each<false>(n, [&](float z, uint32_t v, double w) {
                     if (bin_of(z) != bin) return;
                     const uint32_t at_member = atomicAdd(&f.members, 1u);
                     s.list[at_member] = Entry{z, v};
-                    s.whole[at_member] = w;
+                    s.weigh[at_member] = w;
                 });
                 return digits<true>((int)members, bin, k != 0, goal, had, weighs, f, weight);
             }
@@ -477,12 +480,12 @@ struct Row {
                 digit_count[d] = 0;
             }
             __syncthreads();
-            each<LIST>(n, [&](float z, uint32_t v, uint64_t w) {
+            each<LIST>(n, [&](float z, uint32_t v, double w) {
                 const uint64_t c = code_of(z, v);
                 if (bin_of(z) != bin || (shift < 56 && c >> (shift + 8) != prefix)) return;
                 const int at_digit = (int)(c >> shift) & 255;
                 atomicAdd(&digit_count[at_digit], 1u);
-                atomicAdd(reinterpret_cast<unsigned long long *>(&digit_weight[at_digit]), (unsigned long long)w);
+                atomicAdd(reinterpret_cast<unsigned long long *>(&digit_weight[at_digit]), (unsigned long long)whole(w));
             });
             __syncthreads();
             if (threadIdx.x < 64) {  // four digits a lane
@@ -549,48 +552,76 @@ struct Row {
         return last;
     }
 
+    // Which thread's `mine` the number leads to: the first whose sums reach over it, or where rounding at the very end leaves none, the last that has
+    // anything. (Sums in floating point need not ascend from thread to thread: their comparison alone could name two threads or none.)
+    struct Drawn {
+        int who;
+        double left, total;  // of the number, once what is before the thread is gone (in that thread alone); of all threads
+    };
+    __device__ __forceinline__ Drawn draw(double mine) const {
+        const BlockScan<double> scan(mine, reinterpret_cast<double *>(s.sums[0]));
+        __syncthreads();
+        scan.write();
+        if (threadIdx.x == 0) {
+            s.finds[0].at = kThreads;
+            s.finds[1].at = -1;
+        }
+        __syncthreads();
+        Drawn d;
+        const double upto = scan.read_upto(&d.total), target = d.total * u;
+        const uint64_t over = __ballot(mine > 0.0 && upto > target), some = __ballot(mine > 0.0);
+        const int first = threadIdx.x & ~63;
+        if (threadIdx.x == first) {
+            if (over) atomicMin(&s.finds[0].at, first + __builtin_ctzll(over));
+            if (some) atomicMax(&s.finds[1].at, first + 63 - __builtin_clzll(some));
+        }
+        __syncthreads();
+        d.who = s.finds[0].at;
+        d.left = target - (upto - mine);
+        if (d.who == kThreads) {
+            d.who = s.finds[1].at;
+            d.left = 1e300;
+        }
+        return d;
+    }
+
     // The token among the candidates up to `last` and above min-p.
     __device__ __forceinline__ void draw_list(int n, uint64_t last) const {
         const int t = threadIdx.x, each_has = (n + kThreads - 1) / kThreads, from = t * each_has, to = from + each_has < n ? from + each_has : n;
-        auto kept = [&](int i) -> uint64_t {
-            if (code_of(s.list[i].x, s.list[i].v) > last) return 0;
-            if (set.min_p > 0.f) {
-                double w;
-                whole(s.list[i].x, &w);
-                if (w < (double)set.min_p) return 0;
-            }
-            return s.whole[i];
+        auto kept = [&](int i) {
+            const double w = s.weigh[i];
+            return code_of(s.list[i].x, s.list[i].v) > last || w < (double)set.min_p ? 0.0 : w;
         };
-        uint64_t mine = 0, total;
+        double mine = 0.0;
         for (int i = from; i < to; ++i) mine += kept(i);
-        uint64_t before = block_scan(mine, s.sums[0], &total);
-        uint64_t target = (uint64_t)((double)total * u);
-        target = target < total ? target : total - 1;
-        if (mine == 0 || before > target || before + mine <= target) return;
+        const Drawn d = draw(mine);
+        if (t != d.who) return;
+        double left = d.left, share = 0.0;
+        int token = 0;
         for (int i = from; i < to; ++i) {
-            const uint64_t w = kept(i);
-            if (before + w > target) {
-                write((int)s.list[i].v, (double)w / (double)total);
-                return;
-            }
-            before += w;
+            const double w = kept(i);
+            if (!(w > 0.0)) continue;
+            token = (int)s.list[i].v;
+            share = w;
+            if (w > left) break;
+            left -= w;
         }
+        write(token, share / d.total);
     }
 
     // The same from the whole row: cut into 256 ranges, whose sums give the range; a wavefront finds the token in it.
     __device__ __forceinline__ void draw_row(int n, uint64_t last) const {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, length = ((n + 255) / 256 + 63) & ~63;
-        uint64_t *ranges = &s.few[0].code;
+        double *ranges = reinterpret_cast<double *>(s.few);
         auto logit = [&](int64_t i) { return i < n ? x[i] : -__builtin_inff(); };
-        auto kept = [&](int64_t i, float z) -> uint64_t {
-            if (!(z > -__builtin_inff()) || code_of(z, (uint32_t)i) > last) return 0;
-            double w;
-            const uint64_t all = whole(z, &w);
-            return w >= (double)set.min_p ? all : 0;
+        auto kept = [&](int64_t i, float z) {
+            if (!(z > -__builtin_inff()) || code_of(z, (uint32_t)i) > last) return 0.0;
+            const double w = weight_of(z);
+            return w < (double)set.min_p ? 0.0 : w;
         };
         __syncthreads();
         for (int g = wave; g < 256; g += kThreads / 64) {
-            uint64_t sum = 0;
+            double sum = 0.0;
             const int64_t end = (g + 1) * (int64_t)length;
             if (end - length < n)
                 for (int64_t i = end - length + lane; i < end; i += kAtOnce * 64) {
@@ -605,27 +636,24 @@ struct Row {
         }
         __syncthreads();
         static_assert(kThreads >= 256, "a thread for each range");
-        const uint64_t mine = threadIdx.x < 256 ? ranges[threadIdx.x] : 0;
-        uint64_t total;
-        const uint64_t before = block_scan(mine, s.sums[0], &total);
-        uint64_t target = (uint64_t)((double)total * u);
-        target = target < total ? target : total - 1;
-        if (mine > 0 && before <= target && before + mine > target) {
-            s.finds[0].at = threadIdx.x;
-            s.finds[0].code = target - before;
-        }
+        const Drawn d = draw(threadIdx.x < 256 ? ranges[threadIdx.x] : 0.0);
+        if ((int)threadIdx.x == d.who) s.finds[0].code = __builtin_bit_cast(uint64_t, d.left);
         __syncthreads();
         if (wave != 0) return;
-        uint64_t left = s.finds[0].code;
-        const int g = s.finds[0].at;
+        double left = __builtin_bit_cast(double, s.finds[0].code), share = 0.0;
+        int token = 0;
         for (int i0 = 0; i0 < length; i0 += 64) {
-            const int64_t i = (int64_t)g * length + i0 + lane;
-            const uint64_t here = kept(i, logit(i)), upto = wave_scan(here, (uint64_t)0, AddOp());
-            if (here > 0 && upto > left && upto - here <= left) write((int)i, (double)here / (double)total);
-            const uint64_t all = lane_value(upto, 63);
-            if (all > left) return;
-            left -= all;
+            const int64_t i = (int64_t)d.who * length + i0 + lane;
+            const double here = kept(i, logit(i)), upto = wave_scan(here, 0.0, AddOp());
+            const uint64_t over = __ballot(here > 0.0 && upto > left), some = __ballot(here > 0.0);
+            if (!some) continue;
+            const int which = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
+            token = (int)((int64_t)d.who * length + i0 + which);
+            share = lane_value(here, which);
+            if (over) break;
+            left -= lane_value(upto, 63);
         }
+        if (lane == 0) write(token, share / d.total);
     }
 
     // Without a filter: the token that `left` of the weight before it leads to, in piece `at`. Where rounding leads past the piece's end, its
@@ -746,9 +774,9 @@ __global__ __launch_bounds__(kThreads) void sample_choice_kernel(const SampleArg
         auto put = [&](int i, int h, Entry one) {
             const uint32_t place = s.places[i] + 64 * h;
             if (place + lane >= s.places[i + 1]) return;
-            const uint64_t w = row.whole(one.x);
+            const double w = row.weight_of(one.x);
             s.list[place + lane] = one;
-            s.whole[place + lane] = w;
+            s.weigh[place + lane] = w;
             row.to_bin(one.x, w);
         };
 #pragma unroll
@@ -768,7 +796,7 @@ __global__ __launch_bounds__(kThreads) void sample_choice_kernel(const SampleArg
         row.clear_bins();
     }
     __syncthreads();
-    row.each<false>((int)p.d.vocab, [&](float z, uint32_t, uint64_t w) { row.to_bin(z, w); });
+    row.each<false>((int)p.d.vocab, [&](float z, uint32_t, double w) { row.to_bin(z, w); });
     __syncthreads();
     last = row.filter<false>((int)p.d.vocab, total * p.unit, limit);
     row.draw_row((int)p.d.vocab, last);

@@ -551,9 +551,9 @@ int32_t fth_dev_logits_process_f32(const fth_logits_desc *d, const float *logits
  * temperature, top_k, top_p and min_p may each be NULL (temperature 1, that filter left out). Logits of -inf are never chosen. A
  * row that holds NaN or +inf or nothing above -inf, or whose settings are out of range (temperature negative or not finite,
  * top_k < 0, top_p or min_p NaN or negative, min_p > 1, uniform outside [0, 1)) gets token -1 and logprob NaN, and bad_index (device, may be NULL)
- * receives the lowest such row, or -1. Exponentials and sums are fp64, since which side of a border a number lies on decides the token; in a
- * row with a filter w counts as a whole multiple of 2^-45 of the largest (2^-44 above 2^17 tokens, a bit less for each doubling), so what is
- * below half of that is not drawn there. Runs repeat bit for bit, and rows do not depend on each other. The workspace (an eighth of the
+ * receives the lowest such row, or -1. Exponentials and sums are fp64, since which side of a border a number lies on decides the token;
+ * where the last token of top-p is looked for, w counts as a whole multiple of 2^-45 of the largest (2^-44 above 2^17 tokens, a bit less for each
+ * doubling). Runs repeat bit for bit, and rows do not depend on each other. The workspace (an eighth of the
  * logits' bytes and a little) is overwritten; what it holds before does not matter. At most 2^30 tokens, 2^20 rows and 2^42 logits. */
 typedef struct fth_sample_desc {
     int64_t rows, vocab, logits_stride; /* elements, >= vocab */

@@ -1,5 +1,5 @@
-"""Sampling against weights in 64 bits that are rounded nowhere: numbers at borders, and
-vocabularies above 131072 tokens, where a lane of the choice has several pieces of a row and, further on, the row too many to list."""
+"""Sampling against weights in 64 bits that are rounded nowhere: log-probabilities of unlikely tokens, the ends and borders of the numbers,
+and vocabularies above 131072 tokens, where a lane of the choice has several pieces of a row and, further on, the row too many to list."""
 import math
 
 import numpy as np
@@ -49,6 +49,45 @@ def agree(hip, x, u, **kw):
         lp = math.log(w[i] / total)
         assert abs(l[r] - lp) <= 2.0 ** -24 * abs(lp) + 2.0 ** -36, (r, t[r], l[r], lp, kw_r)
     return t, l
+
+
+@pytest.mark.parametrize("kw", [dict(top_k=41), dict(top_k=500), dict(min_p=1e-30), dict(top_k=45, min_p=1e-27), dict(top_k=20000), dict(top_k=20000, min_p=1e-30), dict()], ids=str)
+def test_unlikely_tokens(hip, kw):
+    """40 tokens at 2^-20 to 2^-85 of the largest weight stand before all others, and the numbers lead to each of them."""
+    vocab = 50257
+    x = np.random.RandomState(1).normal(-80.0, 2.0, (1, vocab)).astype(np.float32)
+    x[0, :40] = np.linspace(-14.0, -59.0, 40)
+    x[0, 20000] = 0.0
+    v, w = kept(x[0], **kw)
+    assert np.array_equal(v[:40], np.arange(40))
+    middle = (running(w) - w / 2)[:40].astype(np.float64) / math.fsum(w)
+    u = np.concatenate([[0.0, 2.0 ** -90], middle[::-1], middle, [2.0 ** -10, 0.5]])
+    rows = len(u)
+    t, l = call(hip, np.repeat(x, rows, 0), u, **{n: np.full(rows, s) for n, s in kw.items()})
+    # Sums of fp64 weights, largest 1: the k-th token of a descending line starts where the ones before it end, to 2^-53 of what they weigh
+    back = np.argsort(-w[:40])  # (they descend)
+    assert np.array_equal(back, np.arange(40))
+    for r in range(rows):
+        i = int(np.searchsorted(v, t[r]))
+        assert v[i] == t[r] and abs(l[r] - math.log(w[i] / math.fsum(w))) <= 2.0 ** -24 * abs(l[r]) + 2.0 ** -36, (r, t[r], l[r])
+    assert t[0] == 0 and t[1] == 0
+    assert t[2:42].tolist() == t[42:82].tolist()[::-1]
+    # to 2^-50 of the likelier ones before it: the first dozen tokens are told apart
+    assert t[42:42 + 12].tolist() == list(range(12)) and t[-1] == 20000
+
+
+def test_the_first_token_that_is_kept(hip):
+    """0 and the smallest numbers lead to the first kept token that has any weight, however little."""
+    for vocab, at in ((70, 3), (5000, 1), (50257, 31000)):
+        for low in (-30.0, -40.0, -100.0, -600.0):
+            x = np.full((6, vocab), -np.inf, np.float32)
+            x[:, at] = low
+            x[:, at + 7] = 1.0
+            x[:, at + 9] = 0.5
+            u = np.array([0.0, 1e-320, 2.0 ** -1000, 0.0, 0.3, 0.9])
+            for kw in (dict(top_k=3), dict(top_k=10, temperature=0.9), dict(top_k=2), dict()):
+                t, _ = agree(hip, x, u, **{n: np.full(6, v) for n, v in kw.items()})
+                assert t[0] == t[3] == (at if kw.get("top_k") != 2 else at + 7)
 
 
 def borders(x, rows, seed, **kw):
