@@ -95,13 +95,12 @@ __device__ __forceinline__ float larger_scale(float had, float needs) { return h
 // What elements are multiplied by: 0 under a scale that is none.
 __device__ __forceinline__ float per_scale(float s) { return s > 0.f ? 1.f / s : 0.f; }
 
-// To nearest even; |x| is within the type's range, or x is not finite (0).
+// To nearest even; |x| is within the type's range. NaN is for e4m3 alone, which has a code for it.
 __device__ __forceinline__ uint32_t to_code(float x, fth::i8) {
-    x = fabsf(x) < __builtin_inff() ? __builtin_rintf(x) : 0.f;
-    return (uint32_t)(int)fminf(fmaxf(x, -127.f), 127.f) & 255u;
+    return (uint32_t)(int)fminf(fmaxf(__builtin_rintf(x), -127.f), 127.f) & 255u;
 }
 __device__ __forceinline__ uint32_t to_code(float x, fth::e4m3) {
-    x = fabsf(x) < __builtin_inff() ? fminf(fmaxf(x, -448.f), 448.f) : 0.f;
+    x = x == x ? fminf(fmaxf(x, -448.f), 448.f) : x;
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false) & 255u;
 }
 
@@ -173,7 +172,7 @@ template <typename T> __global__ __launch_bounds__(64) void append_scaled_kernel
         const float shrink = had * per;
         for (int64_t x = lane; x < (int64_t)(run.row - run.first) * hd; x += 64) {
             const int row = run.first + (int)(x / hd), c = (int)(x % hd);
-            store(row, c, fth::to_f32(dst[row * p.c.row_stride + c]) * shrink);
+            store(row, c, now == now ? fth::to_f32(dst[row * p.c.row_stride + c]) * shrink : 0.f);
         }
         if (lane == 0) *scale = now;
     }
