@@ -90,10 +90,10 @@ template <typename T> __device__ __forceinline__ float scale_for(float largest) 
     const int e = __builtin_amdgcn_frexp_expf(largest) - (std::is_same<T, fth::i8>::value ? 7 : 9) + (m > (std::is_same<T, fth::i8>::value ? 0.9921875f : 0.875f));
     return __builtin_ldexpf(1.f, e < -126 ? -126 : e);
 }
-// Which of two scales holds: the larger, NaN before all.
-__device__ __forceinline__ float larger_scale(float had, float needs) { return had != had || needs != needs ? __builtin_nanf("") : had > needs ? had : needs; }
-// What elements are multiplied by: 0 under a scale that is none.
-__device__ __forceinline__ float per_scale(float s) { return s > 0.f ? 1.f / s : 0.f; }
+// Which of two scales holds: the larger (what was there may be negative, where something else has filled the cache), NaN before all.
+__device__ __forceinline__ float larger_scale(float had, float needs) { return had != had || needs != needs ? __builtin_nanf("") : fabsf(had) > needs ? had : needs; }
+// What elements are multiplied by: 0 under a scale that is none or subnormal (such a one holds for zeros alone).
+__device__ __forceinline__ float per_scale(float s) { return fabsf(s) >= 0x1p-126f ? 1.f / s : 0.f; }
 
 // To nearest even; |x| is within the type's range. NaN is for e4m3 alone, which has a code for it.
 __device__ __forceinline__ uint32_t to_code(float x, fth::i8) {

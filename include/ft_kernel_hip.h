@@ -504,7 +504,8 @@ void fth_dev_paged_scales_contiguous(fth_paged_scales *sc, const fth_paged_cache
  * for a block of zeros, else a power of two (2^-126 at least), the smallest whose 127 (448) multiples reach the largest element
  * that the block was given since its first position was written; NaN if one of those was not finite, and then all of the
  * block is NaN to whoever reads it. Elements are rounded to nearest even multiples. Where tokens raise the scale of a block, what
- * the block holds before them is rounded to the new scale (e4m3: exact but for what becomes subnormal; NaN codes stay NaN). A prompt gets the scales
+ * the block holds before them is rounded to the new scale (e4m3: exact but for what becomes subnormal; NaN codes stay NaN). A scale
+ * that something else has given the block holds as long as its size is the larger, a negative one too; one that is not finite stays. A prompt gets the scales
  * that its tokens one by one would get. What a block holds at and behind the positions written counts as gone: a
  * sequence that is cut back goes on from there, and a token at the first position of a block starts it anew.
  * Tokens of one block stand one after the other in the call, positions ascending by one; one that follows a token of its block
