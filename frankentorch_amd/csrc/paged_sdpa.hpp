@@ -119,7 +119,9 @@ template <typename T, typename Args> __global__ __launch_bounds__(64) void paged
                 if (page >= 0 && lane < n) {
                     const int64_t i = (int64_t)page * p.sc.page_stride + hk * p.sc.head_stride + (int)p.by_block((uint32_t)(key - index * page_size));
                     ks = p.k_scales[i];
-                    vs[lane] = p.v_scales[i];
+                    const float v = p.v_scales[i];
+                    ks = __builtin_fmaf(ks, 0.f, ks);  // infinite: NaN
+                    vs[lane] = __builtin_fmaf(v, 0.f, v);
                 }
             }
             if (page >= 0 && lane < n) {

@@ -265,7 +265,11 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
         for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(q[i][e]));
     big = rows_reduce(big, MaxOp());
     const int up = big > 0.f && big < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(big) : 0;
-    const float down = __builtin_ldexpf(1.f, -up);
+    // What a score is multiplied by beside its key's scale: 2^-up scale2, of which `rest` has the power of two that would take it out of range (queries near
+    // the ends of float32).
+    const int over = __builtin_amdgcn_frexp_expf(p.scale2) - up, cut = over > 96 ? over - 96 : over < -96 ? over + 96 : 0;
+    const float factor = __builtin_ldexpf(p.scale2, -up - cut), rest = __builtin_ldexpf(1.f, cut);
+    const bool far = __any(cut != 0);
 #pragma unroll
     for (int i = 0; i < 2 * NK; ++i)
 #pragma unroll
@@ -304,8 +308,15 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
                     ks[s][r] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_ks), (j + s) & 63));
                     vs[s][r] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_vs), (j + s) & 63));
                 }
-                by[s][r] = ((ANY ? __shfl(ks[s][0], 4 * g + r) : ks[s][r % NL]) * down) * p.scale2;
+                const float k_scale = ANY ? __shfl(ks[s][0], 4 * g + r) : ks[s][r % NL];
+                by[s][r] = __builtin_fmaf(k_scale, 0.f, k_scale * factor);  // NaN for an infinite one, whatever its scores' sign (V's give NaN by their parts)
             }
+        if (far) {
+#pragma unroll
+            for (int s = 0; s < H; ++s)
+#pragma unroll
+                for (int r = 0; r < NS; ++r) by[s][r] *= rest;
+        }
         Place next[H];
         if constexpr (more) {
             if constexpr (ANY) {

@@ -1,9 +1,10 @@
-"""8-bit caches that something else has filled: NaN codes, scales that are negative, subnormal or infinite."""
+"""8-bit caches that something else has filled: NaN codes, scales that are negative, subnormal or infinite, in appends and in attention."""
 import numpy as np
 import pytest
 
 from scaled_case import Scaled, codes, values
 from test_gpu_paged_append_scaled import Call, ragged
+from test_gpu_paged_sdpa_scaled import expected, made, queries, run
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +78,47 @@ def test_scales_of_any_kind_before_the_tokens(hip, lead, dtype, had):
             # half a step: of whole numbers 1/2; of e4m3 2^-4 of the number, 2^-10 where it is subnormal; and 2^-22 for quotients by scales that are no powers of two
             step = 0.5 * abs(float(now)) if dtype == "i8" else np.maximum(np.abs(want) * 2.0 ** -4, abs(float(now)) * 2.0 ** -10)
             assert np.all(np.abs(held * float(now) - want) <= step * (1 + 2.0 ** -10) + np.abs(want) * 2.0 ** -22), (size, w)
+
+
+# ---- attention --------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["i8", "e4m3"])
+@pytest.mark.parametrize("d,page,block", [(64, 16, 16), (128, 16, 4), (128, 16, 1), (64, 8, 8), (80, 16, 16), (20, 16, 4)])
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+def test_a_scale_that_is_not_finite_is_nan(hip, dtype, d, page, block, value):
+    """Whoever sees the block gets NaN, whatever the sign of the scores that an infinite scale of K would give and whatever the codes; nobody else does."""
+    lens, hkv, new, hq = [100, 100, 100, 40], 2, 3, 4
+    p = made(71, lens, hkv, d, page, block, dtype)
+    q = np.abs(queries(len(lens), new, hq, d))
+    one = 1 if dtype == "i8" else 0x38
+    for s, sign in ((0, 0), (1, 1)):  # scores of one sign in the block of K
+        start = 20 - 20 % block
+        for pos in range(start, start + block):
+            r = p.row_at(s, pos, 0)
+            p.codes[0][r:r + d] = (256 - one if dtype == "i8" else one | 128) if sign else one
+    ref = expected(p, q, 0.2, lens)
+    p.scales[0][p.scale_at(0, 20, 0)] = value
+    p.scales[0][p.scale_at(1, 20, 0)] = value
+    p.scales[1][p.scale_at(2, 20, 1)] = value
+    got = run(hip, p, q, 0.2, lens)
+    nan = np.zeros(ref.shape, bool)
+    nan[0, :, :2] = nan[1, :, :2] = nan[2, :, 2:] = True
+    assert np.array_equal(np.isnan(got), nan)
+    assert np.max(np.abs(got[~nan] - ref[~nan])) <= 2e-5 * np.max(np.abs(ref[~nan]))
+
+
+@pytest.mark.parametrize("dtype", ["i8", "e4m3"])
+@pytest.mark.parametrize("block", [16, 4, 1])
+@pytest.mark.parametrize("size", [1e-37, 1e-33, 1e30, 1e35])
+def test_queries_near_the_ends_of_float32(hip, dtype, block, size):
+    """Scales of K bring the scores back: what scores are multiplied by goes through neither end."""
+    lens, d = [150, 33], 128
+    p = made(74, lens, 2, d, 16, block, dtype)
+    for s, n in enumerate(lens):
+        for pos in range(0, n, block):
+            for h in range(2):
+                p.scales[0][p.scale_at(s, pos, h)] /= np.float32(size)
+    q = (queries(2, 2, 4, d) * np.float32(size)).astype(np.float32)
+    got, ref = run(hip, p, q, 0.1, lens), expected(p, q, 0.1, lens)
+    assert np.max(np.abs(got - ref)) <= 2e-5 * np.max(np.abs(ref))
