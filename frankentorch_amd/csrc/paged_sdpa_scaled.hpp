@@ -9,7 +9,7 @@
 //     score meets the scale of its key's block in fp32 afterwards.
 //   * V as bf16, against weights that have met the scale of their key's block in fp32 and are cut into three parts of bf16, whose sum they
 //     are. They carry a factor of 2^40, which keeps the third part of every weight an output of fp32 can show above the smallest bf16; where that
-//     overflows (scales of V beyond 2^70) the share is walked again with 2^-24.
+//     overflows (scales of V beyond 2^70) the share is walked twice more, for the keys with scales of V below 2^48, and for the others with 2^-24.
 // e4m3 becomes either type two at a time by one instruction of gfx950; whole numbers become f16 by the bits of 1024 + 128 + x, bf16 through fp32.
 //
 // Measured: 64 sequences of 1024 to 8191 keys, 32 query heads on 8 of 128, e4m3, blocks of 16 (614 MB): 111 us, 5.6 TB/s (one wavefront a row 3660;
@@ -150,12 +150,22 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
         return make_int2(p.table[seq * p.c.table_stride + index], key - index * (int)p.c.page_size);
     };
     int2 ahead64;
+    // Which keys this walk has, 0: all, 1: those with scales of V below 2^48, 2: the others; their scales (of the others: 0).
+    int part = 0;
+    bool others = false;
+    auto of_part = [&](float s) __attribute__((always_inline)) {
+        if (part == 0) return s;
+        const bool below = fabsf(s) < 0x1p48f;
+        others |= !below;
+        return below == (part == 1) ? s : 0.f;
+    };
     auto look_ahead = [&](int j0) __attribute__((always_inline)) {
         mine = place_of(ahead64);
         if constexpr (SIXTEEN) {
             const int64_t at = mine.page + p.by_block((uint32_t)mine.in_page);
             my_ks = KS[at];
             my_vs = VS[at];
+            my_vs = of_part(my_vs);
         }
         ahead64 = page_ahead(j0 + 64);
     };
@@ -311,11 +321,15 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
                 const float k_scale = ANY ? __shfl(ks[s][0], 4 * g + r) : ks[s][r % NL];
                 by[s][r] = __builtin_fmaf(k_scale, 0.f, k_scale * factor);  // NaN for an infinite one, whatever its scores' sign (V's give NaN by their parts)
             }
-        if (far) {
+        if (far || (!SIXTEEN && part > 0)) {
 #pragma unroll
-            for (int s = 0; s < H; ++s)
+            for (int s = 0; s < H; ++s) {
 #pragma unroll
                 for (int r = 0; r < NS; ++r) by[s][r] *= rest;
+                if constexpr (!SIXTEEN)
+#pragma unroll
+                    for (int r = 0; r < NL; ++r) vs[s][r] = of_part(vs[s][r]);
+            }
         }
         Place next[H];
         if constexpr (more) {
@@ -439,12 +453,14 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
             }
         }
     };
-    for (float unit = 0x1p40f;; unit = 0x1p-24f) {
+    // All tiles of this wavefront; whether something in the outputs is not finite.
+    auto walk = [&]() __attribute__((always_inline)) {
+        const float unit = part < 2 ? 0x1p40f : 0x1p-24f;
         m_run = -__builtin_inff();
         l_run = l_before = 0.f;
 #pragma unroll
         for (int e = 0; e < NE; ++e) o[e] = before[e] = F4{0.f, 0.f, 0.f, 0.f};
-        if (wave >= tiles) break;
+        if (wave >= tiles) return false;
         int t = wave;
         for (; t + kWaves < tiles; t += kWaves) step(t, unit, std::true_type());
         step(t, unit, std::false_type());
@@ -456,10 +472,27 @@ __device__ __forceinline__ void scaled_segment(const ScaledArgs &p, float *lds_o
             for (int r = 0; r < 4; ++r) {
                 o[e][r] += before[e][r];
                 check = __builtin_fmaf(o[e][r], 0.f, check);
-                o[e][r] *= unit > 1.f ? 0x1p-40f : 0x1p24f;
+                o[e][r] *= part < 2 ? 0x1p-40f : 0x1p24f;
             }
-        if (unit < 1.f || !__any(!(check == 0.f))) break;
-        begin();
+        return __any(!(check == 0.f)) != 0;
+    };
+    if (walk()) {  // with code of its own (as one loop, in which a branch of every tile asks which part it is: heads of 80, i8, 64 sequences of up to 8191 keys 116 -> 122 us)
+        for (;;) {
+            ++part;
+            begin();
+            walk();
+            if (part == 1 && !__any(others)) break;  // (the same as before: what is not finite comes from elsewhere)
+            float *mine = lds_o + (wave * 16 + lr) * (DP + 4);  // this wavefront's place holds the first part for the second
+#pragma unroll
+            for (int e = 0; e < NE; ++e)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float &x = mine[(4 * g + r) * NE + e];
+                    if (part == 1) x = o[e][r];
+                    else o[e][r] += x;
+                }
+            if (part == 2) break;
+        }
     }
 
     bad = __any(bad);

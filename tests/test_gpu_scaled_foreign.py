@@ -1,4 +1,7 @@
-"""8-bit caches that something else has filled: NaN codes, scales that are negative, subnormal or infinite, in appends and in attention."""
+"""8-bit caches that something else has filled: NaN codes, scales that are negative, subnormal or infinite, in appends and in attention; scales
+of V from one end of float32 to the other in one sequence."""
+import math
+
 import numpy as np
 import pytest
 
@@ -122,3 +125,50 @@ def test_queries_near_the_ends_of_float32(hip, dtype, block, size):
     q = (queries(2, 2, 4, d) * np.float32(size)).astype(np.float32)
     got, ref = run(hip, p, q, 0.1, lens), expected(p, q, 0.1, lens)
     assert np.max(np.abs(got - ref)) <= 2e-5 * np.max(np.abs(ref))
+
+
+@pytest.mark.parametrize("dtype", ["i8", "e4m3"])
+@pytest.mark.parametrize("d,block", [(64, 16), (128, 1), (64, 4), (20, 4)])
+@pytest.mark.parametrize("large", [1e24, 1e30, 2.0 ** 108])
+def test_scales_of_v_far_apart(hip, dtype, d, block, large):
+    """One block of V has a scale that takes the products beyond float32's range under the factor that weights otherwise carry, and codes of 0 in half of its columns;
+    the others are from 1e-36 to 1. Every output is compared by itself, with the sum of its terms' sizes. Scores are below 8: roundings of them move a
+    weight by 3 x 8 log2(e) x 2^-24, the products' and the sums' add as much again, far below 2e-5."""
+    n, hkv = 300, 2
+    p = made(72, [n], hkv, d, 16, block, dtype)
+    q = queries(1, 2, 4, d, std=0.3)
+    rng = np.random.RandomState(9)
+    for h in range(hkv):
+        for pos in range(0, n, block):
+            p.scales[0][p.scale_at(0, pos, h)] = 0.01
+            p.scales[1][p.scale_at(0, pos, h)] = 10.0 ** rng.uniform(-36, -33) if h else 10.0 ** rng.uniform(-36, 0)
+        p.scales[1][p.scale_at(0, 100, h)] = large
+        for pos in range(100 - 100 % block, 100 - 100 % block + block):
+            r = p.row_at(0, pos, h)
+            p.codes[1][r:r + d // 2] = 0
+    got, ref = run(hip, p, q, 0.05, [n]), expected(p, q, 0.05, [n])
+    p.codes[1] = np.abs(np.clip(p.codes[1].view(np.int8).astype(np.int32), -127, 127)).astype(np.uint8) if dtype == "i8" else p.codes[1] & 127
+    p.scales[1] = np.abs(p.scales[1])
+    size = expected(p, q, 0.05, [n])
+    assert np.all(np.isfinite(got)) and np.all(np.abs(got - ref) <= 2e-5 * size)
+
+
+@pytest.mark.parametrize("dtype", ["i8", "e4m3"])
+@pytest.mark.parametrize("block", [1, 4, 16])
+@pytest.mark.parametrize("low,high", [(0.01, 30.0), (1e-30, 1e-28), (1e20, 1e30), (1e-20, 1e20)])
+def test_each_output_by_itself(hip, dtype, block, low, high):
+    """Scales of any size and sign, each output against the sum of its own terms' sizes (scores stay below 60: 3 roundings of 60 log2(e) units of 2^-24
+    and a few more of the products are within 2e-5)."""
+    lens, hkv, d = [300, 40], 2, 64
+    p = made(73, lens, hkv, d, 16, block, dtype)
+    rng = np.random.RandomState(5)
+    q = queries(2, 1, 4, d, std=0.5)
+    for s, n in enumerate(lens):
+        for pos in range(0, n, block):
+            for h in range(hkv):
+                p.scales[0][p.scale_at(s, pos, h)] = rng.uniform(0.001, 0.004) * rng.choice([-1, 1])
+                p.scales[1][p.scale_at(s, pos, h)] = math.exp(rng.uniform(math.log(low), math.log(high))) * rng.choice([-1, 1, 1])
+    got, ref = run(hip, p, q, 0.125, lens), expected(p, q, 0.125, lens)
+    p.codes[1] = np.abs(np.clip(p.codes[1].view(np.int8).astype(np.int32), -127, 127)).astype(np.uint8) if dtype == "i8" else p.codes[1] & 127
+    p.scales[1] = np.abs(p.scales[1])
+    assert np.all(np.abs(got - ref) <= 2e-5 * expected(p, q, 0.125, lens))
