@@ -533,7 +533,8 @@ def paged_scales(cache, block) -> _lib.PagedScales:
 def paged_append_scaled(cache, scales, desc, q, k, v, cosines, sines, block_table, seq_ids, positions, q_out, k_cache, v_cache, k_scales, v_scales, bad_index=None,
                         stream=None):
     """paged_append into a cache of 8 bits: elements are rounded to multiples of their block's scale, which grows to what the block's
-    largest element needs. Tokens of one block stand one after the other, positions ascending."""
+    largest element needs. Tokens of one block stand one after the other, positions ascending by one: from the first that does not, the block's are
+    left out, and `bad_index` receives that one's number."""
     check(_lib.load().fth_dev_paged_append_scaled_f32(C.byref(cache), C.byref(scales), C.byref(desc), _ptr(q), _ptr(k), _ptr(v), _ptr(cosines), _ptr(sines),
                                                       _ptr(block_table), _ptr(seq_ids), _ptr(positions), _ptr(q_out), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales),
                                                       _ptr(v_scales), _ptr(bad_index), stream))

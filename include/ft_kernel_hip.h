@@ -509,7 +509,8 @@ void fth_dev_paged_scales_contiguous(fth_paged_scales *sc, const fth_paged_cache
  * that its tokens one by one would get. What a block holds at and behind the positions written counts as gone: a
  * sequence that is cut back goes on from there, and a token at the first position of a block starts it anew.
  * Tokens of one block stand one after the other in the call, positions ascending by one; one that follows a token of its block
- * without being at the next position is left out and reported like one without a place, but for its queries, which are rotated.
+ * without being at the next position is left out and reported like one without a place, and so is all that follows it in the block,
+ * also what goes on from the tokens before it or from itself; their queries are rotated. (In blocks of one position that is a place that comes again.)
  * Tokens of one block in two places of the list leave that block unspecified (nothing else). */
 int32_t fth_dev_paged_append_scaled_f32(const fth_paged_cache *c, const fth_paged_scales *sc, const fth_paged_append_desc *d, const float *q, const float *k,
                                         const float *v, const float *cosines, const float *sines, const int32_t *block_table, const int32_t *seq_ids,
