@@ -5,7 +5,7 @@
 // one after the other in the call; whoever has its first token does all of it, so that no two workgroups touch one block. A run ends at the first token
 // that is not at the next position: that one is reported, and what follows it in the block belongs to no run.
 //
-// Bound by reading the rows and writing the queries once: 3 prompts of up to 7001 tokens, 32 query heads on 8 of 128, e4m3, blocks of 48: 115 us, 5.9
+// Bound by reading the rows and writing the queries once: 3 prompts of up to 7001 tokens, 32 query heads on 8 of 128, e4m3, blocks of 48: 113 us, 6.0
 // TB/s (element by element 473; a wavefront a run that first asks for its place 156). Short calls wait for loads that depend on each
 // other, position -> page -> scale: 5.6 us for a step of 64 sequences, where an empty launch takes 5.
 

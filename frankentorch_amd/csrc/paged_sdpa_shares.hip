@@ -115,6 +115,9 @@ Plan plan(const fth_paged_cache &c, const fth_paged_sdpa_desc &d) {
     // up to 5000, bf16: 117 / 103; 128 on heads of 256 of up to 1500, bf16: 198 / 165; 512 of 1000 on one head: 51 / 56, 1024 of 20 keys:
     // 19 / 33, where beginning a pair costs more than waiting for one), two where their tiles would not keep enough bytes on the way (the first
     // of these: 204 / 209, the second 202 / 210, heads of 64, bf16: 108 / 103).
+    // Caches of 8 bits by the same bytes (us): even / shares of 512 KB / one each, 64 of up to 8191 120 / 132 / 139, on 12 heads of 64 of up to 12000 129 / 136 /
+    // 153, 128 on heads of 256 of up to 3000 180 / 213 / 183; shares from 512 KB on instead, 64 of up to 3000 56 / 60, on 12 heads of 64 of up to 5000 69 / 77, 128 on
+    // heads of 256 of up to 1500 104 / 129; two workgroups a compute unit / one, the first two of these 120 / 129 and 129 / 156.
     p.even = p.enough = 0;
     p.step_log2 = 7;
     if (p.tiles && large && c.num_seqs <= 256) {
@@ -128,7 +131,9 @@ Plan plan(const fth_paged_cache &c, const fth_paged_sdpa_desc &d) {
     // average, and that is read once (us, with / without: one sequence of 131071, bf16 87 / 99, fp32 180 / 196; 64 of up to 8191,
     // bf16 217 / 229 in shares of 512 KB; 16 of up to 3967, four queries, f16, 260 MB 38.5 / 36.3, fp32, 520 MB 79 / 72; by the even
     // shares of today 196 / 220). The host knows the bound alone: where it is far above the lengths, calls that read one cache again and
-    // again lose (under 131072: 4 sequences of 3000 keys 47.5 / 34, 16 of 1000 22.4 / 17.2, 64 of 300 or 600 level).
+    // again lose (under 131072: 4 sequences of 3000 keys 47.5 / 34, 16 of 1000 22.4 / 17.2, 64 of 300 or 600 level). Caches of 8 bits, with / without: 64 of up to
+    // 8191 120 / 127, on 12 heads of 64 of up to 12000 129 / 137, 128 on heads of 256 of up to 3000 180 / 186; below the bound 64 of up to 4000 level, 24 38.6 / 34.2, one
+    // of 131071, 269 MB, 50.6 / 55.5 where two take turns and 49 / 46 where it is read again.
     p.nt = p.row_tiles == 1 && 2.0 * (double)c.num_seqs * (double)most * (double)c.kv_heads * (double)c.head_dim * (double)size > 500.0 * (1 << 20);
     return p;
 }

@@ -17,8 +17,10 @@
 // exponential (31 + 8.3). 64 rows of 50257 17.4 (9.4 + 8.7: 4.4 for reading, 3 for exponentials, 2.4 for the candidates), 16 10.6, 1 13.3. Slower were: pieces of 1024 logits (twice the
 // candidates), wavefronts that take several pieces with the next one's loads ahead and bounds of 72 or 64 registers, the last three by spills (87, 80 and
 // 90 us for the pieces); candidates straight to memory, a branch each (25.9); one thread to rank each member of a bin (the choice 17.1). Level: eight wavefronts a SIMD instead of six. The choice by 512 threads 20.9, 256 32.3 us.
-// Rows that the candidates do not decide (a nucleus of tens of thousands, top-k 20000) are read three times more, by one workgroup: 131071 logits 225 us,
-// 50257 88 to 106 (one logit a thread at a time, all members of a bin ranked: 690 and 137 to 154), most of it fp64 exponentials and atomics in LDS.
+// Rows that the candidates do not decide (a nucleus of tens of thousands, top-k 20000) are read again by one workgroup: once for the bins, once for each
+// border (top-k, top-p) or eight times where the border's bin has more than kList members, once for the draw, each time with an fp64 exponential a logit
+// and atomics in LDS. 131071 normal logits 156 to 193 us, 50257 90 to 108, 200 rows of 131071 192 to 237; 131071 equal logits 1730 us with one border, 3180
+// with two, 50257 730 and 1330 (of two values half of that). Vocabularies above kPlaces pieces, 2^20 tokens, are always read so.
 
 #include <type_traits>
 
