@@ -5,7 +5,7 @@ import math
 import numpy as np
 import pytest
 
-from frankentorch_amd.device import DeviceBuffer
+from frankentorch_amd.device import DeviceBuffer, Stream
 from test_gpu_sample import call, numbers
 
 pytestmark = pytest.mark.gpu
@@ -171,3 +171,31 @@ def test_rows_that_cannot_be_sampled_in_large_vocabularies(hip):
     for kw in (dict(), dict(top_k=np.full(4, 20), top_p=np.full(4, 0.9))):
         t, l = call(hip, x, numbers(8, 4), bad=bad, **kw)
         assert t[0] >= 0 and t[1:].tolist() == [-1] * 3 and np.all(np.isnan(l[1:])) and bad.to_host()[0] == 1
+
+
+def test_two_calls_at_once(hip):
+    """Calls on two streams, each with its workspace, give what they give alone."""
+    rows, vocab = 24, 50257
+    rng = np.random.RandomState(11)
+    x = [rng.normal(0.0, 2.0, (rows, vocab)).astype(np.float32) for _ in range(2)]
+    u = [numbers(s, rows) for s in (21, 22)]
+    kw = [dict(top_k=np.full(rows, 40, np.int32), top_p=np.full(rows, 0.9, np.float32)), dict(top_p=np.full(rows, 0.999, np.float32))]
+    alone = [call(hip, x[i], u[i], **kw[i]) for i in range(2)]
+    desc = hip.sample_desc(rows, vocab)
+    streams = [Stream() for _ in range(2)]
+    ops = []
+    for i in range(2):
+        k, p = (None if kw[i].get(n) is None else DeviceBuffer.from_host(kw[i][n]) for n in ("top_k", "top_p"))
+        ops.append([DeviceBuffer.from_host(x[i]), k, p, DeviceBuffer.from_host(u[i])])
+    outs = [[(DeviceBuffer((rows,), np.int32), DeviceBuffer((rows,))) for _ in range(10)] for _ in range(2)]
+    work = [hip.sample_workspace(desc) for _ in range(2)]
+    hip.synchronize()
+    for n in range(10):
+        for i in range(2):
+            logits, k, p, number = ops[i]
+            hip.sample(desc, logits, None, k, p, None, number, *outs[i][n], workspace=work[i], stream=streams[i].handle)
+    for s in streams:
+        s.synchronize()
+    for i in range(2):
+        for tokens, lp in outs[i]:
+            assert np.array_equal(tokens.to_host(), alone[i][0]) and np.array_equal(lp.to_host().view(np.uint32), alone[i][1].view(np.uint32))
